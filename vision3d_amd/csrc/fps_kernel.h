@@ -7,7 +7,7 @@
 //   * The cloud stays ON CHIP for the whole kernel: every thread keeps PPT points (x, y, z, running min-distance) in
 //     VGPRs -- a CU has 512 KiB of them, 3x its LDS -- so a round touches no global memory (the reference re-reads
 //     20 B/point/round through L2).
-//   * arg-max per round = per-thread strict-'>' scan (packed fp32 math) -> every lane asks an LDS coordinate table for
+//   * arg-max per round = per-thread strict-'>' scan (points taken in pairs) -> every lane asks an LDS coordinate table for
 //     ITS best point (one 16-byte read per lane, issued before the wave reduction and in flight under it: only the
 //     winner lane's answer is used, but which lane wins is not known yet and the read costs no VALU time) -> six-step
 //     DPP max butterfly per wave -> the winner lane writes ONE 20-byte record (x, y, z, distance | priority) into the
@@ -244,7 +244,7 @@ __global__ __launch_bounds__(THREADS) void fps_kernel(const float* __restrict__ 
     int bi = 0;
     float wmax;
     if constexpr (MODE != kFpsStream) {
-      // Scan: two points per packed fp32 instruction (v_pk_add / v_pk_mul: same IEEE results as the scalar forms), the
+      // Scan: two points at a time (scalar instructions: the build turns the packed fp32 forms off, see the Makefile), the
       // running maximum by v_max3 (no compare, no mask hazard on the chain).  WHICH point holds the maximum -- the first
       // one in scan order, :67's strict '>' -- and the wave's maximum come out of fps_pick's interleaved block.
 #pragma unroll

@@ -38,8 +38,8 @@ __device__ __forceinline__ T sq_dist(T qx, T qy, T qz, T sx, T sy, T sz) {
   return (dx * dx + dy * dy) + dz * dz;
 }
 
-// Two queries against one support in packed fp32 (v_pk_add_f32 / v_pk_mul_f32: per-element IEEE results identical
-// to the scalar form, half the instructions); the double variant is two scalar evaluations.
+// Two queries against one support as float pairs (the build turns packed fp32 instructions off, see the Makefile: each
+// element is a scalar operation with the IEEE result of sq_dist); the double variant is two scalar evaluations.
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef unsigned pd_u32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void sq_dist_pair(float qx0, float qy0, float qz0, float qx1, float qy1, float qz1, float sx,
