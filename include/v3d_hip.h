@@ -428,6 +428,59 @@ int v3d_point_to_node_partition_f32(const float* points, const float* nodes, int
 int v3d_point_to_node_knn(const void* workspace, int64_t N, int64_t M, int K, int64_t* node_knn_indices,
                           uint8_t* node_knn_masks, int device, void* stream);
 
+/* ---- transformer layers over packs: layer normalisation ----------------------------------------------------------------
+ * Element types of the calls below (`dtype`): features, outputs and gradients share one; statistics and sums are fp32.
+ *
+ * v3d_layer_norm_fwd: feats (rows,C), residual (rows,C) or NULL, weight / bias (C) of `weight_dtype` (the features' type or
+ * V3D_F32) or NULL (1 / 0) -> out (rows,C) = (t - mean) * rstd * weight + bias with t = feats + residual, the mean and the
+ * (biased, centred) variance of the row in fp32, rstd = 1 / sqrt(var + eps).  mean / rstd (rows) fp32: both or neither.
+ * v3d_layer_norm_bwd: grad (rows,C) of out, the forward's inputs and statistics -> grad_feats (rows,C) (NULL = not wanted;
+ * it is the residual's gradient too), grad_weight / grad_bias (C) of `weight_dtype` (either may be NULL), rows >= 1.  The
+ * column sums are added in a fixed order: the same bits every time.  `workspace`: v3d_layer_norm_bwd_workspace_bytes bytes,
+ * 256-B aligned, or NULL (stream-ordered allocation); not touched without grad_weight and grad_bias.
+ * Rows may start at any element (no alignment is asked for); C <= V3D_NORM_MAX_CHANNELS (half of it in fp32). */
+#define V3D_F32 0
+#define V3D_F16 1
+#define V3D_BF16 2
+#define V3D_NORM_MAX_CHANNELS 16384
+int v3d_layer_norm_fwd(const void* feats, const void* residual, const void* weight, const void* bias, void* out,
+                       float* mean, float* rstd, int dtype, int weight_dtype, int64_t rows, int64_t C, float eps,
+                       int device, void* stream);
+size_t v3d_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t C);
+int v3d_layer_norm_bwd(const void* grad, const void* feats, const void* residual, const void* weight, const float* mean,
+                       const float* rstd, void* grad_feats, void* grad_weight, void* grad_bias, int dtype,
+                       int weight_dtype, int64_t rows, int64_t C, void* workspace, size_t workspace_bytes, int device,
+                       void* stream);
+
+/* ---- transformer layers over packs: attention --------------------------------------------------------------------------
+ * v3d_attention_pack_fwd: q (total_q,H,D), k and v (total_s,KV,D): packs of B sequences with q_lengths / s_lengths (B) i64
+ * rows each (device data, never read on the host); H % KV == 0, query head h reads key head h / (H / KV).  Per sequence
+ *   out[i,h,:] = sum_j softmax_j(scale * q[i,h,:] . k[j,h',:]) v[j,h',:]
+ * over all keys j of the sequence or, with `causal`, over j <= i + (s_len - q_len): the last query sees every key.  A query
+ * that sees no key yields zeros; an infinity or NaN in a key or value that a query does not see does not reach it.  Rows
+ * behind the last sequence are written as zeros; lengths that overrun the totals are cut.  out (total_q,H,D) contiguous;
+ * lse (total_q,H) fp32 = natural log of the row's sum of exponentials (-inf without keys), what the backward needs; or NULL.
+ * `strides` (host array, elements): q row, q head, k row, k head, v row, v head -- the last dimension is contiguous, rows
+ * need no alignment.  Products of 16-bit types are exact, the probabilities are rounded to the type before they meet the
+ * values; scores, statistics and sums are fp32.  D <= V3D_ATTENTION_MAX_HEAD_SIZE, 0 < scale < inf.
+ *
+ * v3d_cached_attention: q (B,tokens,H,D) = the newest `tokens` tokens of every sequence, k_cache / v_cache
+ * (B,capacity,KV,D), lengths (B) i64 = filled rows, the new ones among them (cut to [0, capacity]): token t sees the rows
+ * j <= lengths[b] - tokens + t.  Rows past a length are never read.  `strides`: q row, q head, k batch, k row, k head,
+ * v batch, v row, v head; q rows are token b * tokens + t.
+ *
+ * workspace: v3d_*_workspace_bytes bytes (0 where the row tiles alone fill the GPU), 256-B aligned, or NULL. */
+#define V3D_ATTENTION_MAX_HEAD_SIZE 256
+size_t v3d_attention_pack_workspace_bytes(int B, int64_t total_q, int64_t total_s, int H, int KV, int D);
+int v3d_attention_pack_fwd(const void* q, const void* k, const void* v, const int64_t* q_lengths,
+                           const int64_t* s_lengths, void* out, float* lse, int dtype, int B, int64_t total_q,
+                           int64_t total_s, int H, int KV, int D, const int64_t* strides, float scale, int causal,
+                           void* workspace, size_t workspace_bytes, int device, void* stream);
+size_t v3d_cached_attention_workspace_bytes(int B, int tokens, int64_t capacity, int H, int KV, int D);
+int v3d_cached_attention(const void* q, const void* k_cache, const void* v_cache, const int64_t* lengths, void* out,
+                         int dtype, int B, int tokens, int64_t capacity, int H, int KV, int D, const int64_t* strides,
+                         float scale, void* workspace, size_t workspace_bytes, int device, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

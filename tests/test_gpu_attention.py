@@ -1,0 +1,337 @@
+"""ops.attention_pack_mode and ops.cached_attention against the definition in 64 bits: types, head sizes, grouped heads,
+ragged packs (empty sequences, sequences without keys, rows behind the last one), strides, masked infinities, refusals."""
+import pytest
+import torch
+
+from vision3d_amd import ops
+
+DEV = "cuda:0"
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def _half(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def _one(q, k, v, causal, scale):
+    """One sequence in 64 bits: (T,H,D), (S,KV,D) -> out, its bound sum_j p |v|, the largest error of a score."""
+    t, h, d = q.shape
+    s, kv, _ = k.shape
+    group = h // kv
+    out, size = torch.zeros_like(q), torch.zeros_like(q)
+    worst = torch.zeros(t, h, 1, dtype=torch.float64)
+    lse = torch.full((t, h), float("-inf"), dtype=torch.float64)
+    for i in range(h):
+        kk, vv = k[:, i // group], v[:, i // group]
+        for row in range(t):
+            n = min(s, max(0, row + s - t + 1)) if causal else s
+            if n == 0:
+                continue
+            logits = (kk[:n] @ q[row, i]) * scale
+            p = torch.softmax(logits, 0)
+            out[row, i] = p @ vv[:n]
+            size[row, i] = p @ vv[:n].abs()
+            lse[row, i] = torch.logsumexp(logits, 0)
+            worst[row, i] = (kk[:n].abs() @ q[row, i].abs()).max() * scale
+    return out, size, worst, lse
+
+
+def _tolerance(dtype, out, size, worst, d):
+    """The output's own rounding; the probabilities' rounding before they meet the values (16-bit types); a score is a sum
+    of d products in 32 bits, off by at most d + 4 half steps of sum |q| |k| (exp2's argument included), which moves its
+    probability and the sum of them by that much; 64 steps for the exponentials and the sums over keys."""
+    scores = (d + 4) * 2.0 ** -24 * worst
+    p = _half(dtype) if dtype != torch.float32 else 0.0
+    return _half(dtype) * out.abs() + size * (p + 2 * scores + 64 * 2.0 ** -24) + 2.0 ** -24
+
+
+def _pack(q_lengths, s_lengths, heads, kv, dim, dtype, seed=0, spare=0, spread=1.0):
+    gen = torch.Generator().manual_seed(seed)
+    mk = lambda n, h: (torch.randn((n, h, dim), generator=gen) * spread).to(dtype)
+    return (mk(sum(q_lengths) + spare, heads), mk(sum(s_lengths) + spare, kv), mk(sum(s_lengths) + spare, kv))
+
+
+def _expect(q, k, v, q_lengths, s_lengths, causal, scale):
+    outs, sizes, worsts, at, key = [], [], [], 0, 0
+    for a, b in zip(q_lengths, s_lengths):
+        o, s, w, _ = _one(q[at:at + a].double(), k[key:key + b].double(), v[key:key + b].double(), causal, scale)
+        outs.append(o), sizes.append(s), worsts.append(w)
+        at, key = at + a, key + b
+    return torch.cat(outs), torch.cat(sizes), torch.cat(worsts)
+
+
+def _check(dtype, q_lengths, s_lengths, heads, kv, dim, causal, seed=0, spare=0, scale=None, spread=1.0):
+    q, k, v = _pack(q_lengths, s_lengths, heads, kv, dim, dtype, seed, spare, spread)
+    out = ops.attention_pack_mode(q.to(DEV), k.to(DEV), v.to(DEV), torch.tensor(q_lengths).to(DEV),
+                                  torch.tensor(s_lengths).to(DEV), scale=scale, causal=causal).cpu()
+    n = sum(q_lengths)
+    want, size, worst = _expect(q, k, v, q_lengths, s_lengths, causal, dim ** -0.5 if scale is None else scale)
+    assert out.dtype == dtype and out.shape == q.shape
+    assert torch.equal(out[n:], torch.zeros_like(out[n:]))
+    off = (out[:n].double() - want).abs()
+    tol = _tolerance(dtype, want, size, worst, dim)
+    assert (off <= tol).all(), f"{(off / tol).max().item():.2f} of the tolerance"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dim", [8, 32, 33, 40, 64, 80, 96, 100, 128, 192, 200, 256])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_head_sizes(dtype, dim, causal):
+    _check(dtype, [70, 1, 0, 33, 5], [70, 1, 0, 33, 5], 2, 1, dim, causal, seed=dim)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("heads,kv", [(1, 1), (3, 3), (6, 3), (8, 1), (14, 2)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_grouped_heads_and_cross_lengths(dtype, heads, kv, causal):
+    # more keys than queries, fewer (the first queries see nothing), none, no queries, one of each
+    _check(dtype, [37, 90, 11, 0, 1, 129], [64, 31, 0, 40, 1, 65], heads, kv, 64, causal, seed=heads, spare=3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_tile_borders(dtype):
+    for n in (1, 31, 32, 33, 63, 64, 65, 127, 128, 129, 191, 257):
+        _check(dtype, [n], [n], 1, 1, 64, True, seed=n)
+        _check(dtype, [3], [n], 2, 1, 64, False, seed=n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_few_rows_many_keys(dtype):
+    # the keys are divided over workgroups and joined
+    _check(dtype, [1], [1500], 1, 1, 128, True)
+    _check(dtype, [1, 1, 2], [900, 3, 1300], 4, 2, 64, True)
+    _check(dtype, [40], [1100], 2, 2, 80, False)
+
+
+@pytest.mark.gpu
+def test_many_short_sequences():
+    gen = torch.Generator().manual_seed(3)
+    lengths = torch.randint(0, 9, (5000,), generator=gen).tolist()  # more sequences than a wave looks up at once
+    _check(torch.float32, lengths, lengths, 1, 1, 16, True)
+    lengths = torch.randint(0, 40, (130,), generator=gen).tolist()
+    _check(torch.bfloat16, lengths, lengths[::-1], 2, 1, 32, False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_large_scores_and_scale(dtype):
+    # scores of some hundreds: the sums live on the running maximum
+    _check(dtype, [70, 20], [140, 20], 2, 1, 64, True, scale=1.0, spread=3.0)
+    _check(dtype, [70, 20], [140, 20], 2, 1, 64, False, scale=1e-6)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_strides_and_alignment(dtype):
+    lengths = torch.tensor([50, 77], device=DEV)
+    for dim in (40, 64):
+        gen = torch.Generator().manual_seed(dim)
+        qkv = torch.randn((127, 8, dim + 3), generator=gen).to(dtype).to(DEV)
+        q, k, v = qkv[:, :4, 1:dim + 1], qkv[:, 4:6, 2:dim + 2], qkv[:, 6:, 3:]  # views at odd elements
+        got = ops.attention_pack_mode(q, k, v, lengths, causal=True)
+        assert torch.equal(got, ops.attention_pack_mode(q.contiguous(), k.contiguous(), v.contiguous(), lengths, causal=True))
+        flip = lambda t: t.transpose(0, 2).contiguous().transpose(0, 2)  # the last dimension is not contiguous
+        assert torch.equal(got, ops.attention_pack_mode(flip(q), flip(k), flip(v), lengths.cpu().int(), causal=True))
+        heads_first = lambda t: t.transpose(0, 1).contiguous().transpose(0, 1)
+        assert torch.equal(got, ops.attention_pack_mode(heads_first(q), heads_first(k), heads_first(v), lengths, causal=True))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_what_is_not_seen_does_not_reach(dtype, bad):
+    q, k, v = (t.to(DEV) for t in _pack([90, 40], [90, 40], 2, 1, 64, dtype))
+    lengths = torch.tensor([90, 40], device=DEV)
+    clean = ops.attention_pack_mode(q, k, v, lengths, causal=True)
+    k2, v2 = k.clone(), v.clone()
+    k2[70], v2[70] = bad, bad  # seen by queries 70 ... 89 of the first sequence only
+    got = ops.attention_pack_mode(q, k2, v2, lengths, causal=True)
+    assert torch.equal(got[:70], clean[:70]) and torch.equal(got[90:], clean[90:])
+    assert not torch.isfinite(got[70:90]).all(dim=2).any()
+    v2 = v.clone()
+    v2[70, 0, 5] = bad  # a value alone spoils its own column only
+    got = ops.attention_pack_mode(q, k, v2, lengths, causal=True)
+    assert torch.equal(got[:70], clean[:70]) and torch.equal(got[90:], clean[90:])
+    assert not torch.isfinite(got[70:90, :, 5]).any()
+    others = [c for c in range(64) if c != 5]
+    off = (got[70:90][:, :, others].double() - clean[70:90][:, :, others].double()).abs()
+    assert (off <= 4 * _half(dtype) * (1 + clean[70:90][:, :, others].double().abs())).all()
+    # a query's infinity or NaN stays with the query; without a mask the next sequence is still not reached
+    q2 = q.clone()
+    q2[11] = bad
+    got = ops.attention_pack_mode(q2, k, v, lengths, causal=True)
+    keep = [i for i in range(130) if i != 11]
+    assert torch.equal(got[keep], clean[keep])
+    v2 = v.clone()
+    v2[89] = bad
+    clean = ops.attention_pack_mode(q, k, v, lengths)
+    assert torch.equal(ops.attention_pack_mode(q, k, v2, lengths)[90:], clean[90:])
+
+
+@pytest.mark.gpu
+def test_lengths_that_do_not_fit():
+    q, k, v = (t.to(DEV) for t in _pack([60], [60], 1, 1, 32, torch.float32))
+    want = ops.attention_pack_mode(q, k, v, torch.tensor([20, 40], device=DEV))
+    got = ops.attention_pack_mode(q, k, v, torch.tensor([20, 4000, 7], device=DEV))  # cut at the total
+    assert torch.equal(got, want)
+    got = ops.attention_pack_mode(q, k, v, torch.tensor([-5, 20, 40, -(1 << 62)], device=DEV))
+    assert torch.equal(got, want)
+    got = ops.attention_pack_mode(q, k, v, torch.tensor([20, 1 << 62, 1 << 62], device=DEV))
+    assert torch.equal(got, want)
+    none = torch.zeros(0, dtype=torch.long, device=DEV)
+    assert torch.equal(ops.attention_pack_mode(q, k, v, none), torch.zeros_like(q))
+    assert ops.attention_pack_mode(q[:0], k, v, torch.tensor([0], device=DEV), torch.tensor([60], device=DEV)).shape == (0, 1, 32)
+    got = ops.attention_pack_mode(q, k[:0], v[:0], torch.tensor([60], device=DEV), torch.tensor([0], device=DEV))
+    assert torch.equal(got, torch.zeros_like(q))
+
+
+def _check_cache(dtype, lengths, tokens, capacity, heads, kv, dim, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    b = len(lengths)
+    q = torch.randn((b, tokens, heads, dim), generator=gen).to(dtype)
+    k = torch.randn((b, capacity, kv, dim), generator=gen).to(dtype)
+    v = torch.randn((b, capacity, kv, dim), generator=gen).to(dtype)
+    for i, n in enumerate(lengths):  # rows past a length may hold anything
+        k[i, max(n, 0):], v[i, max(n, 0):] = float("nan"), float("inf")
+    got = ops.cached_attention(q.to(DEV), k.to(DEV), v.to(DEV), torch.tensor(lengths).to(DEV)).cpu()
+    for i, n in enumerate(lengths):
+        n = min(max(n, 0), capacity)
+        want, size, worst, _ = _one(q[i].double(), k[i, :n].double(), v[i, :n].double(), True, dim ** -0.5)
+        off = (got[i].double() - want).abs()
+        tol = _tolerance(dtype, want, size, worst, dim)
+        assert (off <= tol).all(), f"{(off / tol).max().item():.2f} of the tolerance"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv,dim", [(1, 1, 64), (8, 2, 128), (6, 3, 80), (40, 1, 33), (4, 4, 256), (2, 1, 32), (4, 2, 192)])
+def test_cache(dtype, heads, kv, dim):
+    _check_cache(dtype, [300, 1, 0, 129, 77, 512], 1, 512, heads, kv, dim, seed=dim)
+    _check_cache(dtype, [70, 3, 600], 5, 600, heads, kv, dim, seed=dim + 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_cache_lengths(dtype):
+    _check_cache(dtype, [2500, 2499, 2049, 64], 1, 2500, 4, 1, 128)
+    _check_cache(dtype, [9], 3, 9, 2, 2, 64)
+    _check_cache(dtype, [2], 7, 40, 2, 1, 64)     # more new tokens than rows: the first see nothing
+    _check_cache(dtype, [-3, 50], 1, 40, 2, 1, 64)  # cut to [0, capacity]
+    _check_cache(dtype, [31 * (i % 5) + i for i in range(70)], 1, 200, 2, 1, 64)
+
+
+@pytest.mark.gpu
+def test_cache_equals_the_packs_last_rows():
+    lengths = [140, 33, 260]
+    q, k, v = (t.to(DEV) for t in _pack(lengths, lengths, 8, 2, 128, torch.bfloat16))
+    whole = ops.attention_pack_mode(q, k, v, torch.tensor(lengths, device=DEV), causal=True)
+    cap = 300
+    kc, vc = (torch.full((3, cap, 2, 128), float("nan"), dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    at = 0
+    for i, n in enumerate(lengths):
+        kc[i, :n], vc[i, :n] = k[at:at + n], v[at:at + n]
+        at += n
+    ends = torch.tensor(lengths).cumsum(0) - 1
+    last = ops.cached_attention(q[ends.to(DEV)].unsqueeze(1), kc, vc, torch.tensor(lengths, device=DEV))
+    off = (last[:, 0].double() - whole[ends.to(DEV)].double()).abs()
+    # two sums of the same products in another order: each is within its rounding of the exact value
+    assert off.max() <= 4 * _half(torch.bfloat16) * 2
+
+
+@pytest.mark.gpu
+def test_other_stream_and_graph_replays():
+    from vision3d_amd import ext
+
+    lengths = torch.tensor([1, 1, 1], device=DEV)
+    keys = torch.tensor([700, 0, 1800], device=DEV)
+    q, k, v = (t.to(DEV) for t in _pack([3], [2500], 4, 2, 64, torch.float16))
+    want = ops.attention_pack_mode(q, k, v, lengths, keys)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = ops.attention_pack_mode(q, k, v, lengths, keys)
+    side.synchronize()
+    assert torch.equal(got, want)
+    out, cached = torch.empty_like(q), torch.empty_like(q).view(3, 1, 4, 64)
+    cache_k, cache_v = k.view(-1)[:3 * 800 * 128].view(3, 800, 2, 64), v.view(-1)[:3 * 800 * 128].view(3, 800, 2, 64)
+
+    def step():
+        ext.attention_pack_forward(q, k, v, lengths, keys, out, None, 0.125, False)
+        ext.cached_attention(q.view(3, 1, 4, 64), cache_k, cache_v, keys, cached, 0.125)
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for n in range(4):
+        q.mul_(1.25)
+        keys[0] -= 100  # the lengths are device data: a replay follows them
+        step()
+        torch.cuda.synchronize()
+        eager = [out.clone(), cached.clone()]
+        out.fill_(float("nan")), cached.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager[0]) and torch.equal(cached, eager[1]), n
+
+
+@pytest.mark.gpu
+def test_refusals():
+    q, k, v = (t.to(DEV) for t in _pack([10], [10], 4, 2, 16, torch.float32))
+    n = torch.tensor([10], device=DEV)
+    with pytest.raises(RuntimeError, match="multiple of the key heads"):
+        ops.attention_pack_mode(q[:, :3], k, v, n)
+    with pytest.raises(RuntimeError, match="expected scalar type"):
+        ops.attention_pack_mode(q, k.half(), v.half(), n)
+    with pytest.raises(RuntimeError, match="not implemented for 'Double'"):
+        ops.attention_pack_mode(q.double(), k.double(), v.double(), n)
+    with pytest.raises(RuntimeError, match="expected q_feats"):
+        ops.attention_pack_mode(q, k, v[:5], n)
+    with pytest.raises(RuntimeError, match="expected q_feats"):
+        ops.attention_pack_mode(q[:, :, :8], k, v, n)
+    with pytest.raises(RuntimeError, match="s_lengths must have shape"):
+        ops.attention_pack_mode(q, k, v, n, torch.tensor([5, 5], device=DEV))
+    with pytest.raises(RuntimeError, match="must have 3 dimensions"):
+        ops.attention_pack_mode(q[0], k, v, n)
+    for scale in (0.0, -1.0, float("inf"), float("nan")):
+        with pytest.raises(RuntimeError, match="scale must be positive"):
+            ops.attention_pack_mode(q, k, v, n, scale=scale)
+    with pytest.raises(RuntimeError, match="head size 257"):
+        big = torch.zeros((4, 1, 257), device=DEV)
+        ops.attention_pack_mode(big, big, big, torch.tensor([4], device=DEV))
+    with pytest.raises(RuntimeError, match="no gradient"):
+        ops.cached_attention(q.view(1, 10, 4, 16).requires_grad_(True), k.view(1, 10, 2, 16), v.view(1, 10, 2, 16), n)
+    q = q.detach()
+    with pytest.raises(RuntimeError, match="expected q_feats"):
+        ops.cached_attention(q.view(2, 5, 4, 16), k.view(1, 10, 2, 16), v.view(1, 10, 2, 16), torch.tensor([5, 5], device=DEV))
+    with pytest.raises(RuntimeError, match="lengths must have shape"):
+        ops.cached_attention(q.view(1, 10, 4, 16), k.view(1, 10, 2, 16), v.view(1, 10, 2, 16), torch.tensor([5, 5], device=DEV))
+
+
+def test_refusals_without_a_gpu():
+    from vision3d_amd import _lib
+
+    t = torch.zeros(4, 2, 8)
+    with pytest.raises(RuntimeError, match="attention_pack_mode: CUDA tensors required"):
+        ops.attention_pack_mode(t, t, t, torch.tensor([4]))
+    with pytest.raises(RuntimeError, match="cached_attention: CUDA tensors required"):
+        ops.cached_attention(t[None], t[None], t[None], torch.tensor([4]))
+    lib = _lib.lib()
+    none = [None] * 7
+
+    def pack(dtype=1, b=1, nq=4, ns=4, h=2, kv=1, d=8, scale=1.0):
+        return lib.v3d_attention_pack_fwd(*none, dtype, b, nq, ns, h, kv, d, None, scale, 0, None, 0, 0, None)
+
+    assert pack(dtype=5) == -1 and pack(h=3, kv=2) == -1 and pack(d=0) == -1 and pack(b=-1) == -1
+    assert pack(scale=0.0) == -1 and pack(scale=float("nan")) == -1 and pack() == -1  # null pointers
+    assert pack(d=257) == -4 and pack(nq=1 << 30) == -4 and pack(ns=(1 << 30) + 1) == -4
+    assert pack(nq=0) == 0
+    # the workspace is asked for only where the keys are divided
+    assert lib.v3d_attention_pack_workspace_bytes(4, 100000, 100000, 8, 8, 64) == 0
+    assert lib.v3d_attention_pack_workspace_bytes(1, 1, 100000, 8, 8, 64) > 0
+    assert lib.v3d_cached_attention_workspace_bytes(1, 1, 64, 8, 8, 64) == 0
+    assert lib.v3d_cached_attention_workspace_bytes(1, 1, 100000, 8, 8, 64) > 0

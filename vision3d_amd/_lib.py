@@ -121,6 +121,17 @@ SIGNATURES = {
     "v3d_rows_csr_build": (_c_int, [_c_ptr, _c_i64, _c_i64] + _WS + _TAIL),
     "v3d_rows_scatter_f32": (
         _c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_i64, _c_i64, _c_int, _c_int, _c_int] + _TAIL),
+    "v3d_layer_norm_fwd": (_c_int, [_c_ptr] * 7 + [_c_int, _c_int, _c_i64, _c_i64, _c_f32] + _TAIL),
+    "v3d_layer_norm_bwd_workspace_bytes": (_c_size, [_c_i64, _c_i64]),
+    "v3d_attention_pack_workspace_bytes": (_c_size, [_c_int, _c_i64, _c_i64, _c_int, _c_int, _c_int]),
+    "v3d_attention_pack_fwd": (
+        _c_int, [_c_ptr] * 7 + [_c_int, _c_int, _c_i64, _c_i64, _c_int, _c_int, _c_int, ctypes.POINTER(_c_i64), _c_f32,
+                                _c_int] + _WS + _TAIL),
+    "v3d_cached_attention_workspace_bytes": (_c_size, [_c_int, _c_int, _c_i64, _c_int, _c_int, _c_int]),
+    "v3d_cached_attention": (
+        _c_int, [_c_ptr] * 5 + [_c_int, _c_int, _c_int, _c_i64, _c_int, _c_int, _c_int, ctypes.POINTER(_c_i64), _c_f32]
+        + _WS + _TAIL),
+    "v3d_layer_norm_bwd": (_c_int, [_c_ptr] * 9 + [_c_int, _c_int, _c_i64, _c_i64] + _WS + _TAIL),
 }
 
 _lib = None

@@ -1,0 +1,446 @@
+// attention.hip -- softmax attention inside the sequences of a pack, and of new tokens against cached keys and values.
+//
+//   s_ij = scale * q_i . k_j over the keys that query i sees,  o_i = sum_j exp(s_ij - m_i) v_j / sum_j exp(s_ij - m_i)
+//
+// Rows: the G = H / KV query heads of a key head are folded into the rows of that head's products (row = token * G + head),
+// so grouped heads read every key once per tile whatever G is, and a single token of 8 heads fills 8 columns of a product
+// instead of one.
+#include <algorithm>
+
+#include "attn.h"
+
+namespace v3d {
+
+constexpr int kAttnWaves = 4;
+constexpr int kAttnRows = 32 * kAttnWaves;  // rows of a workgroup's tile
+
+__host__ __device__ constexpr int attn_pow2(int hd) { return hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
+template <typename T, int HD>
+constexpr int attn_keys() { return HD * (int)sizeof(T) > 512 ? 32 : 64; }  // keys of a tile: at most 64 KiB of LDS
+
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void attn_forward_kernel(const AttnArgs a) {
+  constexpr int HDP = attn_pow2(HD);
+  constexpr int BN = attn_keys<T, HD>();
+  constexpr int NT = BN / 32;                       // 32-key blocks of a tile
+  constexpr int E = 16 / (int)sizeof(T);
+  constexpr int STEPS = HD / Mma<T>::kStep;         // product steps over the head size
+  constexpr int USTEPS = 32 / Mma<T>::kStep;        // product steps over a 32-key block
+  constexpr int DT = HD / 32;
+  constexpr Place kV = sizeof(T) == 2 ? kTranspose : kScalar;
+  typedef typename Mma<T>::Op Op;
+  __shared__ T lds_k[BN * HDP];
+  __shared__ T lds_v[BN * HDP];
+  __shared__ int lds_bad;
+
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int half = lane >> 5;
+  int64_t id = blockIdx.x;
+  const int kvh = (int)(id % a.KV);
+  id /= a.KV;
+  const int split = (int)(id % a.splits);
+  id /= a.splits;
+  const AttnSeq seq = locate_rows<kAttnRows>(a, id);
+  if (!seq.found) {  // the launch covers a bound: the rest of it clears the rows behind the last sequence
+    if (a.capacity == 0 && split == 0) {
+      const int64_t rows = (a.total_q - seq.q_end) * a.G;
+      for (int i = threadIdx.x; i < kAttnRows; i += 256) {
+        const int64_t r = seq.spare * kAttnRows + i;
+        if (r >= rows) break;
+        const int64_t at = (seq.q_end + r / a.G) * a.H + (int64_t)kvh * a.G + r % a.G;
+        for (int d = 0; d < a.D; ++d) static_cast<T*>(a.out)[at * a.D + d] = (T)0.f;
+        if (a.lse) a.lse[at] = -__builtin_inff();
+      }
+    }
+    return;
+  }
+  const int rows = seq.q_len * a.G;
+  if (seq.tile * kAttnRows >= rows) return;  // lengths that overrun the total were cut
+  const int row = seq.tile * kAttnRows + wave * 32 + (lane & 31);
+  const int token = min(row, rows - 1) / a.G;
+  const int head = kvh * a.G + min(row, rows - 1) % a.G;
+  auto limit_of = [&](int tok) {
+    return a.causal ? max(0, min(seq.s_len, tok + seq.s_len - seq.q_len + 1)) : seq.s_len;
+  };
+  const int limit = limit_of(token);  // this lane's query sees keys [0, limit)
+  // the wave's and the workgroup's first and last rows bound what they have to look at
+  const int wave_first = min(seq.tile * kAttnRows + wave * 32, rows - 1);
+  const int wave_last = min(seq.tile * kAttnRows + wave * 32 + 31, rows - 1);
+  const bool wave_live = seq.tile * kAttnRows + wave * 32 < rows;
+  const int wave_least = limit_of(wave_first / a.G), wave_most = wave_live ? limit_of(wave_last / a.G) : 0;
+  const int most = limit_of(min(seq.tile * kAttnRows + kAttnRows - 1, rows - 1) / a.G);
+  const int least = limit_of(min(seq.tile * kAttnRows, rows - 1) / a.G);
+
+  const int tiles = (most + BN - 1) / BN;
+  const int per_split = (tiles + a.splits - 1) / a.splits;
+  const int t_begin = split * per_split, t_end = min(tiles, t_begin + per_split);
+
+  const T* q = static_cast<const T*>(a.q) + (seq.q_off + token) * a.q_row + (int64_t)head * a.q_head;
+  const T* k = static_cast<const T*>(a.k) + seq.b * a.k_batch + seq.s_off * a.k_row + (int64_t)kvh * a.k_head;
+  const T* v = static_cast<const T*>(a.v) + seq.b * a.v_batch + seq.s_off * a.v_row + (int64_t)kvh * a.v_head;
+
+  Op qf[STEPS];
+#pragma unroll
+  for (int st = 0; st < STEPS; ++st) {
+    const Chunk<T> c = load_chunk<T>(q, st * 2 * E + E * half, a.D, true);
+#pragma unroll
+    for (int j = 0; j < E; ++j) qf[st][j] = c.v[j];
+  }
+
+  const float c2 = a.scale * kLog2e;
+  float m = -__builtin_inff(), l = 0.f;
+  f32x16 o[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d) o[d] = zero16();
+
+  for (int t = t_begin; t < t_end; ++t) {
+    const int key0 = t * BN;
+    __syncthreads();
+    if (threadIdx.x == 0) lds_bad = 0;
+    __syncthreads();
+    bool bad = false;
+    constexpr int CPR = HD / E;
+    for (int i = threadIdx.x; i < BN * CPR; i += 256) {
+      const int r = i / CPR, c = i % CPR;
+      const bool live = key0 + r < seq.s_len;
+      const Chunk<T> kc = load_chunk<T>(k + (int64_t)(key0 + r) * a.k_row, c * E, a.D, live);
+      const Chunk<T> vc = load_chunk<T>(v + (int64_t)(key0 + r) * a.v_row, c * E, a.D, live);
+      *reinterpret_cast<Chunk<T>*>(lds_k + tile_at<T, HDP, kOperand>(r, c * E)) = kc;
+      *reinterpret_cast<Chunk<T>*>(lds_v + tile_at<T, HDP, kV>(r, c * E)) = vc;
+      bad |= chunk_nonfinite(vc);
+    }
+    if (key0 + BN > least && bad) lds_bad = 1;
+    __syncthreads();
+    if (key0 >= wave_most) continue;
+
+    f32x16 s[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      s[n] = zero16();
+#pragma unroll
+      for (int st = 0; st < STEPS; ++st)
+        s[n] = Mma<T>::run(read_cols<T, HDP>(lds_k, n * 32 + (lane & 31), st, half), qf[st], s[n]);
+    }
+    const bool masked = key0 + BN > wave_least;
+    if (masked) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (key0 + n * 32 + acc_row(r, half) >= limit) s[n][r] = -__builtin_inff();
+    }
+    // running maximum: of the lane, then with the lane that holds the other keys of this query
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[n][r]);
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    const float m_new = fmaxf(m, top);
+    const float base = m_new == -__builtin_inff() ? 0.f : m_new * c2;
+    const float alpha = exp2_fast(m * c2 - base);
+    m = m_new;
+    float sum = 0.f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[n][r] = exp2_fast(fmaf(s[n][r], c2, -base));
+        sum += s[n][r];
+      }
+    l = l * alpha + sum;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+
+    // An infinity or NaN among the values of a tile that some query sees in part must not reach the queries that do not
+    // see it (0 * inf): the product takes the finite values, then the others are added key by key where they are seen.
+    const bool apart = masked && lds_bad;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int u = 0; u < USTEPS; ++u) {
+        const Op p = pack_rows<T>(s[n], u);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          Op w = read_rows<T, HDP>(lds_v, n * 32, u, d * 32, lane);
+          if (apart) w = keep_finite<T>(w, true);
+          o[d] = Mma<T>::run(w, p, o[d]);
+        }
+      }
+    if (apart) {
+#pragma unroll 1
+      for (int key = 0; key < BN; ++key) {
+        const bool seen = key0 + key < limit;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          f32x16 one = zero16();
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int u = 0; u < USTEPS; ++u) {
+              Op p = pack_rows<T>(s[n], u);
+              Op w = keep_finite<T>(read_rows<T, HDP>(lds_v, n * 32, u, d * 32, lane), false);
+              constexpr int R = sizeof(T) == 2 ? 8 : 4;
+#pragma unroll
+              for (int j = 0; j < R; ++j) {
+                const bool mine = n * 32 + acc_row(u * R + j, half) == key;
+                p[j] = mine ? p[j] : (T)0.f;
+                w[j] = mine ? w[j] : (T)0.f;
+              }
+              one = Mma<T>::run(w, p, one);
+            }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[d][r] = seen ? o[d][r] + one[r] : o[d][r];
+        }
+      }
+    }
+  }
+
+  l += __shfl_xor(l, 32, 64);
+  if (row >= rows) return;
+  if (a.splits == 1) {
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // a NaN sum stays a NaN
+    T* out = static_cast<T*>(a.out) + ((seq.q_off + token) * a.H + head) * a.D;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int col = d * 32 + 8 * g + 4 * half;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (col + j < a.D) out[col + j] = from_f32<T>(o[d][g * 4 + j] * inv);
+      }
+    if (a.lse && half == 0)
+      a.lse[(seq.q_off + token) * a.H + head] = l == 0.f ? -__builtin_inff() : m * a.scale + logf(l);
+    return;
+  }
+  const int64_t part = (((int64_t)id * a.KV + kvh) * a.splits + split) * kAttnRows + wave * 32 + (lane & 31);
+  float* po = a.part_o + part * a.D;
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int col = d * 32 + 8 * g + 4 * half;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (col + j < a.D) po[col + j] = o[d][g * 4 + j];
+    }
+  if (half == 0) {
+    a.part_ml[part * 2] = m;
+    a.part_ml[part * 2 + 1] = l;
+  }
+}
+
+// Joins the parts of a row tile's keys: one wave per row, lanes over the columns.
+template <typename T, int TILE>
+__global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int GROUPS = TILE / 4;  // workgroups of 4 rows per tile
+  int64_t id = blockIdx.x;
+  const int at = (int)(id % GROUPS) * 4 + wave;
+  id /= GROUPS;
+  const int kvh = (int)(id % a.KV);
+  id /= a.KV;
+  const AttnSeq seq = locate_rows<TILE>(a, id);
+  if (!seq.found) return;
+  const int row = seq.tile * TILE + at;
+  if (row >= seq.q_len * a.G) return;
+  const int64_t part = (((int64_t)id * a.KV + kvh) * a.splits) * TILE + at;
+  const float c2 = a.scale * kLog2e;
+  float m = -__builtin_inff();
+  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[(part + (int64_t)s * TILE) * 2]);
+  const float base = m == -__builtin_inff() ? 0.f : m * c2;
+  float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < a.splits; ++s) {
+    const int64_t p = part + (int64_t)s * TILE;
+    const float f = exp2_fast(fmaf(a.part_ml[p * 2], c2, -base));
+    l = fmaf(a.part_ml[p * 2 + 1], f, l);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (lane + 64 * j < a.D) o[j] = fmaf(a.part_o[p * a.D + lane + 64 * j], f, o[j]);
+  }
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  const int64_t out = (seq.q_off + row / a.G) * a.H + (int64_t)kvh * a.G + row % a.G;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (lane + 64 * j < a.D) static_cast<T*>(a.out)[out * a.D + lane + 64 * j] = from_f32<T>(o[j] * inv);
+  if (a.lse && lane == 0) a.lse[out] = l == 0.f ? -__builtin_inff() : m * a.scale + logf(l);
+}
+
+// ---- launches ----------------------------------------------------------------------------------------------------------
+struct AttnPlan {
+  int64_t tiles;    // row tiles (a bound in a pack)
+  int splits;
+  size_t bytes;     // workspace
+};
+
+inline AttnPlan attn_plan(int B, int64_t total_q, int64_t longest, int tokens, int KV, int G, int D) {
+  AttnPlan p;
+  p.tiles = tokens > 0 ? B * ceil_div((int64_t)tokens * G, kAttnRows) : ceil_div(total_q * G, kAttnRows) + B;
+  const int64_t groups = p.tiles * KV;
+  // keys are divided only where the row tiles leave compute units idle; a part has at least 4 key tiles of the bound
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(groups, 1), longest / 256));
+  p.splits = std::min(p.splits, 64);
+  p.bytes = p.splits > 1 ? (size_t)(groups * p.splits * kAttnRows) * (size_t)(D + 2) * sizeof(float) : 0;
+  return p;
+}
+
+template <typename T, int HD>
+int attn_forward_launch(const AttnArgs& a, int64_t tiles, hipStream_t stream, const char* what) {
+  hipLaunchKernelGGL((attn_forward_kernel<T, HD>), dim3((unsigned)(tiles * a.KV * a.splits)), dim3(256), 0, stream, a);
+  int rc = launch_status(what);
+  if (rc == 0 && a.splits > 1) {
+    hipLaunchKernelGGL((attn_join_kernel<T, kAttnRows>), dim3((unsigned)(tiles * a.KV * (kAttnRows / 4))), dim3(256), 0,
+                       stream, a);
+    rc = launch_status(what);
+  }
+  return rc;
+}
+
+template <typename T>
+int attn_forward_type(const AttnArgs& a, int64_t tiles, hipStream_t stream, const char* what) {
+  switch (attn_head_size(a.D)) {
+    case 32: return attn_forward_launch<T, 32>(a, tiles, stream, what);
+    case 64: return attn_forward_launch<T, 64>(a, tiles, stream, what);
+    case 96: return attn_forward_launch<T, 96>(a, tiles, stream, what);
+    case 128: return attn_forward_launch<T, 128>(a, tiles, stream, what);
+    case 192: return attn_forward_launch<T, 192>(a, tiles, stream, what);
+    default: return attn_forward_launch<T, 256>(a, tiles, stream, what);
+  }
+}
+
+int attn_check(const char* what, int dtype, int B, int64_t total_q, int64_t total_s, int H, int KV, int D,
+               float scale) {
+  V3D_REQUIRE(dtype == V3D_F32 || dtype == V3D_F16 || dtype == V3D_BF16, what, "unknown element type");
+  V3D_REQUIRE(B >= 0 && total_q >= 0 && total_s >= 0 && H >= 1 && KV >= 1 && D >= 1, what, "bad shape");
+  V3D_REQUIRE(H % KV == 0, what, "the query heads must be a multiple of the key heads");
+  V3D_REQUIRE(scale > 0.f && scale < __builtin_inff(), what, "the scale must be positive and finite");
+  if (D > V3D_ATTENTION_MAX_HEAD_SIZE) {
+    set_last_error("%s: head size %d, at most %d", what, D, V3D_ATTENTION_MAX_HEAD_SIZE);
+    return V3D_ERR_SIZE_LIMIT;
+  }
+  const int64_t most = (int64_t)1 << 30;
+  if (total_q > most / H || total_s > most || B > (1 << 24)) {
+    set_last_error("%s: more than 2^30 rows (query rows count once per head)", what);
+    return V3D_ERR_SIZE_LIMIT;
+  }
+  return 0;
+}
+
+int attn_forward_run(AttnArgs& a, int dtype, const AttnPlan& plan, void* workspace, size_t workspace_bytes, int device,
+                     void* stream, const char* what) {
+  if (plan.tiles * a.KV * plan.splits > ((int64_t)1 << 31) / 64) {
+    set_last_error("%s: too many tiles", what);
+    return V3D_ERR_SIZE_LIMIT;
+  }
+  DeviceGuard guard(device);
+  if (guard.rc != 0) return guard.rc;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  a.splits = plan.splits;
+  Scratch ws;
+  if (plan.bytes > 0) {
+    const int rc = ws.acquire(what, workspace, workspace_bytes, plan.bytes, s);
+    if (rc != 0) return rc;
+    a.part_o = reinterpret_cast<float*>(ws.base);
+    a.part_ml = a.part_o + plan.tiles * a.KV * a.splits * kAttnRows * a.D;
+  }
+  int rc = dtype == V3D_F32   ? attn_forward_type<float>(a, plan.tiles, s, what)
+           : dtype == V3D_F16 ? attn_forward_type<f16>(a, plan.tiles, s, what)
+                              : attn_forward_type<bf16>(a, plan.tiles, s, what);
+  return ws.release(what, rc);
+}
+
+}  // namespace v3d
+
+extern "C" {
+
+size_t v3d_attention_pack_workspace_bytes(int B, int64_t total_q, int64_t total_s, int H, int KV, int D) {
+  if (B <= 0 || total_q <= 0 || H <= 0 || KV <= 0 || H % KV != 0 || D <= 0) return 0;
+  return v3d::attn_plan(B, total_q, total_s, 0, KV, H / KV, D).bytes;
+}
+
+int v3d_attention_pack_fwd(const void* q, const void* k, const void* v, const int64_t* q_lengths,
+                           const int64_t* s_lengths, void* out, float* lse, int dtype, int B, int64_t total_q,
+                           int64_t total_s, int H, int KV, int D, const int64_t* strides, float scale, int causal,
+                           void* workspace, size_t workspace_bytes, int device, void* stream) {
+  using namespace v3d;
+  const char* what = "attention_pack";
+  int rc = attn_check(what, dtype, B, total_q, total_s, H, KV, D, scale);
+  if (rc != 0) return rc;
+  if (total_q == 0) return 0;
+  V3D_REQUIRE(q && out && strides && (B == 0 || (q_lengths && s_lengths)) && (total_s == 0 || (k && v)), what,
+              "null pointer");
+  AttnArgs a{};
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.out = out;
+  a.lse = lse;
+  a.q_lengths = q_lengths;
+  a.s_lengths = s_lengths;
+  a.total_q = total_q;
+  a.total_s = total_s;
+  a.q_row = strides[0];
+  a.q_head = strides[1];
+  a.k_row = strides[2];
+  a.k_head = strides[3];
+  a.v_row = strides[4];
+  a.v_head = strides[5];
+  a.B = B;
+  a.H = H;
+  a.KV = KV;
+  a.G = H / KV;
+  a.D = D;
+  a.scale = scale;
+  a.causal = causal;
+  return attn_forward_run(a, dtype, attn_plan(B, total_q, total_s, 0, KV, a.G, D), workspace, workspace_bytes, device,
+                          stream, what);
+}
+
+size_t v3d_cached_attention_workspace_bytes(int B, int tokens, int64_t capacity, int H, int KV, int D) {
+  if (B <= 0 || tokens <= 0 || H <= 0 || KV <= 0 || H % KV != 0 || D <= 0) return 0;
+  return v3d::attn_plan(B, (int64_t)B * tokens, capacity, tokens, KV, H / KV, D).bytes;
+}
+
+int v3d_cached_attention(const void* q, const void* k_cache, const void* v_cache, const int64_t* lengths, void* out,
+                         int dtype, int B, int tokens, int64_t capacity, int H, int KV, int D, const int64_t* strides,
+                         float scale, void* workspace, size_t workspace_bytes, int device, void* stream) {
+  using namespace v3d;
+  const char* what = "cached_attention";
+  V3D_REQUIRE(B >= 0 && tokens >= 0 && capacity >= 1, what, "bad shape");
+  int rc = attn_check(what, dtype, B, (int64_t)B * tokens, capacity, H, KV, D, scale);
+  if (rc != 0) return rc;
+  if (B == 0 || tokens == 0) return 0;
+  V3D_REQUIRE(q && k_cache && v_cache && lengths && out && strides, what, "null pointer");
+  AttnArgs a{};
+  a.q = q;
+  a.k = k_cache;
+  a.v = v_cache;
+  a.out = out;
+  a.s_lengths = lengths;
+  a.total_q = (int64_t)B * tokens;
+  a.total_s = capacity;
+  a.q_row = strides[0];
+  a.q_head = strides[1];
+  a.k_batch = strides[2];
+  a.k_row = strides[3];
+  a.k_head = strides[4];
+  a.v_batch = strides[5];
+  a.v_row = strides[6];
+  a.v_head = strides[7];
+  a.capacity = capacity;
+  a.tokens = tokens;
+  a.B = B;
+  a.H = H;
+  a.KV = KV;
+  a.G = H / KV;
+  a.D = D;
+  a.scale = scale;
+  a.causal = 1;
+  return attn_forward_run(a, dtype, attn_plan(B, a.total_q, capacity, tokens, KV, a.G, D), workspace, workspace_bytes,
+                          device, stream, what);
+}
+
+}  // extern "C"

@@ -1,0 +1,339 @@
+// attn.h -- what the attention kernels share: arguments, the way from a workgroup to its sequence, tiles in LDS and the
+// matrix instructions' operands.
+#ifndef V3D_CSRC_ATTN_H_
+#define V3D_CSRC_ATTN_H_
+
+#include "common.h"
+#include "numeric.h"
+
+namespace v3d {
+
+typedef float f32x4v __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// Element strides throughout.  Rows of the keys: row j of sequence b is at (first row of b + j) * row stride in a pack,
+// at b * batch stride + j * row stride in a cache (`capacity` > 0).
+struct AttnArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;                 // (total_q, H, D) contiguous
+  float* lse;                // (total_q, H) natural log of the sum of exponentials, -inf for a row without keys; or NULL
+  const int64_t* q_lengths;  // (B), NULL in a cache: every sequence has `tokens` queries
+  const int64_t* s_lengths;  // (B)
+  int64_t total_q, total_s;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head, k_batch, v_batch;
+  int64_t capacity;
+  int tokens;
+  int B, H, KV, G, D;        // G = H / KV query heads share a key head
+  float scale;
+  int causal;
+  int splits;                // parts that the keys of a row tile are divided into
+  float* part_o;             // splits > 1: (tile, KV, split, rows of a tile, D) unnormalised rows ...
+  float* part_ml;            // ... and (tile, KV, split, rows of a tile, 2): maximum (of the unscaled scores) and sum
+};
+
+// A workgroup's sequence.  All fields are wave-uniform.
+struct AttnSeq {
+  int b = 0;
+  int tile = 0;              // row tile (or key tile) inside the sequence
+  bool found = false;
+  int64_t q_off = 0, s_off = 0;
+  int q_len = 0, s_len = 0;
+  int64_t spare = 0;         // !found: how many tiles past the last one
+  int64_t q_end = 0, s_end = 0;  // !found: rows that belong to a sequence
+};
+
+__device__ __forceinline__ int64_t uniform64(int64_t v) {
+  const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)v), hi = __builtin_amdgcn_readfirstlane((unsigned)(v >> 32));
+  return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ int64_t clamp64(int64_t v, int64_t hi) { return v < 0 ? 0 : (v < hi ? v : hi); }
+
+__device__ __forceinline__ int64_t lanes_prefix(int64_t v, int lane) {  // inclusive
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t o = __shfl_up(v, d, 64);
+    if (lane >= d) v += o;
+  }
+  return v;
+}
+
+// Tile `t` of the pack: sequence b has ceil(rows_b / TILE) tiles, rows_b = q_len * G (BY_KEYS: s_len).  The lengths are
+// device data, so the launch covers the bound total / TILE + B and the kernels look their sequence up here: every wave
+// by itself, one lane per sequence (per ceil(B / 64) sequences), no LDS and no barrier.  Negative lengths count as 0;
+// lengths that overrun the totals are cut, so that no row outside the buffers is ever addressed.
+template <int TILE, bool BY_KEYS>
+__device__ __forceinline__ AttnSeq locate(const AttnArgs& a, int64_t t) {
+  const int lane = threadIdx.x & 63;
+  AttnSeq r;
+  const int per = (a.B + 63) >> 6;
+  auto tiles = [&](int64_t q, int64_t s) -> int64_t { return ((BY_KEYS ? s : q * a.G) + TILE - 1) / TILE; };
+  auto len_q = [&](int i) { return clamp64(a.q_lengths[i], a.total_q); };
+  auto len_s = [&](int i) { return clamp64(a.s_lengths[i], a.total_s); };
+  int64_t sq = 0, ss = 0, st = 0;
+  for (int e = 0; e < per; ++e) {
+    const int i = lane * per + e;
+    if (i < a.B) {
+      const int64_t q = len_q(i), s = len_s(i);
+      sq += q;
+      ss += s;
+      st += tiles(q, s);
+    }
+  }
+  int64_t iq = lanes_prefix(sq, lane), is = lanes_prefix(ss, lane), it = lanes_prefix(st, lane);
+  const int64_t all = __shfl(it, 63, 64);
+  if (t >= all) {
+    r.spare = uniform64(t - all);
+    r.q_end = uniform64(clamp64(__shfl(iq, 63, 64), a.total_q));
+    r.s_end = uniform64(clamp64(__shfl(is, 63, 64), a.total_s));
+    return r;
+  }
+  const int src = __builtin_ctzll(__ballot(it > t));  // the first lane whose tiles reach past t
+  int64_t q0 = __shfl(iq - sq, src, 64), s0 = __shfl(is - ss, src, 64), t0 = __shfl(it - st, src, 64);
+  int b = src;
+  int64_t q = __shfl(sq, src, 64), s = __shfl(ss, src, 64);
+  if (per > 1) {
+    for (int e0 = 0;; e0 += 64) {  // ends: the lane's tiles reach past t
+      const int i = src * per + e0 + lane;
+      const bool in = e0 + lane < per && i < a.B;
+      const int64_t lq = in ? len_q(i) : 0, ls = in ? len_s(i) : 0, lt = in ? tiles(lq, ls) : 0;
+      const int64_t pq = lanes_prefix(lq, lane), ps = lanes_prefix(ls, lane), pt = lanes_prefix(lt, lane);
+      const uint64_t hit = __ballot(t0 + pt > t);
+      if (hit != 0) {
+        const int at = __builtin_ctzll(hit);
+        b = src * per + e0 + at;
+        q = __shfl(lq, at, 64);
+        s = __shfl(ls, at, 64);
+        q0 += __shfl(pq - lq, at, 64);
+        s0 += __shfl(ps - ls, at, 64);
+        t0 += __shfl(pt - lt, at, 64);
+        break;
+      }
+      if (e0 + 64 >= per) return r;  // not reached
+      q0 += __shfl(pq, 63, 64);
+      s0 += __shfl(ps, 63, 64);
+      t0 += __shfl(pt, 63, 64);
+    }
+  }
+  q0 = clamp64(q0, a.total_q);
+  s0 = clamp64(s0, a.total_s);
+  r.found = true;
+  r.b = __builtin_amdgcn_readfirstlane(b);
+  r.tile = (int)uniform64(t - t0);
+  r.q_off = uniform64(q0);
+  r.s_off = uniform64(s0);
+  r.q_len = (int)uniform64(clamp64(q, a.total_q - q0));
+  r.s_len = (int)uniform64(clamp64(s, a.total_s - s0));
+  return r;
+}
+
+// The same for a cache: the geometry is known on the host, only the filled length is read.
+template <int TILE>
+__device__ __forceinline__ AttnSeq locate_cache(const AttnArgs& a, int64_t t) {
+  AttnSeq r;
+  const int per = (int)(((int64_t)a.tokens * a.G + TILE - 1) / TILE);
+  r.b = (int)(t / per);
+  r.tile = (int)(t % per);
+  r.found = r.b < a.B;
+  if (!r.found) return r;
+  r.q_off = (int64_t)r.b * a.tokens;
+  r.q_len = a.tokens;
+  r.s_len = (int)uniform64(clamp64(a.s_lengths[r.b], a.capacity));
+  return r;
+}
+
+template <int TILE>
+__device__ __forceinline__ AttnSeq locate_rows(const AttnArgs& a, int64_t t) {
+  return a.capacity > 0 ? locate_cache<TILE>(a, t) : locate<TILE, false>(a, t);
+}
+
+// ---- tiles in LDS ------------------------------------------------------------------------------------------------------
+// A tile is ROWS rows of HDP elements (the head size rounded up to a power of two), moved in 16-byte chunks.  Chunks sit
+// at permuted places of their row so that the reads below touch every bank once:
+//   kOperand: 16 consecutive rows are read at one column, 16 bytes each -> XOR with the row;
+//   kTranspose (16-bit): 4 consecutive rows are read at 64 consecutive bytes each -> 64-byte groups XOR with the row;
+//   kScalar (fp32): two rows, four apart, are read at 128 consecutive bytes each.
+enum Place { kOperand, kTranspose, kScalar };
+
+template <typename T, int HDP, Place P>
+__device__ __forceinline__ int place(int row, int chunk) {
+  constexpr int CPR = HDP * (int)sizeof(T) / 16;
+  if constexpr (P == kOperand) {
+    if constexpr (CPR >= 16) return chunk ^ (row & 15);
+    return chunk ^ ((row / (16 / CPR)) & (CPR - 1));
+  } else if constexpr (P == kTranspose) {
+    if constexpr (CPR >= 16) return chunk ^ ((row & 3) << 2);
+    if constexpr (CPR == 8) return chunk ^ (((row >> 1) & 1) << 2);
+    return chunk;
+  } else {
+    if constexpr (CPR >= 16) return chunk ^ (((row >> 2) & 1) << 3);
+    return chunk;
+  }
+}
+
+// Offset in elements of element `col` of `row`.
+template <typename T, int HDP, Place P>
+__device__ __forceinline__ int tile_at(int row, int col) {
+  constexpr int E = 16 / (int)sizeof(T);
+  return row * HDP + place<T, HDP, P>(row, col / E) * E + col % E;
+}
+
+template <typename T>
+struct alignas(16) Chunk {
+  T v[16 / sizeof(T)];
+};
+
+// One 16-byte chunk of a row in memory: columns [c0, c0 + E) of D; zeros where `live` is false or past D.
+template <typename T>
+__device__ __forceinline__ Chunk<T> load_chunk(const T* row, int c0, int D, bool live) {
+  constexpr int E = 16 / (int)sizeof(T);
+  Chunk<T> c;
+  if (live && c0 + E <= D) {
+    const Packed<T, E> p = *reinterpret_cast<const Packed<T, E>*>(row + c0);
+#pragma unroll
+    for (int j = 0; j < E; ++j) c.v[j] = p.v[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < E; ++j) c.v[j] = (live && c0 + j < D) ? row[c0 + j] : (T)0.f;
+  }
+  return c;
+}
+
+// Whether a chunk holds an infinity or a NaN.
+template <typename T>
+__device__ __forceinline__ bool chunk_nonfinite(const Chunk<T>& c) {
+  bool bad = false;
+#pragma unroll
+  for (int j = 0; j < 16 / (int)sizeof(T); ++j) {
+    const float f = to_f32(c.v[j]);
+    bad |= !(__builtin_fabsf(f) < __builtin_inff());
+  }
+  return bad;
+}
+
+// ---- matrix instructions -----------------------------------------------------------------------------------------------
+// Everything is built on the 32 x 32 result layout: lane l holds column l % 32, register r holds row
+// 8 (r / 4) + 4 (l / 32) + r % 4 (`acc_row`).  The scores are computed transposed (keys x queries): a lane owns ONE query,
+// so its maximum, sum and rescaling are scalars of the lane, and the probabilities are the next product's operand in the
+// registers where they were computed -- the keys of a product are summed in any order, so the values are read in the
+// order in which the result layout holds the keys (no lane exchange in between).
+__device__ __forceinline__ constexpr int acc_row(int r, int half) { return 8 * (r / 4) + 4 * half + r % 4; }
+
+// Operands of one product step: 16-bit types take 16 summands a step (8 per lane: 8 half + j), fp32 8 summands as four
+// instructions of two (4 per lane: 4 half + j).
+template <typename T>
+struct Mma;
+
+template <>
+struct Mma<bf16> {
+  typedef bf16 Op __attribute__((ext_vector_type(8)));
+  static constexpr int kStep = 16;
+  static __device__ __forceinline__ f32x16 run(Op a, Op b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Mma<f16> {
+  typedef f16 Op __attribute__((ext_vector_type(8)));
+  static constexpr int kStep = 16;
+  static __device__ __forceinline__ f32x16 run(Op a, Op b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Mma<float> {
+  typedef float Op __attribute__((ext_vector_type(4)));
+  static constexpr int kStep = 8;
+  static __device__ __forceinline__ f32x16 run(Op a, Op b, f32x16 c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+  }
+};
+
+// The A (or B) operand of a product step whose summands are COLUMNS of the tile: row `row`, columns
+// [step * kStep + E * half, + E), one 16-byte read (kOperand placement).
+template <typename T, int HDP>
+__device__ __forceinline__ typename Mma<T>::Op read_cols(const T* tile, int row, int step, int half) {
+  constexpr int E = 16 / (int)sizeof(T);
+  return *reinterpret_cast<const typename Mma<T>::Op*>(tile + tile_at<T, HDP, kOperand>(row, step * 2 * E + E * half));
+}
+
+// The A operand of a product step whose summands are ROWS of the tile, in the order of the result layout: step u of a
+// 32-row block covers registers [u * R, u * R + R) of that layout (R = 8 for 16-bit types, 4 for fp32).  Lane l stands for
+// column d0 + l % 32.
+template <typename T, int HDP>
+__device__ __forceinline__ typename Mma<T>::Op read_rows(const T* tile, int row0, int u, int d0, int lane) {
+  if constexpr (sizeof(T) == 2) {
+    // gfx950's transposing LDS read: 16 lanes read 4 rows x 16 columns (lane i: row i / 4, columns 4 (i % 4) ..) and each
+    // is handed its column's 4 rows.
+    const int i = lane & 15;
+    const int half = lane >> 5;
+    const int col = d0 + (lane & 16) + 4 * (i & 3);
+    union {
+      s16x4 part[2];
+      typename Mma<T>::Op op;
+    } r;
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const int row = row0 + 16 * u + 8 * p + 4 * half + (i >> 2);
+      T* at = const_cast<T*>(tile) + tile_at<T, HDP, kTranspose>(row, col);
+      r.part[p] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) s16x4*)reinterpret_cast<s16x4*>(at));
+    }
+    return r.op;
+  } else {
+    typename Mma<T>::Op op;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      op[j] = tile[tile_at<T, HDP, kScalar>(row0 + 8 * u + 4 * (lane >> 5) + j, d0 + (lane & 31))];
+    return op;
+  }
+}
+
+// The result layout's registers [u * R, u * R + R) of a 32 x 32 block as the B operand that goes with read_rows.
+template <typename T>
+__device__ __forceinline__ typename Mma<T>::Op pack_rows(const f32x16& p, int u) {
+  constexpr int R = sizeof(T) == 2 ? 8 : 4;
+  typename Mma<T>::Op op;
+#pragma unroll
+  for (int j = 0; j < R; ++j) op[j] = from_f32<T>(p[u * R + j]);
+  return op;
+}
+
+// The finite values of an operand, the others as zeros (`finite`), or the other way round.
+template <typename T>
+__device__ __forceinline__ typename Mma<T>::Op keep_finite(typename Mma<T>::Op op, bool finite) {
+#pragma unroll
+  for (int j = 0; j < 16 / (int)sizeof(T); ++j) {
+    const bool is = __builtin_fabsf(to_f32((T)op[j])) < __builtin_inff();
+    op[j] = is == finite ? op[j] : (T)0.f;
+  }
+  return op;
+}
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }  // v_exp_f32; 2^-inf = 0
+
+__device__ __forceinline__ f32x16 zero16() {
+  f32x16 z;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) z[r] = 0.f;
+  return z;
+}
+
+// Host side: the smallest built head size that holds D, 0 if there is none.
+inline int attn_head_size(int D) {
+  for (int hd : {32, 64, 96, 128, 192, 256})
+    if (D <= hd) return hd;
+  return 0;
+}
+
+}  // namespace v3d
+
+#endif

@@ -52,6 +52,10 @@ __all__ = [
     "kpconv_gather_backward",
     "point_to_node_partition",
     "point_to_node_knn",
+    "attention_pack_forward",
+    "cached_attention",
+    "layer_norm_forward",
+    "layer_norm_backward",
     "radius_neighbors",
     "grid_subsampling",
     "sample_nodes_with_fps",
@@ -993,6 +997,190 @@ def kpconv_gather_backward(q_points, s_points, neighbor_indices, kernel_points, 
         q_points.data_ptr(), s_points.data_ptr(), neighbor_indices.data_ptr(), kernel_points.data_ptr(),
         grad_weighted.data_ptr(), grad_neighbors.data_ptr(), M, s_points.shape[0], H, K, C, float(sigma), dev, stream),
         "kpconv_gather_backward")
+
+
+# --------------------------------------------------------------------------------------------------------
+# Transformer layers over packs (no counterpart in the reference's extension: its layers call torch).
+# --------------------------------------------------------------------------------------------------------
+_ELEMENTS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # V3D_F32, V3D_F16, V3D_BF16
+
+
+def _element(t, name):
+    try:
+        return _ELEMENTS[t.dtype]
+    except KeyError:
+        raise RuntimeError(f'"{name}" not implemented for \'{_TYPE_NAMES.get(t.dtype, t.dtype)}\'') from None
+
+
+def _same_device(name, ref, *others):
+    for o in others:
+        if o is not None and o.device != ref.device:
+            raise RuntimeError(f"{name}: all tensors must be on one device, got {ref.device} and {o.device}")
+
+
+def _layer_norm_check(name, feats, residual, weight, bias):
+    _check_cuda_contiguous(feats, "feats")
+    if feats.dim() != 2:
+        raise RuntimeError(f"{name}: feats must have shape (N, C)")
+    if residual is not None:
+        _check_cuda_contiguous(residual, "residual")
+        _same_dtype(name, feats, residual)
+        if residual.shape != feats.shape:
+            raise RuntimeError(f"{name}: residual must have the shape of feats")
+    for t, n in ((weight, "weight"), (bias, "bias")):
+        if t is not None:
+            _check_cuda_contiguous(t, n)
+            if tuple(t.shape) != (feats.shape[1],):
+                raise RuntimeError(f"{name}: {n} must have shape {(feats.shape[1],)}")
+    if weight is not None and bias is not None:
+        _same_dtype(name, weight, bias)
+    _same_device(name, feats, residual, weight, bias)
+    affine = weight if weight is not None else bias
+    return _element(feats, name), _element(feats if affine is None else affine, name)
+
+
+def layer_norm_forward(feats, residual, weight, bias, targets, mean, rstd, eps):
+    """targets (N, C) = layer norm of ``feats`` (+ ``residual``); ``mean`` / ``rstd`` (N,) fp32 or None; see
+    include/v3d_hip.h."""
+    dtype, wdtype = _layer_norm_check("layer_norm_forward", feats, residual, weight, bias)
+    _check_cuda_contiguous(targets, "targets")
+    _same_dtype("layer_norm_forward", feats, targets)
+    if targets.shape != feats.shape:
+        raise RuntimeError("layer_norm_forward: targets must have the shape of feats")
+    rows, channels = feats.shape
+    for t, n in ((mean, "mean"), (rstd, "rstd")):
+        if t is not None:
+            _check_cuda_contiguous(t, n)
+            _check_float(t, n)
+            if tuple(t.shape) != (rows,):
+                raise RuntimeError(f"layer_norm_forward: {n} must have shape {(rows,)}")
+    _same_device("layer_norm_forward", feats, targets, mean, rstd)
+    dev, stream = _where(feats)
+    _lib.check(_lib.lib().v3d_layer_norm_fwd(feats.data_ptr(), _ptr(residual), _ptr(weight), _ptr(bias),
+                                             targets.data_ptr(), _ptr(mean), _ptr(rstd), dtype, wdtype, rows, channels,
+                                             float(eps), dev, stream), "layer_norm_forward")
+
+
+def layer_norm_backward(target_grads, feats, residual, weight, mean, rstd, feats_grads, weight_grads, bias_grads):
+    """The gradients of ``layer_norm_forward``: each of the three outputs may be None (not wanted)."""
+    name = "layer_norm_backward"
+    dtype, wdtype = _layer_norm_check(name, feats, residual, weight, None)
+    rows, channels = feats.shape
+    for t, n, shape in ((target_grads, "target_grads", feats.shape), (feats_grads, "feats_grads", feats.shape),
+                        (weight_grads, "weight_grads", (channels,)), (bias_grads, "bias_grads", (channels,)),
+                        (mean, "mean", (rows,)), (rstd, "rstd", (rows,))):
+        if t is not None:
+            _check_cuda_contiguous(t, n)
+            if tuple(t.shape) != tuple(shape):
+                raise RuntimeError(f"{name}: {n} must have shape {tuple(shape)}")
+    _check_float(mean, "mean")
+    _check_float(rstd, "rstd")
+    _same_dtype(name, feats, target_grads, *([] if feats_grads is None else [feats_grads]))
+    sums = [t for t in (weight_grads, bias_grads) if t is not None]
+    if sums:
+        _same_dtype(name, sums[0], *sums[1:], *([] if weight is None else [weight]))
+        wdtype = _element(sums[0], name)
+    _same_device(name, feats, target_grads, mean, rstd, feats_grads, weight_grads, bias_grads)
+    dev, stream = _where(feats)
+    lib = _lib.lib()
+    ws, wp, wn = _ws_args(lib.v3d_layer_norm_bwd_workspace_bytes(rows, channels) if sums else 0, feats)
+    _lib.check(lib.v3d_layer_norm_bwd(target_grads.data_ptr(), feats.data_ptr(), _ptr(residual), _ptr(weight),
+                                      mean.data_ptr(), rstd.data_ptr(), _ptr(feats_grads), _ptr(weight_grads),
+                                      _ptr(bias_grads), dtype, wdtype, rows, channels, wp, wn, dev, stream), name)
+
+
+def _heads(name, t, arg, dims):
+    """Features (.., heads, D) of any strides but the last, which is 1."""
+    if not t.is_cuda:
+        raise RuntimeError(f"{arg} must be a CUDA tensor")
+    if t.dim() != dims:
+        raise RuntimeError(f"{name}: {arg} must have {dims} dimensions, got {t.dim()}")
+    if t.size(-1) > 1 and t.stride(-1) != 1:
+        raise RuntimeError(f"{name}: the last dimension of {arg} must be contiguous")
+
+
+def _lengths(name, t, arg, count):
+    _check_cuda_contiguous(t, arg)
+    _check_long(t, arg)
+    if tuple(t.shape) != (count,):
+        raise RuntimeError(f"{name}: {arg} must have shape {(count,)}")
+
+
+def _strides(*values):
+    import ctypes
+
+    return (ctypes.c_int64 * len(values))(*values)
+
+
+def _attention_check(name, q, k, v, q_lengths, s_lengths):
+    _heads(name, q, "q_feats", 3)
+    _heads(name, k, "k_feats", 3)
+    _heads(name, v, "v_feats", 3)
+    dtype = _element(q, name)
+    _same_dtype(name, q, k, v)
+    if v.shape != k.shape or k.size(2) != q.size(2):
+        raise RuntimeError(f"{name}: expected q_feats (N, H, D), k_feats and v_feats (M, KV, D)")
+    _lengths(name, q_lengths, "q_lengths", q_lengths.numel())
+    _lengths(name, s_lengths, "s_lengths", q_lengths.numel())
+    _same_device(name, q, k, v, q_lengths, s_lengths)
+    return dtype, _strides(q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1))
+
+
+def attention_pack_forward(q_feats, k_feats, v_feats, q_lengths, s_lengths, targets, lse, scale, causal):
+    """targets (N, H, D) = attention of ``q_feats`` (N, H, D) over ``k_feats`` / ``v_feats`` (M, KV, D) inside every
+    sequence of the pack, ``lse`` (N, H) fp32 or None; see include/v3d_hip.h."""
+    name = "attention_pack_forward"
+    dtype, strides = _attention_check(name, q_feats, k_feats, v_feats, q_lengths, s_lengths)
+    _check_cuda_contiguous(targets, "targets")
+    _same_dtype(name, q_feats, targets)
+    if targets.shape != q_feats.shape:
+        raise RuntimeError(f"{name}: targets must have the shape of q_feats")
+    N, H, D = q_feats.shape
+    if lse is not None:
+        _check_cuda_contiguous(lse, "lse")
+        _check_float(lse, "lse")
+        if tuple(lse.shape) != (N, H):
+            raise RuntimeError(f"{name}: lse must have shape {(N, H)}")
+    _same_device(name, q_feats, targets, lse)
+    B, M, KV = q_lengths.numel(), k_feats.size(0), k_feats.size(1)
+    dev, stream = _where(q_feats)
+    lib = _lib.lib()
+    ws, wp, wn = _ws_args(lib.v3d_attention_pack_workspace_bytes(B, N, M, H, KV, D), q_feats)
+    _lib.check(lib.v3d_attention_pack_fwd(q_feats.data_ptr(), k_feats.data_ptr(), v_feats.data_ptr(),
+                                          q_lengths.data_ptr(), s_lengths.data_ptr(), targets.data_ptr(), _ptr(lse),
+                                          dtype, B, N, M, H, KV, D, strides, float(scale), int(bool(causal)), wp, wn,
+                                          dev, stream), name)
+
+
+def cached_attention(q_feats, k_cache, v_cache, lengths, targets, scale):
+    """targets (B, T, H, D) = attention of the newest T tokens of every sequence over its cache (B, C, KV, D), of which
+    ``lengths`` (B,) rows are filled; see include/v3d_hip.h."""
+    name = "cached_attention"
+    _heads(name, q_feats, "q_feats", 4)
+    _heads(name, k_cache, "k_cache", 4)
+    _heads(name, v_cache, "v_cache", 4)
+    _check_cuda_contiguous(targets, "targets")
+    dtype = _element(q_feats, name)
+    _same_dtype(name, q_feats, k_cache, v_cache, targets)
+    B, T, H, D = q_feats.shape
+    if targets.shape != q_feats.shape:
+        raise RuntimeError(f"{name}: targets must have the shape of q_feats")
+    if k_cache.shape != v_cache.shape or k_cache.size(0) != B or k_cache.size(3) != D:
+        raise RuntimeError(f"{name}: expected q_feats (B, T, H, D), k_cache and v_cache (B, C, KV, D)")
+    if B > 1 and T > 0 and q_feats.stride(0) != T * q_feats.stride(1):
+        raise RuntimeError(f"{name}: the tokens of q_feats must be at one stride")
+    _lengths(name, lengths, "lengths", B)
+    _same_device(name, q_feats, k_cache, v_cache, lengths, targets)
+    C, KV = k_cache.size(1), k_cache.size(2)
+    q_row = q_feats.stride(1) if T > 1 else q_feats.stride(0)
+    strides = _strides(q_row, q_feats.stride(2), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
+                       v_cache.stride(0), v_cache.stride(1), v_cache.stride(2))
+    dev, stream = _where(q_feats)
+    lib = _lib.lib()
+    ws, wp, wn = _ws_args(lib.v3d_cached_attention_workspace_bytes(B, T, C, H, KV, D), q_feats)
+    _lib.check(lib.v3d_cached_attention(q_feats.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), lengths.data_ptr(),
+                                        targets.data_ptr(), dtype, B, T, C, H, KV, D, strides, float(scale), wp, wn,
+                                        dev, stream), name)
 
 
 # --------------------------------------------------------------------------------------------------------

@@ -5,6 +5,7 @@ Same names, signatures, return values and error behaviour as the reference wrapp
 ``vision3d_amd.ext`` (hand-written gfx950 kernels behind a C ABI).  ``vision3d_amd.install()`` registers this
 package as ``vision3d.ops`` / ``vision3d.ext`` so unchanged model code imports it.
 """
+from .attention import attention_pack_mode, cached_attention
 from .ball_query import ball_query, ball_query_multi
 from .conversion import batch_to_pack, batch_to_pack_with_lengths, pack_to_batch
 from .furthest_point_sample import furthest_point_sample
@@ -14,6 +15,7 @@ from .group_gather import group_gather
 from .knn import knn, knn_pack_mode
 from .knn_points import knn_points
 from .kpconv import kpconv, kpconv_gather
+from .layer_norm import layer_norm
 from .matching import (extract_correspondences_from_feats, extract_correspondences_from_scores,
                        extract_correspondences_from_scores_threshold, extract_correspondences_from_scores_topk)
 from .superpoint_matching import SuperPointMatchingGlobalTopk, SuperPointMatchingMutualTopk
@@ -39,4 +41,5 @@ __all__ = [
     "naive_radius_search_pack_mode",
     "index_select", "local_maxpool_pack_mode", "global_avgpool_pack_mode", "nearest_interpolate_pack_mode",
     "knn_interpolate_pack_mode", "build_grid_and_radius_graph_pyramid", "sa_group", "edge_group", "kpconv_gather", "kpconv", "point_to_node_partition", "ball_query_partition",
+    "attention_pack_mode", "cached_attention", "layer_norm",
 ]

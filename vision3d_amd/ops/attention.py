@@ -1,0 +1,69 @@
+"""Softmax attention of the transformer layers over packs: inside every sequence (cloud) of a pack, and of new tokens
+against a cache of keys and values.  The reference's layers pad a pack to a batch, mask, and materialise the (N, M) scores
+of every head; here the scores live in registers, sequences of any lengths lie one behind the other, and the lengths stay
+on the device (no synchronisation).
+"""
+from typing import Optional
+
+import torch
+from torch import Tensor
+
+from .. import ext
+
+
+def _require_cuda(name, *tensors):
+    if not all(t.is_cuda for t in tensors):
+        raise RuntimeError(f"{name}: CUDA tensors required (no CPU fallback in vision3d_amd)")
+
+
+def _rows(t: Tensor) -> Tensor:
+    """Any strides but the last dimension's; a gradient or input without a unit stride there is copied."""
+    return t if t.size(-1) <= 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def _scale(scale, dim):
+    return float(dim) ** -0.5 if scale is None else float(scale)
+
+
+def attention_pack_mode(q_feats: Tensor, k_feats: Tensor, v_feats: Tensor, q_lengths: Tensor,
+                        s_lengths: Optional[Tensor] = None, scale: Optional[float] = None, causal: bool = False) -> Tensor:
+    """q_feats (N, H, D), k_feats and v_feats (M, KV, D), lengths (B,) -> (N, H, D): per sequence and head the softmax over
+    ``scale * q . k`` (``scale`` = D ** -0.5 if None) of its keys, applied to its values.
+
+    H is a multiple of KV: query head h reads key head ``h // (H // KV)``.  ``s_lengths`` None: the keys are the queries'
+    sequences (self-attention).  ``causal``: query i of a sequence sees the keys j <= i + (s_length - q_length), so the last
+    query sees them all.  A query without keys yields zeros and has no gradient; what a query does not see does not reach
+    it, infinities and NaN included.  Rows behind the last sequence come out as zeros.  fp32, fp16 or bf16, D <= 256; the
+    inputs may be views of one projection (only the last dimension has to be contiguous).
+    """
+    s_lengths = q_lengths if s_lengths is None else s_lengths
+    _require_cuda("attention_pack_mode", q_feats, k_feats, v_feats)
+    dev = q_feats.device
+    q_lengths = q_lengths.to(device=dev, dtype=torch.long).contiguous()
+    s_lengths = s_lengths.to(device=dev, dtype=torch.long).contiguous()
+    scale = _scale(scale, q_feats.size(-1))
+    q, k, v = _rows(q_feats), _rows(k_feats), _rows(v_feats)
+    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    ext.attention_pack_forward(q, k, v, q_lengths, s_lengths, out, None, scale, causal)
+    return out
+
+
+def cached_attention(q_feats: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: Tensor,
+                     scale: Optional[float] = None) -> Tensor:
+    """q_feats (B, T, H, D) = the newest T tokens of B sequences, k_cache and v_cache (B, C, KV, D), lengths (B,) = filled
+    rows of each cache, the new tokens' among them -> (B, T, H, D).
+
+    Token t sees the rows j <= lengths[b] - T + t; rows past a length are never read (they may hold anything).  The serving
+    form of ``attention_pack_mode(..., causal=True)``: no gradient, the keys are divided over the whole GPU however few the
+    sequences are.  Only the last dimension of each tensor has to be contiguous.
+    """
+    _require_cuda("cached_attention", q_feats, k_cache, v_cache)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q_feats, k_cache, v_cache)):
+        raise RuntimeError("cached_attention: no gradient; call it under torch.no_grad() or use attention_pack_mode")
+    lengths = lengths.to(device=q_feats.device, dtype=torch.long).contiguous()
+    q, k, v = _rows(q_feats), _rows(k_cache), _rows(v_cache)
+    if q.dim() == 4 and q.size(0) > 1 and q.stride(0) != q.size(1) * q.stride(1):
+        q = q.contiguous()
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    ext.cached_attention(q, k, v, lengths, out, _scale(scale, q.size(-1)))
+    return out

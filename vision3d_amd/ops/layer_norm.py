@@ -1,0 +1,73 @@
+"""Layer normalisation of feature rows, the norm of the transformer layers over packs (the reference's layers call
+``torch.nn.LayerNorm``; a post-norm layer adds the residual first: here the sum is formed inside the kernel).
+
+One kernel forward; backward recomputes the sum and the normalised rows from the inputs and the saved (mean, rstd), so
+nothing of the input's size is kept besides the inputs themselves.  The gradients of the weight and the bias are added in
+a fixed order (no atomics).
+"""
+from typing import Optional
+
+import torch
+from torch import Tensor
+
+from .. import ext
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, feats, weight, bias, eps, residual):
+        out = torch.empty_like(feats)
+        mean = torch.empty((feats.shape[0],), dtype=torch.float32, device=feats.device)
+        rstd = torch.empty_like(mean)
+        ext.layer_norm_forward(feats, residual, weight, bias, out, mean, rstd, eps)
+        ctx.save_for_backward(feats, weight, residual, mean, rstd)
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        feats, weight, residual, mean, rstd = ctx.saved_tensors
+        need_feats = ctx.needs_input_grad[0] or ctx.needs_input_grad[4]
+        need_weight, need_bias = ctx.needs_input_grad[1], ctx.needs_input_grad[2]
+        grad_feats = torch.empty_like(feats) if need_feats else None
+        channels = feats.shape[1:]
+        grad_weight = feats.new_empty(channels, dtype=weight.dtype) if need_weight else None
+        grad_bias = feats.new_empty(channels, dtype=ctx.bias_dtype) if need_bias else None
+        if feats.shape[0] == 0:  # no rows: the column sums are empty
+            for t in (grad_weight, grad_bias):
+                if t is not None:
+                    t.zero_()
+        else:
+            ext.layer_norm_backward(grad.contiguous(), feats, residual, weight, mean, rstd, grad_feats, grad_weight,
+                                    grad_bias)
+        return (grad_feats if ctx.needs_input_grad[0] else None, grad_weight, grad_bias, None,
+                grad_feats if ctx.needs_input_grad[4] else None)
+
+
+def layer_norm(feats: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5,
+               residual: Optional[Tensor] = None) -> Tensor:
+    """feats (*, C) (+ residual of the same shape), weight / bias (C,) -> (*, C): every row normalised to mean 0 and
+    variance 1 (biased, + eps), scaled and shifted.
+
+    fp32, fp16 or bf16 features; weight and bias in the features' type or fp32.  Statistics and sums are fp32; the output
+    has the features' type.  At most 16384 channels (8192 in fp32).  Gradients flow to all four tensors.
+    """
+    for t in (feats, weight, bias, residual):
+        if t is not None and not t.is_cuda:
+            raise RuntimeError("layer_norm: CUDA tensors required (no CPU fallback in vision3d_amd)")
+    if feats.dim() < 1:
+        raise RuntimeError("layer_norm: feats must have a channel dimension")
+    shape = feats.shape
+    if residual is not None:
+        if residual.shape != shape:
+            raise RuntimeError("layer_norm: residual must have the shape of feats")
+        residual = residual.reshape(-1, shape[-1]).contiguous()
+    rows = feats.reshape(-1, shape[-1]).contiguous()
+    weight = None if weight is None else weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (rows, weight, bias, residual)):
+        return _LayerNorm.apply(rows, weight, bias, float(eps), residual).view(shape)
+    out = torch.empty_like(rows)
+    ext.layer_norm_forward(rows, residual, weight, bias, out, None, None, eps)
+    return out.view(shape)
