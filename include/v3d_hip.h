@@ -469,6 +469,10 @@ int v3d_layer_norm_bwd(const void* grad, const void* feats, const void* residual
  * j <= lengths[b] - tokens + t.  Rows past a length are never read.  `strides`: q row, q head, k batch, k row, k head,
  * v batch, v row, v head; q rows are token b * tokens + t.
  *
+ * v3d_attention_pack_bwd: grad (total_q,H,D) of out and the forward's inputs, out and lse -> grad_q (total_q,H,D), grad_k
+ * and grad_v (total_s,KV,D), all contiguous and fully written (zeros behind the last sequence); key heads sum over their
+ * query heads.  No atomics: the same bits every time.
+ *
  * workspace: v3d_*_workspace_bytes bytes (0 where the row tiles alone fill the GPU), 256-B aligned, or NULL. */
 #define V3D_ATTENTION_MAX_HEAD_SIZE 256
 size_t v3d_attention_pack_workspace_bytes(int B, int64_t total_q, int64_t total_s, int H, int KV, int D);
@@ -476,6 +480,12 @@ int v3d_attention_pack_fwd(const void* q, const void* k, const void* v, const in
                            const int64_t* s_lengths, void* out, float* lse, int dtype, int B, int64_t total_q,
                            int64_t total_s, int H, int KV, int D, const int64_t* strides, float scale, int causal,
                            void* workspace, size_t workspace_bytes, int device, void* stream);
+size_t v3d_attention_pack_bwd_workspace_bytes(int B, int64_t total_q, int64_t total_s, int H, int KV, int D);
+int v3d_attention_pack_bwd(const void* grad, const void* q, const void* k, const void* v, const void* out,
+                           const float* lse, const int64_t* q_lengths, const int64_t* s_lengths, void* grad_q,
+                           void* grad_k, void* grad_v, int dtype, int B, int64_t total_q, int64_t total_s, int H, int KV,
+                           int D, const int64_t* strides, float scale, int causal, void* workspace,
+                           size_t workspace_bytes, int device, void* stream);
 size_t v3d_cached_attention_workspace_bytes(int B, int tokens, int64_t capacity, int H, int KV, int D);
 int v3d_cached_attention(const void* q, const void* k_cache, const void* v_cache, const int64_t* lengths, void* out,
                          int dtype, int B, int tokens, int64_t capacity, int H, int KV, int D, const int64_t* strides,

@@ -11,10 +11,6 @@
 
 namespace v3d {
 
-constexpr int kAttnWaves = 4;
-constexpr int kAttnRows = 32 * kAttnWaves;  // rows of a workgroup's tile
-
-__host__ __device__ constexpr int attn_pow2(int hd) { return hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
 template <typename T, int HD>
 constexpr int attn_keys() { return HD * (int)sizeof(T) > 512 ? 32 : 64; }  // keys of a tile: at most 64 KiB of LDS
 
@@ -27,7 +23,6 @@ __global__ __launch_bounds__(256) void attn_forward_kernel(const AttnArgs a) {
   constexpr int STEPS = HD / Mma<T>::kStep;         // product steps over the head size
   constexpr int USTEPS = 32 / Mma<T>::kStep;        // product steps over a 32-key block
   constexpr int DT = HD / 32;
-  constexpr Place kV = sizeof(T) == 2 ? kTranspose : kScalar;
   typedef typename Mma<T>::Op Op;
   __shared__ T lds_k[BN * HDP];
   __shared__ T lds_v[BN * HDP];
@@ -105,8 +100,8 @@ __global__ __launch_bounds__(256) void attn_forward_kernel(const AttnArgs a) {
       const bool live = key0 + r < seq.s_len;
       const Chunk<T> kc = load_chunk<T>(k + (int64_t)(key0 + r) * a.k_row, c * E, a.D, live);
       const Chunk<T> vc = load_chunk<T>(v + (int64_t)(key0 + r) * a.v_row, c * E, a.D, live);
-      *reinterpret_cast<Chunk<T>*>(lds_k + tile_at<T, HDP, kOperand>(r, c * E)) = kc;
-      *reinterpret_cast<Chunk<T>*>(lds_v + tile_at<T, HDP, kV>(r, c * E)) = vc;
+      *reinterpret_cast<Chunk<T>*>(lds_k + tile_at<T, HDP>(r, c * E)) = kc;
+      *reinterpret_cast<Chunk<T>*>(lds_v + tile_at<T, HDP>(r, c * E)) = vc;
       bad |= chunk_nonfinite(vc);
     }
     if (key0 + BN > least && bad) lds_bad = 1;

@@ -151,34 +151,29 @@ __device__ __forceinline__ AttnSeq locate_rows(const AttnArgs& a, int64_t t) {
 }
 
 // ---- tiles in LDS ------------------------------------------------------------------------------------------------------
-// A tile is ROWS rows of HDP elements (the head size rounded up to a power of two), moved in 16-byte chunks.  Chunks sit
-// at permuted places of their row so that the reads below touch every bank once:
-//   kOperand: 16 consecutive rows are read at one column, 16 bytes each -> XOR with the row;
-//   kTranspose (16-bit): 4 consecutive rows are read at 64 consecutive bytes each -> 64-byte groups XOR with the row;
-//   kScalar (fp32): two rows, four apart, are read at 128 consecutive bytes each.
-enum Place { kOperand, kTranspose, kScalar };
-
-template <typename T, int HDP, Place P>
+// A tile is some rows of HDP elements (the head size rounded up to a power of two), moved in 16-byte chunks.  It is read in
+// two ways: 16 consecutive rows at one column, 16 bytes each (read_cols), and along the rows (read_rows: 4 consecutive rows
+// at 64 consecutive bytes for 16-bit types, two rows 4 apart at 128 bytes for fp32).  Chunks sit at their column XOR f(row),
+// f chosen so that both ways touch each of the 64 banks once: f takes 16 values over 16 rows that start a bank line, and
+// its bits that move 64 (fp32: 128) bytes change between the rows of one read_rows access.
+template <typename T, int HDP>
 __device__ __forceinline__ int place(int row, int chunk) {
   constexpr int CPR = HDP * (int)sizeof(T) / 16;
-  if constexpr (P == kOperand) {
-    if constexpr (CPR >= 16) return chunk ^ (row & 15);
-    return chunk ^ ((row / (16 / CPR)) & (CPR - 1));
-  } else if constexpr (P == kTranspose) {
-    if constexpr (CPR >= 16) return chunk ^ ((row & 3) << 2);
-    if constexpr (CPR == 8) return chunk ^ (((row >> 1) & 1) << 2);
-    return chunk;
+  if constexpr (sizeof(T) == 2) {
+    if constexpr (CPR >= 16) return chunk ^ (((row & 3) << 2) | ((row >> 2) & 3));
+    if constexpr (CPR == 8) return chunk ^ ((((row >> 1) & 1) << 2) | ((row >> 2) & 3));
+    return chunk ^ ((row >> 2) & 3);
   } else {
-    if constexpr (CPR >= 16) return chunk ^ (((row >> 2) & 1) << 3);
-    return chunk;
+    if constexpr (CPR >= 16) return chunk ^ ((((row >> 2) & 1) << 3) | (((row >> 3) & 1) << 2) | (row & 3));
+    return chunk ^ ((row >> 1) & 7);
   }
 }
 
 // Offset in elements of element `col` of `row`.
-template <typename T, int HDP, Place P>
+template <typename T, int HDP>
 __device__ __forceinline__ int tile_at(int row, int col) {
   constexpr int E = 16 / (int)sizeof(T);
-  return row * HDP + place<T, HDP, P>(row, col / E) * E + col % E;
+  return row * HDP + place<T, HDP>(row, col / E) * E + col % E;
 }
 
 template <typename T>
@@ -255,11 +250,11 @@ struct Mma<float> {
 };
 
 // The A (or B) operand of a product step whose summands are COLUMNS of the tile: row `row`, columns
-// [step * kStep + E * half, + E), one 16-byte read (kOperand placement).
+// [step * kStep + E * half, + E), one 16-byte read.
 template <typename T, int HDP>
 __device__ __forceinline__ typename Mma<T>::Op read_cols(const T* tile, int row, int step, int half) {
   constexpr int E = 16 / (int)sizeof(T);
-  return *reinterpret_cast<const typename Mma<T>::Op*>(tile + tile_at<T, HDP, kOperand>(row, step * 2 * E + E * half));
+  return *reinterpret_cast<const typename Mma<T>::Op*>(tile + tile_at<T, HDP>(row, step * 2 * E + E * half));
 }
 
 // The A operand of a product step whose summands are ROWS of the tile, in the order of the result layout: step u of a
@@ -280,7 +275,7 @@ __device__ __forceinline__ typename Mma<T>::Op read_rows(const T* tile, int row0
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
       const int row = row0 + 16 * u + 8 * p + 4 * half + (i >> 2);
-      T* at = const_cast<T*>(tile) + tile_at<T, HDP, kTranspose>(row, col);
+      T* at = const_cast<T*>(tile) + tile_at<T, HDP>(row, col);
       r.part[p] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
           (__attribute__((address_space(3))) s16x4*)reinterpret_cast<s16x4*>(at));
     }
@@ -289,7 +284,7 @@ __device__ __forceinline__ typename Mma<T>::Op read_rows(const T* tile, int row0
     typename Mma<T>::Op op;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      op[j] = tile[tile_at<T, HDP, kScalar>(row0 + 8 * u + 4 * (lane >> 5) + j, d0 + (lane & 31))];
+      op[j] = tile[tile_at<T, HDP>(row0 + 8 * u + 4 * (lane >> 5) + j, d0 + (lane & 31))];
     return op;
   }
 }
@@ -327,6 +322,13 @@ __device__ __forceinline__ f32x16 zero16() {
   return z;
 }
 
+__host__ __device__ constexpr int attn_pow2(int hd) { return hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
+
+constexpr int kAttnWaves = 4;
+constexpr int kAttnRows = 32 * kAttnWaves;  // rows (or keys) of a workgroup's tile
+
+// Host side: the argument checks of every entry point (attention.hip).
+int attn_check(const char* what, int dtype, int B, int64_t total_q, int64_t total_s, int H, int KV, int D, float scale);
 // Host side: the smallest built head size that holds D, 0 if there is none.
 inline int attn_head_size(int D) {
   for (int hd : {32, 64, 96, 128, 192, 256})

@@ -53,6 +53,7 @@ __all__ = [
     "point_to_node_partition",
     "point_to_node_knn",
     "attention_pack_forward",
+    "attention_pack_backward",
     "cached_attention",
     "layer_norm_forward",
     "layer_norm_backward",
@@ -1150,6 +1151,34 @@ def attention_pack_forward(q_feats, k_feats, v_feats, q_lengths, s_lengths, targ
                                           q_lengths.data_ptr(), s_lengths.data_ptr(), targets.data_ptr(), _ptr(lse),
                                           dtype, B, N, M, H, KV, D, strides, float(scale), int(bool(causal)), wp, wn,
                                           dev, stream), name)
+
+
+def attention_pack_backward(target_grads, q_feats, k_feats, v_feats, targets, lse, q_lengths, s_lengths, q_grads, k_grads,
+                            v_grads, scale, causal):
+    """The gradients of ``attention_pack_forward``, from its inputs, its ``targets`` and its ``lse``."""
+    name = "attention_pack_backward"
+    dtype, strides = _attention_check(name, q_feats, k_feats, v_feats, q_lengths, s_lengths)
+    N, H, D = q_feats.shape
+    B, M, KV = q_lengths.numel(), k_feats.size(0), k_feats.size(1)
+    for t, n, shape in ((target_grads, "target_grads", (N, H, D)), (targets, "targets", (N, H, D)),
+                        (q_grads, "q_grads", (N, H, D)), (k_grads, "k_grads", (M, KV, D)), (v_grads, "v_grads", (M, KV, D))):
+        _check_cuda_contiguous(t, n)
+        _same_dtype(name, q_feats, t)
+        if tuple(t.shape) != shape:
+            raise RuntimeError(f"{name}: {n} must have shape {shape}")
+    _check_cuda_contiguous(lse, "lse")
+    _check_float(lse, "lse")
+    if tuple(lse.shape) != (N, H):
+        raise RuntimeError(f"{name}: lse must have shape {(N, H)}")
+    _same_device(name, q_feats, target_grads, targets, lse, q_grads, k_grads, v_grads)
+    dev, stream = _where(q_feats)
+    lib = _lib.lib()
+    ws, wp, wn = _ws_args(lib.v3d_attention_pack_bwd_workspace_bytes(B, N, M, H, KV, D), q_feats)
+    _lib.check(lib.v3d_attention_pack_bwd(target_grads.data_ptr(), q_feats.data_ptr(), k_feats.data_ptr(),
+                                          v_feats.data_ptr(), targets.data_ptr(), lse.data_ptr(), q_lengths.data_ptr(),
+                                          s_lengths.data_ptr(), q_grads.data_ptr(), k_grads.data_ptr(),
+                                          v_grads.data_ptr(), dtype, B, N, M, H, KV, D, strides, float(scale),
+                                          int(bool(causal)), wp, wn, dev, stream), name)
 
 
 def cached_attention(q_feats, k_cache, v_cache, lengths, targets, scale):

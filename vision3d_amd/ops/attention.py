@@ -25,6 +25,27 @@ def _scale(scale, dim):
     return float(dim) ** -0.5 if scale is None else float(scale)
 
 
+class _AttentionPack(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, q_lengths, s_lengths, scale, causal):
+        q, k, v = _rows(q), _rows(k), _rows(v)
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+        ext.attention_pack_forward(q, k, v, q_lengths, s_lengths, out, lse, scale, causal)
+        ctx.save_for_backward(q, k, v, out, lse, q_lengths, s_lengths)
+        ctx.scale, ctx.causal = scale, causal
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        q, k, v, out, lse, q_lengths, s_lengths = ctx.saved_tensors
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        ext.attention_pack_backward(grad.contiguous(), q, k, v, out, lse, q_lengths, s_lengths, dq, dk, dv, ctx.scale,
+                                    ctx.causal)
+        return dq, dk, dv, None, None, None, None
+
+
 def attention_pack_mode(q_feats: Tensor, k_feats: Tensor, v_feats: Tensor, q_lengths: Tensor,
                         s_lengths: Optional[Tensor] = None, scale: Optional[float] = None, causal: bool = False) -> Tensor:
     """q_feats (N, H, D), k_feats and v_feats (M, KV, D), lengths (B,) -> (N, H, D): per sequence and head the softmax over
@@ -33,7 +54,7 @@ def attention_pack_mode(q_feats: Tensor, k_feats: Tensor, v_feats: Tensor, q_len
     H is a multiple of KV: query head h reads key head ``h // (H // KV)``.  ``s_lengths`` None: the keys are the queries'
     sequences (self-attention).  ``causal``: query i of a sequence sees the keys j <= i + (s_length - q_length), so the last
     query sees them all.  A query without keys yields zeros and has no gradient; what a query does not see does not reach
-    it, infinities and NaN included.  Rows behind the last sequence come out as zeros.  fp32, fp16 or bf16, D <= 256; the
+    it, infinities and NaN included (in the forward).  Rows behind the last sequence come out as zeros.  fp32, fp16 or bf16, D <= 256; the
     inputs may be views of one projection (only the last dimension has to be contiguous).
     """
     s_lengths = q_lengths if s_lengths is None else s_lengths
@@ -42,6 +63,8 @@ def attention_pack_mode(q_feats: Tensor, k_feats: Tensor, v_feats: Tensor, q_len
     q_lengths = q_lengths.to(device=dev, dtype=torch.long).contiguous()
     s_lengths = s_lengths.to(device=dev, dtype=torch.long).contiguous()
     scale = _scale(scale, q_feats.size(-1))
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q_feats, k_feats, v_feats)):
+        return _AttentionPack.apply(q_feats, k_feats, v_feats, q_lengths, s_lengths, scale, causal)
     q, k, v = _rows(q_feats), _rows(k_feats), _rows(v_feats)
     out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     ext.attention_pack_forward(q, k, v, q_lengths, s_lengths, out, None, scale, causal)
