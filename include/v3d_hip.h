@@ -459,7 +459,7 @@ int v3d_layer_norm_bwd(const void* grad, const void* feats, const void* residual
  * over all keys j of the sequence or, with `causal`, over j <= i + (s_len - q_len): the last query sees every key.  A query
  * that sees no key yields zeros; an infinity or NaN in a key or value that a query does not see does not reach it.  Rows
  * behind the last sequence are written as zeros; lengths that overrun the totals are cut.  out (total_q,H,D) contiguous;
- * lse (total_q,H) fp32 = natural log of the row's sum of exponentials (-inf without keys), what the backward needs; or NULL.
+ * lse (total_q,H) fp32 = log2 of the row's sum of exp(score) (-inf without keys), what the backward needs; or NULL.
  * `strides` (host array, elements): q row, q head, k row, k head, v row, v head -- the last dimension is contiguous, rows
  * need no alignment.  Products of 16-bit types are exact, the probabilities are rounded to the type before they meet the
  * values; scores, statistics and sums are fp32.  D <= V3D_ATTENTION_MAX_HEAD_SIZE, 0 < scale < inf.

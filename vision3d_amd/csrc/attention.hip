@@ -11,11 +11,13 @@
 
 namespace v3d {
 
+// Keys of a tile: two tiles of keys and values (one worked on, one arriving) stay within 64 KiB up to 512-byte rows, so that
+// two workgroups share a CU.
 template <typename T, int HD>
-constexpr int attn_keys() { return HD * (int)sizeof(T) > 512 ? 32 : 64; }  // keys of a tile: at most 64 KiB of LDS
+constexpr int attn_keys() { return HD * (int)sizeof(T) > 256 ? 32 : 64; }
 
 template <typename T, int HD>
-__global__ __launch_bounds__(256) void attn_forward_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(256, HD * sizeof(T) <= 256 ? 2 : 1) void attn_forward_kernel(const AttnArgs a) {
   constexpr int HDP = attn_pow2(HD);
   constexpr int BN = attn_keys<T, HD>();
   constexpr int NT = BN / 32;                       // 32-key blocks of a tile
@@ -24,9 +26,9 @@ __global__ __launch_bounds__(256) void attn_forward_kernel(const AttnArgs a) {
   constexpr int USTEPS = 32 / Mma<T>::kStep;        // product steps over a 32-key block
   constexpr int DT = HD / 32;
   typedef typename Mma<T>::Op Op;
-  __shared__ T lds_k[BN * HDP];
-  __shared__ T lds_v[BN * HDP];
-  __shared__ int lds_bad;
+  __shared__ T lds_k[2][BN * HDP];
+  __shared__ T lds_v[2][BN * HDP];
+  __shared__ int lds_bad[2];
 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int half = lane >> 5;
@@ -59,10 +61,9 @@ __global__ __launch_bounds__(256) void attn_forward_kernel(const AttnArgs a) {
   };
   const int limit = limit_of(token);  // this lane's query sees keys [0, limit)
   // the wave's and the workgroup's first and last rows bound what they have to look at
-  const int wave_first = min(seq.tile * kAttnRows + wave * 32, rows - 1);
-  const int wave_last = min(seq.tile * kAttnRows + wave * 32 + 31, rows - 1);
   const bool wave_live = seq.tile * kAttnRows + wave * 32 < rows;
-  const int wave_least = limit_of(wave_first / a.G), wave_most = wave_live ? limit_of(wave_last / a.G) : 0;
+  const int wave_least = __builtin_amdgcn_readfirstlane(limit);
+  const int wave_most = wave_live ? limit_of(min(seq.tile * kAttnRows + wave * 32 + 31, rows - 1) / a.G) : 0;
   const int most = limit_of(min(seq.tile * kAttnRows + kAttnRows - 1, rows - 1) / a.G);
   const int least = limit_of(min(seq.tile * kAttnRows, rows - 1) / a.G);
 
@@ -76,152 +77,152 @@ __global__ __launch_bounds__(256) void attn_forward_kernel(const AttnArgs a) {
 
   Op qf[STEPS];
 #pragma unroll
-  for (int st = 0; st < STEPS; ++st) {
-    const Chunk<T> c = load_chunk<T>(q, st * 2 * E + E * half, a.D, true);
-#pragma unroll
-    for (int j = 0; j < E; ++j) qf[st][j] = c.v[j];
-  }
+  for (int st = 0; st < STEPS; ++st) qf[st] = load_op<T>(q, st * 2 * E + E * half, a.D, true);
+
+  // The tile after the one that is worked on is on its way in registers meanwhile.
+  TileStage<T, HD, BN> stage_k, stage_v;
+  if (threadIdx.x < 2) lds_bad[threadIdx.x] = 0;
+  auto fetch = [&](int t) {
+    stage_k.fetch(k + (int64_t)t * BN * a.k_row, a.k_row, a.D, seq.s_len - t * BN);
+    stage_v.fetch(v + (int64_t)t * BN * a.v_row, a.v_row, a.D, seq.s_len - t * BN);
+  };
+  auto place_tile = [&](int t, int buf) {
+    stage_k.store(lds_k[buf]);
+    stage_v.store(lds_v[buf]);
+    // values of a tile that some query sees in part: see below
+    if (t * BN + BN > least && stage_v.nonfinite()) lds_bad[buf] = t + 1;
+  };
 
   const float c2 = a.scale * kLog2e;
-  float m = -__builtin_inff(), l = 0.f;
+  float m = -__builtin_inff(), l = 0.f;  // running maximum of scale * log2(e) * score, and the sum of 2^(that - m)
   f32x16 o[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) o[d] = zero16();
 
-  for (int t = t_begin; t < t_end; ++t) {
+  auto work = [&](int t, auto buffer) {
+    constexpr int buf = decltype(buffer)::value;
     const int key0 = t * BN;
-    __syncthreads();
-    if (threadIdx.x == 0) lds_bad = 0;
-    __syncthreads();
-    bool bad = false;
-    constexpr int CPR = HD / E;
-    for (int i = threadIdx.x; i < BN * CPR; i += 256) {
-      const int r = i / CPR, c = i % CPR;
-      const bool live = key0 + r < seq.s_len;
-      const Chunk<T> kc = load_chunk<T>(k + (int64_t)(key0 + r) * a.k_row, c * E, a.D, live);
-      const Chunk<T> vc = load_chunk<T>(v + (int64_t)(key0 + r) * a.v_row, c * E, a.D, live);
-      *reinterpret_cast<Chunk<T>*>(lds_k + tile_at<T, HDP>(r, c * E)) = kc;
-      *reinterpret_cast<Chunk<T>*>(lds_v + tile_at<T, HDP>(r, c * E)) = vc;
-      bad |= chunk_nonfinite(vc);
-    }
-    if (key0 + BN > least && bad) lds_bad = 1;
-    __syncthreads();
-    if (key0 >= wave_most) continue;
-
+    const bool active = key0 < wave_most;
     f32x16 s[NT];
+    if (active) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      s[n] = zero16();
+      for (int n = 0; n < NT; ++n) s[n] = zero16();
 #pragma unroll
       for (int st = 0; st < STEPS; ++st)
-        s[n] = Mma<T>::run(read_cols<T, HDP>(lds_k, n * 32 + (lane & 31), st, half), qf[st], s[n]);
-    }
-    const bool masked = key0 + BN > wave_least;
-    if (masked) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          s[n] = Mma<T>::run(read_cols<T, HDP>(lds_k[buf], n * 32 + (lane & 31), st, half), qf[st], s[n]);
+      if (key0 + BN > wave_least) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (key0 + n * 32 + acc_row(r, half) >= limit) s[n][r] = -__builtin_inff();
+      }
+      // maximum of the lane, then with the lane that holds the other keys of this query
+      float top = -__builtin_inff();
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (key0 + n * 32 + acc_row(r, half) >= limit) s[n][r] = -__builtin_inff();
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[n][r]);
+      top = halves_max(top) * c2;
+      // The maximum moves only when a probability would exceed 2^8: what was summed is rescaled rarely, and a stale
+      // maximum costs no accuracy (16-bit probabilities keep their relative precision up to 2^8, the sums are fp32).
+      if (__any(top > m + 8.f)) {
+        const float m_new = fmaxf(m, top);
+        const float alpha = m_new == -__builtin_inff() ? 1.f : exp2_fast(m - m_new);
+        m = m_new;
+        l *= alpha;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+      }
+      const float base = m == -__builtin_inff() ? 0.f : m;
+      float sum = 0.f;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[n][r] = exp2_fast(fmaf(s[n][r], c2, -base));
+          sum += s[n][r];
+        }
+      l += sum;
     }
-    // running maximum: of the lane, then with the lane that holds the other keys of this query
-    float top = -__builtin_inff();
+    if (lds_bad[buf] == t + 1) {
+      // An infinity or NaN among the values of a tile that some query sees in part must not reach the queries that do not
+      // see it (0 * inf).  It is added key by key to the queries that do, then cleared for the product.  The probabilities
+      // wait in the keys' place, which nobody reads any more.
+      __syncthreads();
+      T* lds_p = lds_k[buf] + wave * (BN * 32);
+      if (active) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[n][r]);
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    const float m_new = fmaxf(m, top);
-    const float base = m_new == -__builtin_inff() ? 0.f : m_new * c2;
-    const float alpha = exp2_fast(m * c2 - base);
-    m = m_new;
-    float sum = 0.f;
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[n][r] = exp2_fast(fmaf(s[n][r], c2, -base));
-        sum += s[n][r];
+          for (int r = 0; r < 16; ++r) lds_p[(n * 32 + acc_row(r, half)) * 32 + (lane & 31)] = from_f32<T>(s[n][r]);
       }
-    l = l * alpha + sum;
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
-
-    // An infinity or NaN among the values of a tile that some query sees in part must not reach the queries that do not
-    // see it (0 * inf): the product takes the finite values, then the others are added key by key where they are seen.
-    const bool apart = masked && lds_bad;
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int u = 0; u < USTEPS; ++u) {
-        const Op p = pack_rows<T>(s[n], u);
-#pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          Op w = read_rows<T, HDP>(lds_v, n * 32, u, d * 32, lane);
-          if (apart) w = keep_finite<T>(w, true);
-          o[d] = Mma<T>::run(w, p, o[d]);
-        }
-      }
-    if (apart) {
+      __syncthreads();
+      if (active) {
 #pragma unroll 1
-      for (int key = 0; key < BN; ++key) {
-        const bool seen = key0 + key < limit;
+        for (int key = 0; key < BN && key0 + key < wave_most; ++key) {
+          const float p = to_f32(lds_p[key * 32 + (lane & 31)]);
+          const bool seen = key0 + key < limit;
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          f32x16 one = zero16();
+          for (int d = 0; d < DT; ++d)
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int u = 0; u < USTEPS; ++u) {
-              Op p = pack_rows<T>(s[n], u);
-              Op w = keep_finite<T>(read_rows<T, HDP>(lds_v, n * 32, u, d * 32, lane), false);
-              constexpr int R = sizeof(T) == 2 ? 8 : 4;
-#pragma unroll
-              for (int j = 0; j < R; ++j) {
-                const bool mine = n * 32 + acc_row(u * R + j, half) == key;
-                p[j] = mine ? p[j] : (T)0.f;
-                w[j] = mine ? w[j] : (T)0.f;
-              }
-              one = Mma<T>::run(w, p, one);
+            for (int r = 0; r < 16; ++r) {
+              const float w = to_f32(lds_v[buf][tile_at<T, HDP>(key, d * 32 + acc_row(r, half))]);
+              if (seen && !(__builtin_fabsf(w) < __builtin_inff())) o[d][r] += p * w;
             }
-#pragma unroll
-          for (int r = 0; r < 16; ++r) o[d][r] = seen ? o[d][r] + one[r] : o[d][r];
         }
       }
+      __syncthreads();
+      for (int i = threadIdx.x; i < BN * HDP; i += 256)
+        if (!(__builtin_fabsf(to_f32(lds_v[buf][i])) < __builtin_inff())) lds_v[buf][i] = (T)0.f;
+      __syncthreads();
+    }
+    if (active) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int u = 0; u < USTEPS; ++u) {
+          const Op p = pack_rows<T>(s[n], u);
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+            o[d] = Mma<T>::run(read_rows<T, HDP>(lds_v[buf], n * 32, u, d * 32, lane), p, o[d]);
+        }
+    }
+  };
+
+  if (t_begin < t_end) {
+    __syncthreads();  // lds_bad
+    fetch(t_begin);
+    place_tile(t_begin, 0);
+    __syncthreads();
+    for (int t = t_begin; t < t_end; t += 2) {
+      if (t + 1 < t_end) fetch(t + 1);
+      work(t, Const<0>{});
+      if (t + 1 < t_end) place_tile(t + 1, 1);
+      __syncthreads();
+      if (t + 1 >= t_end) break;
+      if (t + 2 < t_end) fetch(t + 2);
+      work(t + 1, Const<1>{});
+      if (t + 2 < t_end) place_tile(t + 2, 0);
+      __syncthreads();
     }
   }
 
-  l += __shfl_xor(l, 32, 64);
+  l = halves_sum(l);
   if (row >= rows) return;
   if (a.splits == 1) {
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // a NaN sum stays a NaN
-    T* out = static_cast<T*>(a.out) + ((seq.q_off + token) * a.H + head) * a.D;
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int col = d * 32 + 8 * g + 4 * half;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (col + j < a.D) out[col + j] = from_f32<T>(o[d][g * 4 + j] * inv);
-      }
-    if (a.lse && half == 0)
-      a.lse[(seq.q_off + token) * a.H + head] = l == 0.f ? -__builtin_inff() : m * a.scale + logf(l);
+    const int64_t at = (seq.q_off + token) * a.H + head;
+    store_rows<T, DT>(static_cast<T*>(a.out) + at * a.D, o, inv, a.D, half);
+    if (a.lse && half == 0) a.lse[at] = l == 0.f ? -__builtin_inff() : m + log2f(l);
     return;
   }
   const int64_t part = (((int64_t)id * a.KV + kvh) * a.splits + split) * kAttnRows + wave * 32 + (lane & 31);
-  float* po = a.part_o + part * a.D;
-#pragma unroll
-  for (int d = 0; d < DT; ++d)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int col = d * 32 + 8 * g + 4 * half;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (col + j < a.D) po[col + j] = o[d][g * 4 + j];
-    }
+  store_rows<float, DT>(a.part_o + part * a.D, o, 1.f, a.D, half);
   if (half == 0) {
     a.part_ml[part * 2] = m;
     a.part_ml[part * 2 + 1] = l;
@@ -243,14 +244,13 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
   const int row = seq.tile * TILE + at;
   if (row >= seq.q_len * a.G) return;
   const int64_t part = (((int64_t)id * a.KV + kvh) * a.splits) * TILE + at;
-  const float c2 = a.scale * kLog2e;
   float m = -__builtin_inff();
   for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[(part + (int64_t)s * TILE) * 2]);
-  const float base = m == -__builtin_inff() ? 0.f : m * c2;
+  const float base = m == -__builtin_inff() ? 0.f : m;
   float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
   for (int s = 0; s < a.splits; ++s) {
     const int64_t p = part + (int64_t)s * TILE;
-    const float f = exp2_fast(fmaf(a.part_ml[p * 2], c2, -base));
+    const float f = exp2_fast(a.part_ml[p * 2] - base);
     l = fmaf(a.part_ml[p * 2 + 1], f, l);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -261,7 +261,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
 #pragma unroll
   for (int j = 0; j < 4; ++j)
     if (lane + 64 * j < a.D) static_cast<T*>(a.out)[out * a.D + lane + 64 * j] = from_f32<T>(o[j] * inv);
-  if (a.lse && lane == 0) a.lse[out] = l == 0.f ? -__builtin_inff() : m * a.scale + logf(l);
+  if (a.lse && lane == 0) a.lse[out] = l == 0.f ? -__builtin_inff() : m + log2f(l);
 }
 
 // ---- launches ----------------------------------------------------------------------------------------------------------

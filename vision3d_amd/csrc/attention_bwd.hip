@@ -25,15 +25,6 @@ struct AttnBwdArgs {
 template <typename T, int HD>
 constexpr int bwd_keys() { return HD * (int)sizeof(T) > 256 ? 32 : 64; }
 
-template <typename T>
-__device__ __forceinline__ typename Mma<T>::Op load_op(const T* row, int c0, int D, bool live) {
-  const Chunk<T> c = load_chunk<T>(row, c0, D, live);
-  typename Mma<T>::Op op;
-#pragma unroll
-  for (int j = 0; j < 16 / (int)sizeof(T); ++j) op[j] = c.v[j];
-  return op;
-}
-
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void attn_backward_q_kernel(const AttnBwdArgs b) {
   constexpr int HDP = attn_pow2(HD);
@@ -98,7 +89,7 @@ __global__ __launch_bounds__(256) void attn_backward_q_kernel(const AttnBwdArgs 
     for (int j = 0; j < E; ++j) delta = fmaf((float)gf[st][j], (float)of[j], delta);
   }
   delta += __shfl_xor(delta, 32, 64);
-  const float lse = a.lse[at] * kLog2e;
+  const float lse = a.lse[at];
   if (half == 0 && row < rows) b.delta[at] = delta;
 
   const float c2 = a.scale * kLog2e;
@@ -232,7 +223,7 @@ __global__ __launch_bounds__(256) void attn_backward_kv_kernel(const AttnBwdArgs
       const int r = row0 + threadIdx.x;
       const int tok = min(r, rows - 1) / a.G, g = min(r, rows - 1) % a.G;
       const int64_t i = (int64_t)tok * a.H + g;
-      lds_lse[threadIdx.x] = lse[i] * kLog2e;
+      lds_lse[threadIdx.x] = lse[i];
       lds_delta[threadIdx.x] = delta[i];
       // keys that the row sees; a row past the last sees none
       lds_limit[threadIdx.x] = r >= rows ? 0 : a.causal ? max(0, min(seq.s_len, tok + seq.s_len - seq.q_len + 1)) : seq.s_len;

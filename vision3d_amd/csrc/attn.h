@@ -13,6 +13,11 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
+__host__ __device__ constexpr int attn_pow2(int hd) { return hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
+
+constexpr int kAttnWaves = 4;
+constexpr int kAttnRows = 32 * kAttnWaves;  // rows (or keys) of a workgroup's tile
+
 // Element strides throughout.  Rows of the keys: row j of sequence b is at (first row of b + j) * row stride in a pack,
 // at b * batch stride + j * row stride in a cache (`capacity` > 0).
 struct AttnArgs {
@@ -20,7 +25,7 @@ struct AttnArgs {
   const void* k;
   const void* v;
   void* out;                 // (total_q, H, D) contiguous
-  float* lse;                // (total_q, H) natural log of the sum of exponentials, -inf for a row without keys; or NULL
+  float* lse;                // (total_q, H) log2 of the sum of exponentials, -inf for a row without keys; or NULL
   const int64_t* q_lengths;  // (B), NULL in a cache: every sequence has `tokens` queries
   const int64_t* s_lengths;  // (B)
   int64_t total_q, total_s;
@@ -32,7 +37,7 @@ struct AttnArgs {
   int causal;
   int splits;                // parts that the keys of a row tile are divided into
   float* part_o;             // splits > 1: (tile, KV, split, rows of a tile, D) unnormalised rows ...
-  float* part_ml;            // ... and (tile, KV, split, rows of a tile, 2): maximum (of the unscaled scores) and sum
+  float* part_ml;            // ... and (tile, KV, split, rows of a tile, 2): maximum (of scale * log2(e) * score) and sum
 };
 
 // A workgroup's sequence.  All fields are wave-uniform.
@@ -197,17 +202,51 @@ __device__ __forceinline__ Chunk<T> load_chunk(const T* row, int c0, int D, bool
   return c;
 }
 
-// Whether a chunk holds an infinity or a NaN.
-template <typename T>
-__device__ __forceinline__ bool chunk_nonfinite(const Chunk<T>& c) {
-  bool bad = false;
+// A tile of ROWS rows on its way from memory to LDS: 256 threads, CH chunks of 16 bytes each, in registers.
+template <typename T, int HD, int ROWS>
+struct TileStage {
+  static constexpr int E = 16 / (int)sizeof(T);
+  static constexpr int CPR = HD / E;                // chunks of a row
+  static constexpr int CH = ROWS * CPR / 256;
+  static_assert(ROWS * CPR % 256 == 0, "whole chunks per thread");
+  Chunk<T> c[CH];
+
+  static __device__ __forceinline__ int row_of(int i) { return (i * 256 + (int)threadIdx.x) / CPR; }
+  static __device__ __forceinline__ int col_of(int i) { return (i * 256 + (int)threadIdx.x) % CPR * E; }
+
+  // Rows [0, count) of those at `base`; the others, and columns from D on, are zeros.
+  __device__ __forceinline__ void fetch(const T* base, int64_t stride, int D, int count) {
+    if (count >= ROWS && D == HD) {
 #pragma unroll
-  for (int j = 0; j < 16 / (int)sizeof(T); ++j) {
-    const float f = to_f32(c.v[j]);
-    bad |= !(__builtin_fabsf(f) < __builtin_inff());
+      for (int i = 0; i < CH; ++i) {
+        const Packed<T, E> p = *reinterpret_cast<const Packed<T, E>*>(base + row_of(i) * stride + col_of(i));
+#pragma unroll
+        for (int j = 0; j < E; ++j) c[i].v[j] = p.v[j];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < CH; ++i) c[i] = load_chunk<T>(base + row_of(i) * stride, col_of(i), D, row_of(i) < count);
+    }
   }
-  return bad;
-}
+  __device__ __forceinline__ void store(T* tile) const {
+    constexpr int HDP = attn_pow2(HD);
+#pragma unroll
+    for (int i = 0; i < CH; ++i) *reinterpret_cast<Chunk<T>*>(tile + tile_at<T, HDP>(row_of(i), col_of(i))) = c[i];
+  }
+  __device__ __forceinline__ bool nonfinite() const {
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+#pragma unroll
+      for (int j = 0; j < E; ++j) bad |= !(__builtin_fabsf(to_f32(c[i].v[j])) < __builtin_inff());
+    return bad;
+  }
+};
+
+template <int N>
+struct Const {
+  static constexpr int value = N;
+};
 
 // ---- matrix instructions -----------------------------------------------------------------------------------------------
 // Everything is built on the 32 x 32 result layout: lane l holds column l % 32, register r holds row
@@ -299,19 +338,46 @@ __device__ __forceinline__ typename Mma<T>::Op pack_rows(const f32x16& p, int u)
   return op;
 }
 
-// The finite values of an operand, the others as zeros (`finite`), or the other way round.
+// Elements [c0, c0 + E) of a row in memory as an operand; zeros past D.
 template <typename T>
-__device__ __forceinline__ typename Mma<T>::Op keep_finite(typename Mma<T>::Op op, bool finite) {
+__device__ __forceinline__ typename Mma<T>::Op load_op(const T* row, int c0, int D, bool live) {
+  const Chunk<T> c = load_chunk<T>(row, c0, D, live);
+  typename Mma<T>::Op op;
 #pragma unroll
-  for (int j = 0; j < 16 / (int)sizeof(T); ++j) {
-    const bool is = __builtin_fabsf(to_f32((T)op[j])) < __builtin_inff();
-    op[j] = is == finite ? op[j] : (T)0.f;
-  }
+  for (int j = 0; j < 16 / (int)sizeof(T); ++j) op[j] = c.v[j];
   return op;
 }
 
+// A result whose column is this lane's row and whose rows are the row's elements, times `f`, to memory.
+template <typename T, int DT>
+__device__ __forceinline__ void store_rows(T* row, const f32x16 (&acc)[DT], float f, int D, int half) {
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int col = d * 32 + 8 * g + 4 * half;
+      const float v[4] = {acc[d][g * 4] * f, acc[d][g * 4 + 1] * f, acc[d][g * 4 + 2] * f, acc[d][g * 4 + 3] * f};
+      if (col + 4 <= D) {
+        store_vec<T, 4>(row + col, v);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (col + j < D) row[col + j] = from_f32<T>(v[j]);
+      }
+    }
+}
+
+// Over the two lanes (l, l + 32) of a column, without LDS.
+__device__ __forceinline__ float halves_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float halves_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr float kLn2 = 0.69314718055994530942f;
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }  // v_exp_f32; 2^-inf = 0
 
@@ -321,11 +387,6 @@ __device__ __forceinline__ f32x16 zero16() {
   for (int r = 0; r < 16; ++r) z[r] = 0.f;
   return z;
 }
-
-__host__ __device__ constexpr int attn_pow2(int hd) { return hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
-
-constexpr int kAttnWaves = 4;
-constexpr int kAttnRows = 32 * kAttnWaves;  // rows (or keys) of a workgroup's tile
 
 // Host side: the argument checks of every entry point (attention.hip).
 int attn_check(const char* what, int dtype, int B, int64_t total_q, int64_t total_s, int H, int KV, int D, float scale);
