@@ -462,7 +462,8 @@ int v3d_layer_norm_bwd(const void* grad, const void* feats, const void* residual
  * lse (total_q,H) fp32 = log2 of the row's sum of exp(score) (-inf without keys), what the backward needs; or NULL.
  * `strides` (host array, elements): q row, q head, k row, k head, v row, v head -- the last dimension is contiguous, rows
  * need no alignment.  Products of 16-bit types are exact, the probabilities are rounded to the type before they meet the
- * values; scores, statistics and sums are fp32.  D <= V3D_ATTENTION_MAX_HEAD_SIZE, 0 < scale < inf.
+ * values; scores, statistics and sums are fp32.  16 bytes <= D <= V3D_ATTENTION_MAX_HEAD_SIZE, 0 < scale < inf; strides are not
+ * negative, key rows do not overlap (a stride of 0 is fine) and 129 token (or key) rows, plus a group's heads, span less than 2^29 elements.
  *
  * v3d_cached_attention: q (B,tokens,H,D) = the newest `tokens` tokens of every sequence, k_cache / v_cache
  * (B,capacity,KV,D), lengths (B) i64 = filled rows, the new ones among them (cut to [0, capacity]): token t sees the rows

@@ -328,6 +328,7 @@ def test_refusals_without_a_gpu():
 
     assert pack(dtype=5) == -1 and pack(h=3, kv=2) == -1 and pack(d=0) == -1 and pack(b=-1) == -1
     assert pack(scale=0.0) == -1 and pack(scale=float("nan")) == -1 and pack() == -1  # null pointers
+    assert pack(d=7) == -1 and pack(dtype=0, d=3) == -1  # less than 16 bytes
     assert pack(d=257) == -4 and pack(nq=1 << 30) == -4 and pack(ns=(1 << 30) + 1) == -4
     assert pack(nq=0) == 0
     # the workspace is asked for only where the keys are divided

@@ -21,7 +21,6 @@ __global__ __launch_bounds__(256, HD * sizeof(T) <= 256 ? 2 : 1) void attn_forwa
   constexpr int HDP = attn_pow2(HD);
   constexpr int BN = attn_keys<T, HD>();
   constexpr int NT = BN / 32;                       // 32-key blocks of a tile
-  constexpr int E = 16 / (int)sizeof(T);
   constexpr int STEPS = HD / Mma<T>::kStep;         // product steps over the head size
   constexpr int USTEPS = 32 / Mma<T>::kStep;        // product steps over a 32-key block
   constexpr int DT = HD / 32;
@@ -36,7 +35,7 @@ __global__ __launch_bounds__(256, HD * sizeof(T) <= 256 ? 2 : 1) void attn_forwa
   const int kvh = (int)(id % a.KV);
   id /= a.KV;
   const int split = (int)(id % a.splits);
-  id /= a.splits;
+  id = (int64_t)(gridDim.x / (a.KV * a.splits)) - 1 - id / a.splits;  // causal: the longest tiles of a sequence start first
   const AttnSeq seq = locate_rows<kAttnRows>(a, id);
   if (!seq.found) {  // the launch covers a bound: the rest of it clears the rows behind the last sequence
     if (a.capacity == 0 && split == 0) {
@@ -54,30 +53,27 @@ __global__ __launch_bounds__(256, HD * sizeof(T) <= 256 ? 2 : 1) void attn_forwa
   const int rows = seq.q_len * a.G;
   if (seq.tile * kAttnRows >= rows) return;  // lengths that overrun the total were cut
   const int row = seq.tile * kAttnRows + wave * 32 + (lane & 31);
-  const int token = min(row, rows - 1) / a.G;
-  const int head = kvh * a.G + min(row, rows - 1) % a.G;
-  auto limit_of = [&](int tok) {
-    return a.causal ? max(0, min(seq.s_len, tok + seq.s_len - seq.q_len + 1)) : seq.s_len;
-  };
-  const int limit = limit_of(token);  // this lane's query sees keys [0, limit)
+  const int token = div_g(a, min(row, rows - 1));
+  const int head = kvh * a.G + min(row, rows - 1) - token * a.G;
+  const int limit = attn_limit(a, seq, token);  // this lane's query sees keys [0, limit)
   // the wave's and the workgroup's first and last rows bound what they have to look at
   const bool wave_live = seq.tile * kAttnRows + wave * 32 < rows;
   const int wave_least = __builtin_amdgcn_readfirstlane(limit);
-  const int wave_most = wave_live ? limit_of(min(seq.tile * kAttnRows + wave * 32 + 31, rows - 1) / a.G) : 0;
-  const int most = limit_of(min(seq.tile * kAttnRows + kAttnRows - 1, rows - 1) / a.G);
-  const int least = limit_of(min(seq.tile * kAttnRows, rows - 1) / a.G);
+  const int wave_most = wave_live ? attn_limit(a, seq, div_g(a, min(seq.tile * kAttnRows + wave * 32 + 31, rows - 1))) : 0;
+  const int most = attn_limit(a, seq, div_g(a, min(seq.tile * kAttnRows + kAttnRows - 1, rows - 1)));
+  const int least = attn_limit(a, seq, div_g(a, min(seq.tile * kAttnRows, rows - 1)));
 
   const int tiles = (most + BN - 1) / BN;
   const int per_split = (tiles + a.splits - 1) / a.splits;
   const int t_begin = split * per_split, t_end = min(tiles, t_begin + per_split);
 
-  const T* q = static_cast<const T*>(a.q) + (seq.q_off + token) * a.q_row + (int64_t)head * a.q_head;
+  const int token0 = div_g(a, seq.tile * kAttnRows);
+  const T* q = static_cast<const T*>(a.q) + (seq.q_off + token0) * a.q_row + (int64_t)kvh * a.G * a.q_head;
   const T* k = static_cast<const T*>(a.k) + seq.b * a.k_batch + seq.s_off * a.k_row + (int64_t)kvh * a.k_head;
   const T* v = static_cast<const T*>(a.v) + seq.b * a.v_batch + seq.s_off * a.v_row + (int64_t)kvh * a.v_head;
 
   Op qf[STEPS];
-#pragma unroll
-  for (int st = 0; st < STEPS; ++st) qf[st] = load_op<T>(q, st * 2 * E + E * half, a.D, true);
+  load_ops<T>(qf, q, (token - token0) * (int)a.q_row + (head - kvh * a.G) * (int)a.q_head, half, a.D);
 
   // The tile after the one that is worked on is on its way in registers meanwhile.
   TileStage<T, HD, BN> stage_k, stage_v;
@@ -87,8 +83,8 @@ __global__ __launch_bounds__(256, HD * sizeof(T) <= 256 ? 2 : 1) void attn_forwa
     stage_v.fetch(v + (int64_t)t * BN * a.v_row, a.v_row, a.D, seq.s_len - t * BN);
   };
   auto place_tile = [&](int t, int buf) {
-    stage_k.store(lds_k[buf]);
-    stage_v.store(lds_v[buf]);
+    stage_k.store(lds_k[buf], a.D);
+    stage_v.store(lds_v[buf], a.D);
     // values of a tile that some query sees in part: see below
     if (t * BN + BN > least && stage_v.nonfinite()) lds_bad[buf] = t + 1;
   };
@@ -257,7 +253,8 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
       if (lane + 64 * j < a.D) o[j] = fmaf(a.part_o[p * a.D + lane + 64 * j], f, o[j]);
   }
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-  const int64_t out = (seq.q_off + row / a.G) * a.H + (int64_t)kvh * a.G + row % a.G;
+  const int token = div_g(a, row);
+  const int64_t out = (seq.q_off + token) * a.H + (int64_t)kvh * a.G + row - token * a.G;
 #pragma unroll
   for (int j = 0; j < 4; ++j)
     if (lane + 64 * j < a.D) static_cast<T*>(a.out)[out * a.D + lane + 64 * j] = from_f32<T>(o[j] * inv);
@@ -311,6 +308,7 @@ int attn_check(const char* what, int dtype, int B, int64_t total_q, int64_t tota
   V3D_REQUIRE(dtype == V3D_F32 || dtype == V3D_F16 || dtype == V3D_BF16, what, "unknown element type");
   V3D_REQUIRE(B >= 0 && total_q >= 0 && total_s >= 0 && H >= 1 && KV >= 1 && D >= 1, what, "bad shape");
   V3D_REQUIRE(H % KV == 0, what, "the query heads must be a multiple of the key heads");
+  V3D_REQUIRE(D >= (dtype == V3D_F32 ? 4 : 8), what, "a head has at least 16 bytes");
   V3D_REQUIRE(scale > 0.f && scale < __builtin_inff(), what, "the scale must be positive and finite");
   if (D > V3D_ATTENTION_MAX_HEAD_SIZE) {
     set_last_error("%s: head size %d, at most %d", what, D, V3D_ATTENTION_MAX_HEAD_SIZE);
@@ -324,8 +322,26 @@ int attn_check(const char* what, int dtype, int B, int64_t total_q, int64_t tota
   return 0;
 }
 
+// A tile's rows are addressed by 32-bit byte offsets from the tile's first row: at most 128 rows of a key tensor, at most
+// 129 tokens and the heads of a group of a query tensor.
+int attn_check_strides(const char* what, const AttnArgs& a) {
+  const int64_t reach = (int64_t)1 << 29;  // elements of 4 bytes
+  auto fits = [&](int64_t row, int64_t head) {
+    return row >= 0 && head >= 0 && row < reach / 130 && head < reach / (2 * a.G) && 129 * row + a.G * head + a.D < reach;
+  };
+  if (!fits(a.q_row, a.q_head) || !fits(a.k_row, 0) || !fits(a.v_row, 0) || !fits((int64_t)a.H * a.D, a.D)) {
+    set_last_error("%s: strides of a query or key row beyond 32-bit tile offsets", what);
+    return V3D_ERR_SIZE_LIMIT;
+  }
+  V3D_REQUIRE((a.k_row == 0 || a.k_row >= a.D) && (a.v_row == 0 || a.v_row >= a.D), what, "key rows overlap");
+  V3D_REQUIRE(a.k_head >= 0 && a.v_head >= 0 && a.k_batch >= 0 && a.v_batch >= 0, what, "negative stride");
+  return 0;
+}
+
 int attn_forward_run(AttnArgs& a, int dtype, const AttnPlan& plan, void* workspace, size_t workspace_bytes, int device,
                      void* stream, const char* what) {
+  const int bad = attn_check_strides(what, a);
+  if (bad != 0) return bad;
   if (plan.tiles * a.KV * plan.splits > ((int64_t)1 << 31) / 64) {
     set_last_error("%s: too many tiles", what);
     return V3D_ERR_SIZE_LIMIT;
@@ -384,10 +400,7 @@ int v3d_attention_pack_fwd(const void* q, const void* k, const void* v, const in
   a.v_row = strides[4];
   a.v_head = strides[5];
   a.B = B;
-  a.H = H;
-  a.KV = KV;
-  a.G = H / KV;
-  a.D = D;
+  attn_heads(a, H, KV, D);
   a.scale = scale;
   a.causal = causal;
   return attn_forward_run(a, dtype, attn_plan(B, total_q, total_s, 0, KV, a.G, D), workspace, workspace_bytes, device,
@@ -428,10 +441,7 @@ int v3d_cached_attention(const void* q, const void* k_cache, const void* v_cache
   a.capacity = capacity;
   a.tokens = tokens;
   a.B = B;
-  a.H = H;
-  a.KV = KV;
-  a.G = H / KV;
-  a.D = D;
+  attn_heads(a, H, KV, D);
   a.scale = scale;
   a.causal = 1;
   return attn_forward_run(a, dtype, attn_plan(B, a.total_q, capacity, tokens, KV, a.G, D), workspace, workspace_bytes,

@@ -22,28 +22,28 @@ struct AttnBwdArgs {
   void* dv;
 };
 
+// Keys (or rows) of a tile that passes by; two of them, of two tensors, in LDS.
 template <typename T, int HD>
-constexpr int bwd_keys() { return HD * (int)sizeof(T) > 256 ? 32 : 64; }
+constexpr int bwd_tile() { return HD * (int)sizeof(T) > 128 ? 32 : 64; }
 
 template <typename T, int HD>
-__global__ __launch_bounds__(256) void attn_backward_q_kernel(const AttnBwdArgs b) {
+__global__ __launch_bounds__(256, HD * sizeof(T) <= 256 ? 2 : 1) void attn_backward_q_kernel(const AttnBwdArgs b) {
   constexpr int HDP = attn_pow2(HD);
-  constexpr int BN = bwd_keys<T, HD>();
+  constexpr int BN = bwd_tile<T, HD>();
   constexpr int NT = BN / 32;
-  constexpr int E = 16 / (int)sizeof(T);
   constexpr int STEPS = HD / Mma<T>::kStep;
   constexpr int USTEPS = 32 / Mma<T>::kStep;
   constexpr int DT = HD / 32;
   typedef typename Mma<T>::Op Op;
-  __shared__ T lds_k[BN * HDP];
-  __shared__ T lds_v[BN * HDP];
+  __shared__ T lds_k[2][BN * HDP];
+  __shared__ T lds_v[2][BN * HDP];
 
   const AttnArgs& a = b.f;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int half = lane >> 5;
   int64_t id = blockIdx.x;
   const int kvh = (int)(id % a.KV);
-  id /= a.KV;
+  id = (int64_t)(gridDim.x / a.KV) - 1 - id / a.KV;  // causal: the longest tiles of a sequence start first
   const AttnSeq seq = locate<kAttnRows, false>(a, id);
   T* dq = static_cast<T*>(b.dq);
   if (!seq.found) {  // rows behind the last sequence have no gradient
@@ -57,38 +57,48 @@ __global__ __launch_bounds__(256) void attn_backward_q_kernel(const AttnBwdArgs 
     return;
   }
   const int rows = seq.q_len * a.G;
-  if (seq.tile * kAttnRows >= rows) return;  // lengths that overrun the total were cut
-  const int row = seq.tile * kAttnRows + wave * 32 + (lane & 31);
-  const int token = min(row, rows - 1) / a.G;
-  const int head = kvh * a.G + min(row, rows - 1) % a.G;
-  auto limit_of = [&](int tok) {
-    return a.causal ? max(0, min(seq.s_len, tok + seq.s_len - seq.q_len + 1)) : seq.s_len;
-  };
-  const int limit = limit_of(token);
-  const bool wave_live = seq.tile * kAttnRows + wave * 32 < rows;
-  const int wave_least = limit_of(min(seq.tile * kAttnRows + wave * 32, rows - 1) / a.G);
-  const int wave_most = wave_live ? limit_of(min(seq.tile * kAttnRows + wave * 32 + 31, rows - 1) / a.G) : 0;
-  const int most = limit_of(min(seq.tile * kAttnRows + kAttnRows - 1, rows - 1) / a.G);
+  const int row0 = seq.tile * kAttnRows;
+  if (row0 >= rows) return;  // lengths that overrun the total were cut
+  const int row = row0 + wave * 32 + (lane & 31);
+  const int token = div_g(a, min(row, rows - 1));
+  const int head = kvh * a.G + min(row, rows - 1) - token * a.G;
+  const int limit = attn_limit(a, seq, token);
+  const int wave_least = __builtin_amdgcn_readfirstlane(limit);
+  const int wave_most =
+      row0 + wave * 32 < rows ? attn_limit(a, seq, div_g(a, min(row0 + wave * 32 + 31, rows - 1))) : 0;
+  const int most = attn_limit(a, seq, div_g(a, min(row0 + kAttnRows - 1, rows - 1)));
 
-  const T* q = static_cast<const T*>(a.q) + (seq.q_off + token) * a.q_row + (int64_t)head * a.q_head;
+  const int token0 = div_g(a, row0);
+  const T* q = static_cast<const T*>(a.q) + (seq.q_off + token0) * a.q_row + (int64_t)kvh * a.G * a.q_head;
   const T* k = static_cast<const T*>(a.k) + seq.s_off * a.k_row + (int64_t)kvh * a.k_head;
   const T* v = static_cast<const T*>(a.v) + seq.s_off * a.v_row + (int64_t)kvh * a.v_head;
   const int64_t at = (seq.q_off + token) * a.H + head;
-  const T* out = static_cast<const T*>(a.out) + at * a.D;
-  const T* grad = static_cast<const T*>(b.grad) + at * a.D;
+  const int64_t at0 = ((seq.q_off + token0) * a.H + (int64_t)kvh * a.G) * a.D;
+  const int at_row = (int)(at * a.D - at0);
+
+  TileStage<T, HD, BN> stage_k, stage_v;
+  auto fetch = [&](int t) {
+    stage_k.fetch(k + (int64_t)t * BN * a.k_row, a.k_row, a.D, seq.s_len - t * BN);
+    stage_v.fetch(v + (int64_t)t * BN * a.v_row, a.v_row, a.D, seq.s_len - t * BN);
+  };
+  auto place_tile = [&](int buf) {
+    stage_k.store(lds_k[buf], a.D);
+    stage_v.store(lds_v[buf], a.D);
+  };
 
   Op qf[STEPS], gf[STEPS];
   float delta = 0.f;
+  load_ops<T>(qf, q, (token - token0) * (int)a.q_row + (head - kvh * a.G) * (int)a.q_head, half, a.D);
+  load_ops<T>(gf, static_cast<const T*>(b.grad) + at0, at_row, half, a.D);
+  {
+    Op of[STEPS];
+    load_ops<T>(of, static_cast<const T*>(a.out) + at0, at_row, half, a.D);
 #pragma unroll
-  for (int st = 0; st < STEPS; ++st) {
-    const int c0 = st * 2 * E + E * half;
-    qf[st] = load_op<T>(q, c0, a.D, true);
-    gf[st] = load_op<T>(grad, c0, a.D, true);
-    const Op of = load_op<T>(out, c0, a.D, true);
+    for (int st = 0; st < STEPS; ++st)
 #pragma unroll
-    for (int j = 0; j < E; ++j) delta = fmaf((float)gf[st][j], (float)of[j], delta);
+      for (int j = 0; j < 16 / (int)sizeof(T); ++j) delta = fmaf((float)gf[st][j], (float)of[st][j], delta);
   }
-  delta += __shfl_xor(delta, 32, 64);
+  delta = halves_sum(delta);
   const float lse = a.lse[at];
   if (half == 0 && row < rows) b.delta[at] = delta;
 
@@ -97,70 +107,68 @@ __global__ __launch_bounds__(256) void attn_backward_q_kernel(const AttnBwdArgs 
 #pragma unroll
   for (int d = 0; d < DT; ++d) acc[d] = zero16();
 
-  const int tiles = (most + BN - 1) / BN;
-  for (int t = 0; t < tiles; ++t) {
+  auto work = [&](int t, auto buffer) {
+    constexpr int buf = decltype(buffer)::value;
     const int key0 = t * BN;
-    __syncthreads();
-    constexpr int CPR = HD / E;
-    for (int i = threadIdx.x; i < BN * CPR; i += 256) {
-      const int r = i / CPR, c = i % CPR;
-      const bool live = key0 + r < seq.s_len;
-      *reinterpret_cast<Chunk<T>*>(lds_k + tile_at<T, HDP>(r, c * E)) =
-          load_chunk<T>(k + (int64_t)(key0 + r) * a.k_row, c * E, a.D, live);
-      *reinterpret_cast<Chunk<T>*>(lds_v + tile_at<T, HDP>(r, c * E)) =
-          load_chunk<T>(v + (int64_t)(key0 + r) * a.v_row, c * E, a.D, live);
-    }
-    __syncthreads();
-    if (key0 >= wave_most) continue;
-    const bool masked = key0 + BN > wave_least;
+    if (key0 >= wave_most) return;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       f32x16 s = zero16(), dp = zero16();
 #pragma unroll
       for (int st = 0; st < STEPS; ++st) {
-        s = Mma<T>::run(read_cols<T, HDP>(lds_k, n * 32 + (lane & 31), st, half), qf[st], s);
-        dp = Mma<T>::run(read_cols<T, HDP>(lds_v, n * 32 + (lane & 31), st, half), gf[st], dp);
+        s = Mma<T>::run(read_cols<T, HDP>(lds_k[buf], n * 32 + (lane & 31), st, half), qf[st], s);
+        dp = Mma<T>::run(read_cols<T, HDP>(lds_v[buf], n * 32 + (lane & 31), st, half), gf[st], dp);
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float p = exp2_fast(fmaf(s[r], c2, -lse));
-        const bool seen = !masked || key0 + n * 32 + acc_row(r, half) < limit;
-        s[r] = seen ? p * (dp[r] - delta) : 0.f;
+      for (int r = 0; r < 16; ++r) s[r] = exp2_fast(fmaf(s[r], c2, -lse)) * (dp[r] - delta);
+      if (key0 + BN > wave_least) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (key0 + n * 32 + acc_row(r, half) >= limit) s[r] = 0.f;
       }
 #pragma unroll
       for (int u = 0; u < USTEPS; ++u) {
         const Op ds = pack_rows<T>(s, u);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) acc[d] = Mma<T>::run(read_rows<T, HDP>(lds_k, n * 32, u, d * 32, lane), ds, acc[d]);
+        for (int d = 0; d < DT; ++d)
+          acc[d] = Mma<T>::run(read_rows<T, HDP>(lds_k[buf], n * 32, u, d * 32, lane), ds, acc[d]);
       }
     }
+  };
+
+  const int tiles = (most + BN - 1) / BN;
+  if (tiles > 0) {
+    fetch(0);
+    place_tile(0);
+    __syncthreads();
+    for (int t = 0; t < tiles; t += 2) {
+      if (t + 1 < tiles) fetch(t + 1);
+      work(t, Const<0>{});
+      if (t + 1 < tiles) place_tile(1);
+      __syncthreads();
+      if (t + 1 >= tiles) break;
+      if (t + 2 < tiles) fetch(t + 2);
+      work(t + 1, Const<1>{});
+      if (t + 2 < tiles) place_tile(0);
+      __syncthreads();
+    }
   }
-  if (row >= rows) return;
-#pragma unroll
-  for (int d = 0; d < DT; ++d)
-#pragma unroll
-    for (int g = 0; g < 4; ++g)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int col = d * 32 + 8 * g + 4 * half + j;
-        if (col < a.D) dq[at * a.D + col] = from_f32<T>(acc[d][g * 4 + j] * a.scale);
-      }
+  if (row < rows) store_rows<T, DT>(dq + at * a.D, acc, a.scale, a.D, half);
 }
 
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void attn_backward_kv_kernel(const AttnBwdArgs b) {
   constexpr int HDP = attn_pow2(HD);
-  constexpr int BM = bwd_keys<T, HD>();  // rows of a tile that passes by
+  constexpr int BM = bwd_tile<T, HD>();
   constexpr int NT = BM / 32;
-  constexpr int E = 16 / (int)sizeof(T);
   constexpr int STEPS = HD / Mma<T>::kStep;
   constexpr int USTEPS = 32 / Mma<T>::kStep;
   constexpr int DT = HD / 32;
   typedef typename Mma<T>::Op Op;
-  __shared__ T lds_q[BM * HDP];
-  __shared__ T lds_g[BM * HDP];
-  __shared__ float lds_lse[BM], lds_delta[BM];
-  __shared__ int lds_limit[BM];
+  __shared__ T lds_q[2][BM * HDP];
+  __shared__ T lds_g[2][BM * HDP];
+  __shared__ float lds_lse[2][BM], lds_delta[2][BM];
+  __shared__ int lds_limit[2][BM];
 
   const AttnArgs& a = b.f;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -179,98 +187,120 @@ __global__ __launch_bounds__(256) void attn_backward_kv_kernel(const AttnBwdArgs
     }
     return;
   }
-  if (seq.tile * kAttnRows >= seq.s_len) return;  // cut
-  const int key = seq.tile * kAttnRows + wave * 32 + (lane & 31);
+  const int key0 = seq.tile * kAttnRows;
+  if (key0 >= seq.s_len) return;  // cut
+  const int wave_key = key0 + wave * 32;
+  const int key = wave_key + (lane & 31);
   const bool live = key < seq.s_len;
   const int rows = seq.q_len * a.G;
-  // rows that see the tile's first key: tokens from (first key) - (s_len - q_len) on
-  const int key0 = seq.tile * kAttnRows;
-  const int token0 = a.causal ? max(0, key0 - (seq.s_len - seq.q_len)) : 0;
-  const int wave_key = key0 + wave * 32;
-  const int wave_token0 = a.causal ? max(0, wave_key - (seq.s_len - seq.q_len)) : 0;
+  // rows that see a key: tokens from key - (s_len - q_len) on
+  const int first = a.causal ? max(0, key0 - (seq.s_len - seq.q_len)) * a.G : 0;
+  const int wave_first = a.causal ? max(0, wave_key - (seq.s_len - seq.q_len)) * a.G : 0;
 
-  const T* k = static_cast<const T*>(a.k) + (seq.s_off + min(key, seq.s_len - 1)) * a.k_row + (int64_t)kvh * a.k_head;
-  const T* v = static_cast<const T*>(a.v) + (seq.s_off + min(key, seq.s_len - 1)) * a.v_row + (int64_t)kvh * a.v_head;
-  Op kf[STEPS], vf[STEPS];
-#pragma unroll
-  for (int st = 0; st < STEPS; ++st) {
-    kf[st] = load_op<T>(k, st * 2 * E + E * half, a.D, live);
-    vf[st] = load_op<T>(v, st * 2 * E + E * half, a.D, live);
-  }
-  const float c2 = a.scale * kLog2e;
-  f32x16 ak[DT], av[DT];
-#pragma unroll
-  for (int d = 0; d < DT; ++d) ak[d] = av[d] = zero16();
-
+  const T* k = static_cast<const T*>(a.k) + (seq.s_off + key0) * a.k_row + (int64_t)kvh * a.k_head;
+  const T* v = static_cast<const T*>(a.v) + (seq.s_off + key0) * a.v_row + (int64_t)kvh * a.v_head;
   const T* q = static_cast<const T*>(a.q) + seq.q_off * a.q_row + (int64_t)kvh * a.G * a.q_head;
   const T* grad = static_cast<const T*>(b.grad) + (seq.q_off * a.H + (int64_t)kvh * a.G) * a.D;
   const float* lse = a.lse + seq.q_off * a.H + kvh * a.G;
   const float* delta = b.delta + seq.q_off * a.H + kvh * a.G;
 
-  for (int row0 = token0 * a.G / BM * BM; row0 < rows; row0 += BM) {
-    __syncthreads();
-    constexpr int CPR = HD / E;
-    for (int i = threadIdx.x; i < BM * CPR; i += 256) {
-      const int r = i / CPR, c = i % CPR;
-      const bool in = row0 + r < rows;
-      const int tok = min(row0 + r, rows - 1) / a.G, g = min(row0 + r, rows - 1) % a.G;
-      *reinterpret_cast<Chunk<T>*>(lds_q + tile_at<T, HDP>(r, c * E)) =
-          load_chunk<T>(q + tok * a.q_row + g * a.q_head, c * E, a.D, in);
-      *reinterpret_cast<Chunk<T>*>(lds_g + tile_at<T, HDP>(r, c * E)) =
-          load_chunk<T>(grad + ((int64_t)tok * a.H + g) * a.D, c * E, a.D, in);
-    }
+  TileStage<T, HD, BM> stage_q, stage_g;
+  float stage_lse = 0.f, stage_delta = 0.f;
+  int stage_limit = 0;
+  auto fetch = [&](int row0) {
+    const int tok0 = div_g(a, row0);
+    stage_q.fetch_at(q + tok0 * a.q_row, [&](int r) {
+      const int tok = div_g(a, row0 + r);
+      return (tok - tok0) * (int)a.q_row + (row0 + r - tok * a.G) * (int)a.q_head;
+    }, a.D, rows - row0);
+    stage_g.fetch_at(grad + (int64_t)tok0 * a.H * a.D, [&](int r) {
+      const int tok = div_g(a, row0 + r);
+      return ((tok - tok0) * a.H + (row0 + r - tok * a.G)) * a.D;
+    }, a.D, rows - row0);
     if (threadIdx.x < BM) {
-      const int r = row0 + threadIdx.x;
-      const int tok = min(r, rows - 1) / a.G, g = min(r, rows - 1) % a.G;
-      const int64_t i = (int64_t)tok * a.H + g;
-      lds_lse[threadIdx.x] = lse[i];
-      lds_delta[threadIdx.x] = delta[i];
-      // keys that the row sees; a row past the last sees none
-      lds_limit[threadIdx.x] = r >= rows ? 0 : a.causal ? max(0, min(seq.s_len, tok + seq.s_len - seq.q_len + 1)) : seq.s_len;
+      const int r = min(row0 + (int)threadIdx.x, rows - 1);
+      const int tok = div_g(a, r);
+      const int64_t i = (int64_t)tok * a.H + (r - tok * a.G);
+      stage_lse = lse[i];
+      stage_delta = delta[i];
+      stage_limit = row0 + (int)threadIdx.x < rows ? attn_limit(a, seq, tok) : 0;  // a row past the last sees no key
     }
-    __syncthreads();
-    if (wave_key >= seq.s_len || row0 + BM <= wave_token0 * a.G) continue;
+  };
+  auto place_tile = [&](int buf) {
+    stage_q.store(lds_q[buf], a.D);
+    stage_g.store(lds_g[buf], a.D);
+    if (threadIdx.x < BM) {
+      lds_lse[buf][threadIdx.x] = stage_lse;
+      lds_delta[buf][threadIdx.x] = stage_delta;
+      lds_limit[buf][threadIdx.x] = stage_limit;
+    }
+  };
+
+  Op kf[STEPS], vf[STEPS];
+  load_ops<T>(kf, k, live ? (key - key0) * (int)a.k_row : -1, half, a.D);
+  load_ops<T>(vf, v, live ? (key - key0) * (int)a.v_row : -1, half, a.D);
+  const float c2 = a.scale * kLog2e;
+  f32x16 ak[DT], av[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d) ak[d] = av[d] = zero16();
+
+  auto work = [&](int row0, auto buffer) {
+    constexpr int buf = decltype(buffer)::value;
+    if (wave_key >= seq.s_len || row0 + BM <= wave_first) return;
+    // every row of the tile sees every key of the wave: the first row's limit is the least
+    const bool whole = row0 + BM <= rows && wave_key + 32 <= __builtin_amdgcn_readfirstlane(lds_limit[buf][0]);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       f32x16 s = zero16(), dp = zero16();
 #pragma unroll
       for (int st = 0; st < STEPS; ++st) {
-        s = Mma<T>::run(read_cols<T, HDP>(lds_q, n * 32 + (lane & 31), st, half), kf[st], s);
-        dp = Mma<T>::run(read_cols<T, HDP>(lds_g, n * 32 + (lane & 31), st, half), vf[st], dp);
+        s = Mma<T>::run(read_cols<T, HDP>(lds_q[buf], n * 32 + (lane & 31), st, half), kf[st], s);
+        dp = Mma<T>::run(read_cols<T, HDP>(lds_g[buf], n * 32 + (lane & 31), st, half), vf[st], dp);
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int i = n * 32 + acc_row(r, half);
-        const bool seen = key < lds_limit[i];
-        const float p = exp2_fast(fmaf(s[r], c2, -lds_lse[i]));
-        s[r] = seen ? p : 0.f;
-        dp[r] = seen ? p * (dp[r] - lds_delta[i]) : 0.f;
+        s[r] = exp2_fast(fmaf(s[r], c2, -lds_lse[buf][i]));
+        dp[r] = s[r] * (dp[r] - lds_delta[buf][i]);
+      }
+      if (!whole) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (key >= lds_limit[buf][n * 32 + acc_row(r, half)]) s[r] = dp[r] = 0.f;
       }
 #pragma unroll
       for (int u = 0; u < USTEPS; ++u) {
         const Op p = pack_rows<T>(s, u), ds = pack_rows<T>(dp, u);
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-          av[d] = Mma<T>::run(read_rows<T, HDP>(lds_g, n * 32, u, d * 32, lane), p, av[d]);
-          ak[d] = Mma<T>::run(read_rows<T, HDP>(lds_q, n * 32, u, d * 32, lane), ds, ak[d]);
+          av[d] = Mma<T>::run(read_rows<T, HDP>(lds_g[buf], n * 32, u, d * 32, lane), p, av[d]);
+          ak[d] = Mma<T>::run(read_rows<T, HDP>(lds_q[buf], n * 32, u, d * 32, lane), ds, ak[d]);
         }
       }
+    }
+  };
+
+  const int begin = first / BM * BM;
+  if (begin < rows) {
+    fetch(begin);
+    place_tile(0);
+    __syncthreads();
+    for (int r = begin; r < rows; r += 2 * BM) {
+      if (r + BM < rows) fetch(r + BM);
+      work(r, Const<0>{});
+      if (r + BM < rows) place_tile(1);
+      __syncthreads();
+      if (r + BM >= rows) break;
+      if (r + 2 * BM < rows) fetch(r + 2 * BM);
+      work(r + BM, Const<1>{});
+      if (r + 2 * BM < rows) place_tile(0);
+      __syncthreads();
     }
   }
   if (!live) return;
   const int64_t at = ((seq.s_off + key) * a.KV + kvh) * a.D;
-#pragma unroll
-  for (int d = 0; d < DT; ++d)
-#pragma unroll
-    for (int g = 0; g < 4; ++g)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int col = d * 32 + 8 * g + 4 * half + j;
-        if (col < a.D) {
-          dk[at + col] = from_f32<T>(ak[d][g * 4 + j] * a.scale);
-          dv[at + col] = from_f32<T>(av[d][g * 4 + j]);
-        }
-      }
+  store_rows<T, DT>(dk + at, ak, a.scale, a.D, half);
+  store_rows<T, DT>(dv + at, av, 1.f, a.D, half);
 }
 
 // ---- launches ----------------------------------------------------------------------------------------------------------
@@ -327,9 +357,6 @@ int v3d_attention_pack_bwd(const void* grad, const void* q, const void* k, const
   V3D_REQUIRE(strides && (B == 0 || (q_lengths && s_lengths)), what, "null pointer");
   V3D_REQUIRE(total_q == 0 || (grad && q && out && lse && grad_q), what, "null pointer");
   V3D_REQUIRE(total_s == 0 || (k && v && grad_k && grad_v), what, "null pointer");
-  DeviceGuard guard(device);
-  if (guard.rc != 0) return guard.rc;
-  hipStream_t s = static_cast<hipStream_t>(stream);
   AttnBwdArgs b{};
   AttnArgs& a = b.f;
   a.q = q;
@@ -348,10 +375,7 @@ int v3d_attention_pack_bwd(const void* grad, const void* q, const void* k, const
   a.v_row = strides[4];
   a.v_head = strides[5];
   a.B = B;
-  a.H = H;
-  a.KV = KV;
-  a.G = H / KV;
-  a.D = D;
+  attn_heads(a, H, KV, D);
   a.scale = scale;
   a.causal = causal;
   a.splits = 1;
@@ -359,6 +383,11 @@ int v3d_attention_pack_bwd(const void* grad, const void* q, const void* k, const
   b.dq = grad_q;
   b.dk = grad_k;
   b.dv = grad_v;
+  rc = attn_check_strides(what, a);
+  if (rc != 0) return rc;
+  DeviceGuard guard(device);
+  if (guard.rc != 0) return guard.rc;
+  hipStream_t s = static_cast<hipStream_t>(stream);
   Scratch ws;
   rc = ws.acquire(what, workspace, workspace_bytes,
                   v3d_attention_pack_bwd_workspace_bytes(B, total_q, total_s, H, KV, D), s);

@@ -33,12 +33,17 @@ struct AttnArgs {
   int64_t capacity;
   int tokens;
   int B, H, KV, G, D;        // G = H / KV query heads share a key head
+  unsigned g_mul, g_shift;   // n / G = mulhi(n, g_mul) >> g_shift for n < 2^31 (G > 1)
   float scale;
   int causal;
   int splits;                // parts that the keys of a row tile are divided into
   float* part_o;             // splits > 1: (tile, KV, split, rows of a tile, D) unnormalised rows ...
   float* part_ml;            // ... and (tile, KV, split, rows of a tile, 2): maximum (of scale * log2(e) * score) and sum
 };
+
+__device__ __forceinline__ int div_g(const AttnArgs& a, int n) {
+  return a.G == 1 ? n : (int)(__umulhi((unsigned)n, a.g_mul) >> a.g_shift);
+}
 
 // A workgroup's sequence.  All fields are wave-uniform.
 struct AttnSeq {
@@ -181,25 +186,29 @@ __device__ __forceinline__ int tile_at(int row, int col) {
   return row * HDP + place<T, HDP>(row, col / E) * E + col % E;
 }
 
-template <typename T>
-struct alignas(16) Chunk {
-  T v[16 / sizeof(T)];
-};
+// Loads go through a buffer descriptor: what lies past its range comes back as zeros without a branch, so all loads of a
+// tile are under way together.  Columns from D on are zeros too: a 16-byte chunk past D is placed out of any range, a chunk
+// that D ends inside is read up to D and shifted into place (hence D >= 16 bytes).
+constexpr int kOutOfRange = 0x7fffffff;
 
-// One 16-byte chunk of a row in memory: columns [c0, c0 + E) of D; zeros where `live` is false or past D.
+__device__ __forceinline__ u32x4 load_buffer(const void* base, int bytes, int offset) {
+  return __builtin_amdgcn_raw_buffer_load_b128(__builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00027000),
+                                               offset, 0, 0);
+}
+
+// The byte offset of the chunk at column `col` of a row that starts at element `at`.
 template <typename T>
-__device__ __forceinline__ Chunk<T> load_chunk(const T* row, int c0, int D, bool live) {
+__device__ __forceinline__ int chunk_offset(int at, int col, int D) {
   constexpr int E = 16 / (int)sizeof(T);
-  Chunk<T> c;
-  if (live && c0 + E <= D) {
-    const Packed<T, E> p = *reinterpret_cast<const Packed<T, E>*>(row + c0);
-#pragma unroll
-    for (int j = 0; j < E; ++j) c.v[j] = p.v[j];
-  } else {
-#pragma unroll
-    for (int j = 0; j < E; ++j) c.v[j] = (live && c0 + j < D) ? row[c0 + j] : (T)0.f;
-  }
-  return c;
+  return col >= D ? kOutOfRange : (at + min(col, D - E)) * (int)sizeof(T);
+}
+template <typename T>
+__device__ __forceinline__ u32x4 chunk_shift(u32x4 c, int col, int D) {
+  constexpr int E = 16 / (int)sizeof(T);
+  const int by = col < D ? max(0, col + E - D) : 0;
+  unsigned __int128 x = __builtin_bit_cast(unsigned __int128, c);
+  x >>= by * 8 * (int)sizeof(T);
+  return __builtin_bit_cast(u32x4, x);
 }
 
 // A tile of ROWS rows on its way from memory to LDS: 256 threads, CH chunks of 16 bytes each, in registers.
@@ -207,38 +216,47 @@ template <typename T, int HD, int ROWS>
 struct TileStage {
   static constexpr int E = 16 / (int)sizeof(T);
   static constexpr int CPR = HD / E;                // chunks of a row
-  static constexpr int CH = ROWS * CPR / 256;
-  static_assert(ROWS * CPR % 256 == 0, "whole chunks per thread");
-  Chunk<T> c[CH];
+  static constexpr int CH = (ROWS * CPR + 255) / 256;
+  static constexpr bool kEven = ROWS * CPR % 256 == 0;  // else the last chunk of some threads repeats the last row's
+  u32x4 c[CH];
 
-  static __device__ __forceinline__ int row_of(int i) { return (i * 256 + (int)threadIdx.x) / CPR; }
+  static __device__ __forceinline__ int row_of(int i) {
+    const int r = (i * 256 + (int)threadIdx.x) / CPR;
+    return kEven ? r : min(r, ROWS - 1);
+  }
   static __device__ __forceinline__ int col_of(int i) { return (i * 256 + (int)threadIdx.x) % CPR * E; }
 
-  // Rows [0, count) of those at `base`; the others, and columns from D on, are zeros.
+  // Rows [0, count) (count >= 1) at `base`, `stride` elements apart (64 strides stay below 2^31 bytes).
   __device__ __forceinline__ void fetch(const T* base, int64_t stride, int D, int count) {
-    if (count >= ROWS && D == HD) {
+    const int bytes = ((min(count, ROWS) - 1) * (int)stride + D) * (int)sizeof(T);
 #pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        const Packed<T, E> p = *reinterpret_cast<const Packed<T, E>*>(base + row_of(i) * stride + col_of(i));
-#pragma unroll
-        for (int j = 0; j < E; ++j) c[i].v[j] = p.v[j];
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < CH; ++i) c[i] = load_chunk<T>(base + row_of(i) * stride, col_of(i), D, row_of(i) < count);
-    }
+    for (int i = 0; i < CH; ++i) c[i] = load_buffer(base, bytes, chunk_offset<T>(row_of(i) * (int)stride, col_of(i), D));
   }
-  __device__ __forceinline__ void store(T* tile) const {
-    constexpr int HDP = attn_pow2(HD);
+  // The same for rows at offsets of their own (elements, non-negative, below 2^29).
+  template <typename Offset>
+  __device__ __forceinline__ void fetch_at(const T* base, Offset offset, int D, int count) {
 #pragma unroll
-    for (int i = 0; i < CH; ++i) *reinterpret_cast<Chunk<T>*>(tile + tile_at<T, HDP>(row_of(i), col_of(i))) = c[i];
+    for (int i = 0; i < CH; ++i)
+      c[i] = load_buffer(base, kOutOfRange,
+                         row_of(i) < count ? chunk_offset<T>(offset(row_of(i)), col_of(i), D) : kOutOfRange);
+  }
+  __device__ __forceinline__ void store(T* tile, int D) {
+    constexpr int HDP = attn_pow2(HD);
+    if (D % E != 0) {
+#pragma unroll
+      for (int i = 0; i < CH; ++i) c[i] = chunk_shift<T>(c[i], col_of(i), D);
+    }
+#pragma unroll
+    for (int i = 0; i < CH; ++i) *reinterpret_cast<u32x4*>(tile + tile_at<T, HDP>(row_of(i), col_of(i))) = c[i];
   }
   __device__ __forceinline__ bool nonfinite() const {
     bool bad = false;
 #pragma unroll
-    for (int i = 0; i < CH; ++i)
+    for (int i = 0; i < CH; ++i) {
+      const Packed<T, E> v = __builtin_bit_cast(Packed<T , E>, c[i]);
 #pragma unroll
-      for (int j = 0; j < E; ++j) bad |= !(__builtin_fabsf(to_f32(c[i].v[j])) < __builtin_inff());
+      for (int j = 0; j < E; ++j) bad |= !(__builtin_fabsf(to_f32(v.v[j])) < __builtin_inff());
+    }
     return bad;
   }
 };
@@ -338,14 +356,18 @@ __device__ __forceinline__ typename Mma<T>::Op pack_rows(const f32x16& p, int u)
   return op;
 }
 
-// Elements [c0, c0 + E) of a row in memory as an operand; zeros past D.
-template <typename T>
-__device__ __forceinline__ typename Mma<T>::Op load_op(const T* row, int c0, int D, bool live) {
-  const Chunk<T> c = load_chunk<T>(row, c0, D, live);
-  typename Mma<T>::Op op;
+// The operands of all product steps over the head size from one row in memory: `at` = this lane's row in elements from
+// `base` (wave-uniform), negative = a row of zeros.
+template <typename T, int STEPS>
+__device__ __forceinline__ void load_ops(typename Mma<T>::Op (&op)[STEPS], const T* base, int at, int half, int D) {
+  constexpr int E = 16 / (int)sizeof(T);
 #pragma unroll
-  for (int j = 0; j < 16 / (int)sizeof(T); ++j) op[j] = c.v[j];
-  return op;
+  for (int st = 0; st < STEPS; ++st) {
+    const int col = st * 2 * E + E * half;
+    u32x4 c = load_buffer(base, kOutOfRange, at < 0 ? kOutOfRange : chunk_offset<T>(at, col, D));
+    if (D % E != 0) c = chunk_shift<T>(c, col, D);
+    op[st] = __builtin_bit_cast(typename Mma<T>::Op, c);
+  }
 }
 
 // A result whose column is this lane's row and whose rows are the row's elements, times `f`, to memory.
@@ -365,6 +387,11 @@ __device__ __forceinline__ void store_rows(T* row, const f32x16 (&acc)[DT], floa
           if (col + j < D) row[col + j] = from_f32<T>(v[j]);
       }
     }
+}
+
+// The mask of a row: its token sees the keys [0, this).
+__device__ __forceinline__ int attn_limit(const AttnArgs& a, const AttnSeq& seq, int token) {
+  return a.causal ? max(0, min(seq.s_len, token + seq.s_len - seq.q_len + 1)) : seq.s_len;
 }
 
 // Over the two lanes (l, l + 32) of a column, without LDS.
@@ -388,8 +415,22 @@ __device__ __forceinline__ f32x16 zero16() {
   return z;
 }
 
+// Host side: the heads, and the division by the group's size as a product (exact for 31-bit numerators: the multiplier is
+// 2^(31 + s) / G rounded up with 2^s >= G, its excess times n stays below 2^(31 + s)).
+inline void attn_heads(AttnArgs& a, int H, int KV, int D) {
+  a.H = H;
+  a.KV = KV;
+  a.G = H / KV;
+  a.D = D;
+  unsigned s = 0;
+  while (((int64_t)1 << s) < a.G) ++s;
+  a.g_mul = s == 0 ? 0u : (unsigned)((((uint64_t)1 << (31 + s)) + a.G - 1) / a.G);
+  a.g_shift = s == 0 ? 0u : s - 1;
+}
+
 // Host side: the argument checks of every entry point (attention.hip).
 int attn_check(const char* what, int dtype, int B, int64_t total_q, int64_t total_s, int H, int KV, int D, float scale);
+int attn_check_strides(const char* what, const AttnArgs& a);
 // Host side: the smallest built head size that holds D, 0 if there is none.
 inline int attn_head_size(int D) {
   for (int hd : {32, 64, 96, 128, 192, 256})

@@ -17,8 +17,13 @@ def _require_cuda(name, *tensors):
 
 
 def _rows(t: Tensor) -> Tensor:
-    """Any strides but the last dimension's; a gradient or input without a unit stride there is copied."""
-    return t if t.size(-1) <= 1 or t.stride(-1) == 1 else t.contiguous()
+    """The strides that the kernels take: any but the last dimension's, which is 1, within 32-bit offsets of a tile; other
+    inputs are copied."""
+    if t.dim() < 3 or t.numel() == 0:
+        return t
+    row, head, unit = t.stride()[-3:]
+    near = 130 * row + t.size(-2) * head + t.size(-1) < 1 << 29
+    return t if unit == 1 and (row == 0 or row >= t.size(-1)) and near else t.contiguous()
 
 
 def _scale(scale, dim):
@@ -54,7 +59,7 @@ def attention_pack_mode(q_feats: Tensor, k_feats: Tensor, v_feats: Tensor, q_len
     H is a multiple of KV: query head h reads key head ``h // (H // KV)``.  ``s_lengths`` None: the keys are the queries'
     sequences (self-attention).  ``causal``: query i of a sequence sees the keys j <= i + (s_length - q_length), so the last
     query sees them all.  A query without keys yields zeros and has no gradient; what a query does not see does not reach
-    it, infinities and NaN included (in the forward).  Rows behind the last sequence come out as zeros.  fp32, fp16 or bf16, D <= 256; the
+    it, infinities and NaN included (in the forward).  Rows behind the last sequence come out as zeros.  fp32, fp16 or bf16, D from 8 (fp32: 4) to 256; the
     inputs may be views of one projection (only the last dimension has to be contiguous).
     """
     s_lengths = q_lengths if s_lengths is None else s_lengths
