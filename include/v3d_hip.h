@@ -459,10 +459,12 @@ int v3d_layer_norm_bwd(const void* grad, const void* feats, const void* residual
  * over all keys j of the sequence or, with `causal`, over j <= i + (s_len - q_len): the last query sees every key.  A query
  * that sees no key yields zeros; an infinity or NaN in a key or value that a query does not see does not reach it.  Rows
  * behind the last sequence are written as zeros; lengths that overrun the totals are cut.  out (total_q,H,D) contiguous;
- * lse (total_q,H) fp32 = log2 of the row's sum of exp(score) (-inf without keys), what the backward needs; or NULL.
+ * rest (total_q,H,D): what rounding to a 16-bit type took from out, for the backward (whose grad . out would otherwise carry
+ * it into every gradient of the row); not written in fp32; or NULL.  lse (total_q,H) fp32 = log2 of the row's sum of exp(score) (-inf without keys), what the backward needs; or NULL.
  * `strides` (host array, elements): q row, q head, k row, k head, v row, v head -- the last dimension is contiguous, rows
  * need no alignment.  Products of 16-bit types are exact, the probabilities are rounded to the type before they meet the
- * values; scores, statistics and sums are fp32.  16 bytes <= D <= V3D_ATTENTION_MAX_HEAD_SIZE, 0 < scale < inf; strides are not
+ * values; scores, statistics and sums are fp32.  fp32 products are formed of bf16 thirds
+ * to 2^-24: an infinity that a query sees comes out as a NaN.  16 bytes <= D <= V3D_ATTENTION_MAX_HEAD_SIZE, 0 < scale < inf; strides are not
  * negative, key rows do not overlap (a stride of 0 is fine) and 129 token (or key) rows, plus a group's heads, span less than 2^29 elements.
  *
  * v3d_cached_attention: q (B,tokens,H,D) = the newest `tokens` tokens of every sequence, k_cache / v_cache
@@ -470,7 +472,7 @@ int v3d_layer_norm_bwd(const void* grad, const void* feats, const void* residual
  * j <= lengths[b] - tokens + t.  Rows past a length are never read.  `strides`: q row, q head, k batch, k row, k head,
  * v batch, v row, v head; q rows are token b * tokens + t.
  *
- * v3d_attention_pack_bwd: grad (total_q,H,D) of out and the forward's inputs, out and lse -> grad_q (total_q,H,D), grad_k
+ * v3d_attention_pack_bwd: grad (total_q,H,D) of out and the forward's inputs, out, rest (or NULL) and lse -> grad_q (total_q,H,D), grad_k
  * and grad_v (total_s,KV,D), all contiguous and fully written (zeros behind the last sequence); key heads sum over their
  * query heads.  No atomics: the same bits every time.
  *
@@ -478,12 +480,12 @@ int v3d_layer_norm_bwd(const void* grad, const void* feats, const void* residual
 #define V3D_ATTENTION_MAX_HEAD_SIZE 256
 size_t v3d_attention_pack_workspace_bytes(int B, int64_t total_q, int64_t total_s, int H, int KV, int D);
 int v3d_attention_pack_fwd(const void* q, const void* k, const void* v, const int64_t* q_lengths,
-                           const int64_t* s_lengths, void* out, float* lse, int dtype, int B, int64_t total_q,
-                           int64_t total_s, int H, int KV, int D, const int64_t* strides, float scale, int causal,
-                           void* workspace, size_t workspace_bytes, int device, void* stream);
+                           const int64_t* s_lengths, void* out, void* rest, float* lse, int dtype, int B,
+                           int64_t total_q, int64_t total_s, int H, int KV, int D, const int64_t* strides, float scale,
+                           int causal, void* workspace, size_t workspace_bytes, int device, void* stream);
 size_t v3d_attention_pack_bwd_workspace_bytes(int B, int64_t total_q, int64_t total_s, int H, int KV, int D);
 int v3d_attention_pack_bwd(const void* grad, const void* q, const void* k, const void* v, const void* out,
-                           const float* lse, const int64_t* q_lengths, const int64_t* s_lengths, void* grad_q,
+                           const void* rest, const float* lse, const int64_t* q_lengths, const int64_t* s_lengths, void* grad_q,
                            void* grad_k, void* grad_v, int dtype, int B, int64_t total_q, int64_t total_s, int H, int KV,
                            int D, const int64_t* strides, float scale, int causal, void* workspace,
                            size_t workspace_bytes, int device, void* stream);

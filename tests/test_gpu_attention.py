@@ -321,7 +321,7 @@ def test_refusals_without_a_gpu():
     with pytest.raises(RuntimeError, match="cached_attention: CUDA tensors required"):
         ops.cached_attention(t[None], t[None], t[None], torch.tensor([4]))
     lib = _lib.lib()
-    none = [None] * 7
+    none = [None] * 8
 
     def pack(dtype=1, b=1, nq=4, ns=4, h=2, kv=1, d=8, scale=1.0):
         return lib.v3d_attention_pack_fwd(*none, dtype, b, nq, ns, h, kv, d, None, scale, 0, None, 0, 0, None)

@@ -125,11 +125,11 @@ SIGNATURES = {
     "v3d_layer_norm_bwd_workspace_bytes": (_c_size, [_c_i64, _c_i64]),
     "v3d_attention_pack_workspace_bytes": (_c_size, [_c_int, _c_i64, _c_i64, _c_int, _c_int, _c_int]),
     "v3d_attention_pack_fwd": (
-        _c_int, [_c_ptr] * 7 + [_c_int, _c_int, _c_i64, _c_i64, _c_int, _c_int, _c_int, ctypes.POINTER(_c_i64), _c_f32,
+        _c_int, [_c_ptr] * 8 + [_c_int, _c_int, _c_i64, _c_i64, _c_int, _c_int, _c_int, ctypes.POINTER(_c_i64), _c_f32,
                                 _c_int] + _WS + _TAIL),
     "v3d_attention_pack_bwd_workspace_bytes": (_c_size, [_c_int, _c_i64, _c_i64, _c_int, _c_int, _c_int]),
     "v3d_attention_pack_bwd": (
-        _c_int, [_c_ptr] * 11 + [_c_int, _c_int, _c_i64, _c_i64, _c_int, _c_int, _c_int, ctypes.POINTER(_c_i64), _c_f32,
+        _c_int, [_c_ptr] * 12 + [_c_int, _c_int, _c_i64, _c_i64, _c_int, _c_int, _c_int, ctypes.POINTER(_c_i64), _c_f32,
                                  _c_int] + _WS + _TAIL),
     "v3d_cached_attention_workspace_bytes": (_c_size, [_c_int, _c_int, _c_i64, _c_int, _c_int, _c_int]),
     "v3d_cached_attention": (

@@ -11,73 +11,226 @@
 
 namespace v3d {
 
-// Keys of a tile: two tiles of keys and values (one worked on, one arriving) stay within 64 KiB up to 512-byte rows, so that
-// two workgroups share a CU.
+__device__ __forceinline__ void wave_order() {  // LDS accesses of a wave stay in program order
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// What a wave carries through its keys: 32 rows, one per lane and half.
 template <typename T, int HD>
-constexpr int attn_keys() { return HD * (int)sizeof(T) > 256 ? 32 : 64; }
+struct AttnWave {
+  typedef typename Kind<T>::U U;
+  static constexpr int HDP = attn_pow2(HD);
+  static constexpr int STEPS = HD / 16;  // product steps over the head size
+  static constexpr int DT = HD / 32;
+
+  Op<T> q[STEPS];
+  f32x16 o[DT];
+  float m = -__builtin_inff(), l = 0.f;  // running maximum of scale * log2(e) * score, and the sum of 2^(that - m)
+  float c2;
+  int lane, half;
+  int row, token, head;
+  int limit;        // this lane's query sees the keys [0, limit)
+  int least, most;  // of the wave's first and last row; most = 0: the wave has no rows
+
+  // `row0`: the wave's first row in the sequence.
+  __device__ __forceinline__ void begin(const AttnArgs& a, const AttnSeq& seq, int kvh, int row0, int rows) {
+    lane = threadIdx.x & 63;
+    half = lane >> 5;
+    row = row0 + (lane & 31);
+    token = div_g(a, min(row, rows - 1));
+    const int g = min(row, rows - 1) - token * a.G;
+    head = kvh * a.G + g;
+    limit = attn_limit(a, seq, token);
+    least = __builtin_amdgcn_readfirstlane(limit);
+    most = row0 < rows ? attn_limit(a, seq, div_g(a, min(row0 + 31, rows - 1))) : 0;
+    c2 = a.scale * kLog2e;
+    const int token0 = div_g(a, min(row0, rows - 1));
+    load_ops<T>(q, static_cast<const T*>(a.q) + (seq.q_off + token0) * a.q_row + (int64_t)kvh * a.G * a.q_head,
+                (token - token0) * (int)a.q_row + g * (int)a.q_head, half, a.D, true);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[d] = zero16();
+  }
+
+  // s = 2^(score - m) of a tile of 32 NT keys from key0 on; m, l and o move on.
+  template <int NT>
+  __device__ __forceinline__ void scores(const U* k, int key0, f32x16 (&s)[NT]) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) s[n] = zero16();
+#pragma unroll
+    for (int st = 0; st < STEPS; ++st)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+        s[n] = product<T>(read_cols<T, HDP, 32 * NT>(k, n * 32 + (lane & 31), st, half), q[st], s[n]);
+    if (key0 + 32 * NT > least) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (key0 + n * 32 + acc_row(r, half) >= limit) s[n][r] = -__builtin_inff();
+    }
+    // maximum of the lane, then with the lane that holds the other keys of this query
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[n][r]);
+    top = halves_max(top) * c2;
+    // The maximum moves only when a probability would exceed 2^8: what was summed is rescaled rarely, and a stale maximum
+    // costs no accuracy (16-bit probabilities keep their relative precision up to 2^8, the sums are fp32).
+    if (__any(top > m + 8.f)) {
+      const float m_new = fmaxf(m, top);
+      const float alpha = m_new == -__builtin_inff() ? 1.f : exp2_fast(m - m_new);
+      m = m_new;
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+    }
+    const float base = m == -__builtin_inff() ? 0.f : m;
+    float sum = 0.f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[n][r] = exp2_fast(fmaf(s[n][r], c2, -base));
+        sum += s[n][r];
+      }
+    l += sum;
+  }
+
+  template <int NT>
+  __device__ __forceinline__ void values(const U* v, const f32x16 (&s)[NT]) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const Op<T> p = pack_rows<T>(s[n], u);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[d] = product<T>(read_rows<T, HDP, 32 * NT>(v, n * 32, u, d * 32, lane), p, o[d]);
+      }
+  }
+
+  // An infinity or NaN among the values of a tile that some query sees in part must not reach the queries that do not see
+  // it (0 * inf).  Key by key it is added to the queries that do -- `p` is 32 x 32 of LDS that is the wave's own --; the
+  // tile's owner then clears it for the product.
+  template <int NT>
+  __device__ __forceinline__ void add_nonfinite(U* p, const U* v, int key0, const f32x16 (&s)[NT]) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      wave_order();
+#pragma unroll
+      for (int r = 0; r < 16; ++r) p[acc_row(r, half) * 32 + (lane & 31)] = from_f32<U>(s[n][r]);
+      wave_order();
+#pragma unroll 1
+      for (int key = 0; key < 32 && key0 + n * 32 + key < most; ++key) {
+        const float pk = to_f32(p[key * 32 + (lane & 31)]);
+        const bool seen = key0 + n * 32 + key < limit;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            float w = 0.f;
+#pragma unroll
+            for (int i = 0; i < Kind<T>::P; ++i)
+              w += to_f32(v[i * (32 * NT * HDP) + tile_at<HDP>(n * 32 + key, d * 32 + acc_row(r, half))]);
+            if (seen && !(__builtin_fabsf(w) < __builtin_inff())) o[d][r] += pk * w;
+          }
+      }
+    }
+  }
+};
+
+template <typename U>
+__device__ __forceinline__ void clear_nonfinite(U* tile, int count, int first, int step) {
+  for (int i = first; i < count; i += step)
+    if (!(__builtin_fabsf(to_f32(tile[i])) < __builtin_inff())) tile[i] = (U)0.f;
+}
+
+// 4 finished values of a row: rounded to the type and, for the backward, what the rounding took.
+template <typename T>
+__device__ __forceinline__ void store_out(const AttnArgs& a, int64_t row, int col, const float (&v)[4]) {
+  store4<T>(static_cast<T*>(a.out) + row * a.D, col, a.D, v);
+  if (sizeof(T) == 2 && a.rest != nullptr) {
+    float left[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) left[j] = v[j] - to_f32(from_f32<T>(v[j]));
+    store4<T>(static_cast<T*>(a.rest) + row * a.D, col, a.D, left);
+  }
+}
+__device__ __forceinline__ float inverse_sum(float l) {
+  return l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no keys: zeros; a NaN stays a NaN
+}
+__device__ __forceinline__ float log_sum(float m, float l) { return l == 0.f ? -__builtin_inff() : m + log2f(l); }
+
+// The launch covers a bound of the pack's tiles: the rest of it clears the rows behind the last sequence.
+template <typename T, int TILE>
+__device__ __forceinline__ void clear_behind(const AttnArgs& a, const AttnSeq& seq, int kvh) {
+  const int64_t rows = (a.total_q - seq.q_end) * a.G;
+  for (int i = threadIdx.x; i < TILE; i += blockDim.x) {
+    const int64_t r = seq.spare * TILE + i;
+    if (r >= rows) break;
+    const int64_t at = (seq.q_end + r / a.G) * a.H + (int64_t)kvh * a.G + r % a.G;
+    for (int d = 0; d < a.D; ++d) {
+      static_cast<T*>(a.out)[at * a.D + d] = (T)0.f;
+      if (a.rest) static_cast<T*>(a.rest)[at * a.D + d] = (T)0.f;
+    }
+    if (a.lse) a.lse[at] = -__builtin_inff();
+  }
+}
+
+// ---- many rows: 128 of them share the tiles of keys and values ---------------------------------------------------------
+// Keys of a tile; two tiles (one worked on, one arriving) of keys and values lie in at most 96 KiB of LDS where that fits:
+// two workgroups a CU with 16-bit heads of up to 128.
+template <typename T, int HD>
+constexpr int attn_keys() { return Kind<T>::P == 1 && HD <= 128 ? 64 : 32; }
+template <typename T, int HD>
+constexpr int attn_buffers() { return Kind<T>::P == 3 && HD > 128 ? 1 : 2; }
+template <typename T, int HD>
+constexpr int attn_occupancy() { return HD <= (Kind<T>::P == 1 ? 128 : 64) ? 2 : 1; }  // waves per SIMD that the registers are kept for
 
 template <typename T, int HD>
-__global__ __launch_bounds__(256, HD * sizeof(T) <= 256 ? 2 : 1) void attn_forward_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(256, (attn_occupancy<T, HD>())) void attn_forward_kernel(const AttnArgs a) {
+  typedef typename Kind<T>::U U;
   constexpr int HDP = attn_pow2(HD);
   constexpr int BN = attn_keys<T, HD>();
-  constexpr int NT = BN / 32;                       // 32-key blocks of a tile
-  constexpr int STEPS = HD / Mma<T>::kStep;         // product steps over the head size
-  constexpr int USTEPS = 32 / Mma<T>::kStep;        // product steps over a 32-key block
-  constexpr int DT = HD / 32;
-  typedef typename Mma<T>::Op Op;
-  __shared__ T lds_k[2][BN * HDP];
-  __shared__ T lds_v[2][BN * HDP];
-  __shared__ int lds_bad[2];
+  constexpr int NT = BN / 32;  // 32-key blocks of a tile
+  constexpr int BUFS = attn_buffers<T, HD>();
+  constexpr int SIZE = Kind<T>::P * BN * HDP;
+  __shared__ __attribute__((aligned(16))) U lds_k[BUFS][SIZE];
+  __shared__ __attribute__((aligned(16))) U lds_v[BUFS][SIZE];
+  __shared__ int lds_bad[BUFS];
 
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int half = lane >> 5;
+  const int wave = threadIdx.x >> 6;
   int64_t id = blockIdx.x;
   const int kvh = (int)(id % a.KV);
   id /= a.KV;
   const int split = (int)(id % a.splits);
   id = (int64_t)(gridDim.x / (a.KV * a.splits)) - 1 - id / a.splits;  // causal: the longest tiles of a sequence start first
   const AttnSeq seq = locate_rows<kAttnRows>(a, id);
-  if (!seq.found) {  // the launch covers a bound: the rest of it clears the rows behind the last sequence
-    if (a.capacity == 0 && split == 0) {
-      const int64_t rows = (a.total_q - seq.q_end) * a.G;
-      for (int i = threadIdx.x; i < kAttnRows; i += 256) {
-        const int64_t r = seq.spare * kAttnRows + i;
-        if (r >= rows) break;
-        const int64_t at = (seq.q_end + r / a.G) * a.H + (int64_t)kvh * a.G + r % a.G;
-        for (int d = 0; d < a.D; ++d) static_cast<T*>(a.out)[at * a.D + d] = (T)0.f;
-        if (a.lse) a.lse[at] = -__builtin_inff();
-      }
-    }
+  if (!seq.found) {
+    if (a.capacity == 0 && split == 0) clear_behind<T, kAttnRows>(a, seq, kvh);
     return;
   }
   const int rows = seq.q_len * a.G;
-  if (seq.tile * kAttnRows >= rows) return;  // lengths that overrun the total were cut
-  const int row = seq.tile * kAttnRows + wave * 32 + (lane & 31);
-  const int token = div_g(a, min(row, rows - 1));
-  const int head = kvh * a.G + min(row, rows - 1) - token * a.G;
-  const int limit = attn_limit(a, seq, token);  // this lane's query sees keys [0, limit)
-  // the wave's and the workgroup's first and last rows bound what they have to look at
-  const bool wave_live = seq.tile * kAttnRows + wave * 32 < rows;
-  const int wave_least = __builtin_amdgcn_readfirstlane(limit);
-  const int wave_most = wave_live ? attn_limit(a, seq, div_g(a, min(seq.tile * kAttnRows + wave * 32 + 31, rows - 1))) : 0;
-  const int most = attn_limit(a, seq, div_g(a, min(seq.tile * kAttnRows + kAttnRows - 1, rows - 1)));
-  const int least = attn_limit(a, seq, div_g(a, min(seq.tile * kAttnRows, rows - 1)));
+  const int row0 = seq.tile * kAttnRows;
+  if (row0 >= rows) return;  // lengths that overrun the total were cut
+  AttnWave<T, HD> w;
+  w.begin(a, seq, kvh, row0 + wave * 32, rows);
+  // the workgroup's first and last rows bound what it has to look at
+  const int most = attn_limit(a, seq, div_g(a, min(row0 + kAttnRows - 1, rows - 1)));
+  const int least = attn_limit(a, seq, div_g(a, row0));
 
   const int tiles = (most + BN - 1) / BN;
   const int per_split = (tiles + a.splits - 1) / a.splits;
   const int t_begin = split * per_split, t_end = min(tiles, t_begin + per_split);
-
-  const int token0 = div_g(a, seq.tile * kAttnRows);
-  const T* q = static_cast<const T*>(a.q) + (seq.q_off + token0) * a.q_row + (int64_t)kvh * a.G * a.q_head;
   const T* k = static_cast<const T*>(a.k) + seq.b * a.k_batch + seq.s_off * a.k_row + (int64_t)kvh * a.k_head;
   const T* v = static_cast<const T*>(a.v) + seq.b * a.v_batch + seq.s_off * a.v_row + (int64_t)kvh * a.v_head;
 
-  Op qf[STEPS];
-  load_ops<T>(qf, q, (token - token0) * (int)a.q_row + (head - kvh * a.G) * (int)a.q_head, half, a.D);
-
   // The tile after the one that is worked on is on its way in registers meanwhile.
-  TileStage<T, HD, BN> stage_k, stage_v;
-  if (threadIdx.x < 2) lds_bad[threadIdx.x] = 0;
+  TileStage<T, HD, BN, 256> stage_k, stage_v;
+  if (threadIdx.x < BUFS) lds_bad[threadIdx.x] = 0;
   auto fetch = [&](int t) {
     stage_k.fetch(k + (int64_t)t * BN * a.k_row, a.k_row, a.D, seq.s_len - t * BN);
     stage_v.fetch(v + (int64_t)t * BN * a.v_row, a.v_row, a.D, seq.s_len - t * BN);
@@ -85,109 +238,23 @@ __global__ __launch_bounds__(256, HD * sizeof(T) <= 256 ? 2 : 1) void attn_forwa
   auto place_tile = [&](int t, int buf) {
     stage_k.store(lds_k[buf], a.D);
     stage_v.store(lds_v[buf], a.D);
-    // values of a tile that some query sees in part: see below
     if (t * BN + BN > least && stage_v.nonfinite()) lds_bad[buf] = t + 1;
   };
-
-  const float c2 = a.scale * kLog2e;
-  float m = -__builtin_inff(), l = 0.f;  // running maximum of scale * log2(e) * score, and the sum of 2^(that - m)
-  f32x16 o[DT];
-#pragma unroll
-  for (int d = 0; d < DT; ++d) o[d] = zero16();
-
   auto work = [&](int t, auto buffer) {
     constexpr int buf = decltype(buffer)::value;
     const int key0 = t * BN;
-    const bool active = key0 < wave_most;
+    const bool active = key0 < w.most;
     f32x16 s[NT];
-    if (active) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n) s[n] = zero16();
-#pragma unroll
-      for (int st = 0; st < STEPS; ++st)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-          s[n] = Mma<T>::run(read_cols<T, HDP>(lds_k[buf], n * 32 + (lane & 31), st, half), qf[st], s[n]);
-      if (key0 + BN > wave_least) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (key0 + n * 32 + acc_row(r, half) >= limit) s[n][r] = -__builtin_inff();
-      }
-      // maximum of the lane, then with the lane that holds the other keys of this query
-      float top = -__builtin_inff();
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[n][r]);
-      top = halves_max(top) * c2;
-      // The maximum moves only when a probability would exceed 2^8: what was summed is rescaled rarely, and a stale
-      // maximum costs no accuracy (16-bit probabilities keep their relative precision up to 2^8, the sums are fp32).
-      if (__any(top > m + 8.f)) {
-        const float m_new = fmaxf(m, top);
-        const float alpha = m_new == -__builtin_inff() ? 1.f : exp2_fast(m - m_new);
-        m = m_new;
-        l *= alpha;
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
-      }
-      const float base = m == -__builtin_inff() ? 0.f : m;
-      float sum = 0.f;
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          s[n][r] = exp2_fast(fmaf(s[n][r], c2, -base));
-          sum += s[n][r];
-        }
-      l += sum;
-    }
+    if (active) w.template scores<NT>(lds_k[buf], key0, s);
     if (lds_bad[buf] == t + 1) {
-      // An infinity or NaN among the values of a tile that some query sees in part must not reach the queries that do not
-      // see it (0 * inf).  It is added key by key to the queries that do, then cleared for the product.  The probabilities
-      // wait in the keys' place, which nobody reads any more.
+      static_assert(BUFS * SIZE >= kAttnWaves * 1024, "room for the waves' probabilities");
+      __syncthreads();  // nobody reads the keys any more: both of their buffers are free until the next tile is placed
+      if (active) w.template add_nonfinite<NT>(lds_k[0] + wave * 1024, lds_v[buf], key0, s);
       __syncthreads();
-      T* lds_p = lds_k[buf] + wave * (BN * 32);
-      if (active) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) lds_p[(n * 32 + acc_row(r, half)) * 32 + (lane & 31)] = from_f32<T>(s[n][r]);
-      }
-      __syncthreads();
-      if (active) {
-#pragma unroll 1
-        for (int key = 0; key < BN && key0 + key < wave_most; ++key) {
-          const float p = to_f32(lds_p[key * 32 + (lane & 31)]);
-          const bool seen = key0 + key < limit;
-#pragma unroll
-          for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const float w = to_f32(lds_v[buf][tile_at<T, HDP>(key, d * 32 + acc_row(r, half))]);
-              if (seen && !(__builtin_fabsf(w) < __builtin_inff())) o[d][r] += p * w;
-            }
-        }
-      }
-      __syncthreads();
-      for (int i = threadIdx.x; i < BN * HDP; i += 256)
-        if (!(__builtin_fabsf(to_f32(lds_v[buf][i])) < __builtin_inff())) lds_v[buf][i] = (T)0.f;
+      clear_nonfinite(lds_v[buf], SIZE, threadIdx.x, 256);
       __syncthreads();
     }
-    if (active) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int u = 0; u < USTEPS; ++u) {
-          const Op p = pack_rows<T>(s[n], u);
-#pragma unroll
-          for (int d = 0; d < DT; ++d)
-            o[d] = Mma<T>::run(read_rows<T, HDP>(lds_v[buf], n * 32, u, d * 32, lane), p, o[d]);
-        }
-    }
+    if (active) w.template values<NT>(lds_v[buf], s);
   };
 
   if (t_begin < t_end) {
@@ -195,37 +262,181 @@ __global__ __launch_bounds__(256, HD * sizeof(T) <= 256 ? 2 : 1) void attn_forwa
     fetch(t_begin);
     place_tile(t_begin, 0);
     __syncthreads();
-    for (int t = t_begin; t < t_end; t += 2) {
-      if (t + 1 < t_end) fetch(t + 1);
-      work(t, Const<0>{});
-      if (t + 1 < t_end) place_tile(t + 1, 1);
-      __syncthreads();
-      if (t + 1 >= t_end) break;
-      if (t + 2 < t_end) fetch(t + 2);
-      work(t + 1, Const<1>{});
-      if (t + 2 < t_end) place_tile(t + 2, 0);
-      __syncthreads();
+    if constexpr (BUFS == 2) {
+      for (int t = t_begin; t < t_end; t += 2) {
+        if (t + 1 < t_end) fetch(t + 1);
+        work(t, Const<0>{});
+        if (t + 1 < t_end) place_tile(t + 1, 1);
+        __syncthreads();
+        if (t + 1 >= t_end) break;
+        if (t + 2 < t_end) fetch(t + 2);
+        work(t + 1, Const<1>{});
+        if (t + 2 < t_end) place_tile(t + 2, 0);
+        __syncthreads();
+      }
+    } else {
+      for (int t = t_begin; t < t_end; ++t) {
+        if (t + 1 < t_end) fetch(t + 1);
+        work(t, Const<0>{});
+        __syncthreads();
+        if (t + 1 < t_end) place_tile(t + 1, 0);
+        __syncthreads();
+      }
     }
   }
 
-  l = halves_sum(l);
-  if (row >= rows) return;
-  if (a.splits == 1) {
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // a NaN sum stays a NaN
-    const int64_t at = (seq.q_off + token) * a.H + head;
-    store_rows<T, DT>(static_cast<T*>(a.out) + at * a.D, o, inv, a.D, half);
-    if (a.lse && half == 0) a.lse[at] = l == 0.f ? -__builtin_inff() : m + log2f(l);
-    return;
-  }
-  const int64_t part = (((int64_t)id * a.KV + kvh) * a.splits + split) * kAttnRows + wave * 32 + (lane & 31);
-  store_rows<float, DT>(a.part_o + part * a.D, o, 1.f, a.D, half);
-  if (half == 0) {
-    a.part_ml[part * 2] = m;
-    a.part_ml[part * 2 + 1] = l;
+  const float l = halves_sum(w.l);
+  if (w.row >= rows) return;
+  const int64_t at = (seq.q_off + w.token) * a.H + w.head;
+  const int64_t part = (((int64_t)id * a.KV + kvh) * a.splits + split) * kAttnRows + wave * 32 + (w.lane & 31);
+  const float inv = a.splits == 1 ? inverse_sum(l) : 1.f;
+#pragma unroll
+  for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int col = d * 32 + 8 * g + 4 * w.half;
+      const float x[4] = {w.o[d][g * 4] * inv, w.o[d][g * 4 + 1] * inv, w.o[d][g * 4 + 2] * inv, w.o[d][g * 4 + 3] * inv};
+      if (a.splits == 1)
+        store_out<T>(a, at, col, x);
+      else
+        store4<float>(a.part_o + part * a.D, col, a.D, x);
+    }
+  if (w.half == 0) {
+    if (a.splits > 1) {
+      a.part_ml[part * 2] = w.m;
+      a.part_ml[part * 2 + 1] = l;
+    } else if (a.lse) {
+      a.lse[at] = log_sum(w.m, l);
+    }
   }
 }
 
-// Joins the parts of a row tile's keys: one wave per row, lanes over the columns.
+// ---- few rows: 32 of them, the waves of a workgroup divide the keys ----------------------------------------------------
+// Bound: the bytes of the keys and values.  A wave fetches its own tiles of 32 keys into its own part of LDS, so there is no
+// barrier in the loop and each wave keeps a tile of keys and one of values in flight; keys and values take turns in one
+// place (a wave's LDS accesses happen in order).  The waves' sums meet in LDS at the end.
+template <typename T, int HD>
+constexpr int few_waves() { return Kind<T>::P == 3 && HD > 128 ? 2 : 4; }
+
+template <typename T, int HD>
+__global__ __launch_bounds__((64 * few_waves<T, HD>())) void attn_few_rows_kernel(const AttnArgs a) {
+  typedef typename Kind<T>::U U;
+  constexpr int HDP = attn_pow2(HD);
+  constexpr int W = few_waves<T, HD>();
+  constexpr int SIZE = Kind<T>::P * 32 * HDP;
+  constexpr int TILES = W * SIZE * (int)sizeof(U), JOIN = 32 * HD * (int)sizeof(float);
+  __shared__ __attribute__((aligned(16))) char lds[TILES > JOIN ? TILES : JOIN];
+  __shared__ U lds_p[W][32 * 32];
+  __shared__ float lds_ml[W][32][2];
+
+  const int wave = threadIdx.x >> 6;
+  int64_t id = blockIdx.x;
+  const int kvh = (int)(id % a.KV);
+  id /= a.KV;
+  const int split = (int)(id % a.splits);
+  id /= a.splits;
+  const AttnSeq seq = locate_rows<32>(a, id);
+  if (!seq.found) {
+    if (a.capacity == 0 && split == 0) clear_behind<T, 32>(a, seq, kvh);
+    return;
+  }
+  const int rows = seq.q_len * a.G;
+  const int row0 = seq.tile * 32;
+  if (row0 >= rows) return;
+  AttnWave<T, HD> w;
+  w.begin(a, seq, kvh, row0, rows);
+  const int tiles = (w.most + 31) / 32;
+  const int per_split = (tiles + a.splits - 1) / a.splits;
+  const int t_end = min(tiles, (split + 1) * per_split);
+  const T* k = static_cast<const T*>(a.k) + seq.b * a.k_batch + seq.s_off * a.k_row + (int64_t)kvh * a.k_head;
+  const T* v = static_cast<const T*>(a.v) + seq.b * a.v_batch + seq.s_off * a.v_row + (int64_t)kvh * a.v_head;
+  U* tile = reinterpret_cast<U*>(lds) + wave * SIZE;
+
+  TileStage<T, HD, 32, 64> stage_k, stage_v;
+  auto fetch_k = [&](int t) { stage_k.fetch(k + (int64_t)t * 32 * a.k_row, a.k_row, a.D, seq.s_len - t * 32); };
+  auto fetch_v = [&](int t) { stage_v.fetch(v + (int64_t)t * 32 * a.v_row, a.v_row, a.D, seq.s_len - t * 32); };
+  int t = __builtin_amdgcn_readfirstlane(split * per_split + wave);
+  if (t < t_end) {
+    fetch_k(t);
+    fetch_v(t);
+  }
+  for (; t < t_end; t += W) {
+    const int key0 = t * 32;
+    f32x16 s[1];
+    wave_order();
+    stage_k.store(tile, a.D);
+    if (t + W < t_end) fetch_k(t + W);
+    wave_order();
+    w.template scores<1>(tile, key0, s);
+    wave_order();
+    stage_v.store(tile, a.D);
+    wave_order();
+    if (key0 + 32 > w.least && __any(stage_v.nonfinite())) {
+      w.template add_nonfinite<1>(lds_p[wave], tile, key0, s);
+      wave_order();
+      clear_nonfinite(tile, SIZE, threadIdx.x & 63, 64);
+      wave_order();
+    }
+    if (t + W < t_end) fetch_v(t + W);
+    w.template values<1>(tile, s);
+  }
+
+  // the waves' parts: maximum, sums, then the rows one wave after another (a fixed order)
+  {
+    const float l = halves_sum(w.l);
+    if (w.half == 0) {
+      lds_ml[wave][w.lane][0] = w.m;
+      lds_ml[wave][w.lane][1] = l;
+    }
+  }
+  __syncthreads();
+  float m = -__builtin_inff(), l = 0.f;
+#pragma unroll
+  for (int i = 0; i < W; ++i) m = fmaxf(m, lds_ml[i][w.lane & 31][0]);
+  const float base = m == -__builtin_inff() ? 0.f : m;
+#pragma unroll
+  for (int i = 0; i < W; ++i) l = fmaf(lds_ml[i][w.lane & 31][1], exp2_fast(lds_ml[i][w.lane & 31][0] - base), l);
+  const float f = exp2_fast(w.m - base) * (a.splits == 1 ? inverse_sum(l) : 1.f);
+  float* join = reinterpret_cast<float*>(lds);
+  auto join_at = [](int r, int col) { return r * HD + (((col >> 2) ^ (r & 7)) << 2); };  // 8 rows at one column: 8 places
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    if (wave == i) {
+#pragma unroll
+      for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          f32x4v* to = reinterpret_cast<f32x4v*>(join + join_at(w.lane & 31, d * 32 + 8 * g + 4 * w.half));
+          f32x4v x = {w.o[d][g * 4] * f, w.o[d][g * 4 + 1] * f, w.o[d][g * 4 + 2] * f, w.o[d][g * 4 + 3] * f};
+          if (i > 0) x += *to;
+          *to = x;
+        }
+    }
+    __syncthreads();
+  }
+  const int64_t part = (((int64_t)id * a.KV + kvh) * a.splits + split) * 32;
+  if (wave == 0 && w.half == 0 && w.row < rows) {
+    if (a.splits > 1) {
+      a.part_ml[(part + w.lane) * 2] = m;
+      a.part_ml[(part + w.lane) * 2 + 1] = l;
+    } else if (a.lse) {
+      a.lse[(seq.q_off + w.token) * a.H + w.head] = log_sum(m, l);
+    }
+  }
+  for (int i = threadIdx.x; i < 32 * (HD / 4); i += 64 * W) {
+    const int r = i / (HD / 4), col = i % (HD / 4) * 4;
+    if (row0 + r >= rows) break;
+    const f32x4v y = *reinterpret_cast<const f32x4v*>(join + join_at(r, col));
+    const float x[4] = {y[0], y[1], y[2], y[3]};
+    const int token = div_g(a, row0 + r);
+    if (a.splits == 1)
+      store_out<T>(a, (seq.q_off + token) * a.H + (int64_t)kvh * a.G + (row0 + r - token * a.G), col, x);
+    else
+      store4<float>(a.part_o + (part + r) * a.D, col, a.D, x);
+  }
+}
+
+// Joins the parts of a row tile's keys: one wave per row, first its lanes over the parts (at most 64), then over the columns.
 template <typename T, int TILE>
 __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -240,66 +451,88 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
   const int row = seq.tile * TILE + at;
   if (row >= seq.q_len * a.G) return;
   const int64_t part = (((int64_t)id * a.KV + kvh) * a.splits) * TILE + at;
-  float m = -__builtin_inff();
-  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[(part + (int64_t)s * TILE) * 2]);
+  const bool mine = lane < a.splits;
+  const float m_part = mine ? a.part_ml[(part + (int64_t)lane * TILE) * 2] : -__builtin_inff();
+  const float l_part = mine ? a.part_ml[(part + (int64_t)lane * TILE) * 2 + 1] : 0.f;
+  float m = m_part;
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
   const float base = m == -__builtin_inff() ? 0.f : m;
-  float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  const float f = exp2_fast(m_part - base);
+  const float l = lanes_sum<64>(l_part * f);
+  __shared__ float factor[4][64];
+  factor[wave][lane] = f;
+  wave_order();
+  const float inv = inverse_sum(l);
+  const int64_t out = [&] {
+    const int token = div_g(a, row);
+    return (seq.q_off + token) * a.H + (int64_t)kvh * a.G + (row - token * a.G);
+  }();
+  const int col = lane * 4;
+  float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
   for (int s = 0; s < a.splits; ++s) {
-    const int64_t p = part + (int64_t)s * TILE;
-    const float f = exp2_fast(a.part_ml[p * 2] - base);
-    l = fmaf(a.part_ml[p * 2 + 1], f, l);
+    const float fs = factor[wave][s];
+    const float* p = a.part_o + (part + (int64_t)s * TILE) * a.D;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (lane + 64 * j < a.D) o[j] = fmaf(a.part_o[p * a.D + lane + 64 * j], f, o[j]);
+    for (int j = 0; j < 4; ++j) o[j] = fmaf(col + j < a.D ? p[col + j] : 0.f, fs, o[j]);
   }
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-  const int token = div_g(a, row);
-  const int64_t out = (seq.q_off + token) * a.H + (int64_t)kvh * a.G + row - token * a.G;
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (lane + 64 * j < a.D) static_cast<T*>(a.out)[out * a.D + lane + 64 * j] = from_f32<T>(o[j] * inv);
-  if (a.lse && lane == 0) a.lse[out] = l == 0.f ? -__builtin_inff() : m + log2f(l);
+  for (int j = 0; j < 4; ++j) o[j] *= inv;
+  store_out<T>(a, out, col, o);
+  if (a.lse && lane == 0) a.lse[out] = log_sum(m, l);
 }
 
 // ---- launches ----------------------------------------------------------------------------------------------------------
 struct AttnPlan {
+  bool few;         // 32-row tiles whose waves divide the keys, else 128-row tiles
   int64_t tiles;    // row tiles (a bound in a pack)
   int splits;
   size_t bytes;     // workspace
+  int tile() const { return few ? 32 : kAttnRows; }
 };
 
-inline AttnPlan attn_plan(int B, int64_t total_q, int64_t longest, int tokens, int KV, int G, int D) {
+// `tokens` > 0: a cache, every sequence has that many queries; else a pack, whose lengths are known on the device only.
+inline AttnPlan attn_plan(int B, int64_t total_q, int64_t total_s, int tokens, int KV, int G, int D) {
   AttnPlan p;
-  p.tiles = tokens > 0 ? B * ceil_div((int64_t)tokens * G, kAttnRows) : ceil_div(total_q * G, kAttnRows) + B;
-  const int64_t groups = p.tiles * KV;
-  // keys are divided only where the row tiles leave compute units idle; a part has at least 4 key tiles of the bound
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(groups, 1), longest / 256));
-  p.splits = std::min(p.splits, 64);
-  p.bytes = p.splits > 1 ? (size_t)(groups * p.splits * kAttnRows) * (size_t)(D + 2) * sizeof(float) : 0;
+  p.few = total_q * G <= (int64_t)32 * B;
+  p.tiles = tokens > 0 ? B * ceil_div((int64_t)tokens * G, p.tile()) : ceil_div(total_q * G, p.tile()) + B;
+  // Keys are divided where the row tiles leave compute units idle (two workgroups on each of 256), as far as every part
+  // of a sequence of the mean length keeps 256 keys.
+  const int64_t groups = std::max<int64_t>(p.tiles * KV, 1), mean = tokens > 0 ? total_s : total_s / std::max(B, 1);
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / groups, mean / 256, 64}));
+  p.bytes = p.splits > 1 ? (size_t)(groups * p.splits * p.tile()) * (size_t)(D + 2) * sizeof(float) : 0;
   return p;
 }
 
 template <typename T, int HD>
-int attn_forward_launch(const AttnArgs& a, int64_t tiles, hipStream_t stream, const char* what) {
-  hipLaunchKernelGGL((attn_forward_kernel<T, HD>), dim3((unsigned)(tiles * a.KV * a.splits)), dim3(256), 0, stream, a);
+int attn_forward_launch(const AttnArgs& a, const AttnPlan& p, hipStream_t stream, const char* what) {
+  const dim3 grid((unsigned)(p.tiles * a.KV * a.splits));
+  if (p.few)
+    hipLaunchKernelGGL((attn_few_rows_kernel<T, HD>), grid, dim3((64 * few_waves<T, HD>())), 0, stream, a);
+  else
+    hipLaunchKernelGGL((attn_forward_kernel<T, HD>), grid, dim3(256), 0, stream, a);
   int rc = launch_status(what);
   if (rc == 0 && a.splits > 1) {
-    hipLaunchKernelGGL((attn_join_kernel<T, kAttnRows>), dim3((unsigned)(tiles * a.KV * (kAttnRows / 4))), dim3(256), 0,
-                       stream, a);
+    const dim3 join((unsigned)(p.tiles * a.KV * (p.tile() / 4)));
+    if (p.few)
+      hipLaunchKernelGGL((attn_join_kernel<T, 32>), join, dim3(256), 0, stream, a);
+    else
+      hipLaunchKernelGGL((attn_join_kernel<T, kAttnRows>), join, dim3(256), 0, stream, a);
     rc = launch_status(what);
   }
   return rc;
 }
 
 template <typename T>
-int attn_forward_type(const AttnArgs& a, int64_t tiles, hipStream_t stream, const char* what) {
+int attn_forward_type(const AttnArgs& a, const AttnPlan& plan, hipStream_t stream, const char* what) {
   switch (attn_head_size(a.D)) {
-    case 32: return attn_forward_launch<T, 32>(a, tiles, stream, what);
-    case 64: return attn_forward_launch<T, 64>(a, tiles, stream, what);
-    case 96: return attn_forward_launch<T, 96>(a, tiles, stream, what);
-    case 128: return attn_forward_launch<T, 128>(a, tiles, stream, what);
-    case 192: return attn_forward_launch<T, 192>(a, tiles, stream, what);
-    default: return attn_forward_launch<T, 256>(a, tiles, stream, what);
+    case 32: return attn_forward_launch<T, 32>(a, plan, stream, what);
+    case 64: return attn_forward_launch<T, 64>(a, plan, stream, what);
+    case 96: return attn_forward_launch<T, 96>(a, plan, stream, what);
+    case 128: return attn_forward_launch<T, 128>(a, plan, stream, what);
+    case 192: return attn_forward_launch<T, 192>(a, plan, stream, what);
+    default: return attn_forward_launch<T, 256>(a, plan, stream, what);
   }
 }
 
@@ -355,11 +588,11 @@ int attn_forward_run(AttnArgs& a, int dtype, const AttnPlan& plan, void* workspa
     const int rc = ws.acquire(what, workspace, workspace_bytes, plan.bytes, s);
     if (rc != 0) return rc;
     a.part_o = reinterpret_cast<float*>(ws.base);
-    a.part_ml = a.part_o + plan.tiles * a.KV * a.splits * kAttnRows * a.D;
+    a.part_ml = a.part_o + plan.tiles * a.KV * a.splits * plan.tile() * a.D;
   }
-  int rc = dtype == V3D_F32   ? attn_forward_type<float>(a, plan.tiles, s, what)
-           : dtype == V3D_F16 ? attn_forward_type<f16>(a, plan.tiles, s, what)
-                              : attn_forward_type<bf16>(a, plan.tiles, s, what);
+  int rc = dtype == V3D_F32   ? attn_forward_type<float>(a, plan, s, what)
+           : dtype == V3D_F16 ? attn_forward_type<f16>(a, plan, s, what)
+                              : attn_forward_type<bf16>(a, plan, s, what);
   return ws.release(what, rc);
 }
 
@@ -373,8 +606,9 @@ size_t v3d_attention_pack_workspace_bytes(int B, int64_t total_q, int64_t total_
 }
 
 int v3d_attention_pack_fwd(const void* q, const void* k, const void* v, const int64_t* q_lengths,
-                           const int64_t* s_lengths, void* out, float* lse, int dtype, int B, int64_t total_q,
-                           int64_t total_s, int H, int KV, int D, const int64_t* strides, float scale, int causal,
+                           const int64_t* s_lengths, void* out, void* rest, float* lse, int dtype, int B,
+                           int64_t total_q, int64_t total_s, int H, int KV, int D, const int64_t* strides, float scale,
+                           int causal,
                            void* workspace, size_t workspace_bytes, int device, void* stream) {
   using namespace v3d;
   const char* what = "attention_pack";
@@ -388,6 +622,7 @@ int v3d_attention_pack_fwd(const void* q, const void* k, const void* v, const in
   a.k = k;
   a.v = v;
   a.out = out;
+  a.rest = dtype == V3D_F32 ? nullptr : rest;
   a.lse = lse;
   a.q_lengths = q_lengths;
   a.s_lengths = s_lengths;

@@ -22,21 +22,23 @@ struct AttnBwdArgs {
   void* dv;
 };
 
-// Keys (or rows) of a tile that passes by; two of them, of two tensors, in LDS.
+// Keys (or rows) of a tile that passes by; two of them (fp32 heads past 128: one), of two tensors, in LDS.
 template <typename T, int HD>
-constexpr int bwd_tile() { return HD * (int)sizeof(T) > 128 ? 32 : 64; }
+constexpr int bwd_tile() { return Kind<T>::P == 1 && HD <= 64 ? 64 : 32; }
+template <typename T, int HD>
+constexpr int bwd_buffers() { return Kind<T>::P == 3 && HD > 128 ? 1 : 2; }
 
 template <typename T, int HD>
-__global__ __launch_bounds__(256, HD * sizeof(T) <= 256 ? 2 : 1) void attn_backward_q_kernel(const AttnBwdArgs b) {
+__global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 128 : 64) ? 2 : 1) void attn_backward_q_kernel(const AttnBwdArgs b) {
   constexpr int HDP = attn_pow2(HD);
   constexpr int BN = bwd_tile<T, HD>();
   constexpr int NT = BN / 32;
-  constexpr int STEPS = HD / Mma<T>::kStep;
-  constexpr int USTEPS = 32 / Mma<T>::kStep;
+  constexpr int BUFS = bwd_buffers<T, HD>();
+  constexpr int STEPS = HD / 16;
   constexpr int DT = HD / 32;
-  typedef typename Mma<T>::Op Op;
-  __shared__ T lds_k[2][BN * HDP];
-  __shared__ T lds_v[2][BN * HDP];
+  typedef typename Kind<T>::U U;
+  __shared__ __attribute__((aligned(16))) U lds_k[BUFS][Kind<T>::P * BN * HDP];
+  __shared__ __attribute__((aligned(16))) U lds_v[BUFS][Kind<T>::P * BN * HDP];
 
   const AttnArgs& a = b.f;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -76,7 +78,7 @@ __global__ __launch_bounds__(256, HD * sizeof(T) <= 256 ? 2 : 1) void attn_backw
   const int64_t at0 = ((seq.q_off + token0) * a.H + (int64_t)kvh * a.G) * a.D;
   const int at_row = (int)(at * a.D - at0);
 
-  TileStage<T, HD, BN> stage_k, stage_v;
+  TileStage<T, HD, BN, 256> stage_k, stage_v;
   auto fetch = [&](int t) {
     stage_k.fetch(k + (int64_t)t * BN * a.k_row, a.k_row, a.D, seq.s_len - t * BN);
     stage_v.fetch(v + (int64_t)t * BN * a.v_row, a.v_row, a.D, seq.s_len - t * BN);
@@ -86,18 +88,21 @@ __global__ __launch_bounds__(256, HD * sizeof(T) <= 256 ? 2 : 1) void attn_backw
     stage_v.store(lds_v[buf], a.D);
   };
 
-  Op qf[STEPS], gf[STEPS];
+  Op<T> qf[STEPS], gf[STEPS];
   float delta = 0.f;
-  load_ops<T>(qf, q, (token - token0) * (int)a.q_row + (head - kvh * a.G) * (int)a.q_head, half, a.D);
-  load_ops<T>(gf, static_cast<const T*>(b.grad) + at0, at_row, half, a.D);
-  {
-    Op of[STEPS];
-    load_ops<T>(of, static_cast<const T*>(a.out) + at0, at_row, half, a.D);
+  load_ops<T>(qf, q, (token - token0) * (int)a.q_row + (head - kvh * a.G) * (int)a.q_head, half, a.D, true);
+  load_ops<T>(gf, static_cast<const T*>(b.grad) + at0, at_row, half, a.D, true);
+  // delta = grad . out, the output as it was before it was rounded
+  auto add_delta = [&](const void* out) {
+    Op<T> of[STEPS];
+    load_ops<T>(of, static_cast<const T*>(out) + at0, at_row, half, a.D, true);
 #pragma unroll
     for (int st = 0; st < STEPS; ++st)
 #pragma unroll
-      for (int j = 0; j < 16 / (int)sizeof(T); ++j) delta = fmaf((float)gf[st][j], (float)of[st][j], delta);
-  }
+      for (int j = 0; j < 8; ++j) delta = fmaf(number(gf[st], j), number(of[st], j), delta);
+  };
+  add_delta(a.out);
+  if (a.rest != nullptr) add_delta(a.rest);
   delta = halves_sum(delta);
   const float lse = a.lse[at];
   if (half == 0 && row < rows) b.delta[at] = delta;
@@ -116,8 +121,8 @@ __global__ __launch_bounds__(256, HD * sizeof(T) <= 256 ? 2 : 1) void attn_backw
       f32x16 s = zero16(), dp = zero16();
 #pragma unroll
       for (int st = 0; st < STEPS; ++st) {
-        s = Mma<T>::run(read_cols<T, HDP>(lds_k[buf], n * 32 + (lane & 31), st, half), qf[st], s);
-        dp = Mma<T>::run(read_cols<T, HDP>(lds_v[buf], n * 32 + (lane & 31), st, half), gf[st], dp);
+        s = product<T>(read_cols<T, HDP, BN>(lds_k[buf], n * 32 + (lane & 31), st, half), qf[st], s);
+        dp = product<T>(read_cols<T, HDP, BN>(lds_v[buf], n * 32 + (lane & 31), st, half), gf[st], dp);
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = exp2_fast(fmaf(s[r], c2, -lse)) * (dp[r] - delta);
@@ -127,11 +132,11 @@ __global__ __launch_bounds__(256, HD * sizeof(T) <= 256 ? 2 : 1) void attn_backw
           if (key0 + n * 32 + acc_row(r, half) >= limit) s[r] = 0.f;
       }
 #pragma unroll
-      for (int u = 0; u < USTEPS; ++u) {
-        const Op ds = pack_rows<T>(s, u);
+      for (int u = 0; u < 2; ++u) {
+        const Op<T> ds = pack_rows<T>(s, u);
 #pragma unroll
         for (int d = 0; d < DT; ++d)
-          acc[d] = Mma<T>::run(read_rows<T, HDP>(lds_k[buf], n * 32, u, d * 32, lane), ds, acc[d]);
+          acc[d] = product<T>(read_rows<T, HDP, BN>(lds_k[buf], n * 32, u, d * 32, lane), ds, acc[d]);
       }
     }
   };
@@ -141,16 +146,26 @@ __global__ __launch_bounds__(256, HD * sizeof(T) <= 256 ? 2 : 1) void attn_backw
     fetch(0);
     place_tile(0);
     __syncthreads();
-    for (int t = 0; t < tiles; t += 2) {
-      if (t + 1 < tiles) fetch(t + 1);
-      work(t, Const<0>{});
-      if (t + 1 < tiles) place_tile(1);
-      __syncthreads();
-      if (t + 1 >= tiles) break;
-      if (t + 2 < tiles) fetch(t + 2);
-      work(t + 1, Const<1>{});
-      if (t + 2 < tiles) place_tile(0);
-      __syncthreads();
+    if constexpr (BUFS == 2) {
+      for (int t = 0; t < tiles; t += 2) {
+        if (t + 1 < tiles) fetch(t + 1);
+        work(t, Const<0>{});
+        if (t + 1 < tiles) place_tile(1);
+        __syncthreads();
+        if (t + 1 >= tiles) break;
+        if (t + 2 < tiles) fetch(t + 2);
+        work(t + 1, Const<1>{});
+        if (t + 2 < tiles) place_tile(0);
+        __syncthreads();
+      }
+    } else {
+      for (int t = 0; t < tiles; ++t) {
+        if (t + 1 < tiles) fetch(t + 1);
+        work(t, Const<0>{});
+        __syncthreads();
+        if (t + 1 < tiles) place_tile(0);
+        __syncthreads();
+      }
     }
   }
   if (row < rows) store_rows<T, DT>(dq + at * a.D, acc, a.scale, a.D, half);
@@ -161,14 +176,14 @@ __global__ __launch_bounds__(256) void attn_backward_kv_kernel(const AttnBwdArgs
   constexpr int HDP = attn_pow2(HD);
   constexpr int BM = bwd_tile<T, HD>();
   constexpr int NT = BM / 32;
-  constexpr int STEPS = HD / Mma<T>::kStep;
-  constexpr int USTEPS = 32 / Mma<T>::kStep;
+  constexpr int BUFS = bwd_buffers<T, HD>();
+  constexpr int STEPS = HD / 16;
   constexpr int DT = HD / 32;
-  typedef typename Mma<T>::Op Op;
-  __shared__ T lds_q[2][BM * HDP];
-  __shared__ T lds_g[2][BM * HDP];
-  __shared__ float lds_lse[2][BM], lds_delta[2][BM];
-  __shared__ int lds_limit[2][BM];
+  typedef typename Kind<T>::U U;
+  __shared__ __attribute__((aligned(16))) U lds_q[BUFS][Kind<T>::P * BM * HDP];
+  __shared__ __attribute__((aligned(16))) U lds_g[BUFS][Kind<T>::P * BM * HDP];
+  __shared__ float lds_lse[BUFS][BM], lds_delta[BUFS][BM];
+  __shared__ int lds_limit[BUFS][BM];
 
   const AttnArgs& a = b.f;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -204,7 +219,7 @@ __global__ __launch_bounds__(256) void attn_backward_kv_kernel(const AttnBwdArgs
   const float* lse = a.lse + seq.q_off * a.H + kvh * a.G;
   const float* delta = b.delta + seq.q_off * a.H + kvh * a.G;
 
-  TileStage<T, HD, BM> stage_q, stage_g;
+  TileStage<T, HD, BM, 256> stage_q, stage_g;
   float stage_lse = 0.f, stage_delta = 0.f;
   int stage_limit = 0;
   auto fetch = [&](int row0) {
@@ -236,9 +251,9 @@ __global__ __launch_bounds__(256) void attn_backward_kv_kernel(const AttnBwdArgs
     }
   };
 
-  Op kf[STEPS], vf[STEPS];
-  load_ops<T>(kf, k, live ? (key - key0) * (int)a.k_row : -1, half, a.D);
-  load_ops<T>(vf, v, live ? (key - key0) * (int)a.v_row : -1, half, a.D);
+  Op<T> kf[STEPS], vf[STEPS];
+  load_ops<T>(kf, k, (key - key0) * (int)a.k_row, half, a.D, live);
+  load_ops<T>(vf, v, (key - key0) * (int)a.v_row, half, a.D, live);
   const float c2 = a.scale * kLog2e;
   f32x16 ak[DT], av[DT];
 #pragma unroll
@@ -254,8 +269,8 @@ __global__ __launch_bounds__(256) void attn_backward_kv_kernel(const AttnBwdArgs
       f32x16 s = zero16(), dp = zero16();
 #pragma unroll
       for (int st = 0; st < STEPS; ++st) {
-        s = Mma<T>::run(read_cols<T, HDP>(lds_q[buf], n * 32 + (lane & 31), st, half), kf[st], s);
-        dp = Mma<T>::run(read_cols<T, HDP>(lds_g[buf], n * 32 + (lane & 31), st, half), vf[st], dp);
+        s = product<T>(read_cols<T, HDP, BM>(lds_q[buf], n * 32 + (lane & 31), st, half), kf[st], s);
+        dp = product<T>(read_cols<T, HDP, BM>(lds_g[buf], n * 32 + (lane & 31), st, half), vf[st], dp);
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
@@ -269,12 +284,12 @@ __global__ __launch_bounds__(256) void attn_backward_kv_kernel(const AttnBwdArgs
           if (key >= lds_limit[buf][n * 32 + acc_row(r, half)]) s[r] = dp[r] = 0.f;
       }
 #pragma unroll
-      for (int u = 0; u < USTEPS; ++u) {
-        const Op p = pack_rows<T>(s, u), ds = pack_rows<T>(dp, u);
+      for (int u = 0; u < 2; ++u) {
+        const Op<T> p = pack_rows<T>(s, u), ds = pack_rows<T>(dp, u);
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-          av[d] = Mma<T>::run(read_rows<T, HDP>(lds_g[buf], n * 32, u, d * 32, lane), p, av[d]);
-          ak[d] = Mma<T>::run(read_rows<T, HDP>(lds_q[buf], n * 32, u, d * 32, lane), ds, ak[d]);
+          av[d] = product<T>(read_rows<T, HDP, BM>(lds_g[buf], n * 32, u, d * 32, lane), p, av[d]);
+          ak[d] = product<T>(read_rows<T, HDP, BM>(lds_q[buf], n * 32, u, d * 32, lane), ds, ak[d]);
         }
       }
     }
@@ -285,16 +300,26 @@ __global__ __launch_bounds__(256) void attn_backward_kv_kernel(const AttnBwdArgs
     fetch(begin);
     place_tile(0);
     __syncthreads();
-    for (int r = begin; r < rows; r += 2 * BM) {
-      if (r + BM < rows) fetch(r + BM);
-      work(r, Const<0>{});
-      if (r + BM < rows) place_tile(1);
-      __syncthreads();
-      if (r + BM >= rows) break;
-      if (r + 2 * BM < rows) fetch(r + 2 * BM);
-      work(r + BM, Const<1>{});
-      if (r + 2 * BM < rows) place_tile(0);
-      __syncthreads();
+    if constexpr (BUFS == 2) {
+      for (int r = begin; r < rows; r += 2 * BM) {
+        if (r + BM < rows) fetch(r + BM);
+        work(r, Const<0>{});
+        if (r + BM < rows) place_tile(1);
+        __syncthreads();
+        if (r + BM >= rows) break;
+        if (r + 2 * BM < rows) fetch(r + 2 * BM);
+        work(r + BM, Const<1>{});
+        if (r + 2 * BM < rows) place_tile(0);
+        __syncthreads();
+      }
+    } else {
+      for (int r = begin; r < rows; r += BM) {
+        if (r + BM < rows) fetch(r + BM);
+        work(r, Const<0>{});
+        __syncthreads();
+        if (r + BM < rows) place_tile(0);
+        __syncthreads();
+      }
     }
   }
   if (!live) return;
@@ -345,7 +370,7 @@ size_t v3d_attention_pack_bwd_workspace_bytes(int B, int64_t total_q, int64_t to
 }
 
 int v3d_attention_pack_bwd(const void* grad, const void* q, const void* k, const void* v, const void* out,
-                           const float* lse, const int64_t* q_lengths, const int64_t* s_lengths, void* grad_q,
+                           const void* rest, const float* lse, const int64_t* q_lengths, const int64_t* s_lengths, void* grad_q,
                            void* grad_k, void* grad_v, int dtype, int B, int64_t total_q, int64_t total_s, int H, int KV,
                            int D, const int64_t* strides, float scale, int causal, void* workspace,
                            size_t workspace_bytes, int device, void* stream) {
@@ -363,6 +388,7 @@ int v3d_attention_pack_bwd(const void* grad, const void* q, const void* k, const
   a.k = k;
   a.v = v;
   a.out = const_cast<void*>(out);
+  a.rest = dtype == V3D_F32 ? nullptr : const_cast<void*>(rest);
   a.lse = const_cast<float*>(lse);
   a.q_lengths = q_lengths;
   a.s_lengths = s_lengths;

@@ -25,6 +25,7 @@ struct AttnArgs {
   const void* k;
   const void* v;
   void* out;                 // (total_q, H, D) contiguous
+  void* rest;                // what rounding took from out, in its type (16-bit types, for the backward); or NULL
   float* lse;                // (total_q, H) log2 of the sum of exponentials, -inf for a row without keys; or NULL
   const int64_t* q_lengths;  // (B), NULL in a cache: every sequence has `tokens` queries
   const int64_t* s_lengths;  // (B)
@@ -160,35 +161,76 @@ __device__ __forceinline__ AttnSeq locate_rows(const AttnArgs& a, int64_t t) {
   return a.capacity > 0 ? locate_cache<TILE>(a, t) : locate<TILE, false>(a, t);
 }
 
-// ---- tiles in LDS ------------------------------------------------------------------------------------------------------
-// A tile is some rows of HDP elements (the head size rounded up to a power of two), moved in 16-byte chunks.  It is read in
-// two ways: 16 consecutive rows at one column, 16 bytes each (read_cols), and along the rows (read_rows: 4 consecutive rows
-// at 64 consecutive bytes for 16-bit types, two rows 4 apart at 128 bytes for fp32).  Chunks sit at their column XOR f(row),
-// f chosen so that both ways touch each of the 64 banks once: f takes 16 values over 16 rows that start a bank line, and
-// its bits that move 64 (fp32: 128) bytes change between the rows of one read_rows access.
-template <typename T, int HDP>
-__device__ __forceinline__ int place(int row, int chunk) {
-  constexpr int CPR = HDP * (int)sizeof(T) / 16;
-  if constexpr (sizeof(T) == 2) {
-    if constexpr (CPR >= 16) return chunk ^ (((row & 3) << 2) | ((row >> 2) & 3));
-    if constexpr (CPR == 8) return chunk ^ ((((row >> 1) & 1) << 2) | ((row >> 2) & 3));
-    return chunk ^ ((row >> 2) & 3);
-  } else {
-    if constexpr (CPR >= 16) return chunk ^ ((((row >> 2) & 1) << 3) | (((row >> 3) & 1) << 2) | (row & 3));
-    return chunk ^ ((row >> 1) & 7);
+// ---- numbers of the products -------------------------------------------------------------------------------------------
+// 16-bit types go into the matrix instructions as they are (exact products, fp32 sums).  An fp32 number goes in as three bf16
+// numbers that add up to it exactly (8 + 8 + 8 bits, cut off, so nothing overflows), and a product of two as the six of the
+// nine partial products that reach 2^-24 of it: the same accuracy as fp32 products in 6 x 32 cycles where the fp32
+// matrix instruction takes 8 x 64.  An infinity among fp32 inputs
+// becomes a NaN where it is seen.
+template <typename T>
+struct Kind {
+  typedef T U;                     // what lies in LDS and goes into the instructions
+  static constexpr int P = 1;      // how many of them make a number
+};
+template <>
+struct Kind<float> {
+  typedef bf16 U;
+  static constexpr int P = 3;
+};
+
+template <typename U>
+struct Vec8;
+template <>
+struct Vec8<bf16> {
+  typedef bf16 type __attribute__((ext_vector_type(8)));
+};
+template <>
+struct Vec8<f16> {
+  typedef f16 type __attribute__((ext_vector_type(8)));
+};
+
+// An operand: 8 numbers of a lane.
+template <typename T>
+struct Op {
+  typename Vec8<typename Kind<T>::U>::type part[Kind<T>::P];
+};
+
+template <typename T>
+__device__ __forceinline__ float number(const Op<T>& op, int j) {
+  float x = 0.f;
+#pragma unroll
+  for (int p = Kind<T>::P - 1; p >= 0; --p) x += to_f32(op.part[p][j]);  // exact
+  return x;
+}
+
+__device__ __forceinline__ Op<float> split8(const float (&x)[8]) {
+  unsigned word[3][4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    unsigned a[3], b[3];
+    float x0 = x[2 * j], x1 = x[2 * j + 1];
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+      a[p] = __float_as_uint(x0);
+      b[p] = __float_as_uint(x1);
+      x0 -= __uint_as_float(a[p] & 0xffff0000u);
+      x1 -= __uint_as_float(b[p] & 0xffff0000u);
+      word[p][j] = __builtin_amdgcn_perm(b[p], a[p], 0x07060302u);  // the upper halves
+    }
   }
+  Op<float> op;
+#pragma unroll
+  for (int p = 0; p < 3; ++p) {
+    const u32x4 w = {word[p][0], word[p][1], word[p][2], word[p][3]};
+    op.part[p] = __builtin_bit_cast(Vec8<bf16>::type, w);
+  }
+  return op;
 }
 
-// Offset in elements of element `col` of `row`.
-template <typename T, int HDP>
-__device__ __forceinline__ int tile_at(int row, int col) {
-  constexpr int E = 16 / (int)sizeof(T);
-  return row * HDP + place<T, HDP>(row, col / E) * E + col % E;
-}
-
+// ---- loads -------------------------------------------------------------------------------------------------------------
 // Loads go through a buffer descriptor: what lies past its range comes back as zeros without a branch, so all loads of a
-// tile are under way together.  Columns from D on are zeros too: a 16-byte chunk past D is placed out of any range, a chunk
-// that D ends inside is read up to D and shifted into place (hence D >= 16 bytes).
+// tile are under way together.  Columns from D on are zeros too: 16 bytes past D are placed out of any range, 16 bytes that
+// D ends inside are read up to D and shifted into place (hence a head of at least 16 bytes).
 constexpr int kOutOfRange = 0x7fffffff;
 
 __device__ __forceinline__ u32x4 load_buffer(const void* base, int bytes, int offset) {
@@ -196,67 +238,125 @@ __device__ __forceinline__ u32x4 load_buffer(const void* base, int bytes, int of
                                                offset, 0, 0);
 }
 
-// The byte offset of the chunk at column `col` of a row that starts at element `at`.
+// 8 numbers as they come from memory.
 template <typename T>
-__device__ __forceinline__ int chunk_offset(int at, int col, int D) {
-  constexpr int E = 16 / (int)sizeof(T);
-  return col >= D ? kOutOfRange : (at + min(col, D - E)) * (int)sizeof(T);
-}
-template <typename T>
-__device__ __forceinline__ u32x4 chunk_shift(u32x4 c, int col, int D) {
-  constexpr int E = 16 / (int)sizeof(T);
-  const int by = col < D ? max(0, col + E - D) : 0;
-  unsigned __int128 x = __builtin_bit_cast(unsigned __int128, c);
-  x >>= by * 8 * (int)sizeof(T);
-  return __builtin_bit_cast(u32x4, x);
-}
+struct Raw {
+  static constexpr int L = (int)sizeof(T) / 2;      // 16-byte loads
+  static constexpr int E = 16 / (int)sizeof(T);     // numbers of a load
+  u32x4 c[L];
 
-// A tile of ROWS rows on its way from memory to LDS: 256 threads, CH chunks of 16 bytes each, in registers.
-template <typename T, int HD, int ROWS>
-struct TileStage {
-  static constexpr int E = 16 / (int)sizeof(T);
-  static constexpr int CPR = HD / E;                // chunks of a row
-  static constexpr int CH = (ROWS * CPR + 255) / 256;
-  static constexpr bool kEven = ROWS * CPR % 256 == 0;  // else the last chunk of some threads repeats the last row's
-  u32x4 c[CH];
-
-  static __device__ __forceinline__ int row_of(int i) {
-    const int r = (i * 256 + (int)threadIdx.x) / CPR;
-    return kEven ? r : min(r, ROWS - 1);
+  // Columns [col, col + 8) of a row that starts at element `at` from `base`; `there` false: zeros.
+  __device__ __forceinline__ void load(const T* base, int bytes, int at, int col, int D, bool there) {
+#pragma unroll
+    for (int l = 0; l < L; ++l) {
+      const int c0 = col + l * E;
+      c[l] = load_buffer(base, bytes, !there || c0 >= D ? kOutOfRange : (at + min(c0, D - E)) * (int)sizeof(T));
+    }
   }
-  static __device__ __forceinline__ int col_of(int i) { return (i * 256 + (int)threadIdx.x) % CPR * E; }
+  __device__ __forceinline__ Op<T> op(int col, int D) const {
+    u32x4 v[L];
+#pragma unroll
+    for (int l = 0; l < L; ++l) {
+      v[l] = c[l];
+      if (D % E != 0) {
+        const int c0 = col + l * E, by = c0 < D ? max(0, c0 + E - D) : 0;
+        unsigned __int128 x = __builtin_bit_cast(unsigned __int128, v[l]);
+        x >>= by * 8 * (int)sizeof(T);
+        v[l] = __builtin_bit_cast(u32x4, x);
+      }
+    }
+    if constexpr (L == 1) {
+      Op<T> r;
+      r.part[0] = __builtin_bit_cast(typename Vec8<T>::type, v[0]);
+      return r;
+    } else {
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = __uint_as_float(v[j / 4][j % 4]);
+      return split8(x);
+    }
+  }
+  __device__ __forceinline__ bool nonfinite() const {
+    bool bad = false;
+#pragma unroll
+    for (int l = 0; l < L; ++l) {
+      const Packed<T, E> v = __builtin_bit_cast(Packed<T , E>, c[l]);
+#pragma unroll
+      for (int j = 0; j < E; ++j) bad |= !(__builtin_fabsf(to_f32(v.v[j])) < __builtin_inff());
+    }
+    return bad;
+  }
+};
 
-  // Rows [0, count) (count >= 1) at `base`, `stride` elements apart (64 strides stay below 2^31 bytes).
+// The operands of all product steps over the head size from one row in memory: `at` = this lane's row in elements from
+// `base` (wave-uniform).
+template <typename T, int STEPS>
+__device__ __forceinline__ void load_ops(Op<T> (&op)[STEPS], const T* base, int at, int half, int D, bool there) {
+  Raw<T> raw[STEPS];
+#pragma unroll
+  for (int st = 0; st < STEPS; ++st) raw[st].load(base, kOutOfRange, at, st * 16 + 8 * half, D, there);
+#pragma unroll
+  for (int st = 0; st < STEPS; ++st) op[st] = raw[st].op(st * 16 + 8 * half, D);
+}
+
+// ---- tiles in LDS ------------------------------------------------------------------------------------------------------
+// A tile is P planes of ROWS rows of HDP 16-bit numbers (the head size rounded up to a power of two), moved in chunks of 8.
+// It is read in two ways: 16 consecutive rows at one chunk (read_cols), and 4 consecutive rows at 64 consecutive bytes
+// (read_rows).  Chunks sit at their column XOR f(row), f chosen so that both ways touch each of the 64 banks once: f takes
+// 16 values over 16 rows that start a bank line, and its bits that move 64 bytes change between consecutive rows.
+template <int HDP>
+__device__ __forceinline__ int place(int row, int chunk) {
+  constexpr int CPR = HDP / 8;
+  if constexpr (CPR >= 16) return chunk ^ (((row & 3) << 2) | ((row >> 2) & 3));
+  if constexpr (CPR == 8) return chunk ^ ((((row >> 1) & 1) << 2) | ((row >> 2) & 3));
+  return chunk ^ ((row >> 2) & 3);
+}
+
+// Offset of element `col` of `row` in a plane.
+template <int HDP>
+__device__ __forceinline__ int tile_at(int row, int col) {
+  return row * HDP + place<HDP>(row, col / 8) * 8 + col % 8;
+}
+
+// A tile on its way from memory to LDS in the registers of THREADS threads.
+template <typename T, int HD, int ROWS, int THREADS>
+struct TileStage {
+  typedef typename Kind<T>::U U;
+  static constexpr int CPR = HD / 8;                // chunks of a row
+  static constexpr int CH = (ROWS * CPR + THREADS - 1) / THREADS;
+  static constexpr bool kEven = ROWS * CPR % THREADS == 0;  // else the last chunk of some threads repeats the last row's
+  Raw<T> c[CH];
+
+  static __device__ __forceinline__ int index(int i) { return i * THREADS + (int)threadIdx.x % THREADS; }
+  static __device__ __forceinline__ int row_of(int i) { return kEven ? index(i) / CPR : min(index(i) / CPR, ROWS - 1); }
+  static __device__ __forceinline__ int col_of(int i) { return index(i) % CPR * 8; }
+
+  // Rows [0, count) (count >= 1) at `base`, `stride` elements apart (a tile spans less than 2^31 bytes).
   __device__ __forceinline__ void fetch(const T* base, int64_t stride, int D, int count) {
     const int bytes = ((min(count, ROWS) - 1) * (int)stride + D) * (int)sizeof(T);
 #pragma unroll
-    for (int i = 0; i < CH; ++i) c[i] = load_buffer(base, bytes, chunk_offset<T>(row_of(i) * (int)stride, col_of(i), D));
+    for (int i = 0; i < CH; ++i) c[i].load(base, bytes, row_of(i) * (int)stride, col_of(i), D, true);
   }
   // The same for rows at offsets of their own (elements, non-negative, below 2^29).
   template <typename Offset>
   __device__ __forceinline__ void fetch_at(const T* base, Offset offset, int D, int count) {
 #pragma unroll
-    for (int i = 0; i < CH; ++i)
-      c[i] = load_buffer(base, kOutOfRange,
-                         row_of(i) < count ? chunk_offset<T>(offset(row_of(i)), col_of(i), D) : kOutOfRange);
+    for (int i = 0; i < CH; ++i) c[i].load(base, kOutOfRange, offset(row_of(i)), col_of(i), D, row_of(i) < count);
   }
-  __device__ __forceinline__ void store(T* tile, int D) {
+  __device__ __forceinline__ void store(U* tile, int D) const {
     constexpr int HDP = attn_pow2(HD);
-    if (D % E != 0) {
 #pragma unroll
-      for (int i = 0; i < CH; ++i) c[i] = chunk_shift<T>(c[i], col_of(i), D);
+    for (int i = 0; i < CH; ++i) {
+      const Op<T> op = c[i].op(col_of(i), D);
+#pragma unroll
+      for (int p = 0; p < Kind<T>::P; ++p)
+        *reinterpret_cast<typename Vec8<U>::type*>(tile + p * (ROWS * HDP) + tile_at<HDP>(row_of(i), col_of(i))) = op.part[p];
     }
-#pragma unroll
-    for (int i = 0; i < CH; ++i) *reinterpret_cast<u32x4*>(tile + tile_at<T, HDP>(row_of(i), col_of(i))) = c[i];
   }
   __device__ __forceinline__ bool nonfinite() const {
     bool bad = false;
 #pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      const Packed<T, E> v = __builtin_bit_cast(Packed<T , E>, c[i]);
-#pragma unroll
-      for (int j = 0; j < E; ++j) bad |= !(__builtin_fabsf(to_f32(v.v[j])) < __builtin_inff());
-    }
+    for (int i = 0; i < CH; ++i) bad |= c[i].nonfinite();
     return bad;
   }
 };
@@ -274,99 +374,103 @@ struct Const {
 // order in which the result layout holds the keys (no lane exchange in between).
 __device__ __forceinline__ constexpr int acc_row(int r, int half) { return 8 * (r / 4) + 4 * half + r % 4; }
 
-// Operands of one product step: 16-bit types take 16 summands a step (8 per lane: 8 half + j), fp32 8 summands as four
-// instructions of two (4 per lane: 4 half + j).
+__device__ __forceinline__ f32x16 mfma(Vec8<bf16>::type a, Vec8<bf16>::type b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma(Vec8<f16>::type a, Vec8<f16>::type b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// c + a b over 16 summands (8 of each half of the lanes); fp32: the partial products from the small to the large.
 template <typename T>
-struct Mma;
+__device__ __forceinline__ f32x16 product(const Op<T>& a, const Op<T>& b, f32x16 c) {
+  if constexpr (Kind<T>::P == 3) {
+    c = mfma(a.part[0], b.part[2], c);
+    c = mfma(a.part[2], b.part[0], c);
+    c = mfma(a.part[1], b.part[1], c);
+    c = mfma(a.part[0], b.part[1], c);
+    c = mfma(a.part[1], b.part[0], c);
+  }
+  return mfma(a.part[0], b.part[0], c);
+}
 
-template <>
-struct Mma<bf16> {
-  typedef bf16 Op __attribute__((ext_vector_type(8)));
-  static constexpr int kStep = 16;
-  static __device__ __forceinline__ f32x16 run(Op a, Op b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-  }
-};
-template <>
-struct Mma<f16> {
-  typedef f16 Op __attribute__((ext_vector_type(8)));
-  static constexpr int kStep = 16;
-  static __device__ __forceinline__ f32x16 run(Op a, Op b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-  }
-};
-template <>
-struct Mma<float> {
-  typedef float Op __attribute__((ext_vector_type(4)));
-  static constexpr int kStep = 8;
-  static __device__ __forceinline__ f32x16 run(Op a, Op b, f32x16 c) {
+// The A operand of a product step whose summands are COLUMNS of the tile: row `row`, columns [16 step + 8 half, + 8).
+template <typename T, int HDP, int ROWS>
+__device__ __forceinline__ Op<T> read_cols(const typename Kind<T>::U* tile, int row, int step, int half) {
+  typedef typename Kind<T>::U U;
+  Op<T> op;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
-    return c;
-  }
-};
-
-// The A (or B) operand of a product step whose summands are COLUMNS of the tile: row `row`, columns
-// [step * kStep + E * half, + E), one 16-byte read.
-template <typename T, int HDP>
-__device__ __forceinline__ typename Mma<T>::Op read_cols(const T* tile, int row, int step, int half) {
-  constexpr int E = 16 / (int)sizeof(T);
-  return *reinterpret_cast<const typename Mma<T>::Op*>(tile + tile_at<T, HDP>(row, step * 2 * E + E * half));
+  for (int p = 0; p < Kind<T>::P; ++p)
+    op.part[p] = *reinterpret_cast<const typename Vec8<U>::type*>(tile + p * (ROWS * HDP) +
+                                                                  tile_at<HDP>(row, step * 16 + 8 * half));
+  return op;
 }
 
 // The A operand of a product step whose summands are ROWS of the tile, in the order of the result layout: step u of a
-// 32-row block covers registers [u * R, u * R + R) of that layout (R = 8 for 16-bit types, 4 for fp32).  Lane l stands for
-// column d0 + l % 32.
-template <typename T, int HDP>
-__device__ __forceinline__ typename Mma<T>::Op read_rows(const T* tile, int row0, int u, int d0, int lane) {
-  if constexpr (sizeof(T) == 2) {
-    // gfx950's transposing LDS read: 16 lanes read 4 rows x 16 columns (lane i: row i / 4, columns 4 (i % 4) ..) and each
-    // is handed its column's 4 rows.
-    const int i = lane & 15;
-    const int half = lane >> 5;
-    const int col = d0 + (lane & 16) + 4 * (i & 3);
+// 32-row block covers registers [8 u, 8 u + 8) of that layout.  Lane l stands for column d0 + l % 32.  gfx950's transposing
+// LDS read: 16 lanes read 4 rows x 16 columns (lane i: row i / 4, columns 4 (i % 4) ..), each is handed its column's 4 rows.
+template <typename T, int HDP, int ROWS>
+__device__ __forceinline__ Op<T> read_rows(const typename Kind<T>::U* tile, int row0, int u, int d0, int lane) {
+  typedef typename Kind<T>::U U;
+  const int i = lane & 15;
+  const int half = lane >> 5;
+  const int col = d0 + (lane & 16) + 4 * (i & 3);
+  Op<T> op;
+#pragma unroll
+  for (int p = 0; p < Kind<T>::P; ++p) {
     union {
-      s16x4 part[2];
-      typename Mma<T>::Op op;
+      s16x4 quad[2];
+      typename Vec8<U>::type all;
     } r;
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      const int row = row0 + 16 * u + 8 * p + 4 * half + (i >> 2);
-      T* at = const_cast<T*>(tile) + tile_at<T, HDP>(row, col);
-      r.part[p] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+    for (int h = 0; h < 2; ++h) {
+      const int row = row0 + 16 * u + 8 * h + 4 * half + (i >> 2);
+      U* at = const_cast<U*>(tile) + p * (ROWS * HDP) + tile_at<HDP>(row, col);
+      r.quad[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
           (__attribute__((address_space(3))) s16x4*)reinterpret_cast<s16x4*>(at));
     }
-    return r.op;
-  } else {
-    typename Mma<T>::Op op;
+    op.part[p] = r.all;
+  }
+  return op;
+}
+
+// The result layout's registers [8 u, 8 u + 8) of a 32 x 32 block as the B operand that goes with read_rows.  16-bit types:
+// rounded to the type, which the values have anyway (half a step of each summand, of either sign).
+template <typename T>
+__device__ __forceinline__ Op<T> pack_rows(const f32x16& x, int u) {
+  if constexpr (Kind<T>::P == 3) {
+    float v[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      op[j] = tile[tile_at<T, HDP>(row0 + 8 * u + 4 * (lane >> 5) + j, d0 + (lane & 31))];
+    for (int j = 0; j < 8; ++j) v[j] = x[u * 8 + j];
+    return split8(v);
+  } else {
+    Op<T> op;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) op.part[0][j] = from_f32<T>(x[u * 8 + j]);
     return op;
   }
 }
 
-// The result layout's registers [u * R, u * R + R) of a 32 x 32 block as the B operand that goes with read_rows.
-template <typename T>
-__device__ __forceinline__ typename Mma<T>::Op pack_rows(const f32x16& p, int u) {
-  constexpr int R = sizeof(T) == 2 ? 8 : 4;
-  typename Mma<T>::Op op;
+constexpr float kLog2e = 1.44269504088896340736f;
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }  // v_exp_f32; 2^-inf = 0
+
+__device__ __forceinline__ f32x16 zero16() {
+  f32x16 z;
 #pragma unroll
-  for (int j = 0; j < R; ++j) op[j] = from_f32<T>(p[u * R + j]);
-  return op;
+  for (int r = 0; r < 16; ++r) z[r] = 0.f;
+  return z;
 }
 
-// The operands of all product steps over the head size from one row in memory: `at` = this lane's row in elements from
-// `base` (wave-uniform), negative = a row of zeros.
-template <typename T, int STEPS>
-__device__ __forceinline__ void load_ops(typename Mma<T>::Op (&op)[STEPS], const T* base, int at, int half, int D) {
-  constexpr int E = 16 / (int)sizeof(T);
+// 4 elements of a row from `col` on, as far as D goes.
+template <typename T>
+__device__ __forceinline__ void store4(T* row, int col, int D, const float (&v)[4]) {
+  if (col + 4 <= D) {
+    store_vec<T, 4>(row + col, v);
+  } else {
 #pragma unroll
-  for (int st = 0; st < STEPS; ++st) {
-    const int col = st * 2 * E + E * half;
-    u32x4 c = load_buffer(base, kOutOfRange, at < 0 ? kOutOfRange : chunk_offset<T>(at, col, D));
-    if (D % E != 0) c = chunk_shift<T>(c, col, D);
-    op[st] = __builtin_bit_cast(typename Mma<T>::Op, c);
+    for (int j = 0; j < 4; ++j)
+      if (col + j < D) row[col + j] = from_f32<T>(v[j]);
   }
 }
 
@@ -377,15 +481,8 @@ __device__ __forceinline__ void store_rows(T* row, const f32x16 (&acc)[DT], floa
   for (int d = 0; d < DT; ++d)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const int col = d * 32 + 8 * g + 4 * half;
       const float v[4] = {acc[d][g * 4] * f, acc[d][g * 4 + 1] * f, acc[d][g * 4 + 2] * f, acc[d][g * 4 + 3] * f};
-      if (col + 4 <= D) {
-        store_vec<T, 4>(row + col, v);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (col + j < D) row[col + j] = from_f32<T>(v[j]);
-      }
+      store4<T>(row, d * 32 + 8 * g + 4 * half, D, v);
     }
 }
 
@@ -402,17 +499,6 @@ __device__ __forceinline__ float halves_max(float x) {
 __device__ __forceinline__ float halves_sum(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-
-constexpr float kLog2e = 1.44269504088896340736f;
-
-__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }  // v_exp_f32; 2^-inf = 0
-
-__device__ __forceinline__ f32x16 zero16() {
-  f32x16 z;
-#pragma unroll
-  for (int r = 0; r < 16; ++r) z[r] = 0.f;
-  return z;
 }
 
 // Host side: the heads, and the division by the group's size as a product (exact for 31-bit numerators: the multiplier is

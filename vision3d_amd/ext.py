@@ -1127,9 +1127,10 @@ def _attention_check(name, q, k, v, q_lengths, s_lengths):
     return dtype, _strides(q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1))
 
 
-def attention_pack_forward(q_feats, k_feats, v_feats, q_lengths, s_lengths, targets, lse, scale, causal):
+def attention_pack_forward(q_feats, k_feats, v_feats, q_lengths, s_lengths, targets, lse, scale, causal, rest=None):
     """targets (N, H, D) = attention of ``q_feats`` (N, H, D) over ``k_feats`` / ``v_feats`` (M, KV, D) inside every
-    sequence of the pack, ``lse`` (N, H) fp32 or None; see include/v3d_hip.h."""
+    sequence of the pack; for the backward: ``lse`` (N, H) fp32 and, of 16-bit types, ``rest`` (N, H, D) = what rounding took
+    from ``targets``; see include/v3d_hip.h."""
     name = "attention_pack_forward"
     dtype, strides = _attention_check(name, q_feats, k_feats, v_feats, q_lengths, s_lengths)
     _check_cuda_contiguous(targets, "targets")
@@ -1142,20 +1143,25 @@ def attention_pack_forward(q_feats, k_feats, v_feats, q_lengths, s_lengths, targ
         _check_float(lse, "lse")
         if tuple(lse.shape) != (N, H):
             raise RuntimeError(f"{name}: lse must have shape {(N, H)}")
-    _same_device(name, q_feats, targets, lse)
+    if rest is not None:
+        _check_cuda_contiguous(rest, "rest")
+        _same_dtype(name, q_feats, rest)
+        if rest.shape != q_feats.shape:
+            raise RuntimeError(f"{name}: rest must have the shape of q_feats")
+    _same_device(name, q_feats, targets, lse, rest)
     B, M, KV = q_lengths.numel(), k_feats.size(0), k_feats.size(1)
     dev, stream = _where(q_feats)
     lib = _lib.lib()
     ws, wp, wn = _ws_args(lib.v3d_attention_pack_workspace_bytes(B, N, M, H, KV, D), q_feats)
     _lib.check(lib.v3d_attention_pack_fwd(q_feats.data_ptr(), k_feats.data_ptr(), v_feats.data_ptr(),
-                                          q_lengths.data_ptr(), s_lengths.data_ptr(), targets.data_ptr(), _ptr(lse),
+                                          q_lengths.data_ptr(), s_lengths.data_ptr(), targets.data_ptr(), _ptr(rest), _ptr(lse),
                                           dtype, B, N, M, H, KV, D, strides, float(scale), int(bool(causal)), wp, wn,
                                           dev, stream), name)
 
 
 def attention_pack_backward(target_grads, q_feats, k_feats, v_feats, targets, lse, q_lengths, s_lengths, q_grads, k_grads,
-                            v_grads, scale, causal):
-    """The gradients of ``attention_pack_forward``, from its inputs, its ``targets`` and its ``lse``."""
+                            v_grads, scale, causal, rest=None):
+    """The gradients of ``attention_pack_forward``, from its inputs, ``targets``, ``lse`` and (16-bit types) ``rest``."""
     name = "attention_pack_backward"
     dtype, strides = _attention_check(name, q_feats, k_feats, v_feats, q_lengths, s_lengths)
     N, H, D = q_feats.shape
@@ -1170,13 +1176,18 @@ def attention_pack_backward(target_grads, q_feats, k_feats, v_feats, targets, ls
     _check_float(lse, "lse")
     if tuple(lse.shape) != (N, H):
         raise RuntimeError(f"{name}: lse must have shape {(N, H)}")
-    _same_device(name, q_feats, target_grads, targets, lse, q_grads, k_grads, v_grads)
+    if rest is not None:
+        _check_cuda_contiguous(rest, "rest")
+        _same_dtype(name, q_feats, rest)
+        if rest.shape != q_feats.shape:
+            raise RuntimeError(f"{name}: rest must have the shape of q_feats")
+    _same_device(name, q_feats, target_grads, targets, lse, q_grads, k_grads, v_grads, rest)
     dev, stream = _where(q_feats)
     lib = _lib.lib()
     ws, wp, wn = _ws_args(lib.v3d_attention_pack_bwd_workspace_bytes(B, N, M, H, KV, D), q_feats)
     _lib.check(lib.v3d_attention_pack_bwd(target_grads.data_ptr(), q_feats.data_ptr(), k_feats.data_ptr(),
-                                          v_feats.data_ptr(), targets.data_ptr(), lse.data_ptr(), q_lengths.data_ptr(),
-                                          s_lengths.data_ptr(), q_grads.data_ptr(), k_grads.data_ptr(),
+                                          v_feats.data_ptr(), targets.data_ptr(), _ptr(rest), lse.data_ptr(),
+                                          q_lengths.data_ptr(), s_lengths.data_ptr(), q_grads.data_ptr(), k_grads.data_ptr(),
                                           v_grads.data_ptr(), dtype, B, N, M, H, KV, D, strides, float(scale),
                                           int(bool(causal)), wp, wn, dev, stream), name)
 

@@ -36,18 +36,20 @@ class _AttentionPack(torch.autograd.Function):
         q, k, v = _rows(q), _rows(k), _rows(v)
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
-        ext.attention_pack_forward(q, k, v, q_lengths, s_lengths, out, lse, scale, causal)
-        ctx.save_for_backward(q, k, v, out, lse, q_lengths, s_lengths)
+        # 16-bit outputs: the backward's grad . out needs what the rounding took from them
+        rest = None if q.dtype == torch.float32 else torch.empty_like(out)
+        ext.attention_pack_forward(q, k, v, q_lengths, s_lengths, out, lse, scale, causal, rest)
+        ctx.save_for_backward(q, k, v, out, rest, lse, q_lengths, s_lengths)
         ctx.scale, ctx.causal = scale, causal
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        q, k, v, out, lse, q_lengths, s_lengths = ctx.saved_tensors
+        q, k, v, out, rest, lse, q_lengths, s_lengths = ctx.saved_tensors
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
         ext.attention_pack_backward(grad.contiguous(), q, k, v, out, lse, q_lengths, s_lengths, dq, dk, dv, ctx.scale,
-                                    ctx.causal)
+                                    ctx.causal, rest)
         return dq, dk, dv, None, None, None, None
 
 
