@@ -172,13 +172,13 @@ def test_other_stream_and_graph_replays():
     assert torch.equal(got, want)
 
     from vision3d_amd import ext
-    rows, channels = x.shape
-    y, mean, rstd = torch.empty_like(x), x.new_empty(rows, dtype=torch.float32), x.new_empty(rows, dtype=torch.float32)
+    rows = x.shape[0]
+    y, stats = torch.empty_like(x), x.new_empty((2, rows), dtype=torch.float32)
     dx, dw, db = torch.empty_like(x), torch.empty_like(w), torch.empty_like(b)
 
     def step():
-        ext.layer_norm_forward(x, r, w, b, y, mean, rstd, 1e-5)
-        ext.layer_norm_backward(g, x, r, w, mean, rstd, dx, dw, db)
+        ext.layer_norm_forward(x, r, w, b, y, stats, 1e-5)
+        ext.layer_norm_backward(g, x, r, w, stats, dx, dw, db)
 
     step()
     graph = torch.cuda.CUDAGraph()

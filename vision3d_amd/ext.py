@@ -9,6 +9,8 @@ messages (``csrc/common/torch_helper.h:9-23``).  Underneath, each call is one C-
 ``knn`` is an alias of ``knn_points``: the reference's Python wrapper calls ``ext_module.knn``
 (``ops/knn_points.py:36``) although the extension registers ``knn_points`` (``pybind.cpp:150``).
 """
+import ctypes
+
 import torch
 
 from . import _lib
@@ -106,8 +108,8 @@ def _same_dtype(kernel, ref, *others):
 
 def _where(t):
     """(device index, raw hipStream_t) of the current stream on the tensor's device."""
-    dev = t.device.index if t.device.index is not None else torch.cuda.current_device()
-    return dev, torch.cuda.current_stream(dev).cuda_stream
+    dev = t.get_device()
+    return dev, torch._C._cuda_getCurrentRawStream(dev)  # current_stream(dev).cuda_stream without the Stream object
 
 
 def _workspace(nbytes, like):
@@ -129,8 +131,6 @@ def _ws_args(nbytes, like):
 def ball_query_multi(q_points, s_points, indices_list, max_radii, num_samples_list):
     """Multi-scale ball query (PointNet++ MSG): up to four (radius, k) scales over the same clouds in one pass; every
     ``indices_list[i]`` (B, M, num_samples_list[i]) arrives zero-filled and leaves equal to ``ball_query`` of that scale."""
-    import ctypes
-
     n = len(indices_list)
     if not (1 <= n <= 4) or len(max_radii) != n or len(num_samples_list) != n:
         raise RuntimeError("ball_query_multi: 1 to 4 scales, one radius and one sample count per output")
@@ -1014,117 +1014,110 @@ def _element(t, name):
 
 
 def _same_device(name, ref, *others):
+    dev = ref.get_device()
     for o in others:
-        if o is not None and o.device != ref.device:
+        if o is not None and o.get_device() != dev:
             raise RuntimeError(f"{name}: all tensors must be on one device, got {ref.device} and {o.device}")
 
 
-def _layer_norm_check(name, feats, residual, weight, bias):
+def _operand(name, t, arg, shape, dtype=None):
+    """An optional contiguous CUDA tensor of one shape and, if given, one element type."""
+    if t is None:
+        return
+    _check_cuda_contiguous(t, arg)
+    if t.shape != shape:
+        raise RuntimeError(f"{name}: {arg} must have shape {tuple(shape)}")
+    if dtype is not None and t.dtype != dtype:
+        raise RuntimeError(f"{name}: expected scalar type {_TYPE_NAMES.get(dtype, dtype)} but found "
+                           f"{_TYPE_NAMES.get(t.dtype, t.dtype)}")
+
+
+def _layer_norm_check(name, feats, residual, weight, bias, stats):
     _check_cuda_contiguous(feats, "feats")
     if feats.dim() != 2:
         raise RuntimeError(f"{name}: feats must have shape (N, C)")
-    if residual is not None:
-        _check_cuda_contiguous(residual, "residual")
-        _same_dtype(name, feats, residual)
-        if residual.shape != feats.shape:
-            raise RuntimeError(f"{name}: residual must have the shape of feats")
-    for t, n in ((weight, "weight"), (bias, "bias")):
-        if t is not None:
-            _check_cuda_contiguous(t, n)
-            if tuple(t.shape) != (feats.shape[1],):
-                raise RuntimeError(f"{name}: {n} must have shape {(feats.shape[1],)}")
-    if weight is not None and bias is not None:
-        _same_dtype(name, weight, bias)
-    _same_device(name, feats, residual, weight, bias)
-    affine = weight if weight is not None else bias
-    return _element(feats, name), _element(feats if affine is None else affine, name)
+    shape = feats.shape
+    _operand(name, residual, "residual", shape, feats.dtype)
+    _operand(name, weight, "weight", shape[1:])
+    _operand(name, bias, "bias", shape[1:], None if weight is None else weight.dtype)
+    _operand(name, stats, "stats", (2, shape[0]), torch.float32)
+    affine = bias if weight is None else weight
+    return _element(feats, name), _element(feats if affine is None else affine, name), shape[0], shape[1]
 
 
-def layer_norm_forward(feats, residual, weight, bias, targets, mean, rstd, eps):
-    """targets (N, C) = layer norm of ``feats`` (+ ``residual``); ``mean`` / ``rstd`` (N,) fp32 or None; see
-    include/v3d_hip.h."""
-    dtype, wdtype = _layer_norm_check("layer_norm_forward", feats, residual, weight, bias)
-    _check_cuda_contiguous(targets, "targets")
-    _same_dtype("layer_norm_forward", feats, targets)
-    if targets.shape != feats.shape:
-        raise RuntimeError("layer_norm_forward: targets must have the shape of feats")
-    rows, channels = feats.shape
-    for t, n in ((mean, "mean"), (rstd, "rstd")):
-        if t is not None:
-            _check_cuda_contiguous(t, n)
-            _check_float(t, n)
-            if tuple(t.shape) != (rows,):
-                raise RuntimeError(f"layer_norm_forward: {n} must have shape {(rows,)}")
-    _same_device("layer_norm_forward", feats, targets, mean, rstd)
+def layer_norm_forward(feats, residual, weight, bias, targets, stats, eps):
+    """targets (N, C) = layer norm of ``feats`` (+ ``residual``); ``stats`` (2, N) fp32 = mean and rstd of the rows, or
+    None; see include/v3d_hip.h."""
+    name = "layer_norm_forward"
+    dtype, wdtype, rows, channels = _layer_norm_check(name, feats, residual, weight, bias, stats)
+    _operand(name, targets, "targets", feats.shape, feats.dtype)
+    _same_device(name, feats, residual, weight, bias, targets, stats)
+    mean = _ptr(stats)
     dev, stream = _where(feats)
     _lib.check(_lib.lib().v3d_layer_norm_fwd(feats.data_ptr(), _ptr(residual), _ptr(weight), _ptr(bias),
-                                             targets.data_ptr(), _ptr(mean), _ptr(rstd), dtype, wdtype, rows, channels,
-                                             float(eps), dev, stream), "layer_norm_forward")
+                                             targets.data_ptr(), mean, None if mean is None else mean + 4 * rows, dtype,
+                                             wdtype, rows, channels, float(eps), dev, stream), name)
 
 
-def layer_norm_backward(target_grads, feats, residual, weight, mean, rstd, feats_grads, weight_grads, bias_grads):
+def layer_norm_backward(target_grads, feats, residual, weight, stats, feats_grads, weight_grads, bias_grads):
     """The gradients of ``layer_norm_forward``: each of the three outputs may be None (not wanted)."""
     name = "layer_norm_backward"
-    dtype, wdtype = _layer_norm_check(name, feats, residual, weight, None)
-    rows, channels = feats.shape
-    for t, n, shape in ((target_grads, "target_grads", feats.shape), (feats_grads, "feats_grads", feats.shape),
-                        (weight_grads, "weight_grads", (channels,)), (bias_grads, "bias_grads", (channels,)),
-                        (mean, "mean", (rows,)), (rstd, "rstd", (rows,))):
-        if t is not None:
-            _check_cuda_contiguous(t, n)
-            if tuple(t.shape) != tuple(shape):
-                raise RuntimeError(f"{name}: {n} must have shape {tuple(shape)}")
-    _check_float(mean, "mean")
-    _check_float(rstd, "rstd")
-    _same_dtype(name, feats, target_grads, *([] if feats_grads is None else [feats_grads]))
-    sums = [t for t in (weight_grads, bias_grads) if t is not None]
-    if sums:
-        _same_dtype(name, sums[0], *sums[1:], *([] if weight is None else [weight]))
-        wdtype = _element(sums[0], name)
-    _same_device(name, feats, target_grads, mean, rstd, feats_grads, weight_grads, bias_grads)
-    dev, stream = _where(feats)
+    sums = weight_grads if weight_grads is not None else bias_grads
+    dtype, wdtype, rows, channels = _layer_norm_check(name, feats, residual, weight, None, stats)
+    _operand(name, target_grads, "target_grads", feats.shape, feats.dtype)
+    _operand(name, feats_grads, "feats_grads", feats.shape, feats.dtype)
+    nbytes = 0
     lib = _lib.lib()
-    ws, wp, wn = _ws_args(lib.v3d_layer_norm_bwd_workspace_bytes(rows, channels) if sums else 0, feats)
-    _lib.check(lib.v3d_layer_norm_bwd(target_grads.data_ptr(), feats.data_ptr(), _ptr(residual), _ptr(weight),
-                                      mean.data_ptr(), rstd.data_ptr(), _ptr(feats_grads), _ptr(weight_grads),
-                                      _ptr(bias_grads), dtype, wdtype, rows, channels, wp, wn, dev, stream), name)
+    if sums is not None:
+        _operand(name, weight_grads, "weight_grads", (channels,), sums.dtype if weight is None else weight.dtype)
+        _operand(name, bias_grads, "bias_grads", (channels,), sums.dtype if weight is None else weight.dtype)
+        wdtype = _element(sums, name)
+        nbytes = lib.v3d_layer_norm_bwd_workspace_bytes(rows, channels)
+    _same_device(name, feats, target_grads, residual, weight, stats, feats_grads, weight_grads, bias_grads)
+    mean = stats.data_ptr()
+    ws, wp, wn = _ws_args(nbytes, feats)
+    dev, stream = _where(feats)
+    _lib.check(lib.v3d_layer_norm_bwd(target_grads.data_ptr(), feats.data_ptr(), _ptr(residual), _ptr(weight), mean,
+                                      mean + 4 * rows, _ptr(feats_grads), _ptr(weight_grads), _ptr(bias_grads), dtype,
+                                      wdtype, rows, channels, wp, wn, dev, stream), name)
 
 
-def _heads(name, t, arg, dims):
-    """Features (.., heads, D) of any strides but the last, which is 1."""
+def _heads(name, t, arg, dims, dtype):
+    """(strides, shape) of features (.., heads, D) of any strides but the last, which is 1."""
     if not t.is_cuda:
         raise RuntimeError(f"{arg} must be a CUDA tensor")
-    if t.dim() != dims:
-        raise RuntimeError(f"{name}: {arg} must have {dims} dimensions, got {t.dim()}")
-    if t.size(-1) > 1 and t.stride(-1) != 1:
+    shape, strides = t.shape, t.stride()
+    if len(shape) != dims:
+        raise RuntimeError(f"{name}: {arg} must have {dims} dimensions, got {len(shape)}")
+    if shape[-1] > 1 and strides[-1] != 1:
         raise RuntimeError(f"{name}: the last dimension of {arg} must be contiguous")
+    if t.dtype != dtype:
+        raise RuntimeError(f"{name}: expected scalar type {_TYPE_NAMES.get(dtype, dtype)} but found "
+                           f"{_TYPE_NAMES.get(t.dtype, t.dtype)}")
+    return strides, shape
 
 
 def _lengths(name, t, arg, count):
     _check_cuda_contiguous(t, arg)
     _check_long(t, arg)
-    if tuple(t.shape) != (count,):
+    if t.shape != (count,):
         raise RuntimeError(f"{name}: {arg} must have shape {(count,)}")
 
 
-def _strides(*values):
-    import ctypes
-
-    return (ctypes.c_int64 * len(values))(*values)
+_Strides6, _Strides8 = ctypes.c_int64 * 6, ctypes.c_int64 * 8
 
 
 def _attention_check(name, q, k, v, q_lengths, s_lengths):
-    _heads(name, q, "q_feats", 3)
-    _heads(name, k, "k_feats", 3)
-    _heads(name, v, "v_feats", 3)
-    dtype = _element(q, name)
-    _same_dtype(name, q, k, v)
-    if v.shape != k.shape or k.size(2) != q.size(2):
+    qs, qshape = _heads(name, q, "q_feats", 3, q.dtype)
+    ks, kshape = _heads(name, k, "k_feats", 3, q.dtype)
+    vs, vshape = _heads(name, v, "v_feats", 3, q.dtype)
+    if vshape != kshape or kshape[2] != qshape[2]:
         raise RuntimeError(f"{name}: expected q_feats (N, H, D), k_feats and v_feats (M, KV, D)")
-    _lengths(name, q_lengths, "q_lengths", q_lengths.numel())
-    _lengths(name, s_lengths, "s_lengths", q_lengths.numel())
-    _same_device(name, q, k, v, q_lengths, s_lengths)
-    return dtype, _strides(q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1))
+    count = q_lengths.numel()
+    _lengths(name, q_lengths, "q_lengths", count)
+    _lengths(name, s_lengths, "s_lengths", count)
+    sizes = (count, qshape[0], kshape[0], qshape[1], kshape[1], qshape[2])  # B, N, M, H, KV, D
+    return _element(q, name), sizes, _Strides6(qs[0], qs[1], ks[0], ks[1], vs[0], vs[1])
 
 
 def attention_pack_forward(q_feats, k_feats, v_feats, q_lengths, s_lengths, targets, lse, scale, causal, rest=None):
@@ -1132,95 +1125,70 @@ def attention_pack_forward(q_feats, k_feats, v_feats, q_lengths, s_lengths, targ
     sequence of the pack; for the backward: ``lse`` (N, H) fp32 and, of 16-bit types, ``rest`` (N, H, D) = what rounding took
     from ``targets``; see include/v3d_hip.h."""
     name = "attention_pack_forward"
-    dtype, strides = _attention_check(name, q_feats, k_feats, v_feats, q_lengths, s_lengths)
-    _check_cuda_contiguous(targets, "targets")
-    _same_dtype(name, q_feats, targets)
-    if targets.shape != q_feats.shape:
-        raise RuntimeError(f"{name}: targets must have the shape of q_feats")
-    N, H, D = q_feats.shape
-    if lse is not None:
-        _check_cuda_contiguous(lse, "lse")
-        _check_float(lse, "lse")
-        if tuple(lse.shape) != (N, H):
-            raise RuntimeError(f"{name}: lse must have shape {(N, H)}")
-    if rest is not None:
-        _check_cuda_contiguous(rest, "rest")
-        _same_dtype(name, q_feats, rest)
-        if rest.shape != q_feats.shape:
-            raise RuntimeError(f"{name}: rest must have the shape of q_feats")
-    _same_device(name, q_feats, targets, lse, rest)
-    B, M, KV = q_lengths.numel(), k_feats.size(0), k_feats.size(1)
-    dev, stream = _where(q_feats)
+    dtype, sizes, strides = _attention_check(name, q_feats, k_feats, v_feats, q_lengths, s_lengths)
+    shape = q_feats.shape
+    _operand(name, targets, "targets", shape, q_feats.dtype)
+    _operand(name, lse, "lse", shape[:2], torch.float32)
+    _operand(name, rest, "rest", shape, q_feats.dtype)
+    _same_device(name, q_feats, k_feats, v_feats, q_lengths, s_lengths, targets, lse, rest)
     lib = _lib.lib()
-    ws, wp, wn = _ws_args(lib.v3d_attention_pack_workspace_bytes(B, N, M, H, KV, D), q_feats)
+    ws, wp, wn = _ws_args(lib.v3d_attention_pack_workspace_bytes(*sizes), q_feats)
+    dev, stream = _where(q_feats)
     _lib.check(lib.v3d_attention_pack_fwd(q_feats.data_ptr(), k_feats.data_ptr(), v_feats.data_ptr(),
-                                          q_lengths.data_ptr(), s_lengths.data_ptr(), targets.data_ptr(), _ptr(rest), _ptr(lse),
-                                          dtype, B, N, M, H, KV, D, strides, float(scale), int(bool(causal)), wp, wn,
-                                          dev, stream), name)
+                                          q_lengths.data_ptr(), s_lengths.data_ptr(), targets.data_ptr(), _ptr(rest),
+                                          _ptr(lse), dtype, *sizes, strides, scale, bool(causal), wp, wn, dev, stream),
+               name)
 
 
 def attention_pack_backward(target_grads, q_feats, k_feats, v_feats, targets, lse, q_lengths, s_lengths, q_grads, k_grads,
                             v_grads, scale, causal, rest=None):
     """The gradients of ``attention_pack_forward``, from its inputs, ``targets``, ``lse`` and (16-bit types) ``rest``."""
     name = "attention_pack_backward"
-    dtype, strides = _attention_check(name, q_feats, k_feats, v_feats, q_lengths, s_lengths)
-    N, H, D = q_feats.shape
-    B, M, KV = q_lengths.numel(), k_feats.size(0), k_feats.size(1)
-    for t, n, shape in ((target_grads, "target_grads", (N, H, D)), (targets, "targets", (N, H, D)),
-                        (q_grads, "q_grads", (N, H, D)), (k_grads, "k_grads", (M, KV, D)), (v_grads, "v_grads", (M, KV, D))):
-        _check_cuda_contiguous(t, n)
-        _same_dtype(name, q_feats, t)
-        if tuple(t.shape) != shape:
-            raise RuntimeError(f"{name}: {n} must have shape {shape}")
-    _check_cuda_contiguous(lse, "lse")
-    _check_float(lse, "lse")
-    if tuple(lse.shape) != (N, H):
-        raise RuntimeError(f"{name}: lse must have shape {(N, H)}")
-    if rest is not None:
-        _check_cuda_contiguous(rest, "rest")
-        _same_dtype(name, q_feats, rest)
-        if rest.shape != q_feats.shape:
-            raise RuntimeError(f"{name}: rest must have the shape of q_feats")
-    _same_device(name, q_feats, target_grads, targets, lse, q_grads, k_grads, v_grads, rest)
-    dev, stream = _where(q_feats)
+    dtype, sizes, strides = _attention_check(name, q_feats, k_feats, v_feats, q_lengths, s_lengths)
+    shape, kshape = q_feats.shape, k_feats.shape
+    _operand(name, target_grads, "target_grads", shape, q_feats.dtype)
+    _operand(name, targets, "targets", shape, q_feats.dtype)
+    _operand(name, lse, "lse", shape[:2], torch.float32)
+    _operand(name, rest, "rest", shape, q_feats.dtype)
+    _operand(name, q_grads, "q_grads", shape, q_feats.dtype)
+    _operand(name, k_grads, "k_grads", kshape, q_feats.dtype)
+    _operand(name, v_grads, "v_grads", kshape, q_feats.dtype)
+    _same_device(name, q_feats, k_feats, v_feats, q_lengths, s_lengths, target_grads, targets, lse, rest, q_grads, k_grads,
+                 v_grads)
     lib = _lib.lib()
-    ws, wp, wn = _ws_args(lib.v3d_attention_pack_bwd_workspace_bytes(B, N, M, H, KV, D), q_feats)
+    ws, wp, wn = _ws_args(lib.v3d_attention_pack_bwd_workspace_bytes(*sizes), q_feats)
+    dev, stream = _where(q_feats)
     _lib.check(lib.v3d_attention_pack_bwd(target_grads.data_ptr(), q_feats.data_ptr(), k_feats.data_ptr(),
                                           v_feats.data_ptr(), targets.data_ptr(), _ptr(rest), lse.data_ptr(),
-                                          q_lengths.data_ptr(), s_lengths.data_ptr(), q_grads.data_ptr(), k_grads.data_ptr(),
-                                          v_grads.data_ptr(), dtype, B, N, M, H, KV, D, strides, float(scale),
-                                          int(bool(causal)), wp, wn, dev, stream), name)
+                                          q_lengths.data_ptr(), s_lengths.data_ptr(), q_grads.data_ptr(),
+                                          k_grads.data_ptr(), v_grads.data_ptr(), dtype, *sizes, strides, scale,
+                                          bool(causal), wp, wn, dev, stream), name)
 
 
 def cached_attention(q_feats, k_cache, v_cache, lengths, targets, scale):
     """targets (B, T, H, D) = attention of the newest T tokens of every sequence over its cache (B, C, KV, D), of which
     ``lengths`` (B,) rows are filled; see include/v3d_hip.h."""
     name = "cached_attention"
-    _heads(name, q_feats, "q_feats", 4)
-    _heads(name, k_cache, "k_cache", 4)
-    _heads(name, v_cache, "v_cache", 4)
-    _check_cuda_contiguous(targets, "targets")
+    qs, shape = _heads(name, q_feats, "q_feats", 4, q_feats.dtype)
+    ks, kshape = _heads(name, k_cache, "k_cache", 4, q_feats.dtype)
+    vs, vshape = _heads(name, v_cache, "v_cache", 4, q_feats.dtype)
+    _operand(name, targets, "targets", shape, q_feats.dtype)
     dtype = _element(q_feats, name)
-    _same_dtype(name, q_feats, k_cache, v_cache, targets)
-    B, T, H, D = q_feats.shape
-    if targets.shape != q_feats.shape:
-        raise RuntimeError(f"{name}: targets must have the shape of q_feats")
-    if k_cache.shape != v_cache.shape or k_cache.size(0) != B or k_cache.size(3) != D:
+    B, T, H, D = shape
+    if kshape != vshape or kshape[0] != B or kshape[3] != D:
         raise RuntimeError(f"{name}: expected q_feats (B, T, H, D), k_cache and v_cache (B, C, KV, D)")
-    if B > 1 and T > 0 and q_feats.stride(0) != T * q_feats.stride(1):
+    if B > 1 and T > 1 and qs[0] != T * qs[1]:
         raise RuntimeError(f"{name}: the tokens of q_feats must be at one stride")
     _lengths(name, lengths, "lengths", B)
     _same_device(name, q_feats, k_cache, v_cache, lengths, targets)
-    C, KV = k_cache.size(1), k_cache.size(2)
-    q_row = q_feats.stride(1) if T > 1 else q_feats.stride(0)
-    strides = _strides(q_row, q_feats.stride(2), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
-                       v_cache.stride(0), v_cache.stride(1), v_cache.stride(2))
-    dev, stream = _where(q_feats)
+    C, KV = kshape[1], kshape[2]
+    strides = _Strides8(qs[1] if T > 1 else qs[0], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2])
     lib = _lib.lib()
     ws, wp, wn = _ws_args(lib.v3d_cached_attention_workspace_bytes(B, T, C, H, KV, D), q_feats)
+    dev, stream = _where(q_feats)
     _lib.check(lib.v3d_cached_attention(q_feats.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), lengths.data_ptr(),
-                                        targets.data_ptr(), dtype, B, T, C, H, KV, D, strides, float(scale), wp, wn,
-                                        dev, stream), name)
+                                        targets.data_ptr(), dtype, B, T, C, H, KV, D, strides, scale, wp, wn, dev,
+                                        stream), name)
 
 
 # --------------------------------------------------------------------------------------------------------

@@ -19,11 +19,20 @@ def _require_cuda(name, *tensors):
 def _rows(t: Tensor) -> Tensor:
     """The strides that the kernels take: any but the last dimension's, which is 1, within 32-bit offsets of a tile; other
     inputs are copied."""
-    if t.dim() < 3 or t.numel() == 0:
+    strides, shape = t.stride(), t.shape
+    if len(shape) < 3 or t.numel() == 0:
         return t
-    row, head, unit = t.stride()[-3:]
-    near = 130 * row + t.size(-2) * head + t.size(-1) < 1 << 29
-    return t if unit == 1 and (row == 0 or row >= t.size(-1)) and near else t.contiguous()
+    row, head, unit = strides[-3:]
+    heads, dim = shape[-2:]
+    near = 130 * row + heads * head + dim < 1 << 29
+    return t if unit == 1 and (row == 0 or row >= dim) and near else t.contiguous()
+
+
+def _lengths(lengths: Tensor, like: Tensor) -> Tensor:
+    """The reference's loops take the lengths on either side and in any integer type; the kernels int64 on the device."""
+    if lengths.dtype != torch.long or lengths.device != like.device:
+        lengths = lengths.to(device=like.device, dtype=torch.long)
+    return lengths.contiguous()
 
 
 def _scale(scale, dim):
@@ -64,17 +73,15 @@ def attention_pack_mode(q_feats: Tensor, k_feats: Tensor, v_feats: Tensor, q_len
     it, infinities and NaN included (in the forward).  Rows behind the last sequence come out as zeros.  fp32, fp16 or bf16, D from 8 (fp32: 4) to 256; the
     inputs may be views of one projection (only the last dimension has to be contiguous).
     """
-    s_lengths = q_lengths if s_lengths is None else s_lengths
     _require_cuda("attention_pack_mode", q_feats, k_feats, v_feats)
-    dev = q_feats.device
-    q_lengths = q_lengths.to(device=dev, dtype=torch.long).contiguous()
-    s_lengths = s_lengths.to(device=dev, dtype=torch.long).contiguous()
-    scale = _scale(scale, q_feats.size(-1))
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q_feats, k_feats, v_feats)):
+    q_lengths = _lengths(q_lengths, q_feats)
+    s_lengths = q_lengths if s_lengths is None else _lengths(s_lengths, q_feats)
+    scale = _scale(scale, q_feats.shape[-1])
+    if torch.is_grad_enabled() and (q_feats.requires_grad or k_feats.requires_grad or v_feats.requires_grad):
         return _AttentionPack.apply(q_feats, k_feats, v_feats, q_lengths, s_lengths, scale, causal)
-    q, k, v = _rows(q_feats), _rows(k_feats), _rows(v_feats)
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    ext.attention_pack_forward(q, k, v, q_lengths, s_lengths, out, None, scale, causal)
+    out = torch.empty(q_feats.shape, dtype=q_feats.dtype, device=q_feats.device)
+    ext.attention_pack_forward(_rows(q_feats), _rows(k_feats), _rows(v_feats), q_lengths, s_lengths, out, None, scale,
+                               causal)
     return out
 
 
@@ -88,12 +95,11 @@ def cached_attention(q_feats: Tensor, k_cache: Tensor, v_cache: Tensor, lengths:
     sequences are.  Only the last dimension of each tensor has to be contiguous.
     """
     _require_cuda("cached_attention", q_feats, k_cache, v_cache)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q_feats, k_cache, v_cache)):
+    if torch.is_grad_enabled() and (q_feats.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         raise RuntimeError("cached_attention: no gradient; call it under torch.no_grad() or use attention_pack_mode")
-    lengths = lengths.to(device=q_feats.device, dtype=torch.long).contiguous()
-    q, k, v = _rows(q_feats), _rows(k_cache), _rows(v_cache)
-    if q.dim() == 4 and q.size(0) > 1 and q.stride(0) != q.size(1) * q.stride(1):
+    q = _rows(q_feats)
+    if q.dim() == 4 and q.shape[1] > 1 and q.shape[0] > 1 and q.stride(0) != q.shape[1] * q.stride(1):
         q = q.contiguous()
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ext.cached_attention(q, k, v, lengths, out, _scale(scale, q.size(-1)))
+    ext.cached_attention(q, _rows(k_cache), _rows(v_cache), _lengths(lengths, q), out, _scale(scale, q.shape[-1]))
     return out

@@ -1,7 +1,7 @@
 """Layer normalisation of feature rows, the norm of the transformer layers over packs (the reference's layers call
 ``torch.nn.LayerNorm``; a post-norm layer adds the residual first: here the sum is formed inside the kernel).
 
-One kernel forward; backward recomputes the sum and the normalised rows from the inputs and the saved (mean, rstd), so
+One kernel forward; backward recomputes the sum and the normalised rows from the inputs and the saved statistics, so
 nothing of the input's size is kept besides the inputs themselves.  The gradients of the weight and the bias are added in
 a fixed order (no atomics).
 """
@@ -17,30 +17,28 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, feats, weight, bias, eps, residual):
         out = torch.empty_like(feats)
-        mean = torch.empty((feats.shape[0],), dtype=torch.float32, device=feats.device)
-        rstd = torch.empty_like(mean)
-        ext.layer_norm_forward(feats, residual, weight, bias, out, mean, rstd, eps)
-        ctx.save_for_backward(feats, weight, residual, mean, rstd)
+        stats = feats.new_empty((2, feats.shape[0]), dtype=torch.float32)
+        ext.layer_norm_forward(feats, residual, weight, bias, out, stats, eps)
+        ctx.save_for_backward(feats, weight, residual, stats)
         ctx.bias_dtype = None if bias is None else bias.dtype
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        feats, weight, residual, mean, rstd = ctx.saved_tensors
+        feats, weight, residual, stats = ctx.saved_tensors
         need_feats = ctx.needs_input_grad[0] or ctx.needs_input_grad[4]
         need_weight, need_bias = ctx.needs_input_grad[1], ctx.needs_input_grad[2]
         grad_feats = torch.empty_like(feats) if need_feats else None
         channels = feats.shape[1:]
-        grad_weight = feats.new_empty(channels, dtype=weight.dtype) if need_weight else None
+        grad_weight = torch.empty_like(weight) if need_weight else None
         grad_bias = feats.new_empty(channels, dtype=ctx.bias_dtype) if need_bias else None
         if feats.shape[0] == 0:  # no rows: the column sums are empty
             for t in (grad_weight, grad_bias):
                 if t is not None:
                     t.zero_()
         else:
-            ext.layer_norm_backward(grad.contiguous(), feats, residual, weight, mean, rstd, grad_feats, grad_weight,
-                                    grad_bias)
+            ext.layer_norm_backward(grad.contiguous(), feats, residual, weight, stats, grad_feats, grad_weight, grad_bias)
         return (grad_feats if ctx.needs_input_grad[0] else None, grad_weight, grad_bias, None,
                 grad_feats if ctx.needs_input_grad[4] else None)
 
@@ -58,16 +56,19 @@ def layer_norm(feats: Tensor, weight: Optional[Tensor] = None, bias: Optional[Te
             raise RuntimeError("layer_norm: CUDA tensors required (no CPU fallback in vision3d_amd)")
     if feats.dim() < 1:
         raise RuntimeError("layer_norm: feats must have a channel dimension")
-    shape = feats.shape
-    if residual is not None:
-        if residual.shape != shape:
-            raise RuntimeError("layer_norm: residual must have the shape of feats")
-        residual = residual.reshape(-1, shape[-1]).contiguous()
-    rows = feats.reshape(-1, shape[-1]).contiguous()
+    if residual is not None and residual.shape != feats.shape:
+        raise RuntimeError("layer_norm: residual must have the shape of feats")
+    if feats.dim() != 2:
+        channels = feats.shape[-1]
+        rows = feats.reshape(-1, channels)
+        return layer_norm(rows, weight, bias, eps, None if residual is None else residual.reshape(-1, channels)).view(
+            feats.shape)
+    feats = feats.contiguous()
     weight = None if weight is None else weight.contiguous()
     bias = None if bias is None else bias.contiguous()
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (rows, weight, bias, residual)):
-        return _LayerNorm.apply(rows, weight, bias, float(eps), residual).view(shape)
-    out = torch.empty_like(rows)
-    ext.layer_norm_forward(rows, residual, weight, bias, out, None, None, eps)
-    return out.view(shape)
+    residual = None if residual is None else residual.contiguous()
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (feats, weight, bias, residual)):
+        return _LayerNorm.apply(feats, weight, bias, eps, residual)
+    out = torch.empty_like(feats)
+    ext.layer_norm_forward(feats, residual, weight, bias, out, None, eps)
+    return out
