@@ -64,10 +64,11 @@ struct AttnWave {
         s[n] = product<T>(read_cols<T, HDP, 32 * NT>(k, n * 32 + (lane & 31), st, half), q[st], s[n]);
     if (key0 + 32 * NT > least) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           if (key0 + n * 32 + acc_row(r, half) >= limit) s[n][r] = -__builtin_inff();
+      }
     }
     // maximum of the lane, then with the lane that holds the other keys of this query
     float top = -__builtin_inff();
@@ -202,7 +203,7 @@ __global__ __launch_bounds__(256, (attn_occupancy<T, HD>())) void attn_forward_k
   __shared__ __attribute__((aligned(16))) U lds_v[BUFS][SIZE];
   __shared__ int lds_bad[BUFS];
 
-  const int wave = threadIdx.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int64_t id = blockIdx.x;
   const int kvh = (int)(id % a.KV);
   id /= a.KV;
@@ -329,7 +330,7 @@ __global__ __launch_bounds__((64 * few_waves<T, HD>())) void attn_few_rows_kerne
   __shared__ U lds_p[W][32 * 32];
   __shared__ float lds_ml[W][32][2];
 
-  const int wave = threadIdx.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int64_t id = blockIdx.x;
   const int kvh = (int)(id % a.KV);
   id /= a.KV;
@@ -439,7 +440,7 @@ __global__ __launch_bounds__((64 * few_waves<T, HD>())) void attn_few_rows_kerne
 // Joins the parts of a row tile's keys: one wave per row, first its lanes over the parts (at most 64), then over the columns.
 template <typename T, int TILE>
 __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   constexpr int GROUPS = TILE / 4;  // workgroups of 4 rows per tile
   int64_t id = blockIdx.x;
   const int at = (int)(id % GROUPS) * 4 + wave;

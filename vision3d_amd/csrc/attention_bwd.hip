@@ -17,6 +17,8 @@ struct AttnBwdArgs {
   AttnArgs f;          // q, k, v, out, lse and the geometry of the forward (never a cache)
   const void* grad;    // (total_q, H, D) contiguous
   float* delta;        // (total_q, H): written by the dq kernel, read by the dk / dv kernel
+  int splits;          // parts that the rows of a key tile are divided into
+  float* part;         // splits > 1: (splits, 2, total_s, KV, D) sums of the parts, dk's and dv's
   void* dq;            // (total_q, H, D), (total_s, KV, D) contiguous
   void* dk;
   void* dv;
@@ -41,12 +43,12 @@ __global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 128 : 64) ? 2 : 1) vo
   __shared__ __attribute__((aligned(16))) U lds_v[BUFS][Kind<T>::P * BN * HDP];
 
   const AttnArgs& a = b.f;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = lane >> 5;
   int64_t id = blockIdx.x;
   const int kvh = (int)(id % a.KV);
   id = (int64_t)(gridDim.x / a.KV) - 1 - id / a.KV;  // causal: the longest tiles of a sequence start first
-  const AttnSeq seq = locate<kAttnRows, false>(a, id);
+  const AttnSeq seq = locate_rows<kAttnRows>(a, id);
   T* dq = static_cast<T*>(b.dq);
   if (!seq.found) {  // rows behind the last sequence have no gradient
     const int64_t rows = (a.total_q - seq.q_end) * a.G;
@@ -172,7 +174,7 @@ __global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 128 : 64) ? 2 : 1) vo
 }
 
 template <typename T, int HD>
-__global__ __launch_bounds__(256) void attn_backward_kv_kernel(const AttnBwdArgs b) {
+__global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 64 : 32) ? 2 : 1) void attn_backward_kv_kernel(const AttnBwdArgs b) {
   constexpr int HDP = attn_pow2(HD);
   constexpr int BM = bwd_tile<T, HD>();
   constexpr int NT = BM / 32;
@@ -182,23 +184,36 @@ __global__ __launch_bounds__(256) void attn_backward_kv_kernel(const AttnBwdArgs
   typedef typename Kind<T>::U U;
   __shared__ __attribute__((aligned(16))) U lds_q[BUFS][Kind<T>::P * BM * HDP];
   __shared__ __attribute__((aligned(16))) U lds_g[BUFS][Kind<T>::P * BM * HDP];
+  // The wave's keys stay in registers, its values in LDS: two waves fit a SIMD, and one's products run under the other's
+  // exponentials (16-bit heads of 128, 8192 tokens: VALUES_REG us with both in registers and one wave).
+  constexpr bool kValuesLds = Kind<T>::P == 1 && HD <= 64;
+  __shared__ __attribute__((aligned(16))) U lds_vt[kValuesLds ? kAttnRows * HDP : 8];
   __shared__ float lds_lse[BUFS][BM], lds_delta[BUFS][BM];
   __shared__ int lds_limit[BUFS][BM];
 
   const AttnArgs& a = b.f;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = lane >> 5;
   int64_t id = blockIdx.x;
   const int kvh = (int)(id % a.KV);
   id /= a.KV;
-  const AttnSeq seq = locate<kAttnRows, true>(a, id);
+  const int split = (int)(id % b.splits);
+  const AttnSeq seq = locate_keys<kAttnRows>(a, id / b.splits);
   T* dk = static_cast<T*>(b.dk);
   T* dv = static_cast<T*>(b.dv);
-  if (!seq.found) {
+  const int64_t plane = a.total_s * a.KV * a.D;
+  float* pk = b.part + 2 * split * plane;
+  float* pv = pk + plane;
+  if (!seq.found) {  // keys behind the last sequence have no gradient
     for (int i = threadIdx.x; i < kAttnRows; i += 256) {
       const int64_t r = seq.s_end + seq.spare * kAttnRows + i;
       if (r >= a.total_s) break;
-      for (int d = 0; d < a.D; ++d) dk[(r * a.KV + kvh) * a.D + d] = dv[(r * a.KV + kvh) * a.D + d] = (T)0.f;
+      for (int64_t d = (r * a.KV + kvh) * a.D; d < (r * a.KV + kvh + 1) * a.D; ++d) {
+        if (b.splits == 1)
+          dk[d] = dv[d] = (T)0.f;
+        else
+          pk[d] = pv[d] = 0.f;
+      }
     }
     return;
   }
@@ -251,9 +266,19 @@ __global__ __launch_bounds__(256) void attn_backward_kv_kernel(const AttnBwdArgs
     }
   };
 
-  Op<T> kf[STEPS], vf[STEPS];
+  Op<T> kf[STEPS], vf[kValuesLds ? 1 : STEPS];
   load_ops<T>(kf, k, (key - key0) * (int)a.k_row, half, a.D, live);
-  load_ops<T>(vf, v, (key - key0) * (int)a.v_row, half, a.D, live);
+  if constexpr (kValuesLds) {
+    TileStage<T, HD, kAttnRows, 256> stage_v;
+    stage_v.fetch(v, a.v_row, a.D, seq.s_len - key0);
+    stage_v.store(lds_vt, a.D);
+  } else {
+    load_ops<T>(vf, v, (key - key0) * (int)a.v_row, half, a.D, live);
+  }
+  auto value = [&](int st) {
+    if constexpr (kValuesLds) return read_cols<T, HDP, kAttnRows>(lds_vt, wave * 32 + (lane & 31), st, half);
+    else return vf[st];
+  };
   const float c2 = a.scale * kLog2e;
   f32x16 ak[DT], av[DT];
 #pragma unroll
@@ -270,7 +295,7 @@ __global__ __launch_bounds__(256) void attn_backward_kv_kernel(const AttnBwdArgs
 #pragma unroll
       for (int st = 0; st < STEPS; ++st) {
         s = product<T>(read_cols<T, HDP, BM>(lds_q[buf], n * 32 + (lane & 31), st, half), kf[st], s);
-        dp = product<T>(read_cols<T, HDP, BM>(lds_g[buf], n * 32 + (lane & 31), st, half), vf[st], dp);
+        dp = product<T>(read_cols<T, HDP, BM>(lds_g[buf], n * 32 + (lane & 31), st, half), value(st), dp);
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
@@ -295,40 +320,80 @@ __global__ __launch_bounds__(256) void attn_backward_kv_kernel(const AttnBwdArgs
     }
   };
 
-  const int begin = first / BM * BM;
-  if (begin < rows) {
+  const int blocks = max(0, (rows - first / BM * BM + BM - 1) / BM), per = (blocks + b.splits - 1) / b.splits;
+  const int begin = first / BM * BM + split * per * BM, end = min(rows, begin + per * BM);
+  if (begin < end) {
     fetch(begin);
     place_tile(0);
     __syncthreads();
     if constexpr (BUFS == 2) {
-      for (int r = begin; r < rows; r += 2 * BM) {
-        if (r + BM < rows) fetch(r + BM);
+      for (int r = begin; r < end; r += 2 * BM) {
+        if (r + BM < end) fetch(r + BM);
         work(r, Const<0>{});
-        if (r + BM < rows) place_tile(1);
+        if (r + BM < end) place_tile(1);
         __syncthreads();
-        if (r + BM >= rows) break;
-        if (r + 2 * BM < rows) fetch(r + 2 * BM);
+        if (r + BM >= end) break;
+        if (r + 2 * BM < end) fetch(r + 2 * BM);
         work(r + BM, Const<1>{});
-        if (r + 2 * BM < rows) place_tile(0);
+        if (r + 2 * BM < end) place_tile(0);
         __syncthreads();
       }
     } else {
-      for (int r = begin; r < rows; r += BM) {
-        if (r + BM < rows) fetch(r + BM);
+      for (int r = begin; r < end; r += BM) {
+        if (r + BM < end) fetch(r + BM);
         work(r, Const<0>{});
         __syncthreads();
-        if (r + BM < rows) place_tile(0);
+        if (r + BM < end) place_tile(0);
         __syncthreads();
       }
     }
   }
   if (!live) return;
   const int64_t at = ((seq.s_off + key) * a.KV + kvh) * a.D;
-  store_rows<T, DT>(dk + at, ak, a.scale, a.D, half);
-  store_rows<T, DT>(dv + at, av, 1.f, a.D, half);
+  if (b.splits == 1) {
+    store_rows<T, DT>(dk + at, ak, a.scale, a.D, half);
+    store_rows<T, DT>(dv + at, av, 1.f, a.D, half);
+  } else {
+    store_rows<float, DT>(pk + at, ak, a.scale, a.D, half);
+    store_rows<float, DT>(pv + at, av, 1.f, a.D, half);
+  }
+}
+
+// Adds the parts in their order, four neighbouring elements a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_backward_join_kernel(const AttnBwdArgs b) {
+  const int64_t plane = b.f.total_s * b.f.KV * b.f.D;
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= plane) return;
+  const float* p = b.part + blockIdx.y * plane + i;
+  T* out = static_cast<T*>(blockIdx.y == 0 ? b.dk : b.dv) + i;
+  if (i + 4 <= plane) {
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < b.splits; ++s) {
+      float y[4];
+      load_vec<float, 4>(p + 2 * s * plane, y);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] += y[j];
+    }
+    store_vec<T, 4>(out, x);
+  } else {
+    for (int j = 0; j < plane - i; ++j) {
+      float x = 0.f;
+      for (int s = 0; s < b.splits; ++s) x += p[2 * s * plane + j];
+      out[j] = from_f32<T>(x);
+    }
+  }
 }
 
 // ---- launches ----------------------------------------------------------------------------------------------------------
+#ifndef KV_TARGET
+#define KV_TARGET 1024
+#endif
+inline int attn_backward_splits(int B, int64_t total_s, int KV) {
+  const int64_t groups = (ceil_div(total_s, kAttnRows) + B) * KV;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(KV_TARGET / groups, 8));
+}
+
 template <typename T, int HD>
 int attn_backward_launch(const AttnBwdArgs& b, hipStream_t stream, const char* what) {
   const AttnArgs& a = b.f;
@@ -339,8 +404,14 @@ int attn_backward_launch(const AttnBwdArgs& b, hipStream_t stream, const char* w
     rc = launch_status(what);
   }
   if (rc == 0 && a.total_s > 0) {
-    hipLaunchKernelGGL((attn_backward_kv_kernel<T, HD>), dim3((unsigned)(s_tiles * a.KV)), dim3(256), 0, stream, b);
+    hipLaunchKernelGGL((attn_backward_kv_kernel<T, HD>), dim3((unsigned)(s_tiles * a.KV * b.splits)), dim3(256), 0,
+                       stream, b);
     rc = launch_status(what);
+    if (rc == 0 && b.splits > 1) {
+      const dim3 grid((unsigned)ceil_div(a.total_s * a.KV * a.D, 1024), 2);
+      hipLaunchKernelGGL((attn_backward_join_kernel<T>), grid, dim3(256), 0, stream, b);
+      rc = launch_status(what);
+    }
   }
   return rc;
 }
@@ -362,11 +433,11 @@ int attn_backward_type(const AttnBwdArgs& b, hipStream_t stream, const char* wha
 extern "C" {
 
 size_t v3d_attention_pack_bwd_workspace_bytes(int B, int64_t total_q, int64_t total_s, int H, int KV, int D) {
-  (void)B;
-  (void)total_s;
-  (void)KV;
-  (void)D;
-  return total_q > 0 && H > 0 ? (size_t)total_q * (size_t)H * sizeof(float) : 0;
+  using namespace v3d;
+  if (B < 0 || total_q < 0 || total_s < 0 || H <= 0 || KV <= 0 || D <= 0) return 0;
+  const int splits = attn_backward_splits(B, total_s, KV);
+  const size_t delta = align_up((size_t)total_q * (size_t)H * sizeof(float), 256);
+  return delta + (splits > 1 ? (size_t)splits * 2 * (size_t)total_s * (size_t)(KV * D) * sizeof(float) : 0);
 }
 
 int v3d_attention_pack_bwd(const void* grad, const void* q, const void* k, const void* v, const void* out,
@@ -419,6 +490,8 @@ int v3d_attention_pack_bwd(const void* grad, const void* q, const void* k, const
                   v3d_attention_pack_bwd_workspace_bytes(B, total_q, total_s, H, KV, D), s);
   if (rc != 0) return rc;
   b.delta = reinterpret_cast<float*>(ws.base);
+  b.splits = attn_backward_splits(B, total_s, KV);
+  b.part = reinterpret_cast<float*>(ws.base + align_up((size_t)total_q * (size_t)H * sizeof(float), 256));
   rc = dtype == V3D_F32   ? attn_backward_type<float>(b, s, what)
        : dtype == V3D_F16 ? attn_backward_type<f16>(b, s, what)
                           : attn_backward_type<bf16>(b, s, what);

@@ -95,7 +95,7 @@ __device__ __forceinline__ AttnSeq locate(const AttnArgs& a, int64_t t) {
     }
   }
   int64_t iq = lanes_prefix(sq, lane), is = lanes_prefix(ss, lane), it = lanes_prefix(st, lane);
-  const int64_t all = __shfl(it, 63, 64);
+  const int64_t all = uniform64(__shfl(it, 63, 64));  // uniform to the compiler: what follows stays in scalar registers
   if (t >= all) {
     r.spare = uniform64(t - all);
     r.q_end = uniform64(clamp64(__shfl(iq, 63, 64), a.total_q));
@@ -156,9 +156,29 @@ __device__ __forceinline__ AttnSeq locate_cache(const AttnArgs& a, int64_t t) {
   return r;
 }
 
+// (The fields once more through readfirstlane: descriptors and loop bounds that the compiler cannot prove uniform cost a
+// loop per load.)
+__device__ __forceinline__ AttnSeq uniform(AttnSeq r) {
+  r.b = __builtin_amdgcn_readfirstlane(r.b);
+  r.tile = __builtin_amdgcn_readfirstlane(r.tile);
+  r.found = __builtin_amdgcn_readfirstlane((int)r.found) != 0;
+  r.q_off = uniform64(r.q_off);
+  r.s_off = uniform64(r.s_off);
+  r.q_len = __builtin_amdgcn_readfirstlane(r.q_len);
+  r.s_len = __builtin_amdgcn_readfirstlane(r.s_len);
+  r.spare = uniform64(r.spare);
+  r.q_end = uniform64(r.q_end);
+  r.s_end = uniform64(r.s_end);
+  return r;
+}
+
 template <int TILE>
 __device__ __forceinline__ AttnSeq locate_rows(const AttnArgs& a, int64_t t) {
-  return a.capacity > 0 ? locate_cache<TILE>(a, t) : locate<TILE, false>(a, t);
+  return uniform(a.capacity > 0 ? locate_cache<TILE>(a, t) : locate<TILE, false>(a, t));
+}
+template <int TILE>
+__device__ __forceinline__ AttnSeq locate_keys(const AttnArgs& a, int64_t t) {
+  return uniform(locate<TILE, true>(a, t));
 }
 
 // ---- numbers of the products -------------------------------------------------------------------------------------------
