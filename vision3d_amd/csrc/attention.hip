@@ -229,60 +229,52 @@ __global__ __launch_bounds__(256, (attn_occupancy<T, HD>())) void attn_forward_k
   const T* k = static_cast<const T*>(a.k) + seq.b * a.k_batch + seq.s_off * a.k_row + (int64_t)kvh * a.k_head;
   const T* v = static_cast<const T*>(a.v) + seq.b * a.v_batch + seq.s_off * a.v_row + (int64_t)kvh * a.v_head;
 
-  // The tile after the one that is worked on is on its way in registers meanwhile.
-  TileStage<T, HD, BN, 256> stage_k, stage_v;
+  // The tile after the one that is worked on is on its way meanwhile: its keys under the scores, its values under the
+  // values' product, through the same registers.
+  TileStage<T, HD, BN, 256> stage;
   if (threadIdx.x < BUFS) lds_bad[threadIdx.x] = 0;
-  auto fetch = [&](int t) {
-    stage_k.fetch(k + (int64_t)t * BN * a.k_row, a.k_row, a.D, seq.s_len - t * BN);
-    stage_v.fetch(v + (int64_t)t * BN * a.v_row, a.v_row, a.D, seq.s_len - t * BN);
-  };
-  auto place_tile = [&](int t, int buf) {
-    stage_k.store(lds_k[buf], a.D);
-    stage_v.store(lds_v[buf], a.D);
-    if (t * BN + BN > least && stage_v.nonfinite()) lds_bad[buf] = t + 1;
+  auto fetch_k = [&](int t) { stage.fetch(k + (int64_t)t * BN * a.k_row, a.k_row, a.D, seq.s_len - t * BN); };
+  auto fetch_v = [&](int t) { stage.fetch(v + (int64_t)t * BN * a.v_row, a.v_row, a.D, seq.s_len - t * BN); };
+  auto place_v = [&](int t, int buf) {
+    stage.store(lds_v[buf], a.D);
+    if (t * BN + BN > least && stage.nonfinite()) lds_bad[buf] = t + 1;
   };
   auto work = [&](int t, auto buffer) {
-    constexpr int buf = decltype(buffer)::value;
+    constexpr int buf = decltype(buffer)::value, other = BUFS - 1 - buf;
     const int key0 = t * BN;
-    const bool active = key0 < w.most;
+    const bool active = key0 < w.most, more = t + 1 < t_end;
     f32x16 s[NT];
+    if (more) fetch_k(t + 1);
     if (active) w.template scores<NT>(lds_k[buf], key0, s);
     if (lds_bad[buf] == t + 1) {
       static_assert(BUFS * SIZE >= kAttnWaves * 1024, "room for the waves' probabilities");
-      __syncthreads();  // nobody reads the keys any more: both of their buffers are free until the next tile is placed
+      __syncthreads();  // nobody reads the keys any more: both of their buffers are free until the next keys are placed
       if (active) w.template add_nonfinite<NT>(lds_k[0] + wave * 1024, lds_v[buf], key0, s);
       __syncthreads();
       clear_nonfinite(lds_v[buf], SIZE, threadIdx.x, 256);
       __syncthreads();
     }
+    if constexpr (BUFS == 1) __syncthreads();
+    if (more) {
+      stage.store(lds_k[other], a.D);
+      fetch_v(t + 1);
+    }
     if (active) w.template values<NT>(lds_v[buf], s);
+    if constexpr (BUFS == 1) __syncthreads();
+    if (more) place_v(t + 1, other);
+    __syncthreads();
   };
 
   if (t_begin < t_end) {
+    fetch_k(t_begin);
+    stage.store(lds_k[0], a.D);
+    fetch_v(t_begin);
     __syncthreads();  // lds_bad
-    fetch(t_begin);
-    place_tile(t_begin, 0);
+    place_v(t_begin, 0);
     __syncthreads();
-    if constexpr (BUFS == 2) {
-      for (int t = t_begin; t < t_end; t += 2) {
-        if (t + 1 < t_end) fetch(t + 1);
-        work(t, Const<0>{});
-        if (t + 1 < t_end) place_tile(t + 1, 1);
-        __syncthreads();
-        if (t + 1 >= t_end) break;
-        if (t + 2 < t_end) fetch(t + 2);
-        work(t + 1, Const<1>{});
-        if (t + 2 < t_end) place_tile(t + 2, 0);
-        __syncthreads();
-      }
-    } else {
-      for (int t = t_begin; t < t_end; ++t) {
-        if (t + 1 < t_end) fetch(t + 1);
-        work(t, Const<0>{});
-        __syncthreads();
-        if (t + 1 < t_end) place_tile(t + 1, 0);
-        __syncthreads();
-      }
+    for (int t = t_begin; t < t_end; t += BUFS) {
+      work(t, Const<0>{});
+      if (BUFS == 2 && t + 1 < t_end) work(t + 1, Const<BUFS - 1>{});
     }
   }
 

@@ -279,6 +279,7 @@ struct Raw {
     for (int l = 0; l < L; ++l) {
       v[l] = c[l];
       if (D % E != 0) {
+        asm volatile("" : "+v"(v[l]));  // stays a branch: as selects the shift would cost every tile of every head size
         const int c0 = col + l * E, by = c0 < D ? max(0, c0 + E - D) : 0;
         unsigned __int128 x = __builtin_bit_cast(unsigned __int128, v[l]);
         x >>= by * 8 * (int)sizeof(T);
