@@ -30,6 +30,42 @@ constexpr int bwd_tile() { return Kind<T>::P == 1 && HD <= 64 ? 64 : 32; }
 template <typename T, int HD>
 constexpr int bwd_buffers() { return Kind<T>::P == 3 && HD > 128 ? 1 : 2; }
 
+// Tiles [0, count) pass by: `fetch` starts the loads of one into registers, `place` puts them into LDS, `work` uses it.  With
+// two buffers a tile is fetched two tiles ahead of its use (a tile's work is shorter than a load's way from memory); loads
+// past the last tile read nothing but are issued all the same, so that waiting for the older ones stays countable.
+template <int BUFS, typename Fetch, typename Place, typename Work>
+__device__ __forceinline__ void pass_tiles(int count, Fetch fetch, Place place, Work work) {
+  if (count <= 0) return;
+  if constexpr (BUFS == 2) {
+    fetch(0, Const<0>{});
+    fetch(1, Const<1>{});
+    place(Const<0>{});
+    __syncthreads();
+    for (int t = 0; t < count; t += 2) {
+      fetch(t + 2, Const<0>{});
+      work(t, Const<0>{});
+      place(Const<1>{});
+      __syncthreads();
+      if (t + 1 >= count) break;
+      fetch(t + 3, Const<1>{});
+      work(t + 1, Const<1>{});
+      place(Const<0>{});
+      __syncthreads();
+    }
+  } else {
+    fetch(0, Const<0>{});
+    place(Const<0>{});
+    __syncthreads();
+    for (int t = 0; t < count; ++t) {
+      fetch(t + 1, Const<0>{});
+      work(t, Const<0>{});
+      __syncthreads();
+      place(Const<0>{});
+      __syncthreads();
+    }
+  }
+}
+
 template <typename T, int HD>
 __global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 128 : 64) ? 2 : 1) void attn_backward_q_kernel(const AttnBwdArgs b) {
   constexpr int HDP = attn_pow2(HD);
@@ -47,7 +83,7 @@ __global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 128 : 64) ? 2 : 1) vo
   const int half = lane >> 5;
   int64_t id = blockIdx.x;
   const int kvh = (int)(id % a.KV);
-  id = (int64_t)(gridDim.x / a.KV) - 1 - id / a.KV;  // causal: the longest tiles of a sequence start first
+  id /= a.KV;
   const AttnSeq seq = locate_rows<kAttnRows>(a, id);
   T* dq = static_cast<T*>(b.dq);
   if (!seq.found) {  // rows behind the last sequence have no gradient
@@ -80,14 +116,14 @@ __global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 128 : 64) ? 2 : 1) vo
   const int64_t at0 = ((seq.q_off + token0) * a.H + (int64_t)kvh * a.G) * a.D;
   const int at_row = (int)(at * a.D - at0);
 
-  TileStage<T, HD, BN, 256> stage_k, stage_v;
-  auto fetch = [&](int t) {
-    stage_k.fetch(k + (int64_t)t * BN * a.k_row, a.k_row, a.D, seq.s_len - t * BN);
-    stage_v.fetch(v + (int64_t)t * BN * a.v_row, a.v_row, a.D, seq.s_len - t * BN);
+  TileStage<T, HD, BN, 256> stage_k[BUFS], stage_v[BUFS];
+  auto fetch = [&](int t, auto to) {
+    stage_k[decltype(to)::value].fetch(k + (int64_t)t * BN * a.k_row, a.k_row, a.D, seq.s_len - t * BN);
+    stage_v[decltype(to)::value].fetch(v + (int64_t)t * BN * a.v_row, a.v_row, a.D, seq.s_len - t * BN);
   };
-  auto place_tile = [&](int buf) {
-    stage_k.store(lds_k[buf], a.D);
-    stage_v.store(lds_v[buf], a.D);
+  auto place_tile = [&](auto from) {
+    stage_k[decltype(from)::value].store(lds_k[decltype(from)::value], a.D);
+    stage_v[decltype(from)::value].store(lds_v[decltype(from)::value], a.D);
   };
 
   Op<T> qf[STEPS], gf[STEPS];
@@ -143,70 +179,54 @@ __global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 128 : 64) ? 2 : 1) vo
     }
   };
 
-  const int tiles = (most + BN - 1) / BN;
-  if (tiles > 0) {
-    fetch(0);
-    place_tile(0);
-    __syncthreads();
-    if constexpr (BUFS == 2) {
-      for (int t = 0; t < tiles; t += 2) {
-        if (t + 1 < tiles) fetch(t + 1);
-        work(t, Const<0>{});
-        if (t + 1 < tiles) place_tile(1);
-        __syncthreads();
-        if (t + 1 >= tiles) break;
-        if (t + 2 < tiles) fetch(t + 2);
-        work(t + 1, Const<1>{});
-        if (t + 2 < tiles) place_tile(0);
-        __syncthreads();
-      }
-    } else {
-      for (int t = 0; t < tiles; ++t) {
-        if (t + 1 < tiles) fetch(t + 1);
-        work(t, Const<0>{});
-        __syncthreads();
-        if (t + 1 < tiles) place_tile(0);
-        __syncthreads();
-      }
-    }
-  }
+  pass_tiles<BUFS>((most + BN - 1) / BN, fetch, place_tile, work);
   if (row < rows) store_rows<T, DT>(dq + at * a.D, acc, a.scale, a.D, half);
 }
 
+// dk and dv of a tile of 32 GROUPS keys.  A wave keeps 32 keys: their operands and both sums, 320 registers with 16-bit heads
+// of 128, one wave on a SIMD.  Where that does not fit the 512 registers two waves share 32 keys, one sums dv, the other dk,
+// and both form s: 40 products instead of 32, but nothing is spilled (16-bit heads of 256: 362 registers otherwise).  Up to
+// there the single wave is faster although it has a SIMD to itself: 8 x 2048 tokens, 16/4 heads of 128, bf16, no mask: 869 us
+// against 932 (633 and 590 TFLOP/s of the 32 products), heads of 64: 404 us against 596.
 template <typename T, int HD>
-__global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 64 : 32) ? 2 : 1) void attn_backward_kv_kernel(const AttnBwdArgs b) {
+constexpr bool kv_roles() { return HD > (Kind<T>::P == 1 ? 128 : 96); }
+template <typename T, int HD>
+constexpr int kv_groups() { return kv_roles<T, HD>() ? 2 : 4; }
+constexpr int kKvThreads = 256;
+
+template <typename T, int HD>
+__global__ __launch_bounds__(kKvThreads, HD <= 32 ? 2 : 1) void attn_backward_kv_kernel(const AttnBwdArgs b) {
   constexpr int HDP = attn_pow2(HD);
-  constexpr int BM = bwd_tile<T, HD>();
+  constexpr int BM = 32;
   constexpr int NT = BM / 32;
   constexpr int BUFS = bwd_buffers<T, HD>();
   constexpr int STEPS = HD / 16;
   constexpr int DT = HD / 32;
+  constexpr int GROUPS = kv_groups<T, HD>(), KEYS = 32 * GROUPS, THREADS = kKvThreads;
+  constexpr bool kRoles = kv_roles<T, HD>();
   typedef typename Kind<T>::U U;
   __shared__ __attribute__((aligned(16))) U lds_q[BUFS][Kind<T>::P * BM * HDP];
   __shared__ __attribute__((aligned(16))) U lds_g[BUFS][Kind<T>::P * BM * HDP];
-  // The wave's keys stay in registers, its values in LDS: two waves fit a SIMD, and one's products run under the other's
-  // exponentials (16-bit heads of 128, 8192 tokens: VALUES_REG us with both in registers and one wave).
-  constexpr bool kValuesLds = Kind<T>::P == 1 && HD <= 64;
-  __shared__ __attribute__((aligned(16))) U lds_vt[kValuesLds ? kAttnRows * HDP : 8];
   __shared__ float lds_lse[BUFS][BM], lds_delta[BUFS][BM];
   __shared__ int lds_limit[BUFS][BM];
 
   const AttnArgs& a = b.f;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = lane >> 5;
+  const bool keys_role = !kRoles || wave >= GROUPS;  // this wave sums dk (without roles dv too), else dv
   int64_t id = blockIdx.x;
   const int kvh = (int)(id % a.KV);
   id /= a.KV;
   const int split = (int)(id % b.splits);
-  const AttnSeq seq = locate_keys<kAttnRows>(a, id / b.splits);
+  const AttnSeq seq = locate_keys<KEYS>(a, id / b.splits);
   T* dk = static_cast<T*>(b.dk);
   T* dv = static_cast<T*>(b.dv);
   const int64_t plane = a.total_s * a.KV * a.D;
   float* pk = b.part + 2 * split * plane;
   float* pv = pk + plane;
   if (!seq.found) {  // keys behind the last sequence have no gradient
-    for (int i = threadIdx.x; i < kAttnRows; i += 256) {
-      const int64_t r = seq.s_end + seq.spare * kAttnRows + i;
+    for (int i = threadIdx.x; i < KEYS; i += THREADS) {
+      const int64_t r = seq.s_end + seq.spare * KEYS + i;
       if (r >= a.total_s) break;
       for (int64_t d = (r * a.KV + kvh) * a.D; d < (r * a.KV + kvh + 1) * a.D; ++d) {
         if (b.splits == 1)
@@ -217,9 +237,9 @@ __global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 64 : 32) ? 2 : 1) voi
     }
     return;
   }
-  const int key0 = seq.tile * kAttnRows;
+  const int key0 = seq.tile * KEYS;
   if (key0 >= seq.s_len) return;  // cut
-  const int wave_key = key0 + wave * 32;
+  const int wave_key = key0 + wave % GROUPS * 32;
   const int key = wave_key + (lane & 31);
   const bool live = key < seq.s_len;
   const int rows = seq.q_len * a.G;
@@ -234,16 +254,20 @@ __global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 64 : 32) ? 2 : 1) voi
   const float* lse = a.lse + seq.q_off * a.H + kvh * a.G;
   const float* delta = b.delta + seq.q_off * a.H + kvh * a.G;
 
-  TileStage<T, HD, BM, 256> stage_q, stage_g;
-  float stage_lse = 0.f, stage_delta = 0.f;
-  int stage_limit = 0;
-  auto fetch = [&](int row0) {
+  const int blocks = max(0, (rows - first / BM * BM + BM - 1) / BM), per = (blocks + b.splits - 1) / b.splits;
+  const int begin = first / BM * BM + split * per * BM, end = min(rows, begin + per * BM);
+  TileStage<T, HD, BM, THREADS> stage_q[BUFS], stage_g[BUFS];
+  float stage_lse[BUFS], stage_delta[BUFS];
+  int stage_limit[BUFS];
+  auto fetch = [&](int t, auto to) {
+    constexpr int st = decltype(to)::value;
+    const int row0 = min(begin + t * BM, rows);
     const int tok0 = div_g(a, row0);
-    stage_q.fetch_at(q + tok0 * a.q_row, [&](int r) {
+    stage_q[st].fetch_at(q + tok0 * a.q_row, [&](int r) {
       const int tok = div_g(a, row0 + r);
       return (tok - tok0) * (int)a.q_row + (row0 + r - tok * a.G) * (int)a.q_head;
     }, a.D, rows - row0);
-    stage_g.fetch_at(grad + (int64_t)tok0 * a.H * a.D, [&](int r) {
+    stage_g[st].fetch_at(grad + (int64_t)tok0 * a.H * a.D, [&](int r) {
       const int tok = div_g(a, row0 + r);
       return ((tok - tok0) * a.H + (row0 + r - tok * a.G)) * a.D;
     }, a.D, rows - row0);
@@ -251,111 +275,95 @@ __global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 64 : 32) ? 2 : 1) voi
       const int r = min(row0 + (int)threadIdx.x, rows - 1);
       const int tok = div_g(a, r);
       const int64_t i = (int64_t)tok * a.H + (r - tok * a.G);
-      stage_lse = lse[i];
-      stage_delta = delta[i];
-      stage_limit = row0 + (int)threadIdx.x < rows ? attn_limit(a, seq, tok) : 0;  // a row past the last sees no key
+      stage_lse[st] = lse[i];
+      stage_delta[st] = delta[i];
+      stage_limit[st] = row0 + (int)threadIdx.x < rows ? attn_limit(a, seq, tok) : 0;  // a row past the last sees no key
     }
   };
-  auto place_tile = [&](int buf) {
-    stage_q.store(lds_q[buf], a.D);
-    stage_g.store(lds_g[buf], a.D);
+  auto place_tile = [&](auto from) {
+    constexpr int buf = decltype(from)::value;
+    stage_q[buf].store(lds_q[buf], a.D);
+    stage_g[buf].store(lds_g[buf], a.D);
     if (threadIdx.x < BM) {
-      lds_lse[buf][threadIdx.x] = stage_lse;
-      lds_delta[buf][threadIdx.x] = stage_delta;
-      lds_limit[buf][threadIdx.x] = stage_limit;
+      lds_lse[buf][threadIdx.x] = stage_lse[buf];
+      lds_delta[buf][threadIdx.x] = stage_delta[buf];
+      lds_limit[buf][threadIdx.x] = stage_limit[buf];
     }
   };
 
-  Op<T> kf[STEPS], vf[kValuesLds ? 1 : STEPS];
+  Op<T> kf[STEPS], vf[STEPS];
   load_ops<T>(kf, k, (key - key0) * (int)a.k_row, half, a.D, live);
-  if constexpr (kValuesLds) {
-    TileStage<T, HD, kAttnRows, 256> stage_v;
-    stage_v.fetch(v, a.v_row, a.D, seq.s_len - key0);
-    stage_v.store(lds_vt, a.D);
-  } else {
-    load_ops<T>(vf, v, (key - key0) * (int)a.v_row, half, a.D, live);
-  }
-  auto value = [&](int st) {
-    if constexpr (kValuesLds) return read_cols<T, HDP, kAttnRows>(lds_vt, wave * 32 + (lane & 31), st, half);
-    else return vf[st];
-  };
+  load_ops<T>(vf, v, (key - key0) * (int)a.v_row, half, a.D, live);
   const float c2 = a.scale * kLog2e;
-  f32x16 ak[DT], av[DT];
+  f32x16 acc[DT], other[kRoles ? 1 : DT];  // of the wave's role, or dk and dv
 #pragma unroll
-  for (int d = 0; d < DT; ++d) ak[d] = av[d] = zero16();
+  for (int d = 0; d < DT; ++d) acc[d] = zero16();
+#pragma unroll
+  for (int d = 0; d < (kRoles ? 1 : DT); ++d) other[d] = zero16();
 
-  auto work = [&](int row0, auto buffer) {
+  auto work = [&](int t, auto buffer) {
     constexpr int buf = decltype(buffer)::value;
+    const int row0 = begin + t * BM;
     if (wave_key >= seq.s_len || row0 + BM <= wave_first) return;
     // every row of the tile sees every key of the wave: the first row's limit is the least
     const bool whole = row0 + BM <= rows && wave_key + 32 <= __builtin_amdgcn_readfirstlane(lds_limit[buf][0]);
+    const U* summed = keys_role ? lds_q[buf] : lds_g[buf];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      f32x16 s = zero16(), dp = zero16();
+      f32x16 s = zero16();
 #pragma unroll
-      for (int st = 0; st < STEPS; ++st) {
+      for (int st = 0; st < STEPS; ++st)
         s = product<T>(read_cols<T, HDP, BM>(lds_q[buf], n * 32 + (lane & 31), st, half), kf[st], s);
-        dp = product<T>(read_cols<T, HDP, BM>(lds_g[buf], n * 32 + (lane & 31), st, half), value(st), dp);
-      }
+      f32x16 p;
+      if (keys_role) {
+        f32x16 dp = zero16();
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int i = n * 32 + acc_row(r, half);
-        s[r] = exp2_fast(fmaf(s[r], c2, -lds_lse[buf][i]));
-        dp[r] = s[r] * (dp[r] - lds_delta[buf][i]);
+        for (int st = 0; st < STEPS; ++st)
+          dp = product<T>(read_cols<T, HDP, BM>(lds_g[buf], n * 32 + (lane & 31), st, half), vf[st], dp);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int i = n * 32 + acc_row(r, half);
+          p[r] = exp2_fast(fmaf(s[r], c2, -lds_lse[buf][i]));
+          s[r] = p[r] * (dp[r] - lds_delta[buf][i]);
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = exp2_fast(fmaf(s[r], c2, -lds_lse[buf][n * 32 + acc_row(r, half)]));
       }
       if (!whole) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (key >= lds_limit[buf][n * 32 + acc_row(r, half)]) s[r] = dp[r] = 0.f;
+          if (key >= lds_limit[buf][n * 32 + acc_row(r, half)]) s[r] = p[r] = 0.f;
       }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const Op<T> p = pack_rows<T>(s, u), ds = pack_rows<T>(dp, u);
+        if constexpr (!kRoles) {
+          const Op<T> y = pack_rows<T>(p, u);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          av[d] = product<T>(read_rows<T, HDP, BM>(lds_g[buf], n * 32, u, d * 32, lane), p, av[d]);
-          ak[d] = product<T>(read_rows<T, HDP, BM>(lds_q[buf], n * 32, u, d * 32, lane), ds, ak[d]);
+          for (int d = 0; d < DT; ++d)
+            other[d] = product<T>(read_rows<T, HDP, BM>(lds_g[buf], n * 32, u, d * 32, lane), y, other[d]);
         }
+        const Op<T> x = pack_rows<T>(s, u);
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+          acc[d] = product<T>(read_rows<T, HDP, BM>(summed, n * 32, u, d * 32, lane), x, acc[d]);
       }
     }
   };
 
-  const int blocks = max(0, (rows - first / BM * BM + BM - 1) / BM), per = (blocks + b.splits - 1) / b.splits;
-  const int begin = first / BM * BM + split * per * BM, end = min(rows, begin + per * BM);
-  if (begin < end) {
-    fetch(begin);
-    place_tile(0);
-    __syncthreads();
-    if constexpr (BUFS == 2) {
-      for (int r = begin; r < end; r += 2 * BM) {
-        if (r + BM < end) fetch(r + BM);
-        work(r, Const<0>{});
-        if (r + BM < end) place_tile(1);
-        __syncthreads();
-        if (r + BM >= end) break;
-        if (r + 2 * BM < end) fetch(r + 2 * BM);
-        work(r + BM, Const<1>{});
-        if (r + 2 * BM < end) place_tile(0);
-        __syncthreads();
-      }
-    } else {
-      for (int r = begin; r < end; r += BM) {
-        if (r + BM < end) fetch(r + BM);
-        work(r, Const<0>{});
-        __syncthreads();
-        if (r + BM < end) place_tile(0);
-        __syncthreads();
-      }
-    }
-  }
+  pass_tiles<BUFS>(max(0, (end - begin + BM - 1) / BM), fetch, place_tile, work);
   if (!live) return;
   const int64_t at = ((seq.s_off + key) * a.KV + kvh) * a.D;
-  if (b.splits == 1) {
-    store_rows<T, DT>(dk + at, ak, a.scale, a.D, half);
-    store_rows<T, DT>(dv + at, av, 1.f, a.D, half);
-  } else {
-    store_rows<float, DT>(pk + at, ak, a.scale, a.D, half);
-    store_rows<float, DT>(pv + at, av, 1.f, a.D, half);
+  const float f = keys_role ? a.scale : 1.f;
+  if (b.splits == 1)
+    store_rows<T, DT>((keys_role ? dk : dv) + at, acc, f, a.D, half);
+  else
+    store_rows<float, DT>((keys_role ? pk : pv) + at, acc, f, a.D, half);
+  if constexpr (!kRoles) {
+    if (b.splits == 1)
+      store_rows<T, DT>(dv + at, other, 1.f, a.D, half);
+    else
+      store_rows<float, DT>(pv + at, other, 1.f, a.D, half);
   }
 }
 
@@ -397,15 +405,16 @@ inline int attn_backward_splits(int B, int64_t total_s, int KV) {
 template <typename T, int HD>
 int attn_backward_launch(const AttnBwdArgs& b, hipStream_t stream, const char* what) {
   const AttnArgs& a = b.f;
-  const int64_t q_tiles = ceil_div(a.total_q * a.G, kAttnRows) + a.B, s_tiles = ceil_div(a.total_s, kAttnRows) + a.B;
+  const int64_t q_tiles = ceil_div(a.total_q * a.G, kAttnRows) + a.B;
+  const int64_t s_tiles = ceil_div(a.total_s, 32 * kv_groups<T, HD>()) + a.B;
   int rc = 0;
   if (a.total_q > 0) {
     hipLaunchKernelGGL((attn_backward_q_kernel<T, HD>), dim3((unsigned)(q_tiles * a.KV)), dim3(256), 0, stream, b);
     rc = launch_status(what);
   }
   if (rc == 0 && a.total_s > 0) {
-    hipLaunchKernelGGL((attn_backward_kv_kernel<T, HD>), dim3((unsigned)(s_tiles * a.KV * b.splits)), dim3(256), 0,
-                       stream, b);
+    hipLaunchKernelGGL((attn_backward_kv_kernel<T, HD>), dim3((unsigned)(s_tiles * a.KV * b.splits)),
+                       dim3(kKvThreads), 0, stream, b);
     rc = launch_status(what);
     if (rc == 0 && b.splits > 1) {
       const dim3 grid((unsigned)ceil_div(a.total_s * a.KV * a.D, 1024), 2);
