@@ -246,7 +246,7 @@ __global__ __launch_bounds__(256, (attn_occupancy<T, HD>())) void attn_forward_k
     f32x16 s[NT];
     if (more) fetch_k(t + 1);
     if (active) w.template scores<NT>(lds_k[buf], key0, s);
-    if (lds_bad[buf] == t + 1) {
+    if (key0 + BN > least && lds_bad[buf] == t + 1) {
       static_assert(BUFS * SIZE >= kAttnWaves * 1024, "room for the waves' probabilities");
       __syncthreads();  // nobody reads the keys any more: both of their buffers are free until the next keys are placed
       if (active) w.template add_nonfinite<NT>(lds_k[0] + wave * 1024, lds_v[buf], key0, s);
@@ -461,18 +461,26 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
     const int token = div_g(a, row);
     return (seq.q_off + token) * a.H + (int64_t)kvh * a.G + (row - token * a.G);
   }();
-  const int col = lane * 4;
+  // as many lanes as the columns need (4 each), the others take other parts
+  const int width = a.D <= 64 ? 16 : (a.D <= 128 ? 32 : 64);
+  const int col = lane % width * 4;
   float o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-  for (int s = 0; s < a.splits; ++s) {
+  for (int s = lane / width; s < a.splits; s += 64 / width) {
     const float fs = factor[wave][s];
     const float* p = a.part_o + (part + (int64_t)s * TILE) * a.D;
 #pragma unroll
     for (int j = 0; j < 4; ++j) o[j] = fmaf(col + j < a.D ? p[col + j] : 0.f, fs, o[j]);
   }
 #pragma unroll
+  for (int d = 32; d >= 16; d >>= 1)
+    if (d >= width) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] += __shfl_xor(o[j], d, 64);
+    }
+#pragma unroll
   for (int j = 0; j < 4; ++j) o[j] *= inv;
-  store_out<T>(a, out, col, o);
+  if (lane < width) store_out<T>(a, out, col, o);
   if (a.lse && lane == 0) a.lse[out] = log_sum(m, l);
 }
 
@@ -493,10 +501,11 @@ inline AttnPlan attn_plan(int B, int64_t total_q, int64_t total_s, int tokens, i
   // (2 x 1024 tokens, 2 key heads of 128): 40 us against 37, keys and values being read by four times as many workgroups.
   p.few = total_q * G <= (int64_t)32 * B || (ceil_div(total_q * G, kAttnRows) + B) * KV <= 64;
   p.tiles = tokens > 0 ? B * ceil_div((int64_t)tokens * G, p.tile()) : ceil_div(total_q * G, p.tile()) + B;
-  // Keys are divided where the row tiles leave compute units idle (two workgroups on each of 256), as far as every part
-  // of a sequence of the mean length keeps 256 keys.
+  // Keys are divided where the row tiles leave compute units idle, as far as every part of a sequence of the mean length
+  // keeps 512 keys: into one workgroup a CU of the 32-row kernel, which is bound by memory (6 caches of 32768 rows, 4 tokens:
+  // 44 us; 512 workgroups, whose parts are twice the bytes to join: 49 us), into two of the other.
   const int64_t groups = std::max<int64_t>(p.tiles * KV, 1), mean = tokens > 0 ? total_s : total_s / std::max(B, 1);
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / groups, mean / 256, 64}));
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(p.few ? 256 : 512) / groups, mean / 512, 64}));
   p.bytes = p.splits > 1 ? (size_t)(groups * p.splits * p.tile()) * (size_t)(D + 2) * sizeof(float) : 0;
   return p;
 }
