@@ -243,6 +243,45 @@ def test_cache_equals_the_packs_last_rows():
 
 
 @pytest.mark.gpu
+def test_cache_beyond_32_bit_offsets():
+    # 2^31 elements of keys and as many of values in one cache: only the last rows carry weight
+    capacity, kv, dim = (1 << 21) + 70, 8, 128
+    k = torch.zeros((1, capacity, kv, dim), dtype=torch.bfloat16, device=DEV)
+    v = torch.zeros_like(k)
+    gen = torch.Generator().manual_seed(0)
+    n = capacity - 5
+    tail = torch.randn((3, kv, dim), generator=gen).to(torch.bfloat16)
+    k[0, n - 3:n], v[0, n - 3:n] = 2.0, tail.to(DEV)
+    k[0, n:], v[0, n:] = float("nan"), float("nan")
+    q = torch.full((1, 1, 16, dim), 2.0, dtype=torch.bfloat16, device=DEV)
+    got = ops.cached_attention(q, k, v, torch.tensor([n], device=DEV))[0, 0].double().cpu()
+    # the three rows' scores are 4 * 128 / sqrt(128) = 45.25, all others 0: their weight is 2^21 e^-45 of the whole
+    want = tail.double().mean(0).repeat_interleave(2, 0)
+    assert (got - want).abs().max() <= 2.0 ** -8 * 4 + 1e-6
+    pack = ops.attention_pack_mode(q[0], k[0, :n], v[0, :n], torch.tensor([1], device=DEV), torch.tensor([n], device=DEV))
+    assert (pack[0].double().cpu() - want).abs().max() <= 2.0 ** -8 * 4 + 1e-6
+
+
+@pytest.mark.gpu
+def test_shared_and_far_rows():
+    # a key row for all (stride 0), rows far apart (a stride beyond what a tile's offsets hold is copied), overlapping rows
+    q, k, v = (t.to(DEV) for t in _pack([50], [50], 2, 2, 64, torch.float16))
+    n = torch.tensor([50], device=DEV)
+    shared = k[:1].expand(50, 2, 64)
+    assert torch.equal(ops.attention_pack_mode(q, shared, v, n), ops.attention_pack_mode(q, shared.contiguous(), v, n))
+    want = ops.attention_pack_mode(q, k, v, n, causal=True)
+    for stride in (1 << 21, 1 << 22, 1 << 23):  # elements between rows
+        far = torch.empty(50 * stride, dtype=torch.float16, device=DEV).view(50, stride)[:, :128].view(50, 2, 64)
+        far.copy_(k)
+        assert torch.equal(ops.attention_pack_mode(q, far, v, n, causal=True), want)
+        far.copy_(q)
+        assert torch.equal(ops.attention_pack_mode(far, k, v, n, causal=True), want)
+        del far
+    over = torch.randn(50 * 32 + 128, device=DEV).to(torch.float16).as_strided((50, 2, 64), (32, 64, 1))
+    assert torch.equal(ops.attention_pack_mode(q, over, over, n), ops.attention_pack_mode(q, over.contiguous(), over.contiguous(), n))
+
+
+@pytest.mark.gpu
 def test_other_stream_and_graph_replays():
     from vision3d_amd import ext
 

@@ -119,6 +119,49 @@ def test_tile_borders(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("count", [2, 63, 64, 65, 200])
+def test_numbers_of_sequences(count, causal):
+    # up to 64 sequences are looked up one to a lane and, causal, numbered by work; more are divided among the lanes
+    gen = torch.Generator().manual_seed(count)
+    lengths = torch.randint(0, 70, (count,), generator=gen).tolist()
+    lengths[count // 2] = 300
+    keys = torch.randint(0, 70, (count,), generator=gen).tolist()
+    keys[-1] = 200
+    _check(torch.bfloat16, lengths, keys, 2, 1, 32, causal, seed=count, spare=5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_nothing_to_do(dtype):
+    q, k, v, g = (t.to(DEV).requires_grad_(True) for t in _inputs([7], [9], 2, 1, 32, dtype, 0))
+    none, zero = torch.zeros(0, dtype=torch.long, device=DEV), torch.zeros(2, dtype=torch.long, device=DEV)
+    for lengths in (none, zero):  # no sequence, or only empty ones: zeros everywhere
+        out = ops.attention_pack_mode(q, k, v, lengths, causal=True)
+        grads = torch.autograd.grad(out, (q, k, v), g.detach())
+        for t in (out, *grads):
+            assert torch.equal(t, torch.zeros_like(t))
+    for qs, ks in ((q[:0], k), (q, k[:0]), (q[:0], k[:0])):  # no queries, no keys, neither
+        vs = v[:ks.shape[0]]
+        out = ops.attention_pack_mode(qs, ks, vs, torch.tensor([qs.shape[0]]), torch.tensor([ks.shape[0]]))
+        grads = torch.autograd.grad(out, (q, k, v), g[:qs.shape[0]].detach())
+        for t in (out, *grads):
+            assert torch.equal(t, torch.zeros_like(t))
+
+
+@pytest.mark.gpu
+def test_lengths_that_overrun_are_cut():
+    q, k, v, g = (t.to(DEV).requires_grad_(True) for t in _inputs([60], [60], 2, 1, 32, torch.float32, 3))
+    grads = []
+    for lengths in ([20, 40], [20, 4000, 7], [-3, 20, 1 << 62, 1 << 62]):
+        out = ops.attention_pack_mode(q, k, v, torch.tensor(lengths, device=DEV), causal=True)
+        grads.append([out, *torch.autograd.grad(out, (q, k, v), g.detach())])
+    for other in grads[1:]:
+        for a, b in zip(grads[0], other):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
 def test_strided_leaves_and_part_of_them():
     lengths = torch.tensor([50, 77], device=DEV)
     qkv = torch.randn((127, 8, 64), device=DEV, requires_grad=True)

@@ -503,7 +503,7 @@ inline AttnPlan attn_plan(int B, int64_t total_q, int64_t total_s, int tokens, i
   p.tiles = tokens > 0 ? B * ceil_div((int64_t)tokens * G, p.tile()) : ceil_div(total_q * G, p.tile()) + B;
   // Keys are divided where the row tiles leave compute units idle, as far as every part of a sequence of the mean length
   // keeps 512 keys: into one workgroup a CU of the 32-row kernel, which is bound by memory (6 caches of 32768 rows, 4 tokens:
-  // 44 us; 512 workgroups, whose parts are twice the bytes to join: 49 us), into two of the other.
+  // 42 us; 512 workgroups, whose parts are twice the bytes to join: 49 us), into two of the other.
   const int64_t groups = std::max<int64_t>(p.tiles * KV, 1), mean = tokens > 0 ? total_s : total_s / std::max(B, 1);
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(p.few ? 256 : 512) / groups, mean / 512, 64}));
   p.bytes = p.splits > 1 ? (size_t)(groups * p.splits * p.tile()) * (size_t)(D + 2) * sizeof(float) : 0;
@@ -580,7 +580,8 @@ int attn_forward_run(AttnArgs& a, int dtype, const AttnPlan& plan, void* workspa
                      void* stream, const char* what) {
   const int bad = attn_check_strides(what, a);
   if (bad != 0) return bad;
-  if (plan.tiles * a.KV * plan.splits > ((int64_t)1 << 31) / 64) {
+  if (plan.tiles * a.KV * plan.splits >= (int64_t)1 << 31 ||
+      (plan.splits > 1 && plan.tiles * a.KV * (plan.tile() / 4) >= (int64_t)1 << 31)) {
     set_last_error("%s: too many tiles", what);
     return V3D_ERR_SIZE_LIMIT;
   }
@@ -606,7 +607,7 @@ int attn_forward_run(AttnArgs& a, int dtype, const AttnPlan& plan, void* workspa
 extern "C" {
 
 size_t v3d_attention_pack_workspace_bytes(int B, int64_t total_q, int64_t total_s, int H, int KV, int D) {
-  if (B <= 0 || total_q <= 0 || H <= 0 || KV <= 0 || H % KV != 0 || D <= 0) return 0;
+  if (B < 0 || total_q <= 0 || total_s < 0 || H <= 0 || KV <= 0 || H % KV != 0 || D <= 0) return 0;
   return v3d::attn_plan(B, total_q, total_s, 0, KV, H / KV, D).bytes;
 }
 

@@ -394,12 +394,12 @@ __global__ __launch_bounds__(256) void attn_backward_join_kernel(const AttnBwdAr
 }
 
 // ---- launches ----------------------------------------------------------------------------------------------------------
-#ifndef KV_TARGET
-#define KV_TARGET 1024
-#endif
+// Parts of a key tile's rows: as many as bring about four workgroups to a CU.  One workgroup fills a CU, and a causal tile at
+// the start of a sequence has all the rows behind it (8192 tokens in 5 sequences, 16/4 heads of 128, bf16: 1 / 2 / 3 parts
+// 468 / 269 / 263 us, and 13 / 18 us to join the parts; 8000 tokens, 4 heads of 64, fp32: 145 / 118 + 11 us).
 inline int attn_backward_splits(int B, int64_t total_s, int KV) {
-  const int64_t groups = (ceil_div(total_s, kAttnRows) + B) * KV;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(KV_TARGET / groups, 8));
+  const int64_t groups = std::max<int64_t>((ceil_div(total_s, kAttnRows) + B) * KV, 1);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(1024 / groups, 8));
 }
 
 template <typename T, int HD>
@@ -491,6 +491,12 @@ int v3d_attention_pack_bwd(const void* grad, const void* q, const void* k, const
   b.dv = grad_v;
   rc = attn_check_strides(what, a);
   if (rc != 0) return rc;
+  if ((ceil_div(total_q * a.G, kAttnRows) + B) * KV >= (int64_t)1 << 31 ||
+      (ceil_div(total_s, 64) + B) * KV * attn_backward_splits(B, total_s, KV) >= (int64_t)1 << 31 ||
+      ceil_div(total_s * KV * D, 1024) >= (int64_t)1 << 31) {
+    set_last_error("%s: too many tiles", what);
+    return V3D_ERR_SIZE_LIMIT;
+  }
   DeviceGuard guard(device);
   if (guard.rc != 0) return guard.rc;
   hipStream_t s = static_cast<hipStream_t>(stream);
