@@ -1054,32 +1054,44 @@ def layer_norm_forward(feats, residual, weight, bias, targets, stats, eps):
     _same_device(name, feats, residual, weight, bias, targets, stats)
     mean = _ptr(stats)
     dev, stream = _where(feats)
-    _lib.check(_lib.lib().v3d_layer_norm_fwd(feats.data_ptr(), _ptr(residual), _ptr(weight), _ptr(bias),
-                                             targets.data_ptr(), mean, None if mean is None else mean + 4 * rows, dtype,
-                                             wdtype, rows, channels, float(eps), dev, stream), name)
+    rc = _lib.lib().v3d_layer_norm_fwd(feats.data_ptr(), _ptr(residual), _ptr(weight), _ptr(bias), targets.data_ptr(), mean,
+                                       None if mean is None else mean + 4 * rows, dtype, wdtype, rows, channels,
+                                       float(eps), dev, stream)
+    if rc != 0:
+        _lib.check(rc, name)
 
 
 def layer_norm_backward(target_grads, feats, residual, weight, stats, feats_grads, weight_grads, bias_grads):
     """The gradients of ``layer_norm_forward``: each of the three outputs may be None (not wanted)."""
     name = "layer_norm_backward"
     sums = weight_grads if weight_grads is not None else bias_grads
-    dtype, wdtype, rows, channels = _layer_norm_check(name, feats, residual, weight, None, stats)
+    _layer_norm_check(name, feats, residual, weight, None, stats)
     _operand(name, target_grads, "target_grads", feats.shape, feats.dtype)
     _operand(name, feats_grads, "feats_grads", feats.shape, feats.dtype)
-    nbytes = 0
-    lib = _lib.lib()
     if sums is not None:
-        _operand(name, weight_grads, "weight_grads", (channels,), sums.dtype if weight is None else weight.dtype)
-        _operand(name, bias_grads, "bias_grads", (channels,), sums.dtype if weight is None else weight.dtype)
-        wdtype = _element(sums, name)
-        nbytes = lib.v3d_layer_norm_bwd_workspace_bytes(rows, channels)
+        dtype = sums.dtype if weight is None else weight.dtype
+        _operand(name, weight_grads, "weight_grads", feats.shape[1:], dtype)
+        _operand(name, bias_grads, "bias_grads", feats.shape[1:], dtype)
+        _element(sums, name)
     _same_device(name, feats, target_grads, residual, weight, stats, feats_grads, weight_grads, bias_grads)
+    _layer_norm_backward(target_grads, feats, residual, weight, stats, feats_grads, weight_grads, bias_grads)
+
+
+def _layer_norm_backward(target_grads, feats, residual, weight, stats, feats_grads, weight_grads, bias_grads):
+    """The launch alone, for the autograd function, whose tensors the forward has checked or the backward has made."""
+    rows, channels = feats.shape
+    sums = weight_grads if weight_grads is not None else bias_grads
+    affine = weight if sums is None else sums
+    lib = _lib.lib()
+    ws, wp, wn = _ws_args(0 if sums is None else lib.v3d_layer_norm_bwd_workspace_bytes(rows, channels), feats)
     mean = stats.data_ptr()
-    ws, wp, wn = _ws_args(nbytes, feats)
     dev, stream = _where(feats)
-    _lib.check(lib.v3d_layer_norm_bwd(target_grads.data_ptr(), feats.data_ptr(), _ptr(residual), _ptr(weight), mean,
-                                      mean + 4 * rows, _ptr(feats_grads), _ptr(weight_grads), _ptr(bias_grads), dtype,
-                                      wdtype, rows, channels, wp, wn, dev, stream), name)
+    rc = lib.v3d_layer_norm_bwd(target_grads.data_ptr(), feats.data_ptr(), _ptr(residual), _ptr(weight), mean,
+                                mean + 4 * rows, _ptr(feats_grads), _ptr(weight_grads), _ptr(bias_grads),
+                                _ELEMENTS[feats.dtype], _ELEMENTS[(feats if affine is None else affine).dtype], rows,
+                                channels, wp, wn, dev, stream)
+    if rc != 0:
+        _lib.check(rc, "layer_norm_backward")
 
 
 def _heads(name, t, arg, dims, dtype):
@@ -1144,7 +1156,7 @@ def attention_pack_backward(target_grads, q_feats, k_feats, v_feats, targets, ls
                             v_grads, scale, causal, rest=None):
     """The gradients of ``attention_pack_forward``, from its inputs, ``targets``, ``lse`` and (16-bit types) ``rest``."""
     name = "attention_pack_backward"
-    dtype, sizes, strides = _attention_check(name, q_feats, k_feats, v_feats, q_lengths, s_lengths)
+    _attention_check(name, q_feats, k_feats, v_feats, q_lengths, s_lengths)
     shape, kshape = q_feats.shape, k_feats.shape
     _operand(name, target_grads, "target_grads", shape, q_feats.dtype)
     _operand(name, targets, "targets", shape, q_feats.dtype)
@@ -1155,14 +1167,26 @@ def attention_pack_backward(target_grads, q_feats, k_feats, v_feats, targets, ls
     _operand(name, v_grads, "v_grads", kshape, q_feats.dtype)
     _same_device(name, q_feats, k_feats, v_feats, q_lengths, s_lengths, target_grads, targets, lse, rest, q_grads, k_grads,
                  v_grads)
+    _attention_pack_backward(target_grads, q_feats, k_feats, v_feats, targets, lse, q_lengths, s_lengths, q_grads, k_grads,
+                             v_grads, scale, causal, rest)
+
+
+def _attention_pack_backward(target_grads, q, k, v, targets, lse, q_lengths, s_lengths, q_grads, k_grads, v_grads, scale,
+                             causal, rest):
+    """The launch alone, for the autograd function, whose tensors the forward has checked or the backward has made."""
+    (N, H, D), (M, KV, _) = q.shape, k.shape
+    B = q_lengths.shape[0]
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
     lib = _lib.lib()
-    ws, wp, wn = _ws_args(lib.v3d_attention_pack_bwd_workspace_bytes(*sizes), q_feats)
-    dev, stream = _where(q_feats)
-    _lib.check(lib.v3d_attention_pack_bwd(target_grads.data_ptr(), q_feats.data_ptr(), k_feats.data_ptr(),
-                                          v_feats.data_ptr(), targets.data_ptr(), _ptr(rest), lse.data_ptr(),
-                                          q_lengths.data_ptr(), s_lengths.data_ptr(), q_grads.data_ptr(),
-                                          k_grads.data_ptr(), v_grads.data_ptr(), dtype, *sizes, strides, scale,
-                                          bool(causal), wp, wn, dev, stream), name)
+    ws, wp, wn = _ws_args(lib.v3d_attention_pack_bwd_workspace_bytes(B, N, M, H, KV, D), q)
+    dev, stream = _where(q)
+    rc = lib.v3d_attention_pack_bwd(target_grads.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), targets.data_ptr(),
+                                    _ptr(rest), lse.data_ptr(), q_lengths.data_ptr(), s_lengths.data_ptr(),
+                                    q_grads.data_ptr(), k_grads.data_ptr(), v_grads.data_ptr(), _ELEMENTS[q.dtype], B, N, M,
+                                    H, KV, D, _Strides6(qs[0], qs[1], ks[0], ks[1], vs[0], vs[1]), scale, bool(causal), wp,
+                                    wn, dev, stream)
+    if rc != 0:
+        _lib.check(rc, "attention_pack_backward")
 
 
 def cached_attention(q_feats, k_cache, v_cache, lengths, targets, scale):

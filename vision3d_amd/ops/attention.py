@@ -57,8 +57,8 @@ class _AttentionPack(torch.autograd.Function):
     def backward(ctx, grad):
         q, k, v, out, rest, lse, q_lengths, s_lengths = ctx.saved_tensors
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        ext.attention_pack_backward(grad.contiguous(), q, k, v, out, lse, q_lengths, s_lengths, dq, dk, dv, ctx.scale,
-                                    ctx.causal, rest)
+        ext._attention_pack_backward(grad.contiguous(), q, k, v, out, lse, q_lengths, s_lengths, dq, dk, dv, ctx.scale,
+                                     ctx.causal, rest)
         return dq, dk, dv, None, None, None, None
 
 

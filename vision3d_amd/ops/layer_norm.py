@@ -27,20 +27,17 @@ class _LayerNorm(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         feats, weight, residual, stats = ctx.saved_tensors
-        need_feats = ctx.needs_input_grad[0] or ctx.needs_input_grad[4]
-        need_weight, need_bias = ctx.needs_input_grad[1], ctx.needs_input_grad[2]
-        grad_feats = torch.empty_like(feats) if need_feats else None
-        channels = feats.shape[1:]
+        need_feats, need_weight, need_bias, _, need_residual = ctx.needs_input_grad
+        grad_feats = torch.empty_like(feats) if need_feats or need_residual else None
         grad_weight = torch.empty_like(weight) if need_weight else None
-        grad_bias = feats.new_empty(channels, dtype=ctx.bias_dtype) if need_bias else None
+        grad_bias = feats.new_empty(feats.shape[1:], dtype=ctx.bias_dtype) if need_bias else None
         if feats.shape[0] == 0:  # no rows: the column sums are empty
             for t in (grad_weight, grad_bias):
                 if t is not None:
                     t.zero_()
         else:
-            ext.layer_norm_backward(grad.contiguous(), feats, residual, weight, stats, grad_feats, grad_weight, grad_bias)
-        return (grad_feats if ctx.needs_input_grad[0] else None, grad_weight, grad_bias, None,
-                grad_feats if ctx.needs_input_grad[4] else None)
+            ext._layer_norm_backward(grad.contiguous(), feats, residual, weight, stats, grad_feats, grad_weight, grad_bias)
+        return grad_feats if need_feats else None, grad_weight, grad_bias, None, grad_feats if need_residual else None
 
 
 def layer_norm(feats: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5,
