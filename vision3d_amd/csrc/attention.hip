@@ -502,9 +502,10 @@ struct AttnPlan {
 inline AttnPlan attn_plan(int B, int64_t total_q, int64_t total_s, int tokens, int KV, int G, int D) {
   AttnPlan p;
   // 32-row tiles where sequences have no more rows than that (a cache's newest tokens), and where 128-row tiles would keep
-  // at most a quarter of the 256 CUs: one sequence of 2048 tokens, 4 heads of 64, bf16: 21 us against 30; twice the tiles
-  // (2 x 1024 tokens, 2 key heads of 128): 40 us against 37, keys and values being read by four times as many workgroups.
-  p.few = total_q * G <= (int64_t)32 * B || (ceil_div(total_q * G, kAttnRows) + B) * KV <= 64;
+  // at most a quarter of the 256 CUs: one sequence of 2048 tokens, 4 heads of 64: 22 us against 26 in bf16 (52 against 47 in
+  // fp32), 8 of 256 tokens in fp32 16 against 21; twice the tiles (2 x 1024 tokens, 2 key heads of 128, bf16): 40 us against
+  // 37, keys and values being read by four times as many workgroups.
+  p.few = total_q * G <= (int64_t)32 * B || ceil_div(total_q * G, kAttnRows) * KV <= 64;
   p.tiles = tokens > 0 ? B * ceil_div((int64_t)tokens * G, p.tile()) : ceil_div(total_q * G, p.tile()) + B;
   // Keys are divided where the row tiles leave compute units idle, as far as every part of a sequence of the mean length
   // keeps 512 keys: into one workgroup a CU of the 32-row kernel, which is bound by memory (6 caches of 32768 rows, 4 tokens:
