@@ -277,6 +277,17 @@ def test_shared_and_far_rows():
         far.copy_(q)
         assert torch.equal(ops.attention_pack_mode(far, k, v, n, causal=True), want)
         del far
+    # one row, one head: their strides mean nothing
+    one = torch.randn(1, 64, device=DEV).half()
+    odd = [one.as_strided((1, 1, 64), st) for st in ((1, 1, 1), (3, 1 << 40, 1), (1 << 40, 5, 1), (0, 0, 1))]
+    for t in odd:
+        got = ops.attention_pack_mode(t, t, t, torch.tensor([1], device=DEV))
+        assert torch.equal(got.view(1, 64), one)
+        got = ops.cached_attention(t[None], t[None], t[None], torch.tensor([1], device=DEV))
+        assert torch.equal(got.view(1, 64), one)
+        leaf = t.detach().requires_grad_(True)
+        out = ops.attention_pack_mode(leaf, t, t, torch.tensor([1], device=DEV))
+        assert not torch.autograd.grad(out, leaf, torch.ones_like(out))[0].any()  # one key: its weight is 1 whatever q is
     over = torch.randn(50 * 32 + 128, device=DEV).to(torch.float16).as_strided((50, 2, 64), (32, 64, 1))
     assert torch.equal(ops.attention_pack_mode(q, over, over, n), ops.attention_pack_mode(q, over.contiguous(), over.contiguous(), n))
 

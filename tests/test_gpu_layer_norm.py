@@ -161,6 +161,24 @@ def test_batched_strided_empty_and_nonfinite():
 
 
 @pytest.mark.gpu
+def test_accumulated_gradients_are_apart():
+    x, r, w, b, g = (v.to(DEV).requires_grad_(True) for v in _inputs(40, 64, torch.float32, True))
+    for k in range(2):  # the second pass adds to what the first left
+        ops.layer_norm(x, w, b, residual=r).backward(g.detach())
+    want = torch.autograd.grad(ops.layer_norm(x, w, b, residual=r), (x, w, b), g.detach())
+    for leaf, one in zip((x, w, b), want):
+        assert torch.equal(leaf.grad, one + one)
+    assert torch.equal(r.grad, x.grad)
+    x.grad.zero_()  # one gradient for two inputs, but not one tensor
+    assert torch.equal(r.grad, want[0] + want[0])
+    # a frozen input, frozen weights: only what is asked for
+    (gr,) = torch.autograd.grad(ops.layer_norm(x.detach(), w.detach(), b.detach(), residual=r), r, g.detach())
+    assert torch.equal(gr, want[0])
+    (gb,) = torch.autograd.grad(ops.layer_norm(x.detach(), None, b), b, g.detach())
+    assert torch.equal(gb, torch.autograd.grad(ops.layer_norm(x.detach(), torch.ones_like(w), b), b, g.detach())[0])
+
+
+@pytest.mark.gpu
 def test_other_stream_and_graph_replays():
     x, r, w, b, g = (v.to(DEV) for v in _inputs(300, 333, torch.bfloat16, True))
     want = ops.layer_norm(x, w, b, residual=r)

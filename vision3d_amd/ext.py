@@ -1095,7 +1095,7 @@ def _layer_norm_backward(target_grads, feats, residual, weight, stats, feats_gra
 
 
 def _heads(name, t, arg, dims, dtype):
-    """(strides, shape) of features (.., heads, D) of any strides but the last, which is 1."""
+    """(strides, shape) of features (.., heads, D) of any strides but the last, which is 1; 0 where there is one entry."""
     if not t.is_cuda:
         raise RuntimeError(f"{arg} must be a CUDA tensor")
     shape, strides = t.shape, t.stride()
@@ -1106,6 +1106,8 @@ def _heads(name, t, arg, dims, dtype):
     if t.dtype != dtype:
         raise RuntimeError(f"{name}: expected scalar type {_TYPE_NAMES.get(dtype, dtype)} but found "
                            f"{_TYPE_NAMES.get(t.dtype, t.dtype)}")
+    if 1 in shape:
+        strides = [0 if n == 1 else s for n, s in zip(shape, strides)]
     return strides, shape
 
 
@@ -1176,7 +1178,7 @@ def _attention_pack_backward(target_grads, q, k, v, targets, lse, q_lengths, s_l
     """The launch alone, for the autograd function, whose tensors the forward has checked or the backward has made."""
     (N, H, D), (M, KV, _) = q.shape, k.shape
     B = q_lengths.shape[0]
-    qs, ks, vs = q.stride(), k.stride(), v.stride()
+    (qs, _), (ks, _), (vs, _) = (_heads("attention_pack_backward", t, "features", 3, q.dtype) for t in (q, k, v))
     lib = _lib.lib()
     ws, wp, wn = _ws_args(lib.v3d_attention_pack_bwd_workspace_bytes(B, N, M, H, KV, D), q)
     dev, stream = _where(q)

@@ -11,26 +11,26 @@ from torch import Tensor
 from .. import ext
 
 
-def _require_cuda(name, *tensors):
-    if not all(t.is_cuda for t in tensors):
+def _require_cuda(name, q, k, v):
+    if not (q.is_cuda and k.is_cuda and v.is_cuda):
         raise RuntimeError(f"{name}: CUDA tensors required (no CPU fallback in vision3d_amd)")
 
 
 def _rows(t: Tensor) -> Tensor:
     """The strides that the kernels take: any but the last dimension's, which is 1, within 32-bit offsets of a tile; other
     inputs are copied."""
-    strides, shape = t.stride(), t.shape
-    if len(shape) < 3 or t.numel() == 0:
+    shape = t.shape
+    if len(shape) < 3 or t.is_contiguous() or t.numel() == 0:
         return t
-    row, head, unit = strides[-3:]
-    heads, dim = shape[-2:]
+    row, head, unit = t.stride()[-3:]
+    rows, heads, dim = shape[-3:]
     near = 130 * row + heads * head + dim < 1 << 29
-    return t if unit == 1 and (row == 0 or row >= dim) and near else t.contiguous()
+    return t if unit == 1 and (rows == 1 or row == 0 or row >= dim) and near else t.contiguous()
 
 
 def _lengths(lengths: Tensor, like: Tensor) -> Tensor:
     """The reference's loops take the lengths on either side and in any integer type; the kernels int64 on the device."""
-    if lengths.dtype != torch.long or lengths.device != like.device:
+    if lengths.dtype != torch.long or not lengths.is_cuda or lengths.get_device() != like.get_device():
         lengths = lengths.to(device=like.device, dtype=torch.long)
     return lengths.contiguous()
 
@@ -43,8 +43,8 @@ class _AttentionPack(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, q_lengths, s_lengths, scale, causal):
         q, k, v = _rows(q), _rows(k), _rows(v)
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+        out = q.new_empty(q.shape)
+        lse = q.new_empty(q.shape[:2], dtype=torch.float32)
         # 16-bit outputs: the backward's grad . out needs what the rounding took from them
         rest = None if q.dtype == torch.float32 else torch.empty_like(out)
         ext.attention_pack_forward(q, k, v, q_lengths, s_lengths, out, lse, scale, causal, rest)
@@ -56,7 +56,7 @@ class _AttentionPack(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         q, k, v, out, rest, lse, q_lengths, s_lengths = ctx.saved_tensors
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
         ext._attention_pack_backward(grad.contiguous(), q, k, v, out, lse, q_lengths, s_lengths, dq, dk, dv, ctx.scale,
                                      ctx.causal, rest)
         return dq, dk, dv, None, None, None, None
@@ -79,7 +79,7 @@ def attention_pack_mode(q_feats: Tensor, k_feats: Tensor, v_feats: Tensor, q_len
     scale = _scale(scale, q_feats.shape[-1])
     if torch.is_grad_enabled() and (q_feats.requires_grad or k_feats.requires_grad or v_feats.requires_grad):
         return _AttentionPack.apply(q_feats, k_feats, v_feats, q_lengths, s_lengths, scale, causal)
-    out = torch.empty(q_feats.shape, dtype=q_feats.dtype, device=q_feats.device)
+    out = q_feats.new_empty(q_feats.shape)
     ext.attention_pack_forward(_rows(q_feats), _rows(k_feats), _rows(v_feats), q_lengths, s_lengths, out, None, scale,
                                causal)
     return out
@@ -100,6 +100,6 @@ def cached_attention(q_feats: Tensor, k_cache: Tensor, v_cache: Tensor, lengths:
     q = _rows(q_feats)
     if q.dim() == 4 and q.shape[1] > 1 and q.shape[0] > 1 and q.stride(0) != q.shape[1] * q.stride(1):
         q = q.contiguous()
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = q.new_empty(q.shape)
     ext.cached_attention(q, _rows(k_cache), _rows(v_cache), _lengths(lengths, q), out, _scale(scale, q.shape[-1]))
     return out
