@@ -6,7 +6,7 @@
 // so grouped heads read every key once per tile whatever G is, and a single token of 8 heads fills 8 columns of a product
 // instead of one.
 //
-// Measured: causal prompt of 12288 tokens in 6 sequences, 32/8 heads of 128, bf16: 308 us = 774 TFLOP/s (matrix pipe 36 % busy,
+// Measured: causal prompt of 12288 tokens in 6 sequences, 32/8 heads of 128, bf16: 308 us = 774 TFLOP/s (matrix pipe 38 % busy,
 // no bank conflicts; two waves a SIMD, bound by the exponentials and by the issue of both); 32 pairs of 512 tokens, 4 heads
 // of 64, fp32: 70 us = 112 TFLOP/s (the library's fp32 product: 153); 32 caches of 2048 ... 8192 rows, one token, 32/8 heads
 // of 128, bf16: 135 us = 4.65 TB/s.
