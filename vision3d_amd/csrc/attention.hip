@@ -29,7 +29,7 @@ struct AttnWave {
   static constexpr int STEPS = HD / 16;  // product steps over the head size
   static constexpr int DT = HD / 32;
 
-  Op<T> q[STEPS];
+  Held<T, HD> q;
   f32x16 o[DT];
   float m = -__builtin_inff(), l = 0.f;  // running maximum of scale * log2(e) * score, and the sum of 2^(that - m)
   float c2;
@@ -37,9 +37,11 @@ struct AttnWave {
   int row, token, head;
   int limit;        // this lane's query sees the keys [0, limit)
   int least, most;  // of the wave's first and last row; most = 0: the wave has no rows
+  int D;
 
   // `row0`: the wave's first row in the sequence.
-  __device__ __forceinline__ void begin(const AttnArgs& a, const AttnSeq& seq, int kvh, int row0, int rows) {
+  __device__ __forceinline__ void begin(const AttnArgs& a, const AttnSeq& seq, int kvh, int row0, int rows, bool load_q) {
+    D = a.D;
     lane = threadIdx.x & 63;
     half = lane >> 5;
     row = row0 + (lane & 31);
@@ -51,22 +53,30 @@ struct AttnWave {
     most = row0 < rows ? attn_limit(a, seq, div_g(a, min(row0 + 31, rows - 1))) : 0;
     c2 = a.scale * kLog2e;
     const int token0 = div_g(a, min(row0, rows - 1));
-    load_ops<T>(q, static_cast<const T*>(a.q) + (seq.q_off + token0) * a.q_row + (int64_t)kvh * a.G * a.q_head,
-                (token - token0) * (int)a.q_row + g * (int)a.q_head, half, a.D, true);
+    if (load_q)
+      q.load(static_cast<const T*>(a.q) + (seq.q_off + token0) * a.q_row + (int64_t)kvh * a.G * a.q_head,
+             (token - token0) * (int)a.q_row + g * (int)a.q_head, half, a.D, true);
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[d] = zero16();
   }
 
   // s = 2^(score - m) of a tile of 32 NT keys from key0 on; m, l and o move on.
-  template <int NT>
-  __device__ __forceinline__ void scores(const U* k, int key0, f32x16 (&s)[NT]) {
+  // kTile: the wave's rows are the tile `rows` in LDS, else they are in q.
+  template <int NT, bool kTile>
+  __device__ __forceinline__ void scores(const U* k, const U* rows, int key0, f32x16 (&s)[NT]) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) s[n] = zero16();
 #pragma unroll
-    for (int st = 0; st < STEPS; ++st)
+    for (int st = 0; st < STEPS; ++st) {
+      Op<T> qs;
+      if constexpr (kTile)
+        qs = read_cols<T, HDP, 32>(rows, lane & 31, st, half);
+      else
+        qs = q.get(st, half, D);
 #pragma unroll
       for (int n = 0; n < NT; ++n)
-        s[n] = product<T>(read_cols<T, HDP, 32 * NT>(k, n * 32 + (lane & 31), st, half), q[st], s[n]);
+        s[n] = product<T>(read_cols<T, HDP, 32 * NT>(k, n * 32 + (lane & 31), st, half), qs, s[n]);
+    }
     if (key0 + 32 * NT > least) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -223,7 +233,7 @@ __global__ __launch_bounds__(256, (attn_occupancy<T, HD>())) void attn_forward_k
   const int row0 = seq.tile * kAttnRows;
   if (row0 >= rows) return;  // lengths that overrun the total were cut
   AttnWave<T, HD> w;
-  w.begin(a, seq, kvh, row0 + wave * 32, rows);
+  w.begin(a, seq, kvh, row0 + wave * 32, rows, true);
   // the workgroup's first and last rows bound what it has to look at
   const int most = attn_limit(a, seq, div_g(a, min(row0 + kAttnRows - 1, rows - 1)));
   const int least = attn_limit(a, seq, div_g(a, row0));
@@ -250,7 +260,7 @@ __global__ __launch_bounds__(256, (attn_occupancy<T, HD>())) void attn_forward_k
     const bool active = key0 < w.most, more = t + 1 < t_end;
     f32x16 s[NT];
     if (more) fetch_k(t + 1);
-    if (active) w.template scores<NT>(lds_k[buf], key0, s);
+    if (active) w.template scores<NT, false>(lds_k[buf], nullptr, key0, s);
     if (key0 + BN > least && lds_bad[buf] == t + 1) {
       static_assert(BUFS * SIZE >= kAttnWaves * 1024, "room for the waves' probabilities");
       __syncthreads();  // nobody reads the keys any more: both of their buffers are free until the next keys are placed
@@ -313,8 +323,15 @@ __global__ __launch_bounds__(256, (attn_occupancy<T, HD>())) void attn_forward_k
 // Bound: the bytes of the keys and values.  A wave fetches its own tiles of 32 keys into its own part of LDS, so there is no
 // barrier in the loop and each wave keeps a tile of keys and one of values in flight; keys and values take turns in one
 // place (a wave's LDS accesses happen in order).  The waves' sums meet in LDS at the end.
+// With large heads the rows stand in LDS, one tile for all waves, and only one of keys and values is on its way at a time, or
+// registers spill (135 with bf16 heads of 256, 604 with fp32 ones).  8 heads, one token, 16 caches of up to 8192 rows: bf16
+// heads of 256 605 -> 130 us (4.9 TB/s), of 192 114 -> 109 us; fp32, up to 4096 rows, of 128 104 -> 94 us (4.0 TB/s), of 256
+// 1571 -> 1272 us (148 registers still spill); fp32 heads of 192 on one key head, five tokens: 210 -> 79 us.  Smaller heads
+// have the registers to keep both on their way.
 template <typename T, int HD>
 constexpr int few_waves() { return Kind<T>::P == 3 && HD > 128 ? 2 : 4; }
+template <typename T, int HD>
+constexpr bool few_large() { return HD > (Kind<T>::P == 1 ? 128 : 64); }
 
 template <typename T, int HD>
 __global__ __launch_bounds__((64 * few_waves<T, HD>())) void attn_few_rows_kernel(const AttnArgs a) {
@@ -324,6 +341,8 @@ __global__ __launch_bounds__((64 * few_waves<T, HD>())) void attn_few_rows_kerne
   constexpr int SIZE = Kind<T>::P * 32 * HDP;
   constexpr int TILES = W * SIZE * (int)sizeof(U), JOIN = 32 * HD * (int)sizeof(float);
   __shared__ __attribute__((aligned(16))) char lds[TILES > JOIN ? TILES : JOIN];
+  constexpr bool kLarge = few_large<T, HD>();
+  __shared__ __attribute__((aligned(16))) U lds_q[kLarge ? SIZE : 8];
   __shared__ U lds_p[W][32 * 32];
   __shared__ float lds_ml[W][32][2];
 
@@ -342,7 +361,17 @@ __global__ __launch_bounds__((64 * few_waves<T, HD>())) void attn_few_rows_kerne
   const int row0 = seq.tile * 32;
   if (row0 >= rows) return;
   AttnWave<T, HD> w;
-  w.begin(a, seq, kvh, row0, rows);
+  w.begin(a, seq, kvh, row0, rows, !kLarge);
+  if constexpr (kLarge) {
+    TileStage<T, HD, 32, 64 * W> stage;
+    const int token0 = div_g(a, row0);
+    stage.fetch_rows(static_cast<const T*>(a.q) + (seq.q_off + token0) * a.q_row + (int64_t)kvh * a.G * a.q_head, [&](int i) {
+      const int token = div_g(a, row0 + i);
+      return (token - token0) * (int)a.q_row + (row0 + i - token * a.G) * (int)a.q_head;
+    }, a.D, rows - row0);
+    stage.store(lds_q, a.D);
+    __syncthreads();
+  }
   const int tiles = (w.most + 31) / 32;
   const int per_split = (tiles + a.splits - 1) / a.splits;
   const int t_end = min(tiles, (split + 1) * per_split);
@@ -350,22 +379,29 @@ __global__ __launch_bounds__((64 * few_waves<T, HD>())) void attn_few_rows_kerne
   const T* v = static_cast<const T*>(a.v) + seq.b * a.v_batch + seq.s_off * a.v_row + (int64_t)kvh * a.v_head;
   U* tile = reinterpret_cast<U*>(lds) + wave * SIZE;
 
-  TileStage<T, HD, 32, 64> stage_k, stage_v;
+  TileStage<T, HD, 32, 64> stage_k, stage_own;
+  auto& stage_v = [&]() -> TileStage<T, HD, 32, 64>& {
+    if constexpr (kLarge) return stage_k;
+    else return stage_own;
+  }();
   auto fetch_k = [&](int t) { stage_k.fetch(k + (int64_t)t * 32 * a.k_row, a.k_row, a.D, seq.s_len - t * 32); };
   auto fetch_v = [&](int t) { stage_v.fetch(v + (int64_t)t * 32 * a.v_row, a.v_row, a.D, seq.s_len - t * 32); };
   int t = __builtin_amdgcn_readfirstlane(split * per_split + wave);
   if (t < t_end) {
     fetch_k(t);
-    fetch_v(t);
+    if (!kLarge) fetch_v(t);
   }
   for (; t < t_end; t += W) {
     const int key0 = t * 32;
     f32x16 s[1];
     wave_order();
     stage_k.store(tile, a.D);
-    if (t + W < t_end) fetch_k(t + W);
+    if (kLarge)
+      fetch_v(t);
+    else if (t + W < t_end)
+      fetch_k(t + W);
     wave_order();
-    w.template scores<1>(tile, key0, s);
+    w.template scores<1, kLarge>(tile, lds_q, key0, s);
     wave_order();
     stage_v.store(tile, a.D);
     wave_order();
@@ -375,7 +411,12 @@ __global__ __launch_bounds__((64 * few_waves<T, HD>())) void attn_few_rows_kerne
       clear_nonfinite(tile, SIZE, threadIdx.x & 63, 64);
       wave_order();
     }
-    if (t + W < t_end) fetch_v(t + W);
+    if (t + W < t_end) {
+      if (kLarge)
+        fetch_k(t + W);
+      else
+        fetch_v(t + W);
+    }
     w.template values<1>(tile, s);
   }
 

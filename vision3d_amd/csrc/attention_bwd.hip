@@ -130,18 +130,20 @@ __global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 128 : 64) ? 2 : 1) vo
     stage_v[decltype(from)::value].store(lds_v[decltype(from)::value], a.D);
   };
 
-  Op<T> qf[STEPS], gf[STEPS];
+  Held<T, HD> qf, gf;
   float delta = 0.f;
-  load_ops<T>(qf, q, (token - token0) * (int)a.q_row + (head - kvh * a.G) * (int)a.q_head, half, a.D, true);
-  load_ops<T>(gf, static_cast<const T*>(b.grad) + at0, at_row, half, a.D, true);
+  qf.load(q, (token - token0) * (int)a.q_row + (head - kvh * a.G) * (int)a.q_head, half, a.D, true);
+  gf.load(static_cast<const T*>(b.grad) + at0, at_row, half, a.D, true);
   // delta = grad . out, the output as it was before it was rounded
   auto add_delta = [&](const void* out) {
-    Op<T> of[STEPS];
-    load_ops<T>(of, static_cast<const T*>(out) + at0, at_row, half, a.D, true);
+    Held<T, HD> of;
+    of.load(static_cast<const T*>(out) + at0, at_row, half, a.D, true);
 #pragma unroll
-    for (int st = 0; st < STEPS; ++st)
+    for (int st = 0; st < STEPS; ++st) {
+      const Op<T> gs = gf.get(st, half, a.D), os = of.get(st, half, a.D);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) delta = fmaf(number(gf[st], j), number(of[st], j), delta);
+      for (int j = 0; j < 8; ++j) delta = fmaf(number(gs, j), number(os, j), delta);
+    }
   };
   add_delta(a.out);
   if (a.rest != nullptr) add_delta(a.rest);
@@ -163,8 +165,8 @@ __global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 128 : 64) ? 2 : 1) vo
       f32x16 s = zero16(), dp = zero16();
 #pragma unroll
       for (int st = 0; st < STEPS; ++st) {
-        s = product<T>(read_cols<T, HDP, BN>(lds_k[buf], n * 32 + (lane & 31), st, half), qf[st], s);
-        dp = product<T>(read_cols<T, HDP, BN>(lds_v[buf], n * 32 + (lane & 31), st, half), gf[st], dp);
+        s = product<T>(read_cols<T, HDP, BN>(lds_k[buf], n * 32 + (lane & 31), st, half), qf.get(st, half, a.D), s);
+        dp = product<T>(read_cols<T, HDP, BN>(lds_v[buf], n * 32 + (lane & 31), st, half), gf.get(st, half, a.D), dp);
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = exp2_fast(fmaf(s[r], c2, -lse)) * (dp[r] - delta);
@@ -267,11 +269,11 @@ __global__ __launch_bounds__(kKvThreads, HD <= 32 ? 2 : 1) void attn_backward_kv
     constexpr int st = decltype(to)::value;
     const int row0 = min(begin + t * BM, rows);
     const int tok0 = div_g(a, row0);
-    stage_q[st].fetch_at(q + tok0 * a.q_row, [&](int r) {
+    stage_q[st].fetch_rows(q + tok0 * a.q_row, [&](int r) {
       const int tok = div_g(a, row0 + r);
       return (tok - tok0) * (int)a.q_row + (row0 + r - tok * a.G) * (int)a.q_head;
     }, a.D, rows - row0);
-    stage_g[st].fetch_at(grad + (int64_t)tok0 * a.H * a.D, [&](int r) {
+    stage_g[st].fetch_rows(grad + (int64_t)tok0 * a.H * a.D, [&](int r) {
       const int tok = div_g(a, row0 + r);
       return ((tok - tok0) * a.H + (row0 + r - tok * a.G)) * a.D;
     }, a.D, rows - row0);
@@ -295,9 +297,9 @@ __global__ __launch_bounds__(kKvThreads, HD <= 32 ? 2 : 1) void attn_backward_kv
     }
   };
 
-  Op<T> kf[STEPS], vf[STEPS];
-  load_ops<T>(kf, k, (key - key0) * (int)a.k_row, half, a.D, live);
-  load_ops<T>(vf, v, (key - key0) * (int)a.v_row, half, a.D, live);
+  Held<T, HD> kf, vf;
+  kf.load(k, (key - key0) * (int)a.k_row, half, a.D, live);
+  vf.load(v, (key - key0) * (int)a.v_row, half, a.D, live);
   const float c2 = a.scale * kLog2e;
   f32x16 acc[DT], other[kRoles ? 1 : DT];  // of the wave's role, or dk and dv
 #pragma unroll
@@ -317,13 +319,13 @@ __global__ __launch_bounds__(kKvThreads, HD <= 32 ? 2 : 1) void attn_backward_kv
       f32x16 s = zero16();
 #pragma unroll
       for (int st = 0; st < STEPS; ++st)
-        s = product<T>(read_cols<T, HDP, BM>(lds_q[buf], n * 32 + (lane & 31), st, half), kf[st], s);
+        s = product<T>(read_cols<T, HDP, BM>(lds_q[buf], n * 32 + (lane & 31), st, half), kf.get(st, half, a.D), s);
       f32x16 p;
       if (keys_role) {
         f32x16 dp = zero16();
 #pragma unroll
         for (int st = 0; st < STEPS; ++st)
-          dp = product<T>(read_cols<T, HDP, BM>(lds_g[buf], n * 32 + (lane & 31), st, half), vf[st], dp);
+          dp = product<T>(read_cols<T, HDP, BM>(lds_g[buf], n * 32 + (lane & 31), st, half), vf.get(st, half, a.D), dp);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int i = n * 32 + acc_row(r, half);

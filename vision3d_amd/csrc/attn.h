@@ -393,6 +393,37 @@ __device__ __forceinline__ void load_ops(Op<T> (&op)[STEPS], const T* base, int 
   for (int st = 0; st < STEPS; ++st) op[st] = raw[st].op(st * 16 + 8 * half, D);
 }
 
+// The operands of all product steps over the head size that a wave keeps for its loop.  fp32 heads of 129 ... 192 are kept as
+// they come from memory, 8 registers a step instead of 12, and split where they are used: 144 registers beside the sums do not
+// fit.  Forward and backward, 8 sequences of about 500 tokens, causal, 8 / 2 heads of 192: 940 -> 828 us.  Heads of 256
+// do not fit either way, and the splits come on top there: 2690 us kept split, 2900 us kept whole.
+template <typename T, int HD>
+struct Held {
+  static constexpr int STEPS = HD / 16;
+  static constexpr bool kLate = Kind<T>::P == 3 && HD > 128 && HD <= 192;
+  Op<T> ops[kLate ? 1 : STEPS];
+  Raw<T> raw[kLate ? STEPS : 1];
+
+  __device__ __forceinline__ void load(const T* base, int at, int half, int D, bool there) {
+    if constexpr (kLate) {
+#pragma unroll
+      for (int st = 0; st < STEPS; ++st) raw[st].load(base, kOutOfRange, at, st * 16 + 8 * half, D, there);
+    } else {
+      load_ops<T>(ops, base, at, half, D, there);
+    }
+  }
+  __device__ __forceinline__ Op<T> get(int st, int half, int D) const {
+    if constexpr (kLate) {
+      Raw<T> r = raw[st];
+#pragma unroll
+      for (int l = 0; l < Raw<T>::L; ++l) asm volatile("" : "+v"(r.c[l]));  // or the split moves out of the loop again
+      return r.op(st * 16 + 8 * half, D);
+    } else {
+      return ops[st];
+    }
+  }
+};
+
 // ---- tiles in LDS ------------------------------------------------------------------------------------------------------
 // A tile is P planes of ROWS rows of HDP 16-bit numbers (the head size rounded up to a power of two), moved in chunks of 8.
 // It is read in two ways: 16 consecutive rows at one chunk (read_cols), and 4 consecutive rows at 64 consecutive bytes
@@ -433,7 +464,7 @@ struct TileStage {
   }
   // The same for rows at offsets of their own (elements, non-negative, below 2^29).
   template <typename Offset>
-  __device__ __forceinline__ void fetch_at(const T* base, Offset offset, int D, int count) {
+  __device__ __forceinline__ void fetch_rows(const T* base, Offset offset, int D, int count) {
 #pragma unroll
     for (int i = 0; i < CH; ++i) c[i].load(base, kOutOfRange, offset(row_of(i)), col_of(i), D, row_of(i) < count);
   }
