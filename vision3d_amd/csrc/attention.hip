@@ -28,6 +28,7 @@ struct AttnWave {
   static constexpr int HDP = attn_pow2(HD);
   static constexpr int STEPS = HD / 16;  // product steps over the head size
   static constexpr int DT = HD / 32;
+  static constexpr bool kAgain = Kind<T>::P == 3 && HD > 192;  // at 192 they fit: 8 x 500 tokens 165 us, 182 us with it
 
   Held<T, HD> q;
   f32x16 o[DT];
@@ -70,12 +71,12 @@ struct AttnWave {
     for (int st = 0; st < STEPS; ++st) {
       Op<T> qs;
       if constexpr (kTile)
-        qs = read_cols<T, HDP, 32>(rows, lane & 31, st, half);
+        qs = read_cols<T, HDP, 32>(rows, again<kAgain>(lane & 31), st, half);
       else
         qs = q.get(st, half, D);
 #pragma unroll
       for (int n = 0; n < NT; ++n)
-        s[n] = product<T>(read_cols<T, HDP, 32 * NT>(k, n * 32 + (lane & 31), st, half), qs, s[n]);
+        s[n] = product<T>(read_cols<T, HDP, 32 * NT>(k, again<kAgain>(n * 32 + (lane & 31)), st, half), qs, s[n]);
     }
     if (key0 + 32 * NT > least) {
 #pragma unroll
@@ -124,7 +125,8 @@ struct AttnWave {
       for (int u = 0; u < 2; ++u) {
         const Op<T> p = pack_rows<T>(s[n], u);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) o[d] = product<T>(read_rows<T, HDP, 32 * NT>(v, n * 32, u, d * 32, lane), p, o[d]);
+        for (int d = 0; d < DT; ++d)
+          o[d] = product<T>(read_rows<T, HDP, 32 * NT>(v, n * 32, u, d * 32, again<kAgain>(lane)), p, o[d]);
       }
   }
 
@@ -326,8 +328,8 @@ __global__ __launch_bounds__(256, (attn_occupancy<T, HD>())) void attn_forward_k
 // With large heads the rows stand in LDS, one tile for all waves, and only one of keys and values is on its way at a time, or
 // registers spill (135 with bf16 heads of 256, 604 with fp32 ones).  8 heads, one token, 16 caches of up to 8192 rows: bf16
 // heads of 256 605 -> 130 us (4.9 TB/s), of 192 114 -> 109 us; fp32, up to 4096 rows, of 128 104 -> 94 us (4.0 TB/s), of 256
-// 1571 -> 1272 us (148 registers still spill); fp32 heads of 192 on one key head, five tokens: 210 -> 79 us.  Smaller heads
-// have the registers to keep both on their way.
+// 1571 -> 670 us with the addresses computed where they are used (1272 us without; 38 registers still spill); fp32 heads of
+// 192 on one key head, five tokens: 210 -> 79 us.  Smaller heads have the registers to keep both on their way.
 template <typename T, int HD>
 constexpr int few_waves() { return Kind<T>::P == 3 && HD > 128 ? 2 : 4; }
 template <typename T, int HD>

@@ -77,6 +77,7 @@ __global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 128 : 64) ? 2 : 1) vo
   constexpr int NT = BN / 32;
   constexpr int BUFS = bwd_buffers<T, HD>();
   constexpr int STEPS = HD / 16;
+  constexpr bool kAgain = Kind<T>::P == 3 && HD > 128;  // see again()
   constexpr int DT = HD / 32;
   typedef typename Kind<T>::U U;
   __shared__ __attribute__((aligned(16))) U lds_k[BUFS][Kind<T>::P * BN * HDP];
@@ -165,8 +166,8 @@ __global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 128 : 64) ? 2 : 1) vo
       f32x16 s = zero16(), dp = zero16();
 #pragma unroll
       for (int st = 0; st < STEPS; ++st) {
-        s = product<T>(read_cols<T, HDP, BN>(lds_k[buf], n * 32 + (lane & 31), st, half), qf.get(st, half, a.D), s);
-        dp = product<T>(read_cols<T, HDP, BN>(lds_v[buf], n * 32 + (lane & 31), st, half), gf.get(st, half, a.D), dp);
+        s = product<T>(read_cols<T, HDP, BN>(lds_k[buf], again<kAgain>(n * 32 + (lane & 31)), st, half), qf.get(st, half, a.D), s);
+        dp = product<T>(read_cols<T, HDP, BN>(lds_v[buf], again<kAgain>(n * 32 + (lane & 31)), st, half), gf.get(st, half, a.D), dp);
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = exp2_fast(fmaf(s[r], c2, -lse)) * (dp[r] - delta);
@@ -180,7 +181,7 @@ __global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 128 : 64) ? 2 : 1) vo
         const Op<T> ds = pack_rows<T>(s, u);
 #pragma unroll
         for (int d = 0; d < DT; ++d)
-          acc[d] = product<T>(read_rows<T, HDP, BN>(lds_k[buf], n * 32, u, d * 32, lane), ds, acc[d]);
+          acc[d] = product<T>(read_rows<T, HDP, BN>(lds_k[buf], n * 32, u, d * 32, again<kAgain>(lane)), ds, acc[d]);
       }
     }
   };
@@ -207,6 +208,7 @@ __global__ __launch_bounds__(kKvThreads, HD <= 32 ? 2 : 1) void attn_backward_kv
   constexpr int NT = BM / 32;
   constexpr int BUFS = bwd_buffers<T, HD>();
   constexpr int STEPS = HD / 16;
+  constexpr bool kAgain = Kind<T>::P == 3 && HD > 128;  // see again()
   constexpr int DT = HD / 32;
   constexpr int GROUPS = kv_groups<T, HD>(), KEYS = 32 * GROUPS, THREADS = kKvThreads;
   constexpr bool kRoles = kv_roles<T, HD>();
@@ -319,13 +321,13 @@ __global__ __launch_bounds__(kKvThreads, HD <= 32 ? 2 : 1) void attn_backward_kv
       f32x16 s = zero16();
 #pragma unroll
       for (int st = 0; st < STEPS; ++st)
-        s = product<T>(read_cols<T, HDP, BM>(lds_q[buf], n * 32 + (lane & 31), st, half), kf.get(st, half, a.D), s);
+        s = product<T>(read_cols<T, HDP, BM>(lds_q[buf], again<kAgain>(n * 32 + (lane & 31)), st, half), kf.get(st, half, a.D), s);
       f32x16 p;
       if (keys_role) {
         f32x16 dp = zero16();
 #pragma unroll
         for (int st = 0; st < STEPS; ++st)
-          dp = product<T>(read_cols<T, HDP, BM>(lds_g[buf], n * 32 + (lane & 31), st, half), vf.get(st, half, a.D), dp);
+          dp = product<T>(read_cols<T, HDP, BM>(lds_g[buf], again<kAgain>(n * 32 + (lane & 31)), st, half), vf.get(st, half, a.D), dp);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int i = n * 32 + acc_row(r, half);
@@ -347,12 +349,12 @@ __global__ __launch_bounds__(kKvThreads, HD <= 32 ? 2 : 1) void attn_backward_kv
           const Op<T> y = pack_rows<T>(p, u);
 #pragma unroll
           for (int d = 0; d < DT; ++d)
-            other[d] = product<T>(read_rows<T, HDP, BM>(lds_g[buf], n * 32, u, d * 32, lane), y, other[d]);
+            other[d] = product<T>(read_rows<T, HDP, BM>(lds_g[buf], n * 32, u, d * 32, again<kAgain>(lane)), y, other[d]);
         }
         const Op<T> x = pack_rows<T>(s, u);
 #pragma unroll
         for (int d = 0; d < DT; ++d)
-          acc[d] = product<T>(read_rows<T, HDP, BM>(summed, n * 32, u, d * 32, lane), x, acc[d]);
+          acc[d] = product<T>(read_rows<T, HDP, BM>(summed, n * 32, u, d * 32, again<kAgain>(lane)), x, acc[d]);
       }
     }
   };

@@ -393,14 +393,12 @@ __device__ __forceinline__ void load_ops(Op<T> (&op)[STEPS], const T* base, int 
   for (int st = 0; st < STEPS; ++st) op[st] = raw[st].op(st * 16 + 8 * half, D);
 }
 
-// The operands of all product steps over the head size that a wave keeps for its loop.  fp32 heads of 129 ... 192 are kept as
-// they come from memory, 8 registers a step instead of 12, and split where they are used: 144 registers beside the sums do not
-// fit.  Forward and backward, 8 sequences of about 500 tokens, causal, 8 / 2 heads of 192: 940 -> 828 us.  Heads of 256
-// do not fit either way, and the splits come on top there: 2690 us kept split, 2900 us kept whole.
+// The operands of all product steps over the head size that a wave keeps for its loop.  fp32 heads past 128 are kept as
+// they come from memory, 8 registers a step instead of 12, and split where they are used: beside the sums there is no room.
 template <typename T, int HD>
 struct Held {
   static constexpr int STEPS = HD / 16;
-  static constexpr bool kLate = Kind<T>::P == 3 && HD > 128 && HD <= 192;
+  static constexpr bool kLate = Kind<T>::P == 3 && HD > 128;
   Op<T> ops[kLate ? 1 : STEPS];
   Raw<T> raw[kLate ? STEPS : 1];
 
@@ -437,6 +435,17 @@ __device__ __forceinline__ int place(int row, int chunk) {
   return chunk ^ ((row >> 2) & 3);
 }
 
+// `x`, such that what is computed from it is computed again in every turn of a loop (kAgain).  The compiler otherwise computes
+// the LDS addresses of a tile once, before the loop, and keeps them all: with fp32 heads past 128 that is more registers than
+// are left, and an address read back from memory costs more than its few instructions.  Training in fp32, 8 sequences of
+// 500 tokens, this and Held together: 8 / 2 heads of 192, causal, 937 -> 770 us (828 us with Held alone), 8 heads of 256
+// 2690 -> 2400 us.
+template <bool kAgain>
+__device__ __forceinline__ int again(int x) {
+  if constexpr (kAgain) asm volatile("" : "+v"(x));
+  return x;
+}
+
 // Offset of element `col` of `row` in a plane.
 template <int HDP>
 __device__ __forceinline__ int tile_at(int row, int col) {
@@ -452,7 +461,8 @@ struct TileStage {
   static constexpr bool kEven = ROWS * CPR % THREADS == 0;  // else the last chunk of some threads repeats the last row's
   Raw<T> c[CH];
 
-  static __device__ __forceinline__ int index(int i) { return i * THREADS + (int)threadIdx.x % THREADS; }
+  static constexpr bool kTight = Kind<T>::P == 3 && HD > 192;  // registers are short
+  static __device__ __forceinline__ int index(int i) { return i * THREADS + again<kTight>((int)threadIdx.x % THREADS); }
   static __device__ __forceinline__ int row_of(int i) { return kEven ? index(i) / CPR : min(index(i) / CPR, ROWS - 1); }
   static __device__ __forceinline__ int col_of(int i) { return index(i) % CPR * 8; }
 
@@ -472,6 +482,7 @@ struct TileStage {
     constexpr int HDP = attn_pow2(HD);
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
+      if constexpr (kTight) __builtin_amdgcn_sched_barrier(0);  // one split at a time
       const Op<T> op = c[i].op(col_of(i), D);
 #pragma unroll
       for (int p = 0; p < Kind<T>::P; ++p)
