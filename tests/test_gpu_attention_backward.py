@@ -346,3 +346,79 @@ def test_refusals():
     (grad,) = torch.autograd.grad(out, leaf, upstream, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):  # no second derivative
         grad.sum().backward()
+
+
+def _dense(q, k, v, g, scale):
+    """One sequence of one head without a mask, in 64 bits: dq, dk, dv."""
+    q, k, v, g = (t.double() for t in (q, k, v, g))
+    p = torch.softmax((q @ k.T) * scale, 1)
+    o = p @ v
+    ds = p * (g @ v.T - (g * o).sum(1, keepdim=True))
+    return (ds @ k) * scale, (ds.T @ q) * scale, p.T @ g
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 192])
+@pytest.mark.parametrize("size", [2.0 ** -16, 2.0 ** -10, 1.0, 2.0 ** 10])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_small_and_large_gradients(dtype, size, dim):
+    # ds is about grad . v / keys: with 2500 keys and gradients of 2^-10 it lies at 2^-18, where fp16 has a few bits left
+    n = 2500
+    q, k, v, g = (t[:, 0] for t in _inputs([n], [n], 1, 1, dim, dtype, seed=dim))
+    g = (g.double() * size).to(dtype)
+    leaves = [t.view(n, 1, dim).to(DEV).requires_grad_(True) for t in (q, k, v)]
+    out = ops.attention_pack_mode(*leaves, torch.tensor([n], device=DEV))
+    got = torch.autograd.grad(out, leaves, g.view(n, 1, dim).to(DEV))
+    # In the 2-norm: p or ds, delta and the gradient itself are rounded (half a step each, of separate entries) and each of
+    # the 32-bit sums adds at most its 100 steps; a fourth half step for their products.  The result's own rounding is
+    # at least half a subnormal step.
+    bound = 4 * _half(dtype) if dtype != torch.float32 else 100 * ULP
+    least = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    for name, a, ref in zip("qkv", got, _dense(q, k, v, g, dim ** -0.5)):
+        off = (a[:, 0].cpu().double() - ref).norm()
+        tol = bound * ref.norm() + least * ref.numel() ** 0.5
+        assert off <= tol, f"d{name}: {(off / tol).item():.2f} of the tolerance"
+
+
+@pytest.mark.gpu
+def test_rows_of_very_different_gradients():
+    # one row's ds does not take the others' bits: each row's dq, and every dk, as if it were alone
+    n, dim = 300, 64
+    q, k, v, g = (t[:, 0] for t in _inputs([n], [n], 1, 1, dim, torch.float16, seed=1))
+    g = (g.double() * 2.0 ** torch.linspace(-20, 10, n)[torch.randperm(n, generator=torch.Generator().manual_seed(0))][:, None]).half()
+    g[7], g[200] = 0, 0  # and rows without any
+    leaves = [t.view(n, 1, dim).to(DEV).requires_grad_(True) for t in (q, k, v)]
+    got = torch.autograd.grad(ops.attention_pack_mode(*leaves, torch.tensor([n], device=DEV)), leaves, g.view(n, 1, dim).to(DEV))
+    want = _dense(q, k, v, g, dim ** -0.5)
+    for a, ref in zip(got, want):
+        off = (a[:, 0].cpu().double() - ref).norm(dim=1)
+        assert (off <= 4 * 2.0 ** -11 * ref.norm(dim=1) + 2.0 ** -25 * dim ** 0.5).all()
+    assert not got[0][7].any() and not got[0][200].any()
+
+
+@pytest.mark.gpu
+def test_products_beyond_the_type():
+    # ds reaches 2^17, past fp16's largest number; the gradients do not
+    n, dim = 4, 64
+    q, k, v, g = (t[:, 0].double() for t in _inputs([n], [n], 1, 1, dim, torch.float16, seed=2))
+    q, k, v, g = (q * 2.0 ** -6).half(), (k * 2.0 ** -6).half(), (v * 2.0 ** 5).half(), (g * 2.0 ** 10).half()
+    p = torch.softmax(q.double() @ k.double().T / 8, 1)
+    assert (p * (g.double() @ v.double().T)).abs().max() > 70000
+    leaves = [t.view(n, 1, dim).to(DEV).requires_grad_(True) for t in (q, k, v)]
+    got = torch.autograd.grad(ops.attention_pack_mode(*leaves, torch.tensor([n], device=DEV)), leaves, g.view(n, 1, dim).to(DEV))
+    for a, ref in zip(got, _dense(q, k, v, g, 0.125)):
+        assert (a[:, 0].cpu().double() - ref).norm() <= 4 * 2.0 ** -11 * ref.norm()
+
+
+@pytest.mark.gpu
+def test_values_gradients_of_many_keys():
+    # a hundred thousand equal keys: p = 10^-5 is a subnormal fp16 number with half its bits
+    n, dim = 100001, 32
+    q, g = torch.ones(1, 1, dim), torch.full((1, 1, dim), 384.0)
+    k, v = torch.full((n, 1, dim), 0.25), torch.ones(n, 1, dim)
+    leaves = [t.half().to(DEV).requires_grad_(True) for t in (q, k, v)]
+    out = ops.attention_pack_mode(*leaves, torch.tensor([1], device=DEV), torch.tensor([n], device=DEV))
+    dv = torch.autograd.grad(out, leaves, g.half().to(DEV))[2].double()
+    # p and the gradient are rounded; the log-sum of n equal terms is off by its own half step (17 of them, in the exponent)
+    want = 384.0 / n
+    assert (dv - want).abs().max() <= want * (2 * 2.0 ** -11 + 32 * 2.0 ** -24)

@@ -23,10 +23,63 @@ struct AttnBwdArgs {
   float* delta;        // (total_q, H): written by the dq kernel, read by the dk / dv kernel
   int splits;          // parts that the rows of a key tile are divided into
   float* part;         // splits > 1: (splits, 2, total_s, KV, D) sums of the parts, dk's and dv's
+  float* grad_norm;    // fp16: (total_q, H) 2-norms of the rows of grad, written by the dq kernel ...
+  float* value_norm;   // ... and (total_s, KV) of the values, written before it; infinities and NaN count as 0
   void* dq;            // (total_q, H, D), (total_s, KV, D) contiguous
   void* dk;
   void* dv;
 };
+
+// ---- the range of fp16 -------------------------------------------------------------------------------------------------
+// fp16 holds 11 bits down to 2^-14 and nothing below 2^-25 or above 2^16, and p, about 1 / keys, and ds, about grad . v / keys,
+// leave that range long before the gradients do (2500 keys, gradients of 2^-10: 5e-3 off, of 2^-13: 5e-2).  So both meet their
+// product times a power of two, which the 32-bit sums are divided by at the end: p times 2^kLift, in the exponent; ds times a
+// factor of its row (dq) or key (dk) that puts a bound of it at 2^11 ... 2^12:
+//   |ds_ij| <= p_ij (|do_i . v_j| + |do_i . o_i|) <= 2 |do_i| max |v_j|,
+// with the 2-norms, the largest taken over the sequence (a factor that follows the largest ds would have to rescale the sums:
+// the registers of heads of 256 spill).  A typical ds of 2000 keys then lies at 2^-2, what is 2^-37 of the bound is still held,
+// and a p that 32-bit scores put past 1 has room.  Costs 2 to 6 % of a training step (8192 causal tokens in 5 sequences, 16/4
+// heads of 128: 464 -> 484 us; 8 x 2048 tokens without a mask 2030 -> 2070 us, 8 us of it the values' norms).
+template <typename T>
+constexpr bool kFp16 = __is_same(T, f16);
+template <typename T>
+constexpr float kLift = kFp16<T> ? 12.f : 0.f;
+
+__device__ __forceinline__ float range_exponent(float bound) {  // e: bound * 2^e in [2^11, 2^12), within what factors can undo
+  return (float)min(max(11 + 127 - (int)(__float_as_uint(bound) >> 23), -60), 60);
+}
+__device__ __forceinline__ float finite_norm(float squares) {
+  const float n = sqrtf(squares);
+  return n < __builtin_inff() ? n : 0.f;
+}
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) x = fmaxf(x, __shfl_xor(x, d, 64));
+  return x;
+}
+
+// 16 lanes a row; a workgroup stays with one key head.
+__global__ __launch_bounds__(256) void attn_value_norm_kernel(const AttnBwdArgs b) {
+  const AttnArgs& a = b.f;
+  const unsigned kvh = blockIdx.x % (unsigned)a.KV, group = blockIdx.x / (unsigned)a.KV, groups = gridDim.x / (unsigned)a.KV;
+  for (int64_t row = group * 16 + threadIdx.x / 16; row < a.total_s; row += groups * 16) {
+    const f16* v = static_cast<const f16*>(a.v) + row * a.v_row + kvh * a.v_head;
+    float sum = 0.f;
+    for (int c = (threadIdx.x & 15) * 8; c < a.D; c += 128) {
+      float x[8];
+      if (c + 8 <= a.D) {
+        load_vec<f16, 8>(v + c, x);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = c + j < a.D ? to_f32(v[c + j]) : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum = fmaf(x[j], x[j], sum);
+    }
+    sum = lanes_sum<16>(sum);
+    if ((threadIdx.x & 15) == 0) b.value_norm[row * a.KV + kvh] = finite_norm(sum);
+  }
+}
 
 // Keys (or rows) of a tile that passes by; two of them (fp32 heads past 128: one), of two tensors, in LDS.
 template <typename T, int HD>
@@ -149,8 +202,30 @@ __global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 128 : 64) ? 2 : 1) vo
   add_delta(a.out);
   if (a.rest != nullptr) add_delta(a.rest);
   delta = halves_sum(delta);
-  const float lse = a.lse[at];
+  float lse = a.lse[at];
   if (half == 0 && row < rows) b.delta[at] = delta;
+  float range = 0.f;  // log2 of what ds is multiplied by: in the exponent, no instruction more
+  if constexpr (kFp16<T>) {
+    float squares = 0.f, most_v = 0.f;
+#pragma unroll
+    for (int st = 0; st < STEPS; ++st) {
+      const Op<T> gs = gf.get(st, half, a.D);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) squares = fmaf(number(gs, j), number(gs, j), squares);
+    }
+    const float norm = finite_norm(halves_sum(squares));
+    if (half == 0 && row < rows) b.grad_norm[at] = norm;
+#pragma unroll 8
+    for (int j = threadIdx.x; j < most; j += 256)
+      most_v = fmaxf(most_v, b.value_norm[(seq.s_off + j) * a.KV + kvh]);
+    __shared__ float lds_norm[4];
+    most_v = wave_max(most_v);
+    if (lane == 0) lds_norm[wave] = most_v;
+    __syncthreads();
+    most_v = fmaxf(fmaxf(lds_norm[0], lds_norm[1]), fmaxf(lds_norm[2], lds_norm[3]));
+    range = range_exponent(2.f * norm * most_v);
+    lse -= range;
+  }
 
   const float c2 = a.scale * kLog2e;
   f32x16 acc[DT];
@@ -187,7 +262,7 @@ __global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 128 : 64) ? 2 : 1) vo
   };
 
   pass_tiles<BUFS>((most + BN - 1) / BN, fetch, place_tile, work);
-  if (row < rows) store_rows<T, DT>(dq + at * a.D, acc, a.scale, a.D, half);
+  if (row < rows) store_rows<T, DT>(dq + at * a.D, acc, a.scale * exp2_fast(-range), a.D, half);
 }
 
 // dk and dv of a tile of 32 GROUPS keys.  A wave keeps 32 keys: their operands and both sums, 320 registers with 16-bit heads
@@ -293,11 +368,28 @@ __global__ __launch_bounds__(kKvThreads, HD <= 32 ? 2 : 1) void attn_backward_kv
     stage_q[buf].store(lds_q[buf], a.D);
     stage_g[buf].store(lds_g[buf], a.D);
     if (threadIdx.x < BM) {
-      lds_lse[buf][threadIdx.x] = stage_lse[buf];
+      lds_lse[buf][threadIdx.x] = stage_lse[buf] - kLift<T>;  // p below is 2^kLift times as large
       lds_delta[buf][threadIdx.x] = stage_delta[buf];
       lds_limit[buf][threadIdx.x] = stage_limit[buf];
     }
   };
+
+  float range = 1.f;  // what ds is multiplied by
+  if constexpr (kFp16<T>) {
+    float most_g = 0.f;
+#pragma unroll 8
+    for (int r = first + threadIdx.x; r < rows; r += THREADS) {
+      const int tok = div_g(a, r);
+      most_g = fmaxf(most_g, b.grad_norm[(seq.q_off + tok) * a.H + kvh * a.G + (r - tok * a.G)]);
+    }
+    __shared__ float lds_norm[4];
+    most_g = wave_max(most_g);
+    if (lane == 0) lds_norm[wave] = most_g;
+    __syncthreads();
+    most_g = fmaxf(fmaxf(lds_norm[0], lds_norm[1]), fmaxf(lds_norm[2], lds_norm[3]));
+    const float norm = live ? b.value_norm[(seq.s_off + key) * a.KV + kvh] : 0.f;
+    range = exp2_fast(range_exponent(2.f * most_g * norm) - kLift<T>);  // p brings its own factor
+  }
 
   Held<T, HD> kf, vf;
   kf.load(k, (key - key0) * (int)a.k_row, half, a.D, live);
@@ -332,7 +424,7 @@ __global__ __launch_bounds__(kKvThreads, HD <= 32 ? 2 : 1) void attn_backward_kv
         for (int r = 0; r < 16; ++r) {
           const int i = n * 32 + acc_row(r, half);
           p[r] = exp2_fast(fmaf(s[r], c2, -lds_lse[buf][i]));
-          s[r] = p[r] * (dp[r] - lds_delta[buf][i]);
+          s[r] = p[r] * (kFp16<T> ? (dp[r] - lds_delta[buf][i]) * range : dp[r] - lds_delta[buf][i]);
         }
       } else {
 #pragma unroll
@@ -362,16 +454,16 @@ __global__ __launch_bounds__(kKvThreads, HD <= 32 ? 2 : 1) void attn_backward_kv
   pass_tiles<BUFS>(max(0, (end - begin + BM - 1) / BM), fetch, place_tile, work);
   if (!live) return;
   const int64_t at = ((seq.s_off + key) * a.KV + kvh) * a.D;
-  const float f = keys_role ? a.scale : 1.f;
+  const float back = exp2_fast(-kLift<T>), f = keys_role ? a.scale * back / range : back;
   if (b.splits == 1)
     store_rows<T, DT>((keys_role ? dk : dv) + at, acc, f, a.D, half);
   else
     store_rows<float, DT>((keys_role ? pk : pv) + at, acc, f, a.D, half);
   if constexpr (!kRoles) {
     if (b.splits == 1)
-      store_rows<T, DT>(dv + at, other, 1.f, a.D, half);
+      store_rows<T, DT>(dv + at, other, back, a.D, half);
     else
-      store_rows<float, DT>(pv + at, other, 1.f, a.D, half);
+      store_rows<float, DT>(pv + at, other, back, a.D, half);
   }
 }
 
@@ -410,13 +502,20 @@ inline int attn_backward_splits(int B, int64_t total_s, int KV) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(1024 / groups, 8));
 }
 
+inline size_t attn_backward_table(int64_t rows, int heads) { return align_up((size_t)rows * (size_t)heads * sizeof(float), 256); }
+
 template <typename T, int HD>
 int attn_backward_launch(const AttnBwdArgs& b, hipStream_t stream, const char* what) {
   const AttnArgs& a = b.f;
   const int64_t q_tiles = ceil_div(a.total_q * a.G, kAttnRows) + a.B;
   const int64_t s_tiles = ceil_div(a.total_s, 32 * kv_groups<T, HD>()) + a.B;
   int rc = 0;
-  if (a.total_q > 0) {
+  if (kFp16<T> && a.total_s > 0) {
+    const int64_t groups = std::min<int64_t>(ceil_div(a.total_s, 16), std::max(65536 / a.KV, 1));
+    hipLaunchKernelGGL(attn_value_norm_kernel, dim3((unsigned)(groups * a.KV)), dim3(256), 0, stream, b);
+    rc = launch_status(what);
+  }
+  if (rc == 0 && a.total_q > 0) {
     hipLaunchKernelGGL((attn_backward_q_kernel<T, HD>), dim3((unsigned)(q_tiles * a.KV)), dim3(256), 0, stream, b);
     rc = launch_status(what);
   }
@@ -453,8 +552,9 @@ size_t v3d_attention_pack_bwd_workspace_bytes(int B, int64_t total_q, int64_t to
   using namespace v3d;
   if (B < 0 || total_q < 0 || total_s < 0 || H <= 0 || KV <= 0 || D <= 0) return 0;
   const int splits = attn_backward_splits(B, total_s, KV);
-  const size_t delta = align_up((size_t)total_q * (size_t)H * sizeof(float), 256);
-  return delta + (splits > 1 ? (size_t)splits * 2 * (size_t)total_s * (size_t)(KV * D) * sizeof(float) : 0);
+  // delta and the rows' norms (of fp16 only, but the type is not asked for)
+  return 2 * attn_backward_table(total_q, H) + attn_backward_table(total_s, KV) +
+         (splits > 1 ? (size_t)splits * 2 * (size_t)total_s * (size_t)(KV * D) * sizeof(float) : 0);
 }
 
 int v3d_attention_pack_bwd(const void* grad, const void* q, const void* k, const void* v, const void* out,
@@ -514,7 +614,9 @@ int v3d_attention_pack_bwd(const void* grad, const void* q, const void* k, const
   if (rc != 0) return rc;
   b.delta = reinterpret_cast<float*>(ws.base);
   b.splits = attn_backward_splits(B, total_s, KV);
-  b.part = reinterpret_cast<float*>(ws.base + align_up((size_t)total_q * (size_t)H * sizeof(float), 256));
+  b.grad_norm = reinterpret_cast<float*>(ws.base + attn_backward_table(total_q, H));
+  b.value_norm = reinterpret_cast<float*>(ws.base + 2 * attn_backward_table(total_q, H));
+  b.part = reinterpret_cast<float*>(ws.base + 2 * attn_backward_table(total_q, H) + attn_backward_table(total_s, KV));
   rc = dtype == V3D_F32   ? attn_backward_type<float>(b, s, what)
        : dtype == V3D_F16 ? attn_backward_type<f16>(b, s, what)
                           : attn_backward_type<bf16>(b, s, what);

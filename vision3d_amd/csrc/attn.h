@@ -566,7 +566,9 @@ __device__ __forceinline__ Op<T> read_rows(const typename Kind<T>::U* tile, int 
 }
 
 // The result layout's registers [8 u, 8 u + 8) of a 32 x 32 block as the B operand that goes with read_rows.  16-bit types:
-// rounded to the type, which the values have anyway (half a step of each summand, of either sign).
+// rounded to the type, as the other factor is (half a step of each summand, of either sign: the matrix instruction takes two
+// operands of one type, and 32-bit summands would cost three products or six).  In bf16 that is relative to the summand
+// whatever its size; what fp16 is to hold is brought into its range first.
 template <typename T>
 __device__ __forceinline__ Op<T> pack_rows(const f32x16& x, int u) {
   if constexpr (Kind<T>::P == 3) {
@@ -583,6 +585,16 @@ __device__ __forceinline__ Op<T> pack_rows(const f32x16& x, int u) {
 }
 
 constexpr float kLog2e = 1.44269504088896340736f;
+
+// Over the two lanes (l, l + 32) of a column, without LDS.
+__device__ __forceinline__ float halves_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float halves_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }  // v_exp_f32; 2^-inf = 0
 
@@ -620,16 +632,6 @@ __device__ __forceinline__ void store_rows(T* row, const f32x16 (&acc)[DT], floa
 // The mask of a row: its token sees the keys [0, this).
 __device__ __forceinline__ int attn_limit(const AttnArgs& a, const AttnSeq& seq, int token) {
   return a.causal ? max(0, min(seq.s_len, token + seq.s_len - seq.q_len + 1)) : seq.s_len;
-}
-
-// Over the two lanes (l, l + 32) of a column, without LDS.
-__device__ __forceinline__ float halves_max(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float halves_sum(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
 // Host side: the heads, and the division by the group's size as a product (exact for 31-bit numerators: the multiplier is
