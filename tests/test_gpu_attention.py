@@ -391,3 +391,25 @@ def test_refusals_without_a_gpu():
     assert lib.v3d_attention_pack_workspace_bytes(1, 1, 100000, 8, 8, 64) > 0
     assert lib.v3d_cached_attention_workspace_bytes(1, 1, 64, 8, 8, 64) == 0
     assert lib.v3d_cached_attention_workspace_bytes(1, 1, 100000, 8, 8, 64) > 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("count", [32768, 1 << 20])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_many_weak_keys_behind_a_strong_one(dtype, count):
+    # each weak key's probability is 2^-25.2 of the strong one's, in fp16 at the edge of nothing; together they are the output
+    k = torch.zeros(1, count, 1, 64, dtype=dtype, device=DEV)
+    v = torch.ones_like(k)
+    k[0, 0], v[0, 0] = 2.1875, 0.0
+    q = torch.ones(1, 1, 1, 64, dtype=dtype, device=DEV)
+    strong = torch.tensor(8 * 2.1875, dtype=torch.float64).exp().item()
+    want = (count - 1) / (count - 1 + strong)
+    cached = ops.cached_attention(q, k, v, torch.tensor([count], device=DEV))
+    one, n = torch.tensor([1], device=DEV), torch.tensor([count], device=DEV)
+    pack = ops.attention_pack_mode(q[0], k[0], v[0], one, n)
+    several = ops.attention_pack_mode(q[0].expand(300, 1, 64).contiguous(), k[0], v[0], one * 300, n)
+    # the probability and the output are rounded to the type (equal values: all in the same direction); scores are exact,
+    # exp2's argument off by a half step of 25, the 32-bit sums by a step per 64 keys of a lane and per joined part
+    tol = want * (2 * _half(dtype) + (26 + count / 64 + 128) * 2.0 ** -24)
+    for out in (cached, pack, several):
+        assert (out.double() - want).abs().max() <= tol

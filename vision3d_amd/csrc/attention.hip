@@ -21,6 +21,11 @@ __device__ __forceinline__ void wave_order() {  // LDS accesses of a wave stay i
   __builtin_amdgcn_wave_barrier();
 }
 
+// fp16 keeps 11 bits down to 2^-14 and nothing below 2^-25, where a long cache still has weight (2^15 keys of 2^-25 are 2^-10 of
+// the row).  The probabilities are formed 2^7 times as large (in the exponent): with the room that a stale maximum asks for, 2^15.
+template <typename T>
+constexpr float kProbLift = __is_same(T, f16) ? 7.f : 0.f;
+
 // What a wave carries through its keys: 32 rows, one per lane and half.
 template <typename T, int HD>
 struct AttnWave {
@@ -32,7 +37,7 @@ struct AttnWave {
 
   Held<T, HD> q;
   f32x16 o[DT];
-  float m = -__builtin_inff(), l = 0.f;  // running maximum of scale * log2(e) * score, and the sum of 2^(that - m)
+  float m = -__builtin_inff(), l = 0.f;  // running maximum of scale * log2(e) * score (less kProbLift), the sum of 2^(that - m)
   float c2;
   int lane, half;
   int row, token, head;
@@ -92,9 +97,9 @@ struct AttnWave {
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[n][r]);
-    top = halves_max(top) * c2;
+    top = halves_max(top) * c2 - kProbLift<T>;
     // The maximum moves only when a probability would exceed 2^8: what was summed is rescaled rarely, and a stale maximum
-    // costs no accuracy (16-bit probabilities keep their relative precision up to 2^8, the sums are fp32).
+    // costs no accuracy (16-bit probabilities keep their relative precision, the sums are fp32).
     if (__any(top > m + 8.f)) {
       const float m_new = fmaxf(m, top);
       const float alpha = m_new == -__builtin_inff() ? 1.f : exp2_fast(m - m_new);
