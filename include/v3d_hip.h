@@ -476,7 +476,8 @@ int v3d_layer_norm_bwd(const void* grad, const void* feats, const void* residual
  * and grad_v (total_s,KV,D), all contiguous and fully written (zeros behind the last sequence); key heads sum over their
  * query heads.  No atomics: the same bits every time.  With 16-bit types the probabilities and ds = p (grad . v - grad . out)
  * are rounded to the type before they meet the other factor, sums are fp32; fp16 ones are scaled by powers of two first, so
- * small and large gradients keep the type's precision.
+ * small and large gradients keep the type's precision.  p is 2^(score - lse) with lse one fp32 number a row: off by 2^-24 of the
+ * scaled score's size, and no number at all past 2^30 of it (the forward has no such bound).
  *
  * workspace: v3d_*_workspace_bytes bytes (0 where the row tiles alone fill the GPU), 256-B aligned, or NULL. */
 #define V3D_ATTENTION_MAX_HEAD_SIZE 256

@@ -413,3 +413,33 @@ def test_many_weak_keys_behind_a_strong_one(dtype, count):
     tol = want * (2 * _half(dtype) + (26 + count / 64 + 128) * 2.0 ** -24)
     for out in (cached, pack, several):
         assert (out.double() - want).abs().max() <= tol
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 192])
+@pytest.mark.parametrize("size", [1e3, 1e5, 1e9, 1e15])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_scores_beyond_the_exponents(dtype, size, dim):
+    # scores of up to 1e30: the row's maximum takes all, whatever 32-bit numbers can no longer tell apart
+    if dtype == torch.float16:
+        size = min(size, 2e4)
+    n = 1500
+    gen = torch.Generator().manual_seed(dim)
+    sign = torch.randint(0, 2, (n, 1, dim), generator=gen) * 2.0 - 1
+    k = (sign * size).to(dtype)
+    assert torch.unique(sign, dim=0).shape[0] == n
+    k = k.to(DEV)  # distinct signs: a key's own product is dim size^2, any other's at least 2 size^2 less
+    v = torch.randn((n, 1, dim), generator=gen).to(dtype).to(DEV)
+    pick = torch.randint(0, n, (400,), generator=gen).to(DEV)
+    one, few, many = (torch.tensor([m], device=DEV) for m in (1, 40, 400))
+    keys = torch.tensor([n], device=DEV)
+    for q, lengths in ((k[pick], many), (k[pick[:40]], few), (k[pick[:1]], one)):
+        assert torch.equal(ops.attention_pack_mode(q, k, v, lengths, keys), v[pick[:q.shape[0]]])
+    got = ops.cached_attention(k[pick[:3]].unsqueeze(1), k.expand(3, n, 1, dim).reshape(3, n, 1, dim),
+                               v.expand(3, n, 1, dim).reshape(3, n, 1, dim), keys.expand(3).contiguous())
+    assert torch.equal(got[:, 0], v[pick[:3]])
+    # all of them equally far below zero: the plain mean
+    least = ops.attention_pack_mode(-k[:1].expand(40, 1, dim).contiguous(), k[:1].expand(n, 1, dim), v, few, keys)
+    want = v.double().mean(0)
+    size = v.double().abs().mean(0)
+    assert ((least.double() - want).abs() <= 2 * _half(dtype) * size + 200 * 2.0 ** -24 * size).all()

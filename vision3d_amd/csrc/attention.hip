@@ -26,6 +26,22 @@ __device__ __forceinline__ void wave_order() {  // LDS accesses of a wave stay i
 template <typename T>
 constexpr float kProbLift = __is_same(T, f16) ? 7.f : 0.f;
 
+// A probability of score s = q . k is 2^(c2 s - base), base = c2 m - kProbLift for the running maximum m and c2 = scale log2(e):
+// one multiply-add.  The rounding of c2 m is the same for the whole row, but past 2^31 it alone leaves the exponent's range: from
+// kProbLarge on a probability is 2^(c2 (s - m) + kProbLift).
+constexpr float kProbLarge = 0x1p20f;
+template <typename T>
+__device__ __forceinline__ float prob_base(float m, float c2) {
+  return (m == -__builtin_inff() ? 0.f : m) * c2 - kProbLift<T>;
+}
+// What probabilities relative to m count relative to `to` >= m.
+template <typename T>
+__device__ __forceinline__ float prob_weight(float m, float to, float c2) {
+  const float from = prob_base<T>(m, c2), base = prob_base<T>(to, c2);
+  const bool fits = __builtin_fabsf(from) < kProbLarge && __builtin_fabsf(base) < kProbLarge && m > -__builtin_inff();
+  return to == -__builtin_inff() ? 1.f : exp2_fast(fits ? from - base : (m - to) * c2);
+}
+
 // What a wave carries through its keys: 32 rows, one per lane and half.
 template <typename T, int HD>
 struct AttnWave {
@@ -37,7 +53,7 @@ struct AttnWave {
 
   Held<T, HD> q;
   f32x16 o[DT];
-  float m = -__builtin_inff(), l = 0.f;  // running maximum of scale * log2(e) * score (less kProbLift), the sum of 2^(that - m)
+  float m = -__builtin_inff(), l = 0.f;  // running maximum of the products q . k, the sum of the probabilities (see scores)
   float c2;
   int lane, half;
   int row, token, head;
@@ -97,12 +113,12 @@ struct AttnWave {
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[n][r]);
-    top = halves_max(top) * c2 - kProbLift<T>;
+    top = halves_max(top);
     // The maximum moves only when a probability would exceed 2^8: what was summed is rescaled rarely, and a stale maximum
     // costs no accuracy (16-bit probabilities keep their relative precision, the sums are fp32).
-    if (__any(top > m + 8.f)) {
+    if (__any((top - m) * c2 > 8.f)) {
       const float m_new = fmaxf(m, top);
-      const float alpha = m_new == -__builtin_inff() ? 1.f : exp2_fast(m - m_new);
+      const float alpha = prob_weight<T>(m, m_new, c2);
       m = m_new;
       l *= alpha;
 #pragma unroll
@@ -110,7 +126,15 @@ struct AttnWave {
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
     }
-    const float base = m == -__builtin_inff() ? 0.f : m;
+    float base = prob_base<T>(m, c2);
+    if (__any(__builtin_fabsf(base) >= kProbLarge)) {
+      const float at = m == -__builtin_inff() ? 0.f : m;
+      base = -kProbLift<T>;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[n][r] -= at;
+    }
     float sum = 0.f;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -185,7 +209,11 @@ __device__ __forceinline__ void store_out(const AttnArgs& a, int64_t row, int co
 __device__ __forceinline__ float inverse_sum(float l) {
   return l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no keys: zeros; a NaN stays a NaN
 }
-__device__ __forceinline__ float log_sum(float m, float l) { return l == 0.f ? -__builtin_inff() : m + log2f(l); }
+// log2 of the row's sum of exp(scale * q . k) from its maximal product and its sum of probabilities.
+template <typename T>
+__device__ __forceinline__ float log_sum(const AttnArgs& a, float m, float l) {
+  return l == 0.f ? -__builtin_inff() : prob_base<T>(m, a.scale * kLog2e) + log2f(l);
+}
 
 // The launch covers a bound of the pack's tiles: the rest of it clears the rows behind the last sequence.
 template <typename T, int TILE>
@@ -321,7 +349,7 @@ __global__ __launch_bounds__(256, (attn_occupancy<T, HD>())) void attn_forward_k
       a.part_ml[part * 2] = w.m;
       a.part_ml[part * 2 + 1] = l;
     } else if (a.lse) {
-      a.lse[at] = log_sum(w.m, l);
+      a.lse[at] = log_sum<T>(a, w.m, l);
     }
   }
 }
@@ -439,10 +467,9 @@ __global__ __launch_bounds__((64 * few_waves<T, HD>())) void attn_few_rows_kerne
   float m = -__builtin_inff(), l = 0.f;
 #pragma unroll
   for (int i = 0; i < W; ++i) m = fmaxf(m, lds_ml[i][w.lane & 31][0]);
-  const float base = m == -__builtin_inff() ? 0.f : m;
 #pragma unroll
-  for (int i = 0; i < W; ++i) l = fmaf(lds_ml[i][w.lane & 31][1], exp2_fast(lds_ml[i][w.lane & 31][0] - base), l);
-  const float f = exp2_fast(w.m - base) * (a.splits == 1 ? inverse_sum(l) : 1.f);
+  for (int i = 0; i < W; ++i) l = fmaf(lds_ml[i][w.lane & 31][1], prob_weight<T>(lds_ml[i][w.lane & 31][0], m, w.c2), l);
+  const float f = prob_weight<T>(w.m, m, w.c2) * (a.splits == 1 ? inverse_sum(l) : 1.f);
   float* join = reinterpret_cast<float*>(lds);
   auto join_at = [](int r, int col) { return r * HD + (((col >> 2) ^ (r & 7)) << 2); };  // 8 rows at one column: 8 places
 #pragma unroll
@@ -466,7 +493,7 @@ __global__ __launch_bounds__((64 * few_waves<T, HD>())) void attn_few_rows_kerne
       a.part_ml[(part + w.lane) * 2] = m;
       a.part_ml[(part + w.lane) * 2 + 1] = l;
     } else if (a.lse) {
-      a.lse[(seq.q_off + w.token) * a.H + w.head] = log_sum(m, l);
+      a.lse[(seq.q_off + w.token) * a.H + w.head] = log_sum<T>(a, m, l);
     }
   }
   for (int i = threadIdx.x; i < 32 * (HD / 4); i += 64 * W) {
@@ -503,8 +530,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
   float m = m_part;
 #pragma unroll
   for (int d = 32; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
-  const float base = m == -__builtin_inff() ? 0.f : m;
-  const float f = exp2_fast(m_part - base);
+  const float f = prob_weight<T>(m_part, m, a.scale * kLog2e);
   const float l = lanes_sum<64>(l_part * f);
   __shared__ float factor[4][64];
   factor[wave][lane] = f;
@@ -534,7 +560,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) o[j] *= inv;
   if (lane < width) store_out<T>(a, out, col, o);
-  if (a.lse && lane == 0) a.lse[out] = log_sum(m, l);
+  if (a.lse && lane == 0) a.lse[out] = log_sum<T>(a, m, l);
 }
 
 // ---- launches ----------------------------------------------------------------------------------------------------------

@@ -39,7 +39,7 @@ struct AttnArgs {
   int causal;
   int splits;                // parts that the keys of a row tile are divided into
   float* part_o;             // splits > 1: (tile, KV, split, rows of a tile, D) unnormalised rows ...
-  float* part_ml;            // ... and (tile, KV, split, rows of a tile, 2): maximum (of scale * log2(e) * score) and sum
+  float* part_ml;            // ... and (tile, KV, split, rows of a tile, 2): maximum (of q . k) and sum
 };
 
 __device__ __forceinline__ int div_g(const AttnArgs& a, int n) {
