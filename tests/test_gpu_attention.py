@@ -443,3 +443,17 @@ def test_scores_beyond_the_exponents(dtype, size, dim):
     want = v.double().mean(0)
     size = v.double().abs().mean(0)
     assert ((least.double() - want).abs() <= 2 * _half(dtype) * size + 200 * 2.0 ** -24 * size).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_newest_token_of_a_long_projection(dtype):
+    # one token a sequence, the sequences 5.7 million elements apart: more than a tile's offsets, but no tile spans two of them
+    x = torch.randn((3, 1400, 32, 128), device=DEV).to(dtype)
+    k, v = (torch.randn((3, 100, 8, 128), device=DEV).to(dtype) for _ in range(2))
+    n = torch.tensor([100, 30, 77], device=DEV)
+    want = ops.cached_attention(x[:, -1:].contiguous(), k, v, n)
+    assert torch.equal(ops.cached_attention(x[:, -1:], k, v, n), want)
+    assert torch.equal(ops.cached_attention(x[:, -1:].transpose(1, 2).contiguous().transpose(1, 2), k, v, n), want)
+    five = ops.cached_attention(x[:, -5:].contiguous(), k, v, n)  # several tokens: copied by the op
+    assert torch.equal(ops.cached_attention(x[:, -5:], k, v, n), five)

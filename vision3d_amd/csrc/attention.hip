@@ -401,8 +401,8 @@ __global__ __launch_bounds__((64 * few_waves<T, HD>())) void attn_few_rows_kerne
     TileStage<T, HD, 32, 64 * W> stage;
     const int token0 = div_g(a, row0);
     stage.fetch_rows(static_cast<const T*>(a.q) + (seq.q_off + token0) * a.q_row + (int64_t)kvh * a.G * a.q_head, [&](int i) {
-      const int token = div_g(a, row0 + i);
-      return (token - token0) * (int)a.q_row + (row0 + i - token * a.G) * (int)a.q_head;
+      const int row = min(row0 + i, rows - 1), token = div_g(a, row);
+      return (token - token0) * (int)a.q_row + (row - token * a.G) * (int)a.q_head;
     }, a.D, rows - row0);
     stage.store(lds_q, a.D);
     __syncthreads();
@@ -641,13 +641,15 @@ int attn_check(const char* what, int dtype, int B, int64_t total_q, int64_t tota
 }
 
 // A tile's rows are addressed by 32-bit byte offsets from the tile's first row: at most 128 rows of a key tensor, at most
-// 129 tokens and the heads of a group of a query tensor.
+// 129 tokens and the heads of a group of a query tensor.  (One new token a sequence of a cache: its row stride leads from
+// sequence to sequence only, which is 64-bit.)
 int attn_check_strides(const char* what, const AttnArgs& a) {
   const int64_t reach = (int64_t)1 << 29;  // elements of 4 bytes
   auto fits = [&](int64_t row, int64_t head) {
     return row >= 0 && head >= 0 && row < reach / 130 && head < reach / (2 * a.G) && 129 * row + a.G * head + a.D < reach;
   };
-  if (!fits(a.q_row, a.q_head) || !fits(a.k_row, 0) || !fits(a.v_row, 0) || !fits((int64_t)a.H * a.D, a.D)) {
+  const bool alone = a.capacity > 0 && a.tokens == 1;
+  if (a.q_row < 0 || !fits(alone ? 0 : a.q_row, a.q_head) || !fits(a.k_row, 0) || !fits(a.v_row, 0) || !fits((int64_t)a.H * a.D, a.D)) {
     set_last_error("%s: strides of a query or key row beyond 32-bit tile offsets", what);
     return V3D_ERR_SIZE_LIMIT;
   }

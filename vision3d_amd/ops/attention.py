@@ -24,8 +24,9 @@ def _rows(t: Tensor) -> Tensor:
         return t
     row, head, unit = t.stride()[-3:]
     rows, heads, dim = shape[-3:]
+    row = 0 if rows == 1 else row
     near = 130 * row + heads * head + dim < 1 << 29
-    return t if unit == 1 and (rows == 1 or row == 0 or row >= dim) and near else t.contiguous()
+    return t if unit == 1 and (row == 0 or row >= dim) and near else t.contiguous()
 
 
 def _lengths(lengths: Tensor, like: Tensor) -> Tensor:
