@@ -457,3 +457,38 @@ def test_newest_token_of_a_long_projection(dtype):
     assert torch.equal(ops.cached_attention(x[:, -1:].transpose(1, 2).contiguous().transpose(1, 2), k, v, n), want)
     five = ops.cached_attention(x[:, -5:].contiguous(), k, v, n)  # several tokens: copied by the op
     assert torch.equal(ops.cached_attention(x[:, -5:], k, v, n), five)
+
+
+@pytest.mark.gpu
+def test_heads_first_layouts_up_to_the_tiles_offsets():
+    # queries of 8 heads on one key head, 38 million elements from head to head: within a tile's offsets (7 of them), taken as
+    # they are; 80 million: beyond, copied
+    n = torch.tensor([300000], device=DEV)
+    k = torch.randn((64, 1, 128), device=DEV).to(torch.bfloat16)
+    s = torch.tensor([64], device=DEV)
+    for rows in (300000, 620000):
+        x = torch.randn((8, rows, 128), device=DEV, dtype=torch.bfloat16)[:, :300000].transpose(0, 1)
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        got = ops.attention_pack_mode(x, k, k, n, s)
+        copied = torch.cuda.max_memory_allocated() - before > 1.5 * got.numel() * 2
+        assert copied == (rows == 620000)
+        assert torch.equal(got, ops.attention_pack_mode(x.contiguous(), k, k, n, s))
+        del got, x
+
+
+@pytest.mark.gpu
+def test_heads_first_cache_is_not_copied():
+    # the distance between a cache's key heads is 64-bit: no tile spans two of them
+    k = torch.randn((1, 8, 530000, 128), device=DEV, dtype=torch.bfloat16).transpose(1, 2)
+    q = torch.randn((1, 1, 32, 128), device=DEV, dtype=torch.bfloat16)
+    n = torch.tensor([200], device=DEV)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    got = ops.cached_attention(q, k, k, n)
+    assert torch.cuda.max_memory_allocated() - before < 1 << 26
+    near = k[:, :200].contiguous()
+    want = ops.attention_pack_mode(q[0], near[0], near[0], torch.tensor([1], device=DEV), n)
+    # the same products summed in another order: each side within its rounding of outputs below 4
+    assert (got[0].double() - want.double()).abs().max() <= 4 * 4 * _half(torch.bfloat16)

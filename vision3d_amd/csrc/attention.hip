@@ -646,7 +646,7 @@ int attn_check(const char* what, int dtype, int B, int64_t total_q, int64_t tota
 int attn_check_strides(const char* what, const AttnArgs& a) {
   const int64_t reach = (int64_t)1 << 29;  // elements of 4 bytes
   auto fits = [&](int64_t row, int64_t head) {
-    return row >= 0 && head >= 0 && row < reach / 130 && head < reach / (2 * a.G) && 129 * row + a.G * head + a.D < reach;
+    return row >= 0 && head >= 0 && row < reach && head < reach && 129 * row + a.G * head + a.D < reach;
   };
   const bool alone = a.capacity > 0 && a.tokens == 1;
   if (a.q_row < 0 || !fits(alone ? 0 : a.q_row, a.q_head) || !fits(a.k_row, 0) || !fits(a.v_row, 0) || !fits((int64_t)a.H * a.D, a.D)) {

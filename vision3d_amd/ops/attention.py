@@ -16,17 +16,22 @@ def _require_cuda(name, q, k, v):
         raise RuntimeError(f"{name}: CUDA tensors required (no CPU fallback in vision3d_amd)")
 
 
-def _rows(t: Tensor) -> Tensor:
-    """The strides that the kernels take: any but the last dimension's, which is 1, within 32-bit offsets of a tile; other
-    inputs are copied."""
+def _rows(t: Tensor, group: int) -> Tensor:
+    """The strides that the kernels take: any but the last dimension's, which is 1, as long as a tile's rows (129 at most, of
+    ``group`` heads: the queries of one key head, or 0 for keys) lie within 32-bit byte offsets; other inputs are copied."""
     shape = t.shape
     if len(shape) < 3 or t.is_contiguous() or t.numel() == 0:
         return t
     row, head, unit = t.stride()[-3:]
     rows, heads, dim = shape[-3:]
-    row = 0 if rows == 1 else row
-    near = 130 * row + heads * head + dim < 1 << 29
+    row, head = 0 if rows == 1 else row, 0 if heads == 1 else head
+    near = 129 * row + group * head + dim < 1 << 29
     return t if unit == 1 and (row == 0 or row >= dim) and near else t.contiguous()
+
+
+def _operands(q: Tensor, k: Tensor, v: Tensor):
+    group = q.shape[-2] // max(k.shape[-2], 1) if q.dim() > 1 and k.dim() > 1 else 1
+    return _rows(q, group), _rows(k, 0), _rows(v, 0)
 
 
 def _lengths(lengths: Tensor, like: Tensor) -> Tensor:
@@ -43,7 +48,7 @@ def _scale(scale, dim):
 class _AttentionPack(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, q_lengths, s_lengths, scale, causal):
-        q, k, v = _rows(q), _rows(k), _rows(v)
+        q, k, v = _operands(q, k, v)
         out = q.new_empty(q.shape)
         lse = q.new_empty(q.shape[:2], dtype=torch.float32)
         # 16-bit outputs: the backward's grad . out needs what the rounding took from them
@@ -81,8 +86,7 @@ def attention_pack_mode(q_feats: Tensor, k_feats: Tensor, v_feats: Tensor, q_len
     if torch.is_grad_enabled() and (q_feats.requires_grad or k_feats.requires_grad or v_feats.requires_grad):
         return _AttentionPack.apply(q_feats, k_feats, v_feats, q_lengths, s_lengths, scale, causal)
     out = q_feats.new_empty(q_feats.shape)
-    ext.attention_pack_forward(_rows(q_feats), _rows(k_feats), _rows(v_feats), q_lengths, s_lengths, out, None, scale,
-                               causal)
+    ext.attention_pack_forward(*_operands(q_feats, k_feats, v_feats), q_lengths, s_lengths, out, None, scale, causal)
     return out
 
 
@@ -98,9 +102,9 @@ def cached_attention(q_feats: Tensor, k_cache: Tensor, v_cache: Tensor, lengths:
     _require_cuda("cached_attention", q_feats, k_cache, v_cache)
     if torch.is_grad_enabled() and (q_feats.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         raise RuntimeError("cached_attention: no gradient; call it under torch.no_grad() or use attention_pack_mode")
-    q = _rows(q_feats)
+    q, k, v = _operands(q_feats, k_cache, v_cache)
     if q.dim() == 4 and q.shape[1] > 1 and q.shape[0] > 1 and q.stride(0) != q.shape[1] * q.stride(1):
         q = q.contiguous()
     out = q.new_empty(q.shape)
-    ext.cached_attention(q, _rows(k_cache), _rows(v_cache), _lengths(lengths, q), out, _scale(scale, q.shape[-1]))
+    ext.cached_attention(q, k, v, _lengths(lengths, q), out, _scale(scale, q.shape[-1]))
     return out
