@@ -492,3 +492,26 @@ def test_heads_first_cache_is_not_copied():
     want = ops.attention_pack_mode(q[0], near[0], near[0], torch.tensor([1], device=DEV), n)
     # the same products summed in another order: each side within its rounding of outputs below 4
     assert (got[0].double() - want.double()).abs().max() <= 4 * 4 * _half(torch.bfloat16)
+
+
+@pytest.mark.gpu
+def test_cost_of_many_sequences():
+    # sixteen times as many short sequences cost about sixteen times as much, forward and backward (not the square of it)
+    def least(count):
+        lengths = torch.full((count,), 4, device=DEV)
+        leaves = [torch.randn((4 * count, 8, 32), device=DEV).to(torch.bfloat16).requires_grad_(True) for _ in range(3)]
+        times = [[], []]
+        for _ in range(6):
+            marks = [torch.cuda.Event(enable_timing=True) for _ in range(3)]
+            marks[0].record()
+            out = ops.attention_pack_mode(*leaves, lengths)
+            marks[1].record()
+            torch.autograd.grad(out, leaves, leaves[0].detach())
+            marks[2].record()
+            torch.cuda.synchronize()
+            for i in range(2):
+                times[i].append(marks[i].elapsed_time(marks[i + 1]))
+        return [min(t) for t in times]
+
+    few, many = least(2048), least(32768)
+    assert many[0] < 48 * few[0] and many[1] < 48 * few[1]

@@ -422,3 +422,31 @@ def test_values_gradients_of_many_keys():
     # p and the gradient are rounded; the log-sum of n equal terms is off by its own half step (17 of them, in the exponent)
     want = 384.0 / n
     assert (dv - want).abs().max() <= want * (2 * 2.0 ** -11 + 32 * 2.0 ** -24)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_thousands_of_short_sequences(dtype):
+    # more than a wave's lanes squared: the table of the sequences is searched in three steps
+    gen = torch.Generator().manual_seed(11)
+    lengths = torch.randint(0, 4, (4500,), generator=gen).tolist()
+    lengths[4000] = 150
+    _check(dtype, lengths, lengths[::-1], 2, 1, 32, True, seed=5, spare=300)
+
+
+@pytest.mark.gpu
+def test_overrunning_lengths_of_many_sequences():
+    gen = torch.Generator().manual_seed(12)
+    lengths = torch.randint(0, 4, (2000,), generator=gen).tolist()
+    n = sum(lengths)
+    q, k, v, g = (t.to(DEV).requires_grad_(True) for t in _inputs([n], [n], 2, 1, 32, torch.float32, 3))
+    lengths[-1] += 2
+    bad = [-7] + lengths
+    bad[-1] = 1 << 62  # cut at the end, what follows has no rows
+    bad += [5] * 100 + [1 << 62]
+    grads = []
+    for some in (lengths[:-1] + [lengths[-1] - 2], bad):
+        out = ops.attention_pack_mode(q, k, v, torch.tensor(some, device=DEV), causal=True)
+        grads.append([out, *torch.autograd.grad(out, (q, k, v), g.detach())])
+    for a, b in zip(*grads):
+        assert torch.equal(a, b)

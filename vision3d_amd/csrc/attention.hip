@@ -563,12 +563,73 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
   if (a.lse && lane == 0) a.lse[out] = log_sum<T>(a, m, l);
 }
 
+// The table of a pack of many sequences, by one workgroup: 1024 sequences at a time, the rows before each, then (of what is left
+// of them within the totals) the tiles.
+__global__ __launch_bounds__(1024) void attn_table_kernel(const AttnArgs a, int64_t* table, int row_tile, int key_tile) {
+  __shared__ int64_t sums[2][2][16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t n = a.B + 1;
+  int64_t before[4] = {0, 0, 0, 0};  // the workgroup's sequences
+  // x, y -> what all threads before this one have of them; adds everybody's to the workgroup's
+  auto scan = [&](int64_t& x, int64_t& y, int which) {
+    const int64_t ix = lanes_prefix(x, lane), iy = lanes_prefix(y, lane);
+    if (lane == 63) {
+      sums[which][0][wave] = ix;
+      sums[which][1][wave] = iy;
+    }
+    __syncthreads();
+    x = before[2 * which] + ix - x;
+    y = before[2 * which + 1] + iy - y;
+#pragma unroll 1
+    for (int w = 0; w < 16; ++w) {
+      if (w < wave) {
+        x += sums[which][0][w];
+        y += sums[which][1][w];
+      }
+      before[2 * which] += sums[which][0][w];
+      before[2 * which + 1] += sums[which][1][w];
+    }
+  };
+  for (int i0 = 0; i0 < a.B; i0 += 1024) {
+    const int i = i0 + threadIdx.x;
+    int64_t q_len = i < a.B ? clamp64(a.q_lengths[i], a.total_q) : 0, s_len = i < a.B ? clamp64(a.s_lengths[i], a.total_s) : 0;
+    int64_t q = q_len, s = s_len;
+    scan(q, s, 0);
+    q = clamp64(q, a.total_q);
+    s = clamp64(s, a.total_s);
+    q_len = clamp64(q_len, a.total_q - q);
+    s_len = clamp64(s_len, a.total_s - s);
+    int64_t row_tiles = (q_len * a.G + row_tile - 1) / row_tile, key_tiles = key_tile > 0 ? (s_len + key_tile - 1) / key_tile : 0;
+    scan(row_tiles, key_tiles, 1);
+    if (i < a.B) {
+      table[i] = q;
+      table[n + i] = s;
+      table[2 * n + i] = row_tiles;
+      if (key_tile > 0) table[3 * n + i] = key_tiles;
+    }
+  }  // (a scan's sums are written again only behind the other scan's barrier)
+  if (threadIdx.x == 0) {
+    table[a.B] = clamp64(before[0], a.total_q);
+    table[n + a.B] = clamp64(before[1], a.total_s);
+    table[2 * n + a.B] = before[2];
+    if (key_tile > 0) table[3 * n + a.B] = before[3];
+  }
+}
+
+int attn_table_launch(AttnArgs& a, void* table, int row_tile, int key_tile, hipStream_t stream, const char* what) {
+  if (a.B <= kAttnWalk) return 0;
+  a.table = static_cast<int64_t*>(table);
+  hipLaunchKernelGGL(attn_table_kernel, dim3(1), dim3(1024), 0, stream, a, static_cast<int64_t*>(table), row_tile, key_tile);
+  return launch_status(what);
+}
+
 // ---- launches ----------------------------------------------------------------------------------------------------------
 struct AttnPlan {
   bool few;         // 32-row tiles whose waves divide the keys, else 128-row tiles
   int64_t tiles;    // row tiles (a bound in a pack)
   int splits;
-  size_t bytes;     // workspace
+  size_t table;     // workspace: the table of the sequences, ...
+  size_t bytes;     // ... and with the parts behind it
   int tile() const { return few ? 32 : kAttnRows; }
 };
 
@@ -586,7 +647,8 @@ inline AttnPlan attn_plan(int B, int64_t total_q, int64_t total_s, int tokens, i
   // 42 us; 512 workgroups, whose parts are twice the bytes to join: 49 us), into two of the other.
   const int64_t groups = std::max<int64_t>(p.tiles * KV, 1), mean = tokens > 0 ? total_s : total_s / std::max(B, 1);
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(p.few ? 256 : 512) / groups, mean / 512, 64}));
-  p.bytes = p.splits > 1 ? (size_t)(groups * p.splits * p.tile()) * (size_t)(D + 2) * sizeof(float) : 0;
+  p.table = tokens > 0 ? 0 : attn_table_bytes(B, 3);
+  p.bytes = p.table + (p.splits > 1 ? (size_t)(groups * p.splits * p.tile()) * (size_t)(D + 2) * sizeof(float) : 0);
   return p;
 }
 
@@ -675,12 +737,14 @@ int attn_forward_run(AttnArgs& a, int dtype, const AttnPlan& plan, void* workspa
   if (plan.bytes > 0) {
     const int rc = ws.acquire(what, workspace, workspace_bytes, plan.bytes, s);
     if (rc != 0) return rc;
-    a.part_o = reinterpret_cast<float*>(ws.base);
+    a.part_o = reinterpret_cast<float*>(ws.base + plan.table);
     a.part_ml = a.part_o + plan.tiles * a.KV * a.splits * plan.tile() * a.D;
   }
-  int rc = dtype == V3D_F32   ? attn_forward_type<float>(a, plan, s, what)
-           : dtype == V3D_F16 ? attn_forward_type<f16>(a, plan, s, what)
-                              : attn_forward_type<bf16>(a, plan, s, what);
+  int rc = plan.table > 0 ? attn_table_launch(a, ws.base, plan.tile(), 0, s, what) : 0;
+  if (rc == 0)
+    rc = dtype == V3D_F32   ? attn_forward_type<float>(a, plan, s, what)
+         : dtype == V3D_F16 ? attn_forward_type<f16>(a, plan, s, what)
+                            : attn_forward_type<bf16>(a, plan, s, what);
   return ws.release(what, rc);
 }
 

@@ -505,12 +505,12 @@ inline int attn_backward_splits(int B, int64_t total_s, int KV) {
 inline size_t attn_backward_table(int64_t rows, int heads) { return align_up((size_t)rows * (size_t)heads * sizeof(float), 256); }
 
 template <typename T, int HD>
-int attn_backward_launch(const AttnBwdArgs& b, hipStream_t stream, const char* what) {
-  const AttnArgs& a = b.f;
+int attn_backward_launch(AttnBwdArgs& b, hipStream_t stream, const char* what) {
+  AttnArgs& a = b.f;
   const int64_t q_tiles = ceil_div(a.total_q * a.G, kAttnRows) + a.B;
   const int64_t s_tiles = ceil_div(a.total_s, 32 * kv_groups<T, HD>()) + a.B;
-  int rc = 0;
-  if (kFp16<T> && a.total_s > 0) {
+  int rc = attn_table_launch(a, const_cast<int64_t*>(a.table), kAttnRows, 32 * kv_groups<T, HD>(), stream, what);
+  if (rc == 0 && kFp16<T> && a.total_s > 0) {
     const int64_t groups = std::min<int64_t>(ceil_div(a.total_s, 16), std::max(65536 / a.KV, 1));
     hipLaunchKernelGGL(attn_value_norm_kernel, dim3((unsigned)(groups * a.KV)), dim3(256), 0, stream, b);
     rc = launch_status(what);
@@ -533,7 +533,7 @@ int attn_backward_launch(const AttnBwdArgs& b, hipStream_t stream, const char* w
 }
 
 template <typename T>
-int attn_backward_type(const AttnBwdArgs& b, hipStream_t stream, const char* what) {
+int attn_backward_type(AttnBwdArgs& b, hipStream_t stream, const char* what) {
   switch (attn_head_size(b.f.D)) {
     case 32: return attn_backward_launch<T, 32>(b, stream, what);
     case 64: return attn_backward_launch<T, 64>(b, stream, what);
@@ -553,7 +553,7 @@ size_t v3d_attention_pack_bwd_workspace_bytes(int B, int64_t total_q, int64_t to
   if (B < 0 || total_q < 0 || total_s < 0 || H <= 0 || KV <= 0 || D <= 0) return 0;
   const int splits = attn_backward_splits(B, total_s, KV);
   // delta and the rows' norms (of fp16 only, but the type is not asked for)
-  return 2 * attn_backward_table(total_q, H) + attn_backward_table(total_s, KV) +
+  return 2 * attn_backward_table(total_q, H) + attn_backward_table(total_s, KV) + attn_table_bytes(B, 4) +
          (splits > 1 ? (size_t)splits * 2 * (size_t)total_s * (size_t)(KV * D) * sizeof(float) : 0);
 }
 
@@ -612,11 +612,18 @@ int v3d_attention_pack_bwd(const void* grad, const void* q, const void* k, const
   rc = ws.acquire(what, workspace, workspace_bytes,
                   v3d_attention_pack_bwd_workspace_bytes(B, total_q, total_s, H, KV, D), s);
   if (rc != 0) return rc;
-  b.delta = reinterpret_cast<float*>(ws.base);
+  char* at = ws.base;
+  auto take = [&](size_t bytes) {
+    char* p = at;
+    at += bytes;
+    return reinterpret_cast<float*>(p);
+  };
+  b.delta = take(attn_backward_table(total_q, H));
+  b.grad_norm = take(attn_backward_table(total_q, H));
+  b.value_norm = take(attn_backward_table(total_s, KV));
+  a.table = reinterpret_cast<int64_t*>(take(attn_table_bytes(B, 4)));
+  b.part = reinterpret_cast<float*>(at);
   b.splits = attn_backward_splits(B, total_s, KV);
-  b.grad_norm = reinterpret_cast<float*>(ws.base + attn_backward_table(total_q, H));
-  b.value_norm = reinterpret_cast<float*>(ws.base + 2 * attn_backward_table(total_q, H));
-  b.part = reinterpret_cast<float*>(ws.base + 2 * attn_backward_table(total_q, H) + attn_backward_table(total_s, KV));
   rc = dtype == V3D_F32   ? attn_backward_type<float>(b, s, what)
        : dtype == V3D_F16 ? attn_backward_type<f16>(b, s, what)
                           : attn_backward_type<bf16>(b, s, what);

@@ -17,6 +17,7 @@ __host__ __device__ constexpr int attn_pow2(int hd) { return hd <= 32 ? 32 : hd 
 
 constexpr int kAttnWaves = 4;
 constexpr int kAttnRows = 32 * kAttnWaves;  // rows (or keys) of a workgroup's tile
+constexpr int kAttnWalk = 256;              // sequences that every wave looks through by itself, see locate
 
 // Element strides throughout.  Rows of the keys: row j of sequence b is at (first row of b + j) * row stride in a pack,
 // at b * batch stride + j * row stride in a cache (`capacity` > 0).
@@ -29,6 +30,7 @@ struct AttnArgs {
   float* lse;                // (total_q, H) log2 of the sum of exponentials, -inf for a row without keys; or NULL
   const int64_t* q_lengths;  // (B), NULL in a cache: every sequence has `tokens` queries
   const int64_t* s_lengths;  // (B)
+  const int64_t* table;      // a pack of more than kAttnWalk sequences: (3 or 4, B + 1), see attn_table_launch
   int64_t total_q, total_s;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head, k_batch, v_batch;
   int64_t capacity;
@@ -89,8 +91,13 @@ __device__ __forceinline__ int wave_sum(int x) {
 
 // Tile number `t` of the pack: sequence b has ceil(rows_b / TILE) tiles, rows_b = q_len * G (BY_KEYS: s_len).  The lengths
 // are device data, so the launch covers the bound total / TILE + B and the kernels look their sequence up here: every wave
-// by itself, one lane per sequence, no LDS and no barrier.  Negative lengths count as 0; lengths that overrun the totals are
-// cut, so that no row outside the buffers is ever addressed.
+// by itself, one lane per sequence (or a few), no LDS and no barrier.  Negative lengths count as 0; lengths that overrun the
+// totals are cut, so that no row outside the buffers is ever addressed.
+//
+// That every wave adds all lengths up costs the square of their number, so more than kAttnWalk sequences are looked up in a table
+// of the rows and tiles before each, which a small kernel writes first: 64 places of it at a time, two steps for 4096 sequences.
+// Sequences of 4 tokens, 8 heads of 32, bf16, forward, without and with the table: 128 sequences 15 / 22 us, 256 22 / 24, 512 45 /
+// 38, 1024 155 / 64, 16384 32000 / 980 us.
 //
 // The causal tiles of up to 64 sequences are numbered by work, the most first, whatever sequence they lie in: a row tile's
 // work grows with its place in the sequence, a key tile's with its distance from the end, so the numbering goes level by
@@ -167,51 +174,70 @@ __device__ __forceinline__ AttnSeq locate(const AttnArgs& a, int64_t t) {
     r.s_len = (int)__shfl(s, src, 64);
     return r;
   }
-  const int per = (a.B + 63) >> 6;
-  int64_t sq = 0, ss = 0, st = 0;
-  for (int e = 0; e < per; ++e) {
-    const int i = lane * per + e;
-    if (i < a.B) {
-      const int64_t q = len_q(i), s = len_s(i);
-      sq += q;
-      ss += s;
-      st += tiles(q, s);
+  if (a.B <= kAttnWalk) {
+    static_assert(kAttnWalk <= 64 * 64, "a lane's sequences are looked at by one wave at once");
+    const int per = (a.B + 63) >> 6;
+    int64_t sq = 0, ss = 0, st = 0;
+    for (int e = 0; e < per; ++e) {
+      const int i = lane * per + e;
+      if (i < a.B) {
+        const int64_t q = len_q(i), s = len_s(i);
+        sq += q;
+        ss += s;
+        st += tiles(q, s);
+      }
     }
-  }
-  const int64_t iq = lanes_prefix(sq, lane), is = lanes_prefix(ss, lane), it = lanes_prefix(st, lane);
-  const int64_t all = uniform64(__shfl(it, 63, 64));  // uniform to the compiler: what follows stays in scalar registers
-  if (t >= all) {
-    r.spare = t - all;
-    r.q_end = clamp64(__shfl(iq, 63, 64), a.total_q);
-    r.s_end = clamp64(__shfl(is, 63, 64), a.total_s);
-    return r;
-  }
-  const int src = __builtin_ctzll(__ballot(it > t));  // the first lane whose tiles reach past t
-  int64_t q0 = __shfl(iq - sq, src, 64), s0 = __shfl(is - ss, src, 64), t0 = __shfl(it - st, src, 64);
-  for (int e0 = 0; e0 < per; e0 += 64) {  // among the lane's sequences, 64 at a time
-    const int i = src * per + e0 + lane;
-    const bool in = e0 + lane < per && i < a.B;
-    const int64_t q = in ? len_q(i) : 0, s = in ? len_s(i) : 0, n = in ? tiles(q, s) : 0;
-    const int64_t pq = lanes_prefix(q, lane), ps = lanes_prefix(s, lane), pt = lanes_prefix(n, lane);
-    const uint64_t hit = __ballot(t0 + pt > t);
-    if (hit != 0) {
-      const int at = __builtin_ctzll(hit);
-      q0 = clamp64(q0 + __shfl(pq - q, at, 64), a.total_q);
-      s0 = clamp64(s0 + __shfl(ps - s, at, 64), a.total_s);
-      r.found = true;
-      r.b = src * per + e0 + at;
-      r.tile = (int)(t - t0 - __shfl(pt - n, at, 64));
-      r.q_off = q0;
-      r.s_off = s0;
-      r.q_len = (int)clamp64(__shfl(q, at, 64), a.total_q - q0);
-      r.s_len = (int)clamp64(__shfl(s, at, 64), a.total_s - s0);
+    const int64_t iq = lanes_prefix(sq, lane), is = lanes_prefix(ss, lane), it = lanes_prefix(st, lane);
+    const int64_t all = uniform64(__shfl(it, 63, 64));  // uniform to the compiler: what follows stays in scalar registers
+    if (t >= all) {
+      r.spare = t - all;
+      r.q_end = clamp64(__shfl(iq, 63, 64), a.total_q);
+      r.s_end = clamp64(__shfl(is, 63, 64), a.total_s);
       return r;
     }
-    q0 += __shfl(pq, 63, 64);
-    s0 += __shfl(ps, 63, 64);
-    t0 += __shfl(pt, 63, 64);
+    const int src = __builtin_ctzll(__ballot(it > t));  // the first lane whose tiles reach past t
+    int64_t q0 = __shfl(iq - sq, src, 64), s0 = __shfl(is - ss, src, 64), t0 = __shfl(it - st, src, 64);
+    const int i = src * per + lane;  // among that lane's sequences
+    const bool in = lane < per && i < a.B;
+    const int64_t q = in ? len_q(i) : 0, s = in ? len_s(i) : 0, n = in ? tiles(q, s) : 0;
+    const int64_t pq = lanes_prefix(q, lane), ps = lanes_prefix(s, lane), pt = lanes_prefix(n, lane);
+    const int at = __builtin_ctzll(__ballot(t0 + pt > t));
+    q0 = clamp64(q0 + __shfl(pq - q, at, 64), a.total_q);
+    s0 = clamp64(s0 + __shfl(ps - s, at, 64), a.total_s);
+    r.found = true;
+    r.b = src * per + at;
+    r.tile = (int)(t - t0 - __shfl(pt - n, at, 64));
+    r.q_off = q0;
+    r.s_off = s0;
+    r.q_len = (int)clamp64(__shfl(q, at, 64), a.total_q - q0);
+    r.s_len = (int)clamp64(__shfl(s, at, 64), a.total_s - s0);
+    return r;
   }
-  return r;  // not reached
+  const int64_t n = a.B + 1;
+  const int64_t* before = a.table + (BY_KEYS ? 3 : 2) * n;  // tiles before a sequence
+  const int64_t all = uniform64(before[a.B]);
+  if (t >= all) {
+    r.spare = t - all;
+    r.q_end = a.table[a.B];
+    r.s_end = a.table[n + a.B];
+    return r;
+  }
+  int low = 0, high = a.B;  // before[low] <= t < before[high]
+  while (high - low > 1) {
+    const int step = (high - low + 63) >> 6;
+    const int at = (int)min((int64_t)high, low + (int64_t)(lane + 1) * step);  // the last lane's is `high`
+    const int src = __builtin_ctzll(__ballot(before[at] > t));
+    high = (int)min((int64_t)high, low + (int64_t)(src + 1) * step);
+    low += src * step;
+  }
+  r.found = true;
+  r.b = low;
+  r.tile = (int)(t - before[low]);
+  r.q_off = a.table[low];
+  r.s_off = a.table[n + low];
+  r.q_len = (int)(a.table[low + 1] - r.q_off);
+  r.s_len = (int)(a.table[n + low + 1] - r.s_off);
+  return r;
 }
 
 // The same for a cache: the geometry is known on the host, only the filled length is read.
@@ -646,6 +672,11 @@ inline void attn_heads(AttnArgs& a, int H, int KV, int D) {
   a.g_mul = s == 0 ? 0u : (unsigned)((((uint64_t)1 << (31 + s)) + a.G - 1) / a.G);
   a.g_shift = s == 0 ? 0u : s - 1;
 }
+
+// Host side: fills `a.table` (attention.hip): first rows of the queries' sequences, of the keys' and the row tiles before each, if
+// key_tile > 0 the key tiles too; the last entry of each is the end of all.
+inline size_t attn_table_bytes(int B, int rows) { return B > kAttnWalk ? align_up((size_t)rows * ((size_t)B + 1) * 8, 256) : 0; }
+int attn_table_launch(AttnArgs& a, void* table, int row_tile, int key_tile, hipStream_t stream, const char* what);
 
 // Host side: the argument checks of every entry point (attention.hip).
 int attn_check(const char* what, int dtype, int B, int64_t total_q, int64_t total_s, int H, int KV, int D, float scale);
