@@ -30,6 +30,8 @@ def _rows(t: Tensor, group: int) -> Tensor:
 
 
 def _operands(q: Tensor, k: Tensor, v: Tensor):
+    if q.is_contiguous() and k.is_contiguous() and v.is_contiguous():
+        return q, k, v
     group = q.shape[-2] // max(k.shape[-2], 1) if q.dim() > 1 and k.dim() > 1 else 1
     return _rows(q, group), _rows(k, 0), _rows(v, 0)
 
