@@ -479,7 +479,8 @@ int v3d_layer_norm_bwd(const void* grad, const void* feats, const void* residual
  * small and large gradients keep the type's precision.  p is 2^(score - lse) with lse one fp32 number a row: off by 2^-24 of the
  * scaled score's size, and no number at all past 2^30 of it (the forward has no such bound).
  *
- * workspace: v3d_*_workspace_bytes bytes (0 where the row tiles alone fill the GPU), 256-B aligned, or NULL. */
+ * At most 2^30 query rows times heads, 2^30 keys and 2^24 tiles: about KV (B + rows / 128), V3D_ERR_SIZE_LIMIT beyond.
+ * workspace: v3d_*_workspace_bytes bytes (0 where few sequences' row tiles alone fill the GPU), 256-B aligned, or NULL. */
 #define V3D_ATTENTION_MAX_HEAD_SIZE 256
 size_t v3d_attention_pack_workspace_bytes(int B, int64_t total_q, int64_t total_s, int H, int KV, int D);
 int v3d_attention_pack_fwd(const void* q, const void* k, const void* v, const int64_t* q_lengths,

@@ -515,3 +515,25 @@ def test_cost_of_many_sequences():
 
     few, many = least(2048), least(32768)
     assert many[0] < 48 * few[0] and many[1] < 48 * few[1]
+
+
+def test_launches_beyond_the_limit_are_refused():
+    # three million sequences of four tokens, eight key heads: more workgroups than a launch holds; nothing is read before
+    import ctypes
+
+    from vision3d_amd import _lib
+
+    lib, at = _lib.lib(), ctypes.c_void_p(1 << 20)
+    strides, cache = (ctypes.c_int64 * 6)(64, 8, 64, 8, 64, 8), (ctypes.c_int64 * 8)(64, 8, 64, 64, 8, 64, 64, 8)
+    count = 3_000_000
+
+    def pack(count, heads):
+        return lib.v3d_attention_pack_fwd(at, at, at, at, at, at, None, None, 1, count, 4 * count, 4 * count, heads, heads, 8,
+                                          strides, 1.0, 0, at, 1 << 40, 0, None)
+
+    assert pack(count, 8) == -4 and pack(1 << 24, 1) == -4
+    assert lib.v3d_attention_pack_bwd(at, at, at, at, at, None, at, at, at, at, at, at, 1, count, 4 * count, 4 * count, 8, 8, 8,
+                                      strides, 1.0, 0, at, 1 << 40, 0, None) == -4
+    assert lib.v3d_attention_pack_bwd(at, at, at, at, at, None, at, at, at, at, at, at, 1, 10, 40, 1 << 30, 8, 8, 8,
+                                      strides, 1.0, 0, at, 1 << 40, 0, None) == -4
+    assert lib.v3d_cached_attention(at, at, at, at, at, 1, count, 1, 1, 8, 8, 8, cache, 1.0, at, 1 << 40, 0, None) == -4

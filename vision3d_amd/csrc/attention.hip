@@ -724,9 +724,9 @@ int attn_forward_run(AttnArgs& a, int dtype, const AttnPlan& plan, void* workspa
                      void* stream, const char* what) {
   const int bad = attn_check_strides(what, a);
   if (bad != 0) return bad;
-  if (plan.tiles * a.KV * plan.splits >= (int64_t)1 << 31 ||
-      (plan.splits > 1 && plan.tiles * a.KV * (plan.tile() / 4) >= (int64_t)1 << 31)) {
-    set_last_error("%s: too many tiles", what);
+  if (plan.tiles * a.KV * plan.splits > kAttnMaxGroups ||
+      (plan.splits > 1 && plan.tiles * a.KV * (plan.tile() / 4) > kAttnMaxGroups)) {
+    set_last_error("%s: more than 2^24 row tiles (every sequence counts as one at least, once per key head)", what);
     return V3D_ERR_SIZE_LIMIT;
   }
   DeviceGuard guard(device);

@@ -599,10 +599,11 @@ int v3d_attention_pack_bwd(const void* grad, const void* q, const void* k, const
   b.dv = grad_v;
   rc = attn_check_strides(what, a);
   if (rc != 0) return rc;
-  if ((ceil_div(total_q * a.G, kAttnRows) + B) * KV >= (int64_t)1 << 31 ||
-      (ceil_div(total_s, 64) + B) * KV * attn_backward_splits(B, total_s, KV) >= (int64_t)1 << 31 ||
-      ceil_div(total_s * KV * D, 1024) >= (int64_t)1 << 31) {
-    set_last_error("%s: too many tiles", what);
+  const int keys = attn_head_size(D) > (dtype == V3D_F32 ? 96 : 128) ? 64 : 128;  // kv_groups
+  if ((ceil_div(total_q * a.G, kAttnRows) + B) * KV > kAttnMaxGroups ||
+      (ceil_div(total_s, keys) + B) * KV * attn_backward_splits(B, total_s, KV) > kAttnMaxGroups ||
+      (attn_backward_splits(B, total_s, KV) > 1 && ceil_div(total_s * KV * D, 1024) > kAttnMaxGroups)) {
+    set_last_error("%s: more than 2^24 row or key tiles (every sequence counts as one at least, once per key head)", what);
     return V3D_ERR_SIZE_LIMIT;
   }
   DeviceGuard guard(device);
