@@ -537,3 +537,26 @@ def test_launches_beyond_the_limit_are_refused():
     assert lib.v3d_attention_pack_bwd(at, at, at, at, at, None, at, at, at, at, at, at, 1, 10, 40, 1 << 30, 8, 8, 8,
                                       strides, 1.0, 0, at, 1 << 40, 0, None) == -4
     assert lib.v3d_cached_attention(at, at, at, at, at, 1, count, 1, 1, 8, 8, 8, cache, 1.0, at, 1 << 40, 0, None) == -4
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused():
+    # no forward-mode derivatives: a tangent is refused, not dropped; what carries none goes through
+    import torch.autograd.forward_ad as fw
+
+    x, w = torch.randn((10, 2, 16), device=DEV), torch.ones(16, device=DEV)
+    n = torch.tensor([10], device=DEV)
+    calls = [lambda t: ops.attention_pack_mode(t, x, x, n), lambda t: ops.attention_pack_mode(x, x, t, n),
+             lambda t: ops.layer_norm(t), lambda t: ops.layer_norm(x, w, residual=t), lambda t: ops.layer_norm(x, t[0, 0])]
+    cached = lambda t: ops.cached_attention(x[None], t[None], x[None], n)
+    with fw.dual_level():
+        dual = fw.make_dual(x, torch.ones_like(x))
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad):
+                for call in calls:
+                    with pytest.raises(NotImplementedError):
+                        call(dual)
+                with pytest.raises(RuntimeError, match="no gradient"):
+                    cached(dual)
+                for call in calls + [cached]:
+                    call(x)

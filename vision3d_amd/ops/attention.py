@@ -9,6 +9,7 @@ import torch
 from torch import Tensor
 
 from .. import ext
+from ._autograd import recorded
 
 
 def _require_cuda(name, q, k, v):
@@ -85,7 +86,7 @@ def attention_pack_mode(q_feats: Tensor, k_feats: Tensor, v_feats: Tensor, q_len
     q_lengths = _lengths(q_lengths, q_feats)
     s_lengths = q_lengths if s_lengths is None else _lengths(s_lengths, q_feats)
     scale = _scale(scale, q_feats.shape[-1])
-    if torch.is_grad_enabled() and (q_feats.requires_grad or k_feats.requires_grad or v_feats.requires_grad):
+    if recorded(q_feats, k_feats, v_feats):
         return _AttentionPack.apply(q_feats, k_feats, v_feats, q_lengths, s_lengths, scale, causal)
     out = q_feats.new_empty(q_feats.shape)
     ext.attention_pack_forward(*_operands(q_feats, k_feats, v_feats), q_lengths, s_lengths, out, None, scale, causal)
@@ -102,7 +103,7 @@ def cached_attention(q_feats: Tensor, k_cache: Tensor, v_cache: Tensor, lengths:
     sequences are.  Only the last dimension of each tensor has to be contiguous.
     """
     _require_cuda("cached_attention", q_feats, k_cache, v_cache)
-    if torch.is_grad_enabled() and (q_feats.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
+    if recorded(q_feats, k_cache, v_cache):
         raise RuntimeError("cached_attention: no gradient; call it under torch.no_grad() or use attention_pack_mode")
     q, k, v = _operands(q_feats, k_cache, v_cache)
     if q.dim() == 4 and q.shape[1] > 1 and q.shape[0] > 1 and q.stride(0) != q.shape[1] * q.stride(1):

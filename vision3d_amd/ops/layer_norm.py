@@ -11,6 +11,7 @@ import torch
 from torch import Tensor
 
 from .. import ext
+from ._autograd import recorded
 
 
 class _LayerNorm(torch.autograd.Function):
@@ -64,7 +65,7 @@ def layer_norm(feats: Tensor, weight: Optional[Tensor] = None, bias: Optional[Te
     weight = None if weight is None else weight.contiguous()
     bias = None if bias is None else bias.contiguous()
     residual = None if residual is None else residual.contiguous()
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (feats, weight, bias, residual)):
+    if recorded(feats, weight, bias, residual):
         return _LayerNorm.apply(feats, weight, bias, eps, residual)
     out = torch.empty_like(feats)
     ext.layer_norm_forward(feats, residual, weight, bias, out, None, eps)
