@@ -474,7 +474,7 @@ int v3d_layer_norm_bwd(const void* grad, const void* feats, const void* residual
  *
  * v3d_attention_pack_bwd: grad (total_q,H,D) of out and the forward's inputs, out, rest (or NULL) and lse -> grad_q (total_q,H,D), grad_k
  * and grad_v (total_s,KV,D), all contiguous and fully written (zeros behind the last sequence); key heads sum over their
- * query heads.  No atomics: the same bits every time.  With 16-bit types the probabilities and ds = p (grad . v - grad . out)
+ * query heads.  grad_q, or grad_k and grad_v together, may be NULL: not wanted.  No atomics: the same bits every time.  With 16-bit types the probabilities and ds = p (grad . v - grad . out)
  * are rounded to the type before they meet the other factor, sums are fp32; fp16 ones are scaled by powers of two first, so
  * small and large gradients keep the type's precision.  p is 2^(score - lse) with lse one fp32 number a row: off by 2^-24 of the
  * scaled score's size, and no number at all past 2^30 of it (the forward has no such bound).

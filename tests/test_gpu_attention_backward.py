@@ -450,3 +450,56 @@ def test_overrunning_lengths_of_many_sequences():
         grads.append([out, *torch.autograd.grad(out, (q, k, v), g.detach())])
     for a, b in zip(*grads):
         assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_only_the_gradients_that_are_wanted(dtype):
+    from vision3d_amd import ext
+
+    n = torch.tensor([130, 0, 45], device=DEV)
+    q, k, v, g = (t.to(DEV) for t in _inputs([175], [175], 4, 2, 64, dtype, 2, spare=4))
+
+    def grads(*wanted):
+        leaves = [t.clone().requires_grad_(w) for t, w in zip((q, k, v), wanted)]
+        out = ops.attention_pack_mode(*leaves, n, causal=True)
+        return torch.autograd.grad(out, [t for t in leaves if t.requires_grad], g)
+
+    dq, dk, dv = grads(True, True, True)
+    for wanted, want in (((1, 0, 0), [dq]), ((0, 1, 0), [dk]), ((0, 0, 1), [dv]), ((0, 1, 1), [dk, dv]), ((1, 0, 1), [dq, dv])):
+        for a, b in zip(grads(*map(bool, wanted)), want):
+            assert torch.equal(a, b)
+    out, lse = torch.empty_like(q), torch.empty(q.shape[:2], device=DEV)
+    ext.attention_pack_forward(q, k, v, n, n, out, lse, 0.125, True)
+    a, b = torch.empty_like(q), [torch.empty_like(k), torch.empty_like(v)]
+    ext.attention_pack_backward(g, q, k, v, out, lse, n, n, None, None, None, 0.125, True)
+    ext.attention_pack_backward(g, q, k, v, out, lse, n, n, a, None, None, 0.125, True)
+    ext.attention_pack_backward(g, q, k, v, out, lse, n, n, None, *b, 0.125, True)
+    both = [torch.empty_like(t) for t in (q, k, v)]
+    ext.attention_pack_backward(g, q, k, v, out, lse, n, n, *both, 0.125, True)
+    for x, y in zip([a, *b], both):
+        assert torch.equal(x, y)
+    with pytest.raises(RuntimeError, match="come together"):
+        ext.attention_pack_backward(g, q, k, v, out, lse, n, n, a, b[0], None, 0.125, True)
+
+
+@pytest.mark.gpu
+def test_frozen_keys_and_values_save_their_kernel():
+    n = torch.tensor([8192], device=DEV)
+    q, k, v = (torch.randn((8192, 8, 64), device=DEV).to(torch.bfloat16) for _ in range(3))
+
+    def least(*wanted):
+        leaves = [t.clone().requires_grad_(w) for t, w in zip((q, k, v), wanted)]
+        out, wanted = ops.attention_pack_mode(*leaves, n), [t for t in leaves if t.requires_grad]
+        times = []
+        for _ in range(6):
+            marks = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+            marks[0].record()
+            torch.autograd.grad(out, wanted, q, retain_graph=True)
+            marks[1].record()
+            torch.cuda.synchronize()
+            times.append(marks[0].elapsed_time(marks[1]))
+        return min(times)
+
+    whole = least(True, True, True)  # dq takes two fifths of it
+    assert least(True, False, False) < 0.75 * whole and least(False, True, True) < 0.9 * whole

@@ -25,7 +25,7 @@ struct AttnBwdArgs {
   float* part;         // splits > 1: (splits, 2, total_s, KV, D) sums of the parts, dk's and dv's
   float* grad_norm;    // fp16: (total_q, H) 2-norms of the rows of grad, written by the dq kernel ...
   float* value_norm;   // ... and (total_s, KV) of the values, written before it; infinities and NaN count as 0
-  void* dq;            // (total_q, H, D), (total_s, KV, D) contiguous
+  void* dq;            // (total_q, H, D) or NULL, (total_s, KV, D), contiguous
   void* dk;
   void* dv;
 };
@@ -145,6 +145,7 @@ __global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 128 : 64) ? 2 : 1) vo
   const AttnSeq seq = locate_rows<kAttnRows>(a, id);
   T* dq = static_cast<T*>(b.dq);
   if (!seq.found) {  // rows behind the last sequence have no gradient
+    if (dq == nullptr) return;
     const int64_t rows = (a.total_q - seq.q_end) * a.G;
     for (int i = threadIdx.x; i < kAttnRows; i += 256) {
       const int64_t r = seq.spare * kAttnRows + i;
@@ -215,6 +216,7 @@ __global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 128 : 64) ? 2 : 1) vo
     }
     const float norm = finite_norm(halves_sum(squares));
     if (half == 0 && row < rows) b.grad_norm[at] = norm;
+    if (dq == nullptr) return;
 #pragma unroll 8
     for (int j = threadIdx.x; j < most; j += 256)
       most_v = fmaxf(most_v, b.value_norm[(seq.s_off + j) * a.KV + kvh]);
@@ -226,6 +228,8 @@ __global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 128 : 64) ? 2 : 1) vo
     range = range_exponent(2.f * norm * most_v);
     lse -= range;
   }
+
+  if (dq == nullptr) return;  // only what the other kernel needs
 
   const float c2 = a.scale * kLog2e;
   f32x16 acc[DT];
@@ -519,7 +523,7 @@ int attn_backward_launch(AttnBwdArgs& b, hipStream_t stream, const char* what) {
     hipLaunchKernelGGL((attn_backward_q_kernel<T, HD>), dim3((unsigned)(q_tiles * a.KV)), dim3(256), 0, stream, b);
     rc = launch_status(what);
   }
-  if (rc == 0 && a.total_s > 0) {
+  if (rc == 0 && a.total_s > 0 && b.dk != nullptr) {
     hipLaunchKernelGGL((attn_backward_kv_kernel<T, HD>), dim3((unsigned)(s_tiles * a.KV * b.splits)),
                        dim3(kKvThreads), 0, stream, b);
     rc = launch_status(what);
@@ -568,8 +572,10 @@ int v3d_attention_pack_bwd(const void* grad, const void* q, const void* k, const
   if (rc != 0) return rc;
   if (total_q == 0 && total_s == 0) return 0;
   V3D_REQUIRE(strides && (B == 0 || (q_lengths && s_lengths)), what, "null pointer");
-  V3D_REQUIRE(total_q == 0 || (grad && q && out && lse && grad_q), what, "null pointer");
-  V3D_REQUIRE(total_s == 0 || (k && v && grad_k && grad_v), what, "null pointer");
+  V3D_REQUIRE(total_q == 0 || (grad && q && out && lse), what, "null pointer");
+  V3D_REQUIRE(total_s == 0 || (k && v), what, "null pointer");
+  V3D_REQUIRE((grad_k == nullptr) == (grad_v == nullptr), what, "grad_k and grad_v come together");
+  if (grad_q == nullptr && grad_k == nullptr) return 0;
   AttnBwdArgs b{};
   AttnArgs& a = b.f;
   a.q = q;

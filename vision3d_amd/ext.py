@@ -1156,7 +1156,8 @@ def attention_pack_forward(q_feats, k_feats, v_feats, q_lengths, s_lengths, targ
 
 def attention_pack_backward(target_grads, q_feats, k_feats, v_feats, targets, lse, q_lengths, s_lengths, q_grads, k_grads,
                             v_grads, scale, causal, rest=None):
-    """The gradients of ``attention_pack_forward``, from its inputs, ``targets``, ``lse`` and (16-bit types) ``rest``."""
+    """The gradients of ``attention_pack_forward``, from its inputs, ``targets``, ``lse`` and (16-bit types) ``rest``;
+    ``q_grads``, or ``k_grads`` and ``v_grads`` together, may be None (not wanted)."""
     name = "attention_pack_backward"
     _attention_check(name, q_feats, k_feats, v_feats, q_lengths, s_lengths)
     shape, kshape = q_feats.shape, k_feats.shape
@@ -1184,8 +1185,8 @@ def _attention_pack_backward(target_grads, q, k, v, targets, lse, q_lengths, s_l
     dev, stream = _where(q)
     rc = lib.v3d_attention_pack_bwd(target_grads.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), targets.data_ptr(),
                                     _ptr(rest), lse.data_ptr(), q_lengths.data_ptr(), s_lengths.data_ptr(),
-                                    q_grads.data_ptr(), k_grads.data_ptr(), v_grads.data_ptr(), _ELEMENTS[q.dtype], B, N, M,
-                                    H, KV, D, _Strides6(qs[0], qs[1], ks[0], ks[1], vs[0], vs[1]), scale, bool(causal), wp,
+                                    _ptr(q_grads), _ptr(k_grads), _ptr(v_grads), _ELEMENTS[q.dtype], B, N, M, H, KV, D,
+                                    _Strides6(qs[0], qs[1], ks[0], ks[1], vs[0], vs[1]), scale, bool(causal), wp,
                                     wn, dev, stream)
     if rc != 0:
         _lib.check(rc, "attention_pack_backward")

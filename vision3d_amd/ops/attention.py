@@ -65,10 +65,12 @@ class _AttentionPack(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         q, k, v, out, rest, lse, q_lengths, s_lengths = ctx.saved_tensors
-        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+        need_q, need_k, need_v = ctx.needs_input_grad[:3]
+        dq = q.new_empty(q.shape) if need_q else None
+        dk, dv = (k.new_empty(k.shape), v.new_empty(v.shape)) if need_k or need_v else (None, None)
         ext._attention_pack_backward(grad.contiguous(), q, k, v, out, lse, q_lengths, s_lengths, dq, dk, dv, ctx.scale,
                                      ctx.causal, rest)
-        return dq, dk, dv, None, None, None, None
+        return dq, dk if need_k else None, dv if need_v else None, None, None, None, None
 
 
 def attention_pack_mode(q_feats: Tensor, k_feats: Tensor, v_feats: Tensor, q_lengths: Tensor,
