@@ -247,3 +247,32 @@ def test_refusals_without_a_gpu():
     assert lib.v3d_layer_norm_fwd(None, None, None, None, None, None, None, 0, 0, 0, 1, 1e-5, 0, None) == 0
     assert lib.v3d_layer_norm_bwd_workspace_bytes(0, 8) == 0
     assert lib.v3d_layer_norm_bwd_workspace_bytes(10 ** 7, 1000) == 1024 * 1000 * 8
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("channels", [8193, 8200, 12289, 16384])
+def test_widest_rows(dtype, channels):
+    test_forward_and_gradients(dtype, channels)  # 1024 threads, two vectors each
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,channels", [(131072 + 777, 8), (65536 + 9, 200), (8192 + 5, 4099)])
+def test_more_rows_than_workgroups_take_at_once(dtype, rows, channels):
+    # the forward's 8192 workgroups take 16, 8 (4) and 1 rows at a time: the last ones come in a second round
+    x, r, w, b, g = (None if v is None else v.to(DEV) for v in _inputs(rows, channels, dtype, True, seed=rows))
+    y, u, t, rstd, dx, dw, db = _formula(_d(x), _d(r), _d(w), _d(b), 1e-5, _d(g))
+    leaves = [v.requires_grad_(True) for v in (x, w, b)]
+    out = ops.layer_norm(*leaves, residual=r)
+    grads = torch.autograd.grad(out, leaves, g)
+    e, big, half = _unit_error(t, rstd), u.abs().clamp(min=1), _half(dtype)
+    tol = half * y.abs() + e * big * w.detach().double().abs() + 2.0 ** -23 * (y.abs() + b.detach().double().abs()) + 2.0 ** -24
+    assert ((out.detach().double() - y).abs() <= tol).all()
+    gw = (g.double() * w.detach().double()).abs()
+    most = gw.amax(1, keepdim=True) + gw + big * (gw * u.abs()).mean(1, keepdim=True)
+    assert ((grads[0].double() - dx).abs() <= half * dx.abs() + rstd * most * (4 * e * big + 60 * 2.0 ** -24) + 2.0 ** -24).all()
+    steps = (rows + 80) * 2.0 ** -24
+    tol = half * dw.abs() + steps * (g.double() * u).abs().sum(0) + (g.double().abs() * e * big).sum(0) + 2.0 ** -24
+    assert ((grads[1].double() - dw).abs() <= tol).all()
+    assert ((grads[2].double() - db).abs() <= half * db.abs() + steps * g.double().abs().sum(0)).all()

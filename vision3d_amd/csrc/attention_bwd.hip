@@ -501,7 +501,7 @@ __global__ __launch_bounds__(256) void attn_backward_join_kernel(const AttnBwdAr
 // Parts of a key tile's rows: as many as bring about four workgroups to a CU.  One workgroup fills a CU, and a causal tile at
 // the start of a sequence has all the rows behind it (8192 tokens in 5 sequences, 16/4 heads of 128, bf16: 1 / 2 / 3 parts
 // 468 / 269 / 263 us, and 13 / 18 us to join the parts; 8000 tokens, 4 heads of 64, fp32: 145 / 118 + 11 us).
-inline int attn_backward_splits(int B, int64_t total_s, int KV) {
+int attn_backward_splits(int B, int64_t total_s, int KV) {
   const int64_t groups = std::max<int64_t>((ceil_div(total_s, kAttnRows) + B) * KV, 1);
   return (int)std::max<int64_t>(1, std::min<int64_t>(1024 / groups, 8));
 }
