@@ -43,13 +43,13 @@ __device__ __forceinline__ float prob_weight(float m, float to, float c2) {
 }
 
 // What a wave carries through its keys: 32 rows, one per lane and half.
-template <typename T, int HD>
+template <typename T, int HD, bool AGAIN>
 struct AttnWave {
   typedef typename Kind<T>::U U;
   static constexpr int HDP = attn_pow2(HD);
   static constexpr int STEPS = HD / 16;  // product steps over the head size
   static constexpr int DT = HD / 32;
-  static constexpr bool kAgain = Kind<T>::P == 3 && HD > 192;  // at 192 they fit: 8 x 500 tokens 165 us, 182 us with it
+  static constexpr bool kAgain = AGAIN;  // see again()
 
   Held<T, HD> q;
   f32x16 o[DT];
@@ -88,16 +88,18 @@ struct AttnWave {
   __device__ __forceinline__ void scores(const U* k, const U* rows, int key0, f32x16 (&s)[NT]) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) s[n] = zero16();
+    if constexpr (!kTile) q.begin();
+    const int at = again<kAgain>(lane) & 31;
 #pragma unroll
     for (int st = 0; st < STEPS; ++st) {
       Op<T> qs;
       if constexpr (kTile)
-        qs = read_cols<T, HDP, 32>(rows, again<kAgain>(lane & 31), st, half);
+        qs = read_cols<T, HDP, 32>(rows, at, st, half);
       else
-        qs = q.get(st, half, D);
+        qs = q.get(st);
 #pragma unroll
       for (int n = 0; n < NT; ++n)
-        s[n] = product<T>(read_cols<T, HDP, 32 * NT>(k, again<kAgain>(n * 32 + (lane & 31)), st, half), qs, s[n]);
+        s[n] = product<T>(read_cols<T, HDP, 32 * NT>(k, n * 32 + at, st, half), qs, s[n]);
     }
     if (key0 + 32 * NT > least) {
 #pragma unroll
@@ -153,9 +155,10 @@ struct AttnWave {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const Op<T> p = pack_rows<T>(s[n], u);
+        const int at = again<kAgain>(lane) & 63;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
-          o[d] = product<T>(read_rows<T, HDP, 32 * NT>(v, n * 32, u, d * 32, again<kAgain>(lane)), p, o[d]);
+          o[d] = product<T>(read_rows<T, HDP, 32 * NT>(v, n * 32, u, d * 32, at), p, o[d]);
       }
   }
 
@@ -267,7 +270,7 @@ __global__ __launch_bounds__(256, (attn_occupancy<T, HD>())) void attn_forward_k
   const int rows = seq.q_len * a.G;
   const int row0 = seq.tile * kAttnRows;
   if (row0 >= rows) return;  // lengths that overrun the total were cut
-  AttnWave<T, HD> w;
+  AttnWave<T, HD, false> w;
   w.begin(a, seq, kvh, row0 + wave * 32, rows, true);
   // the workgroup's first and last rows bound what it has to look at
   const int most = attn_limit(a, seq, div_g(a, min(row0 + kAttnRows - 1, rows - 1)));
@@ -358,11 +361,12 @@ __global__ __launch_bounds__(256, (attn_occupancy<T, HD>())) void attn_forward_k
 // Bound: the bytes of the keys and values.  A wave fetches its own tiles of 32 keys into its own part of LDS, so there is no
 // barrier in the loop and each wave keeps a tile of keys and one of values in flight; keys and values take turns in one
 // place (a wave's LDS accesses happen in order).  The waves' sums meet in LDS at the end.
-// With large heads the rows stand in LDS, one tile for all waves, and only one of keys and values is on its way at a time, or
-// registers spill (135 with bf16 heads of 256, 604 with fp32 ones).  8 heads, one token, 16 caches of up to 8192 rows: bf16
-// heads of 256 605 -> 130 us (4.9 TB/s), of 192 114 -> 109 us; fp32, up to 4096 rows, of 128 104 -> 94 us (4.0 TB/s), of 256
-// 1571 -> 670 us with the addresses computed where they are used (1272 us without; 38 registers still spill); fp32 heads of
-// 192 on one key head, five tokens: 210 -> 79 us.  Smaller heads have the registers to keep both on their way.
+// With large heads the rows stand in LDS, one tile for all waves, and only one of keys and values is on its way at a time, of
+// fp32 heads past 128 only half a tile, or registers spill (135 with bf16 heads of 256, 604 with fp32 ones).  8 heads, one token,
+// 16 caches of up to 8192 rows: bf16 heads of 256 605 -> 130 us (4.9 TB/s), of 192 114 -> 109 us; fp32, up to 4096 rows, of 128
+// 104 -> 94 us (4.0 TB/s), of 256 670 us with whole tiles, 522 with halves, 430 with the threads' columns fixed (1.2 TB/s: bound by
+// the splitting into thirds); fp32 heads of 192 on one key head, five tokens: 210 -> 77 us.  Smaller heads have the registers to
+// keep both on their way.
 template <typename T, int HD>
 constexpr int few_waves() { return Kind<T>::P == 3 && HD > 128 ? 2 : 4; }
 template <typename T, int HD>
@@ -395,7 +399,7 @@ __global__ __launch_bounds__((64 * few_waves<T, HD>())) void attn_few_rows_kerne
   const int rows = seq.q_len * a.G;
   const int row0 = seq.tile * 32;
   if (row0 >= rows) return;
-  AttnWave<T, HD> w;
+  AttnWave<T, HD, (Kind<T>::P == 3 && HD > 192)> w;
   w.begin(a, seq, kvh, row0, rows, !kLarge);
   if constexpr (kLarge) {
     TileStage<T, HD, 32, 64 * W> stage;
@@ -414,13 +418,15 @@ __global__ __launch_bounds__((64 * few_waves<T, HD>())) void attn_few_rows_kerne
   const T* v = static_cast<const T*>(a.v) + seq.b * a.v_batch + seq.s_off * a.v_row + (int64_t)kvh * a.v_head;
   U* tile = reinterpret_cast<U*>(lds) + wave * SIZE;
 
-  TileStage<T, HD, 32, 64> stage_k, stage_own;
-  auto& stage_v = [&]() -> TileStage<T, HD, 32, 64>& {
+  constexpr bool kHalf = Kind<T>::P == 3 && HD > 128;
+  constexpr int SR = kHalf ? 16 : 32;
+  TileStage<T, HD, SR, 64, 32> stage_k, stage_own;
+  auto& stage_v = [&]() -> TileStage<T, HD, SR, 64, 32>& {
     if constexpr (kLarge) return stage_k;
     else return stage_own;
   }();
-  auto fetch_k = [&](int t) { stage_k.fetch(k + (int64_t)t * 32 * a.k_row, a.k_row, a.D, seq.s_len - t * 32); };
-  auto fetch_v = [&](int t) { stage_v.fetch(v + (int64_t)t * 32 * a.v_row, a.v_row, a.D, seq.s_len - t * 32); };
+  auto fetch_k = [&](int t, int r = 0) { stage_k.fetch(k + (int64_t)(t * 32 + r) * a.k_row, a.k_row, a.D, seq.s_len - t * 32 - r); };
+  auto fetch_v = [&](int t, int r = 0) { stage_v.fetch(v + (int64_t)(t * 32 + r) * a.v_row, a.v_row, a.D, seq.s_len - t * 32 - r); };
   int t = __builtin_amdgcn_readfirstlane(split * per_split + wave);
   if (t < t_end) {
     fetch_k(t);
@@ -431,6 +437,10 @@ __global__ __launch_bounds__((64 * few_waves<T, HD>())) void attn_few_rows_kerne
     f32x16 s[1];
     wave_order();
     stage_k.store(tile, a.D);
+    if constexpr (kHalf) {
+      fetch_k(t, 16);
+      stage_k.store(tile + 16 * HDP, a.D);
+    }
     if (kLarge)
       fetch_v(t);
     else if (t + W < t_end)
@@ -439,8 +449,15 @@ __global__ __launch_bounds__((64 * few_waves<T, HD>())) void attn_few_rows_kerne
     w.template scores<1, kLarge>(tile, lds_q, key0, s);
     wave_order();
     stage_v.store(tile, a.D);
+    const bool partly = key0 + 32 > w.least;
+    bool bad = partly && stage_v.nonfinite();
+    if constexpr (kHalf) {
+      fetch_v(t, 16);
+      stage_v.store(tile + 16 * HDP, a.D);
+      if (partly) bad |= stage_v.nonfinite();
+    }
     wave_order();
-    if (key0 + 32 > w.least && __any(stage_v.nonfinite())) {
+    if (partly && __any(bad)) {
       w.template add_nonfinite<1>(lds_p[wave], tile, key0, s);
       wave_order();
       clear_nonfinite(tile, SIZE, threadIdx.x & 63, 64);

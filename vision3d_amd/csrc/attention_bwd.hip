@@ -130,7 +130,7 @@ __global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 128 : 64) ? 2 : 1) vo
   constexpr int NT = BN / 32;
   constexpr int BUFS = bwd_buffers<T, HD>();
   constexpr int STEPS = HD / 16;
-  constexpr bool kAgain = Kind<T>::P == 3 && HD > 128;  // see again()
+  constexpr bool kAgain = Kind<T>::P == 3 && HD > 192;  // see again()
   constexpr int DT = HD / 32;
   typedef typename Kind<T>::U U;
   __shared__ __attribute__((aligned(16))) U lds_k[BUFS][Kind<T>::P * BN * HDP];
@@ -193,9 +193,11 @@ __global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 128 : 64) ? 2 : 1) vo
   auto add_delta = [&](const void* out) {
     Held<T, HD> of;
     of.load(static_cast<const T*>(out) + at0, at_row, half, a.D, true);
+    gf.begin();
+    of.begin();
 #pragma unroll
     for (int st = 0; st < STEPS; ++st) {
-      const Op<T> gs = gf.get(st, half, a.D), os = of.get(st, half, a.D);
+      const Op<T> gs = gf.get(st), os = of.get(st);
 #pragma unroll
       for (int j = 0; j < 8; ++j) delta = fmaf(number(gs, j), number(os, j), delta);
     }
@@ -208,9 +210,10 @@ __global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 128 : 64) ? 2 : 1) vo
   float range = 0.f;  // log2 of what ds is multiplied by: in the exponent, no instruction more
   if constexpr (kFp16<T>) {
     float squares = 0.f, most_v = 0.f;
+    gf.begin();
 #pragma unroll
     for (int st = 0; st < STEPS; ++st) {
-      const Op<T> gs = gf.get(st, half, a.D);
+      const Op<T> gs = gf.get(st);
 #pragma unroll
       for (int j = 0; j < 8; ++j) squares = fmaf(number(gs, j), number(gs, j), squares);
     }
@@ -243,10 +246,13 @@ __global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 128 : 64) ? 2 : 1) vo
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       f32x16 s = zero16(), dp = zero16();
+      qf.begin();
+      gf.begin();
+      const int cols = again<kAgain>(lane) & 31;
 #pragma unroll
       for (int st = 0; st < STEPS; ++st) {
-        s = product<T>(read_cols<T, HDP, BN>(lds_k[buf], again<kAgain>(n * 32 + (lane & 31)), st, half), qf.get(st, half, a.D), s);
-        dp = product<T>(read_cols<T, HDP, BN>(lds_v[buf], again<kAgain>(n * 32 + (lane & 31)), st, half), gf.get(st, half, a.D), dp);
+        s = product<T>(read_cols<T, HDP, BN>(lds_k[buf], n * 32 + cols, st, half), qf.get(st), s);
+        dp = product<T>(read_cols<T, HDP, BN>(lds_v[buf], n * 32 + cols, st, half), gf.get(st), dp);
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = exp2_fast(fmaf(s[r], c2, -lse)) * (dp[r] - delta);
@@ -258,9 +264,10 @@ __global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 128 : 64) ? 2 : 1) vo
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const Op<T> ds = pack_rows<T>(s, u);
+        const int at = again<kAgain>(lane) & 63;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
-          acc[d] = product<T>(read_rows<T, HDP, BN>(lds_k[buf], n * 32, u, d * 32, again<kAgain>(lane)), ds, acc[d]);
+          acc[d] = product<T>(read_rows<T, HDP, BN>(lds_k[buf], n * 32, u, d * 32, at), ds, acc[d]);
       }
     }
   };
@@ -287,7 +294,7 @@ __global__ __launch_bounds__(kKvThreads, HD <= 32 ? 2 : 1) void attn_backward_kv
   constexpr int NT = BM / 32;
   constexpr int BUFS = bwd_buffers<T, HD>();
   constexpr int STEPS = HD / 16;
-  constexpr bool kAgain = Kind<T>::P == 3 && HD > 128;  // see again()
+  constexpr bool kAgain = Kind<T>::P == 3 && HD > 192;  // see again()
   constexpr int DT = HD / 32;
   constexpr int GROUPS = kv_groups<T, HD>(), KEYS = 32 * GROUPS, THREADS = kKvThreads;
   constexpr bool kRoles = kv_roles<T, HD>();
@@ -415,15 +422,18 @@ __global__ __launch_bounds__(kKvThreads, HD <= 32 ? 2 : 1) void attn_backward_kv
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       f32x16 s = zero16();
+      kf.begin();
+      if (keys_role) vf.begin();
+      const int cols = again<kAgain>(lane) & 31;
 #pragma unroll
       for (int st = 0; st < STEPS; ++st)
-        s = product<T>(read_cols<T, HDP, BM>(lds_q[buf], again<kAgain>(n * 32 + (lane & 31)), st, half), kf.get(st, half, a.D), s);
+        s = product<T>(read_cols<T, HDP, BM>(lds_q[buf], n * 32 + cols, st, half), kf.get(st), s);
       f32x16 p;
       if (keys_role) {
         f32x16 dp = zero16();
 #pragma unroll
         for (int st = 0; st < STEPS; ++st)
-          dp = product<T>(read_cols<T, HDP, BM>(lds_g[buf], again<kAgain>(n * 32 + (lane & 31)), st, half), vf.get(st, half, a.D), dp);
+          dp = product<T>(read_cols<T, HDP, BM>(lds_g[buf], n * 32 + cols, st, half), vf.get(st), dp);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int i = n * 32 + acc_row(r, half);
@@ -441,16 +451,17 @@ __global__ __launch_bounds__(kKvThreads, HD <= 32 ? 2 : 1) void attn_backward_kv
       }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
+        const int at = again<kAgain>(lane) & 63;
         if constexpr (!kRoles) {
           const Op<T> y = pack_rows<T>(p, u);
 #pragma unroll
           for (int d = 0; d < DT; ++d)
-            other[d] = product<T>(read_rows<T, HDP, BM>(lds_g[buf], n * 32, u, d * 32, again<kAgain>(lane)), y, other[d]);
+            other[d] = product<T>(read_rows<T, HDP, BM>(lds_g[buf], n * 32, u, d * 32, at), y, other[d]);
         }
         const Op<T> x = pack_rows<T>(s, u);
 #pragma unroll
         for (int d = 0; d < DT; ++d)
-          acc[d] = product<T>(read_rows<T, HDP, BM>(summed, n * 32, u, d * 32, again<kAgain>(lane)), x, acc[d]);
+          acc[d] = product<T>(read_rows<T, HDP, BM>(summed, n * 32, u, d * 32, at), x, acc[d]);
       }
     }
   };

@@ -419,29 +419,53 @@ __device__ __forceinline__ void load_ops(Op<T> (&op)[STEPS], const T* base, int 
   for (int st = 0; st < STEPS; ++st) op[st] = raw[st].op(st * 16 + 8 * half, D);
 }
 
-// The operands of all product steps over the head size that a wave keeps for its loop.  fp32 heads past 128 are kept as
-// they come from memory, 8 registers a step instead of 12, and split where they are used: beside the sums there is no room.
+// `x`, such that what is computed from it is computed again in every turn of a loop (kAgain).  The compiler otherwise computes
+// the LDS addresses of a tile once, before the loop, and keeps them all: with fp32 heads past 192 that is more registers than
+// are left, and an address read back from memory costs more than its few instructions (where `x` is masked afterwards, so that
+// its range is known: 134 -> 80 instructions a chunk).
+template <bool kAgain>
+__device__ __forceinline__ int again(int x) {
+  if constexpr (kAgain) asm volatile("" : "+v"(x));
+  return x;
+}
+
+// The operands of all product steps over the head size that a wave uses in its loop: kept in registers, but fp32 heads past 128
+// are read again from the cache where they are used, kAhead steps ahead, and split there: beside the sums there is no room (48 to
+// 173 registers spilled).  Training in fp32, 8 heads, 8 sequences of 500 tokens: heads of 256 2405 -> 1415 us, of 160 1155 -> 1016;
+// 1, 3, 4 and 8 steps ahead 1590, 1560, 1590 and 1690 for 1545 us (before the addresses of `again`).
 template <typename T, int HD>
 struct Held {
   static constexpr int STEPS = HD / 16;
+  static constexpr int kAhead = 2;
   static constexpr bool kLate = Kind<T>::P == 3 && HD > 128;
   Op<T> ops[kLate ? 1 : STEPS];
-  Raw<T> raw[kLate ? STEPS : 1];
+  Raw<T> raw[kLate ? kAhead : 1];
+  const T* base;
+  int at, half, D;
+  bool there;
 
-  __device__ __forceinline__ void load(const T* base, int at, int half, int D, bool there) {
+  __device__ __forceinline__ void load(const T* from, int row, int h, int d, bool in) {
+    base = from;
+    at = row;
+    half = h;
+    D = d;
+    there = in;
+    if constexpr (!kLate) load_ops<T>(ops, from, row, half, D, in);
+  }
+  // Before the steps of a turn of the loop.
+  __device__ __forceinline__ void begin() {
     if constexpr (kLate) {
+      at = again<true>(at);
 #pragma unroll
-      for (int st = 0; st < STEPS; ++st) raw[st].load(base, kOutOfRange, at, st * 16 + 8 * half, D, there);
-    } else {
-      load_ops<T>(ops, base, at, half, D, there);
+      for (int st = 0; st < kAhead; ++st) raw[st].load(base, kOutOfRange, at, st * 16 + 8 * half, D, there);
     }
   }
-  __device__ __forceinline__ Op<T> get(int st, int half, int D) const {
+  // The operand of step st, in order.
+  __device__ __forceinline__ Op<T> get(int st) {
     if constexpr (kLate) {
-      Raw<T> r = raw[st];
-#pragma unroll
-      for (int l = 0; l < Raw<T>::L; ++l) asm volatile("" : "+v"(r.c[l]));  // or the split moves out of the loop again
-      return r.op(st * 16 + 8 * half, D);
+      const Op<T> op = raw[st % kAhead].op(st * 16 + 8 * half, D);
+      if (st + kAhead < STEPS) raw[st % kAhead].load(base, kOutOfRange, at, (st + kAhead) * 16 + 8 * half, D, there);
+      return op;
     } else {
       return ops[st];
     }
@@ -461,17 +485,6 @@ __device__ __forceinline__ int place(int row, int chunk) {
   return chunk ^ ((row >> 2) & 3);
 }
 
-// `x`, such that what is computed from it is computed again in every turn of a loop (kAgain).  The compiler otherwise computes
-// the LDS addresses of a tile once, before the loop, and keeps them all: with fp32 heads past 128 that is more registers than
-// are left, and an address read back from memory costs more than its few instructions.  Training in fp32, 8 sequences of
-// 500 tokens, this and Held together: 8 / 2 heads of 192, causal, 937 -> 770 us (828 us with Held alone), 8 heads of 256
-// 2690 -> 2400 us.
-template <bool kAgain>
-__device__ __forceinline__ int again(int x) {
-  if constexpr (kAgain) asm volatile("" : "+v"(x));
-  return x;
-}
-
 // Offset of element `col` of `row` in a plane.
 template <int HDP>
 __device__ __forceinline__ int tile_at(int row, int col) {
@@ -479,7 +492,7 @@ __device__ __forceinline__ int tile_at(int row, int col) {
 }
 
 // A tile on its way from memory to LDS in the registers of THREADS threads.
-template <typename T, int HD, int ROWS, int THREADS>
+template <typename T, int HD, int ROWS, int THREADS, int PLANE = ROWS>  // PLANE: rows of a plane of the tile
 struct TileStage {
   typedef typename Kind<T>::U U;
   static constexpr int CPR = HD / 8;                // chunks of a row
@@ -488,9 +501,13 @@ struct TileStage {
   Raw<T> c[CH];
 
   static constexpr bool kTight = Kind<T>::P == 3 && HD > 192;  // registers are short
-  static __device__ __forceinline__ int index(int i) { return i * THREADS + again<kTight>((int)threadIdx.x % THREADS); }
-  static __device__ __forceinline__ int row_of(int i) { return kEven ? index(i) / CPR : min(index(i) / CPR, ROWS - 1); }
-  static __device__ __forceinline__ int col_of(int i) { return index(i) % CPR * 8; }
+  static constexpr bool kFixed = THREADS % CPR == 0;          // a thread stays with one column
+  static __device__ __forceinline__ int thread() { return again<kTight>((int)threadIdx.x) & (THREADS - 1); }
+  static __device__ __forceinline__ int row_of(int i) {
+    const int row = kFixed ? i * (THREADS / CPR) + thread() / CPR : (i * THREADS + thread()) / CPR;
+    return kEven ? row : min(row, ROWS - 1);
+  }
+  static __device__ __forceinline__ int col_of(int i) { return (kFixed ? thread() : i * THREADS + thread()) % CPR * 8; }
 
   // Rows [0, count) at `base`, `stride` elements apart (a tile spans less than 2^31 bytes); count <= 0: nothing is read.
   __device__ __forceinline__ void fetch(const T* base, int64_t stride, int D, int count) {
@@ -512,7 +529,7 @@ struct TileStage {
       const Op<T> op = c[i].op(col_of(i), D);
 #pragma unroll
       for (int p = 0; p < Kind<T>::P; ++p)
-        *reinterpret_cast<typename Vec8<U>::type*>(tile + p * (ROWS * HDP) + tile_at<HDP>(row_of(i), col_of(i))) = op.part[p];
+        *reinterpret_cast<typename Vec8<U>::type*>(tile + p * (PLANE * HDP) + tile_at<HDP>(row_of(i), col_of(i))) = op.part[p];
     }
   }
   __device__ __forceinline__ bool nonfinite() const {
