@@ -494,9 +494,10 @@ int v3d_attention_pack_bwd(const void* grad, const void* q, const void* k, const
                            int D, const int64_t* strides, float scale, int causal, void* workspace,
                            size_t workspace_bytes, int device, void* stream);
 /* What the calls above do with a pack of these sizes (each pointer may be NULL): the rows of a tile of the forward (32: the waves
- * of a workgroup divide the keys; 128), the parts that its keys are divided into, and the backward's parts of a key tile's rows. */
-int v3d_attention_pack_plan(int B, int64_t total_q, int64_t total_s, int H, int KV, int D, int* row_tile, int* key_parts,
-                            int* row_parts);
+ * of a workgroup divide the keys; 128) and the parts that its keys are divided into; the backward's parts of a row tile's keys
+ * (dq) and of a key tile's rows (dk, dv). */
+int v3d_attention_pack_plan(int dtype, int B, int64_t total_q, int64_t total_s, int H, int KV, int D, int* row_tile,
+                            int* key_parts, int* grad_key_parts, int* grad_row_parts);
 size_t v3d_cached_attention_workspace_bytes(int B, int tokens, int64_t capacity, int H, int KV, int D);
 int v3d_cached_attention(const void* q, const void* k_cache, const void* v_cache, const int64_t* lengths, void* out,
                          int dtype, int B, int tokens, int64_t capacity, int H, int KV, int D, const int64_t* strides,

@@ -16,13 +16,13 @@ def _half(dtype):
     return torch.finfo(dtype).eps / 2
 
 
-def _plan(lengths, keys, heads, kv, dim, spare=0):
-    """(rows of a forward tile, parts of its keys, parts of a backward key tile's rows)."""
-    out = [ctypes.c_int() for _ in range(3)]
-    rc = _lib.lib().v3d_attention_pack_plan(len(lengths), sum(lengths) + spare, sum(keys) + spare, heads, kv, dim,
-                                            *(ctypes.byref(x) for x in out))
+def _plan(lengths, keys, heads, kv, dim, spare=0, dtype=torch.float32):
+    """(rows of a forward tile, parts of its keys, parts of a backward key tile's rows, parts of a backward row tile's keys)."""
+    out = [ctypes.c_int() for _ in range(4)]
+    rc = _lib.lib().v3d_attention_pack_plan(TYPES.index(dtype), len(lengths), sum(lengths) + spare, sum(keys) + spare, heads, kv,
+                                            dim, *(ctypes.byref(x) for x in out))
     assert rc == 0
-    return tuple(x.value for x in out)
+    return out[0].value, out[1].value, out[3].value, out[2].value
 
 
 def _rows(lengths):
@@ -244,11 +244,64 @@ def test_gradients_of_long_packs(dtype, dim, causal):
     # 128-row tiles forward, whole key tiles of eight heads backward, up to 64 sequences (causal: numbered by work)
     lengths = [700, 1, 0, 900, 257, 400, 33, 128, 810, 1300, 640, 1000, 1024, 901, 100]
     keys = lengths[::-1]
-    assert _plan(lengths, keys, 8, 8, dim) == (128, 1, 1)
+    assert _plan(lengths, keys, 8, 8, dim) == (128, 1, 1, 1)
     _gradients(dtype, lengths, keys, 8, 8, dim, causal, seed=dim)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dim", [32, 64, 80, 128, 192, 256])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gradients_of_divided_row_tiles(dtype, dim, causal):
+    # few queries, many keys: the keys of a row tile are divided; the short sequence's later parts have none, the last has no keys
+    lengths, keys = [140, 70, 1, 0, 200], [2900, 1500, 700, 40, 0]
+    assert _plan(lengths, keys, 4, 2, dim, 30, dtype)[3] == (8 if dtype == torch.float32 else 2)
+    _gradients(dtype, lengths, keys, 4, 2, dim, causal, seed=dim, spare=30)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_replays_of_divided_tiles(dtype):
+    # every kernel of a training step under capture: the table, the norms, both divided gradients and their joins
+    from vision3d_amd import ext
+
+    lengths, keys = [2] * 260, [5] * 259 + [160000 // 260 * 260 - 5 * 259]
+    q, k, v, g = _inputs(lengths, keys, 2, 1, 64, dtype, 4)
+    assert _plan(lengths, keys, 2, 1, 64, 0, dtype)[2] == 1
+    few = [60, 50], [1500, 1400]
+    q2, k2, v2, g2 = _inputs(*few, 2, 1, 64, dtype, 5)
+    plan = _plan(*few, 2, 1, 64, 0, dtype)
+    assert plan[2] > 1 and plan[3] > 1
+    args, args2 = _tensors(lengths, keys), _tensors(*few)
+    outs = [[torch.empty_like(t) for t in (a, a, b, c)] + [torch.empty(a.shape[:2], device=DEV)] for a, b, c in ((q, k, v), (q2, k2, v2))]
+
+    def step():
+        for (a, b, c, d, n), (out, dq, dk, dv, lse) in zip(((q, k, v, g, args), (q2, k2, v2, g2, args2)), outs):
+            ext.attention_pack_forward(a, b, c, *n, out, lse, 0.125, True)
+            ext.attention_pack_backward(d, a, b, c, out, lse, *n, dq, dk, dv, 0.125, True)
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for n in range(4):
+        q.mul_(1.1), g2.mul_(0.5)
+        args[1][7] += 3  # the lengths are device data: a replay follows them
+        args[1][-1] -= 3
+        step()
+        torch.cuda.synchronize()
+        eager = [t.clone() for o in outs for t in o]
+        for o in outs:
+            for t in o:
+                t.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(eager, (t for o in outs for t in o)):
+            assert torch.equal(a, b), n
+
+
 def test_the_plan_refuses_what_is_no_pack():
-    plan = _lib.lib().v3d_attention_pack_plan
-    assert plan(1, 10, 10, 4, 2, 64, None, None, None) == 0
-    assert plan(1, 10, 10, 4, 3, 64, None, None, None) == -1 and plan(-1, 10, 10, 4, 2, 64, None, None, None) == -1
+    plan, none = _lib.lib().v3d_attention_pack_plan, [None] * 4
+    assert plan(0, 1, 10, 10, 4, 2, 64, *none) == 0
+    assert plan(0, 1, 10, 10, 4, 3, 64, *none) == -1 and plan(0, -1, 10, 10, 4, 2, 64, *none) == -1
+    assert plan(3, 1, 10, 10, 4, 2, 64, *none) == -1 and plan(0, 1, 10, 10, 4, 2, 257, *none) == -4

@@ -124,7 +124,8 @@ SIGNATURES = {
     "v3d_layer_norm_fwd": (_c_int, [_c_ptr] * 7 + [_c_int, _c_int, _c_i64, _c_i64, _c_f32] + _TAIL),
     "v3d_layer_norm_bwd_workspace_bytes": (_c_size, [_c_i64, _c_i64]),
     "v3d_attention_pack_workspace_bytes": (_c_size, [_c_int, _c_i64, _c_i64, _c_int, _c_int, _c_int]),
-    "v3d_attention_pack_plan": (_c_int, [_c_int, _c_i64, _c_i64, _c_int, _c_int, _c_int] + [ctypes.POINTER(_c_int)] * 3),
+    "v3d_attention_pack_plan": (
+        _c_int, [_c_int, _c_int, _c_i64, _c_i64, _c_int, _c_int, _c_int] + [ctypes.POINTER(_c_int)] * 4),
     "v3d_attention_pack_fwd": (
         _c_int, [_c_ptr] * 8 + [_c_int, _c_int, _c_i64, _c_i64, _c_int, _c_int, _c_int, ctypes.POINTER(_c_i64), _c_f32,
                                 _c_int] + _WS + _TAIL),

@@ -774,15 +774,16 @@ size_t v3d_attention_pack_workspace_bytes(int B, int64_t total_q, int64_t total_
   return v3d::attn_plan(B, total_q, total_s, 0, KV, H / KV, D).bytes;
 }
 
-int v3d_attention_pack_plan(int B, int64_t total_q, int64_t total_s, int H, int KV, int D, int* row_tile, int* key_parts,
-                            int* row_parts) {
+int v3d_attention_pack_plan(int dtype, int B, int64_t total_q, int64_t total_s, int H, int KV, int D, int* row_tile,
+                            int* key_parts, int* grad_key_parts, int* grad_row_parts) {
   using namespace v3d;
-  const char* what = "attention_pack_plan";
-  V3D_REQUIRE(B >= 0 && total_q >= 0 && total_s >= 0 && H >= 1 && KV >= 1 && H % KV == 0 && D >= 1, what, "bad shape");
+  const int rc = attn_check("attention_pack_plan", dtype, B, total_q, total_s, H, KV, D, 1.f);
+  if (rc != 0) return rc;
   const AttnPlan plan = attn_plan(B, total_q, total_s, 0, KV, H / KV, D);
   if (row_tile != nullptr) *row_tile = plan.tile();
   if (key_parts != nullptr) *key_parts = plan.splits;
-  if (row_parts != nullptr) *row_parts = attn_backward_splits(B, total_s, KV);
+  if (grad_key_parts != nullptr) *grad_key_parts = attn_backward_q_splits(dtype, B, total_q, total_s, KV, H / KV);
+  if (grad_row_parts != nullptr) *grad_row_parts = attn_backward_splits(B, total_s, KV, D);
   return 0;
 }
 

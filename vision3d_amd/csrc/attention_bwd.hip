@@ -21,6 +21,8 @@ struct AttnBwdArgs {
   AttnArgs f;          // q, k, v, out, lse and the geometry of the forward (never a cache)
   const void* grad;    // (total_q, H, D) contiguous
   float* delta;        // (total_q, H): written by the dq kernel, read by the dk / dv kernel
+  int q_splits;        // parts that the keys of a row tile are divided into
+  float* part_q;       // q_splits > 1: (q_splits, total_q, H, D) sums of the parts
   int splits;          // parts that the rows of a key tile are divided into
   float* part;         // splits > 1: (splits, 2, total_s, KV, D) sums of the parts, dk's and dv's
   float* grad_norm;    // fp16: (total_q, H) 2-norms of the rows of grad, written by the dq kernel ...
@@ -142,8 +144,10 @@ __global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 128 : 64) ? 2 : 1) vo
   int64_t id = blockIdx.x;
   const int kvh = (int)(id % a.KV);
   id /= a.KV;
-  const AttnSeq seq = locate_rows<kAttnRows>(a, id);
+  const int split = (int)(id % b.q_splits);
+  const AttnSeq seq = locate_rows<kAttnRows>(a, id / b.q_splits);
   T* dq = static_cast<T*>(b.dq);
+  float* pq = b.part_q + split * (a.total_q * a.H * a.D);
   if (!seq.found) {  // rows behind the last sequence have no gradient
     if (dq == nullptr) return;
     const int64_t rows = (a.total_q - seq.q_end) * a.G;
@@ -151,7 +155,12 @@ __global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 128 : 64) ? 2 : 1) vo
       const int64_t r = seq.spare * kAttnRows + i;
       if (r >= rows) break;
       const int64_t at = (seq.q_end + r / a.G) * a.H + (int64_t)kvh * a.G + r % a.G;
-      for (int d = 0; d < a.D; ++d) dq[at * a.D + d] = (T)0.f;
+      for (int64_t d = at * a.D; d < (at + 1) * a.D; ++d) {
+        if (b.q_splits == 1)
+          dq[d] = (T)0.f;
+        else
+          pq[d] = 0.f;
+      }
     }
     return;
   }
@@ -166,6 +175,8 @@ __global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 128 : 64) ? 2 : 1) vo
   const int wave_most =
       row0 + wave * 32 < rows ? attn_limit(a, seq, div_g(a, min(row0 + wave * 32 + 31, rows - 1))) : 0;
   const int most = attn_limit(a, seq, div_g(a, min(row0 + kAttnRows - 1, rows - 1)));
+  const int tiles = (most + BN - 1) / BN, per_split = (tiles + b.q_splits - 1) / b.q_splits;
+  const int t_begin = split * per_split, t_end = min(tiles, t_begin + per_split);
 
   const int token0 = div_g(a, row0);
   const T* q = static_cast<const T*>(a.q) + (seq.q_off + token0) * a.q_row + (int64_t)kvh * a.G * a.q_head;
@@ -177,8 +188,9 @@ __global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 128 : 64) ? 2 : 1) vo
 
   TileStage<T, HD, BN, 256> stage_k[BUFS], stage_v[BUFS];
   auto fetch = [&](int t, auto to) {
-    stage_k[decltype(to)::value].fetch(k + (int64_t)t * BN * a.k_row, a.k_row, a.D, seq.s_len - t * BN);
-    stage_v[decltype(to)::value].fetch(v + (int64_t)t * BN * a.v_row, a.v_row, a.D, seq.s_len - t * BN);
+    const int key0 = (t_begin + t) * BN;
+    stage_k[decltype(to)::value].fetch(k + (int64_t)key0 * a.k_row, a.k_row, a.D, seq.s_len - key0);
+    stage_v[decltype(to)::value].fetch(v + (int64_t)key0 * a.v_row, a.v_row, a.D, seq.s_len - key0);
   };
   auto place_tile = [&](auto from) {
     stage_k[decltype(from)::value].store(lds_k[decltype(from)::value], a.D);
@@ -206,7 +218,7 @@ __global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 128 : 64) ? 2 : 1) vo
   if (a.rest != nullptr) add_delta(a.rest);
   delta = halves_sum(delta);
   float lse = a.lse[at];
-  if (half == 0 && row < rows) b.delta[at] = delta;
+  if (split == 0 && half == 0 && row < rows) b.delta[at] = delta;
   float range = 0.f;  // log2 of what ds is multiplied by: in the exponent, no instruction more
   if constexpr (kFp16<T>) {
     float squares = 0.f, most_v = 0.f;
@@ -218,7 +230,7 @@ __global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 128 : 64) ? 2 : 1) vo
       for (int j = 0; j < 8; ++j) squares = fmaf(number(gs, j), number(gs, j), squares);
     }
     const float norm = finite_norm(halves_sum(squares));
-    if (half == 0 && row < rows) b.grad_norm[at] = norm;
+    if (split == 0 && half == 0 && row < rows) b.grad_norm[at] = norm;
     if (dq == nullptr) return;
 #pragma unroll 8
     for (int j = threadIdx.x; j < most; j += 256)
@@ -241,7 +253,7 @@ __global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 128 : 64) ? 2 : 1) vo
 
   auto work = [&](int t, auto buffer) {
     constexpr int buf = decltype(buffer)::value;
-    const int key0 = t * BN;
+    const int key0 = (t_begin + t) * BN;
     if (key0 >= wave_most) return;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -272,8 +284,12 @@ __global__ __launch_bounds__(256, HD <= (Kind<T>::P == 1 ? 128 : 64) ? 2 : 1) vo
     }
   };
 
-  pass_tiles<BUFS>((most + BN - 1) / BN, fetch, place_tile, work);
-  if (row < rows) store_rows<T, DT>(dq + at * a.D, acc, a.scale * exp2_fast(-range), a.D, half);
+  pass_tiles<BUFS>(t_end - t_begin, fetch, place_tile, work);
+  if (row >= rows) return;
+  if (b.q_splits == 1)
+    store_rows<T, DT>(dq + at * a.D, acc, a.scale * exp2_fast(-range), a.D, half);
+  else
+    store_rows<float, DT>(pq + at * a.D, acc, a.scale * exp2_fast(-range), a.D, half);
 }
 
 // dk and dv of a tile of 32 GROUPS keys.  A wave keeps 32 keys: their operands and both sums, 320 registers with 16-bit heads
@@ -482,19 +498,20 @@ __global__ __launch_bounds__(kKvThreads, HD <= 32 ? 2 : 1) void attn_backward_kv
   }
 }
 
-// Adds the parts in their order, four neighbouring elements a thread.
+// Adds the parts (planes `step` apart) in their order, four neighbouring elements a thread; blockIdx.y: which of two tensors, one
+// plane behind the other.
 template <typename T>
-__global__ __launch_bounds__(256) void attn_backward_join_kernel(const AttnBwdArgs b) {
-  const int64_t plane = b.f.total_s * b.f.KV * b.f.D;
+__global__ __launch_bounds__(256) void attn_backward_join_kernel(const float* part, int parts, int64_t step, int64_t plane,
+                                                                 void* first, void* second) {
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   if (i >= plane) return;
-  const float* p = b.part + blockIdx.y * plane + i;
-  T* out = static_cast<T*>(blockIdx.y == 0 ? b.dk : b.dv) + i;
+  const float* p = part + blockIdx.y * plane + i;
+  T* out = static_cast<T*>(blockIdx.y == 0 ? first : second) + i;
   if (i + 4 <= plane) {
     float x[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < b.splits; ++s) {
+    for (int s = 0; s < parts; ++s) {
       float y[4];
-      load_vec<float, 4>(p + 2 * s * plane, y);
+      load_vec<float, 4>(p + s * step, y);
 #pragma unroll
       for (int j = 0; j < 4; ++j) x[j] += y[j];
     }
@@ -502,19 +519,35 @@ __global__ __launch_bounds__(256) void attn_backward_join_kernel(const AttnBwdAr
   } else {
     for (int j = 0; j < plane - i; ++j) {
       float x = 0.f;
-      for (int s = 0; s < b.splits; ++s) x += p[2 * s * plane + j];
+      for (int s = 0; s < parts; ++s) x += p[s * step + j];
       out[j] = from_f32<T>(x);
     }
   }
 }
 
 // ---- launches ----------------------------------------------------------------------------------------------------------
-// Parts of a key tile's rows: as many as bring about four workgroups to a CU.  One workgroup fills a CU, and a causal tile at
-// the start of a sequence has all the rows behind it (8192 tokens in 5 sequences, 16/4 heads of 128, bf16: 1 / 2 / 3 parts
-// 468 / 269 / 263 us, and 13 / 18 us to join the parts; 8000 tokens, 4 heads of 64, fp32: 145 / 118 + 11 us).
-int attn_backward_splits(int B, int64_t total_s, int KV) {
-  const int64_t groups = std::max<int64_t>((ceil_div(total_s, kAttnRows) + B) * KV, 1);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(1024 / groups, 8));
+// Parts of a key tile's rows: one workgroup fills a CU, so the parts are chosen that leave the fewest rows to walk in all rounds
+// of the 256 CUs (3 tiles of 128 or 64 keys on 3 heads of 256, fp32, in 8 / 6 parts: 336 / 252 workgroups, 501 / 340 us), the
+// more the better the balance: a causal tile at the start of a sequence has all the rows behind it (8192 tokens in 5 sequences,
+// 16/4 heads of 128, bf16: 1 / 2 / 3 parts 468 / 269 / 263 us, and 13 / 18 us to join the parts; 8000 tokens, 4 heads of 64, fp32:
+// 145 / 118 + 11 us).
+int attn_backward_splits(int B, int64_t total_s, int KV, int D) {
+  const int keys = attn_head_size(D) > 128 ? 64 : 128;
+  const int64_t groups = std::max<int64_t>((ceil_div(total_s, keys) + B) * KV, 1);
+  int best = 1;
+  for (int parts = 2; parts <= 8 && groups * parts * keys <= 1024 * 128; ++parts)
+    if (ceil_div(groups * parts, 256) * best <= ceil_div(groups * best, 256) * parts) best = parts;
+  return best;
+}
+
+// Parts of a row tile's keys: where the row tiles leave compute units idle, into one workgroup a CU as far as every part of a
+// sequence of the mean length keeps 128 keys (fp32) or 512 (16-bit types, whose tiles pass eight times as fast; the join is a
+// launch).  Training, fp32, 11 sequences of 46 queries and 916 keys, one head of 192: 708 us whole, 436 / 365 / 335 us with 256 /
+// 128 / 64 keys a part; one sequence of 761, one head of 256: 531 us, 395 / 313 / 291; bf16, 200 queries and 32768 keys, one head of
+// 128: 1002 -> 168 us.
+int attn_backward_q_splits(int dtype, int B, int64_t total_q, int64_t total_s, int KV, int G) {
+  const int64_t groups = std::max<int64_t>((ceil_div(total_q * G, kAttnRows) + B) * KV, 1), mean = total_s / std::max(B, 1);
+  return (int)std::max<int64_t>(1, std::min<int64_t>({256 / groups, mean / (dtype == V3D_F32 ? 128 : 512), 16}));
 }
 
 inline size_t attn_backward_table(int64_t rows, int heads) { return align_up((size_t)rows * (size_t)heads * sizeof(float), 256); }
@@ -531,16 +564,23 @@ int attn_backward_launch(AttnBwdArgs& b, hipStream_t stream, const char* what) {
     rc = launch_status(what);
   }
   if (rc == 0 && a.total_q > 0) {
-    hipLaunchKernelGGL((attn_backward_q_kernel<T, HD>), dim3((unsigned)(q_tiles * a.KV)), dim3(256), 0, stream, b);
+    hipLaunchKernelGGL((attn_backward_q_kernel<T, HD>), dim3((unsigned)(q_tiles * a.KV * b.q_splits)), dim3(256), 0, stream, b);
     rc = launch_status(what);
+    if (rc == 0 && b.q_splits > 1) {
+      const int64_t plane = a.total_q * a.H * a.D;
+      hipLaunchKernelGGL((attn_backward_join_kernel<T>), dim3((unsigned)ceil_div(plane, 1024)), dim3(256), 0, stream, b.part_q,
+                         b.q_splits, plane, plane, b.dq, b.dq);
+      rc = launch_status(what);
+    }
   }
   if (rc == 0 && a.total_s > 0 && b.dk != nullptr) {
     hipLaunchKernelGGL((attn_backward_kv_kernel<T, HD>), dim3((unsigned)(s_tiles * a.KV * b.splits)),
                        dim3(kKvThreads), 0, stream, b);
     rc = launch_status(what);
     if (rc == 0 && b.splits > 1) {
-      const dim3 grid((unsigned)ceil_div(a.total_s * a.KV * a.D, 1024), 2);
-      hipLaunchKernelGGL((attn_backward_join_kernel<T>), grid, dim3(256), 0, stream, b);
+      const int64_t plane = a.total_s * a.KV * a.D;
+      hipLaunchKernelGGL((attn_backward_join_kernel<T>), dim3((unsigned)ceil_div(plane, 1024), 2), dim3(256), 0, stream, b.part,
+                         b.splits, 2 * plane, plane, b.dk, b.dv);
       rc = launch_status(what);
     }
   }
@@ -565,10 +605,11 @@ extern "C" {
 
 size_t v3d_attention_pack_bwd_workspace_bytes(int B, int64_t total_q, int64_t total_s, int H, int KV, int D) {
   using namespace v3d;
-  if (B < 0 || total_q < 0 || total_s < 0 || H <= 0 || KV <= 0 || D <= 0) return 0;
-  const int splits = attn_backward_splits(B, total_s, KV);
-  // delta and the rows' norms (of fp16 only, but the type is not asked for)
+  if (B < 0 || total_q < 0 || total_s < 0 || H <= 0 || KV <= 0 || H % KV != 0 || D <= 0) return 0;
+  // delta and the rows' norms (of fp16 only, but the type is not asked for), the table, the parts
+  const int splits = attn_backward_splits(B, total_s, KV, D), q_splits = attn_backward_q_splits(V3D_F32, B, total_q, total_s, KV, H / KV);
   return 2 * attn_backward_table(total_q, H) + attn_backward_table(total_s, KV) + attn_table_bytes(B, 4) +
+         (q_splits > 1 ? align_up((size_t)q_splits * (size_t)total_q * (size_t)(H * D) * sizeof(float), 256) : 0) +
          (splits > 1 ? (size_t)splits * 2 * (size_t)total_s * (size_t)(KV * D) * sizeof(float) : 0);
 }
 
@@ -618,8 +659,8 @@ int v3d_attention_pack_bwd(const void* grad, const void* q, const void* k, const
   if (rc != 0) return rc;
   const int keys = attn_head_size(D) > (dtype == V3D_F32 ? 96 : 128) ? 64 : 128;  // kv_groups
   if ((ceil_div(total_q * a.G, kAttnRows) + B) * KV > kAttnMaxGroups ||
-      (ceil_div(total_s, keys) + B) * KV * attn_backward_splits(B, total_s, KV) > kAttnMaxGroups ||
-      (attn_backward_splits(B, total_s, KV) > 1 && ceil_div(total_s * KV * D, 1024) > kAttnMaxGroups)) {
+      (ceil_div(total_s, keys) + B) * KV * attn_backward_splits(B, total_s, KV, D) > kAttnMaxGroups ||
+      (attn_backward_splits(B, total_s, KV, D) > 1 && ceil_div(total_s * KV * D, 1024) > kAttnMaxGroups)) {
     set_last_error("%s: more than 2^24 row or key tiles (every sequence counts as one at least, once per key head)", what);
     return V3D_ERR_SIZE_LIMIT;
   }
@@ -640,8 +681,11 @@ int v3d_attention_pack_bwd(const void* grad, const void* q, const void* k, const
   b.grad_norm = take(attn_backward_table(total_q, H));
   b.value_norm = take(attn_backward_table(total_s, KV));
   a.table = reinterpret_cast<int64_t*>(take(attn_table_bytes(B, 4)));
+  const int q_splits = attn_backward_q_splits(V3D_F32, B, total_q, total_s, KV, a.G);  // the most of all types
+  b.part_q = take(q_splits > 1 ? align_up((size_t)q_splits * (size_t)total_q * (size_t)(H * D) * sizeof(float), 256) : 0);
   b.part = reinterpret_cast<float*>(at);
-  b.splits = attn_backward_splits(B, total_s, KV);
+  b.q_splits = grad_q == nullptr ? 1 : attn_backward_q_splits(dtype, B, total_q, total_s, KV, a.G);
+  b.splits = attn_backward_splits(B, total_s, KV, D);
   rc = dtype == V3D_F32   ? attn_backward_type<float>(b, s, what)
        : dtype == V3D_F16 ? attn_backward_type<f16>(b, s, what)
                           : attn_backward_type<bf16>(b, s, what);

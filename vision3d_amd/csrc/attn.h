@@ -695,8 +695,9 @@ inline void attn_heads(AttnArgs& a, int H, int KV, int D) {
 inline size_t attn_table_bytes(int B, int rows) { return B > kAttnWalk ? align_up((size_t)rows * ((size_t)B + 1) * 8, 256) : 0; }
 int attn_table_launch(AttnArgs& a, void* table, int row_tile, int key_tile, hipStream_t stream, const char* what);
 
-// Host side: parts that the rows of a key tile of the backward are divided into (attention_bwd.hip).
-int attn_backward_splits(int B, int64_t total_s, int KV);
+// Host side: parts that a row tile's keys and a key tile's rows are divided into in the backward (attention_bwd.hip).
+int attn_backward_q_splits(int dtype, int B, int64_t total_q, int64_t total_s, int KV, int G);
+int attn_backward_splits(int B, int64_t total_s, int KV, int D);
 
 constexpr int64_t kAttnMaxGroups = ((int64_t)1 << 24) - 1;  // a launch holds less than 2^32 threads, 256 a workgroup
 
