@@ -6,10 +6,10 @@
 // so grouped heads read every key once per tile whatever G is, and a single token of 8 heads fills 8 columns of a product
 // instead of one.
 //
-// Measured: causal prompt of 12288 tokens in 6 sequences, 32/8 heads of 128, bf16: 308 us = 774 TFLOP/s (matrix pipe 38 % busy,
-// no bank conflicts; two waves a SIMD, bound by the exponentials and by the issue of both); 32 pairs of 512 tokens, 4 heads
-// of 64, fp32: 70 us = 112 TFLOP/s (the library's fp32 product: 153); 32 caches of 2048 ... 8192 rows, one token, 32/8 heads
-// of 128, bf16: 135 us = 4.65 TB/s.
+// Measured: causal prompt of 12288 tokens in 6 sequences, 32/8 heads of 128, bf16: 300 us = 790 TFLOP/s (296 to 315 us from card
+// to card; matrix pipe 38 % busy, no bank conflicts; two waves a SIMD, bound by the exponentials and by the issue of both); 32
+// pairs of 512 tokens, 4 heads of 64, fp32: 70 us = 112 TFLOP/s (the library's fp32 product: 153); 32 caches of 2048 ... 8192
+// rows, one token, 32/8 heads of 128, bf16: 137 us = 4.6 TB/s.
 #include <algorithm>
 
 #include "attn.h"
@@ -54,6 +54,8 @@ struct AttnWave {
   Held<T, HD> q;
   f32x16 o[DT];
   float m = -__builtin_inff(), l = 0.f;  // running maximum of the products q . k, the sum of the probabilities (see scores)
+  float base = -kProbLift<T>;  // of m
+  bool large = false;          // some base of the wave is beyond kProbLarge
   float c2;
   int lane, half;
   int row, token, head;
@@ -122,16 +124,18 @@ struct AttnWave {
       const float m_new = fmaxf(m, top);
       const float alpha = prob_weight<T>(m, m_new, c2);
       m = m_new;
+      base = prob_base<T>(m, c2);
+      large = __any(__builtin_fabsf(base) >= kProbLarge);
       l *= alpha;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
     }
-    float base = prob_base<T>(m, c2);
-    if (__any(__builtin_fabsf(base) >= kProbLarge)) {
+    float from = base;
+    if (large) {
       const float at = m == -__builtin_inff() ? 0.f : m;
-      base = -kProbLift<T>;
+      from = -kProbLift<T>;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -142,7 +146,7 @@ struct AttnWave {
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        s[n][r] = exp2_fast(fmaf(s[n][r], c2, -base));
+        s[n][r] = exp2_fast(fmaf(s[n][r], c2, -from));
         sum += s[n][r];
       }
     l += sum;
@@ -449,15 +453,14 @@ __global__ __launch_bounds__((64 * few_waves<T, HD>())) void attn_few_rows_kerne
     w.template scores<1, kLarge>(tile, lds_q, key0, s);
     wave_order();
     stage_v.store(tile, a.D);
-    const bool partly = key0 + 32 > w.least;
-    bool bad = partly && stage_v.nonfinite();
+    bool first = false;  // of a tile that comes in halves
     if constexpr (kHalf) {
+      first = key0 + 32 > w.least && stage_v.nonfinite();
       fetch_v(t, 16);
       stage_v.store(tile + 16 * HDP, a.D);
-      if (partly) bad |= stage_v.nonfinite();
     }
     wave_order();
-    if (partly && __any(bad)) {
+    if (key0 + 32 > w.least && __any(first || stage_v.nonfinite())) {
       w.template add_nonfinite<1>(lds_p[wave], tile, key0, s);
       wave_order();
       clear_nonfinite(tile, SIZE, threadIdx.x & 63, 64);
@@ -654,9 +657,11 @@ struct AttnPlan {
 inline AttnPlan attn_plan(int B, int64_t total_q, int64_t total_s, int tokens, int KV, int G, int D) {
   AttnPlan p;
   // 32-row tiles where sequences have no more rows than that (a cache's newest tokens), and where 128-row tiles would keep
-  // at most a quarter of the 256 CUs: one sequence of 2048 tokens, 4 heads of 64: 22 us against 26 in bf16 (52 against 47 in
-  // fp32), 8 of 256 tokens in fp32 16 against 21; twice the tiles (2 x 1024 tokens, 2 key heads of 128, bf16): 40 us against
-  // 37, keys and values being read by four times as many workgroups.
+  // at most a quarter of the 256 CUs.  32-row against 128-row tiles: one sequence of 1000 tokens, 4 heads of 64: bf16 15 / 23 us,
+  // fp32 29 / 64; 4 x 500 tokens, 4 heads of 256: 32 / 61, 178 / 246; at the border itself (one sequence of 2048 tokens, 4 heads
+  // of 64) 22 / 25 and 50 / 46, with twice the tiles (2 x 1024 tokens, 2 key heads of 128, bf16) 40 / 37: keys and values are then
+  // read by four times as many workgroups.  (Against thousands of keys, which 128-row tiles divide more often, the rule costs:
+  // 2 x 500 tokens, 4000 keys, 4 heads of 64: bf16 39 / 26, fp32 94 / 48.)
   p.few = total_q * G <= (int64_t)32 * B || ceil_div(total_q * G, kAttnRows) * KV <= 64;
   p.tiles = tokens > 0 ? B * ceil_div((int64_t)tokens * G, p.tile()) : ceil_div(total_q * G, p.tile()) + B;
   // Keys are divided where the row tiles leave compute units idle, as far as every part of a sequence of the mean length
