@@ -459,25 +459,28 @@ int v3d_layer_norm_bwd(const void* grad, const void* feats, const void* residual
  * over all keys j of the sequence or, with `causal`, over j <= i + (s_len - q_len): the last query sees every key.  A query
  * that sees no key yields zeros; an infinity or NaN in a key or value that a query does not see does not reach it.  Rows
  * behind the last sequence are written as zeros; lengths that overrun the totals are cut.  out (total_q,H,D) contiguous;
- * rest (total_q,H,D): what rounding to a 16-bit type took from out, for the backward (whose grad . out would otherwise carry
- * it into every gradient of the row); not written in fp32; or NULL.  lse (total_q,H) fp32 = log2 of the row's sum of exp(score) (-inf without keys), what the backward needs; or NULL.
- * `strides` (host array, elements): q row, q head, k row, k head, v row, v head -- the last dimension is contiguous, rows
- * need no alignment.  Products of 16-bit types are exact, the probabilities are rounded to the type before they meet the
- * values; scores, statistics and sums are fp32.  fp32 products are formed of bf16 thirds
- * to 2^-24: an infinity that a query sees comes out as a NaN.  16 bytes <= D <= V3D_ATTENTION_MAX_HEAD_SIZE, 0 < scale < inf; strides are not
- * negative, key rows do not overlap (a stride of 0 is fine) and 129 token (or key) rows, plus a group's heads, span less than 2^29 elements.
+ * rest (total_q,H,D): what rounding to a 16-bit type took from out, for the backward (whose grad . out would otherwise
+ * carry it into every gradient of the row); not written in fp32; or NULL.  lse (total_q,H) fp32 = log2 of the row's sum
+ * of exp(score) (-inf without keys), what the backward needs; or NULL.
+ * `strides` (host array, elements): q row, q head, k row, k head, v row, v head -- the last dimension is contiguous,
+ * rows need no alignment.  Products of 16-bit types are exact, the probabilities are rounded to the type before they
+ * meet the values; scores, statistics and sums are fp32.  fp32 products are formed of bf16 thirds to 2^-24: an infinity
+ * that a query sees comes out as a NaN.  16 bytes <= D <= V3D_ATTENTION_MAX_HEAD_SIZE, 0 < scale < inf; strides are not
+ * negative, key rows do not overlap (a stride of 0 is fine) and 129 token (or key) rows, plus a group's heads, span less
+ * than 2^29 elements.
  *
  * v3d_cached_attention: q (B,tokens,H,D) = the newest `tokens` tokens of every sequence, k_cache / v_cache
  * (B,capacity,KV,D), lengths (B) i64 = filled rows, the new ones among them (cut to [0, capacity]): token t sees the rows
  * j <= lengths[b] - tokens + t.  Rows past a length are never read.  `strides`: q row, q head, k batch, k row, k head,
  * v batch, v row, v head; q rows are token b * tokens + t.
  *
- * v3d_attention_pack_bwd: grad (total_q,H,D) of out and the forward's inputs, out, rest (or NULL) and lse -> grad_q (total_q,H,D), grad_k
- * and grad_v (total_s,KV,D), all contiguous and fully written (zeros behind the last sequence); key heads sum over their
- * query heads.  grad_q, or grad_k and grad_v together, may be NULL: not wanted.  No atomics: the same bits every time.  With 16-bit types the probabilities and ds = p (grad . v - grad . out)
- * are rounded to the type before they meet the other factor, sums are fp32; fp16 ones are scaled by powers of two first, so
- * small and large gradients keep the type's precision.  p is 2^(score - lse) with lse one fp32 number a row: off by 2^-24 of the
- * scaled score's size, and no number at all past 2^30 of it (the forward has no such bound).
+ * v3d_attention_pack_bwd: grad (total_q,H,D) of out and the forward's inputs, out, rest (or NULL) and lse -> grad_q
+ * (total_q,H,D), grad_k and grad_v (total_s,KV,D), all contiguous and fully written (zeros behind the last sequence);
+ * key heads sum over their query heads.  grad_q, or grad_k and grad_v together, may be NULL: not wanted.  No atomics:
+ * the same bits every time.  With 16-bit types the probabilities and ds = p (grad . v - grad . out) are rounded to the
+ * type before they meet the other factor, sums are fp32; fp16 ones are scaled by powers of two first, so small and large
+ * gradients keep the type's precision.  p is 2^(score - lse) with lse one fp32 number a row: off by 2^-24 of the scaled
+ * score's size, and no number at all past 2^30 of it (the forward has no such bound).
  *
  * At most 2^30 query rows times heads, 2^30 keys and 2^24 tiles: about KV (B + rows / 128), V3D_ERR_SIZE_LIMIT beyond.
  * workspace: v3d_*_workspace_bytes bytes (0 where few sequences' row tiles alone fill the GPU), 256-B aligned, or NULL. */

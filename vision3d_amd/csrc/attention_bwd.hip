@@ -6,7 +6,8 @@
 // Two kernels, each the owner of what it writes, so there are no atomics and the same input gives the same bits: one goes
 // over the keys of a row tile (dq, and delta on the way), one over the rows of a key tile (dk, dv; the rows of all G query
 // heads of a key head are folded, so the sum over a group needs nothing extra).  Both form s and dp again: 7 products
-// instead of the 5 that the sums need, where a single kernel would add dq with atomics in fp32.
+// instead of the 5 that the sums need, where a single kernel would add dq with atomics in fp32.  Where tiles leave compute units
+// idle, the keys of a row tile and the rows of a key tile are divided and their sums joined in a fixed order.
 //
 // Measured, 8 x 2048 tokens, 16/4 heads of 128, bf16, no mask: dq 449 us = 918 TFLOP/s (two waves a SIMD), dk / dv 869 us = 633
 // TFLOP/s (one wave: its products and exponentials take turns).  8192 causal tokens in 5 sequences: dq 130 us, dk / dv 260 us

@@ -81,8 +81,9 @@ def attention_pack_mode(q_feats: Tensor, k_feats: Tensor, v_feats: Tensor, q_len
     H is a multiple of KV: query head h reads key head ``h // (H // KV)``.  ``s_lengths`` None: the keys are the queries'
     sequences (self-attention).  ``causal``: query i of a sequence sees the keys j <= i + (s_length - q_length), so the last
     query sees them all.  A query without keys yields zeros and has no gradient; what a query does not see does not reach
-    it, infinities and NaN included (in the forward).  Rows behind the last sequence come out as zeros.  fp32, fp16 or bf16, D from 8 (fp32: 4) to 256; the
-    inputs may be views of one projection (only the last dimension has to be contiguous).
+    it, infinities and NaN included (in the forward).  Rows behind the last sequence come out as zeros.  fp32, fp16 or bf16,
+    D from 8 (fp32: 4) to 256; the inputs may be views of one projection (only the last dimension has to be contiguous).
+    Gradients of the tensors that ask for them; no second and no forward-mode derivative.
     """
     _require_cuda("attention_pack_mode", q_feats, k_feats, v_feats)
     q_lengths = _lengths(q_lengths, q_feats)

@@ -46,8 +46,9 @@ def layer_norm(feats: Tensor, weight: Optional[Tensor] = None, bias: Optional[Te
     """feats (*, C) (+ residual of the same shape), weight / bias (C,) -> (*, C): every row normalised to mean 0 and
     variance 1 (biased, + eps), scaled and shifted.
 
-    fp32, fp16 or bf16 features; weight and bias both in the features' type or both in fp32.  Statistics and sums are fp32; the output
-    has the features' type.  At most 16384 channels (8192 in fp32).  Gradients flow to all four tensors.
+    fp32, fp16 or bf16 features; weight and bias both in the features' type or both in fp32.  Statistics and sums are fp32;
+    the output has the features' type.  At most 16384 channels (8192 in fp32).  Gradients flow to all four tensors; no second
+    and no forward-mode derivative.
     """
     for t in (feats, weight, bias, residual):
         if t is not None and not t.is_cuda:
