@@ -35,7 +35,7 @@ struct AttnBwdArgs {
 
 // ---- the range of fp16 -------------------------------------------------------------------------------------------------
 // fp16 holds 11 bits down to 2^-14 and nothing below 2^-25 or above 2^16, and p, about 1 / keys, and ds, about grad . v / keys,
-// leave that range long before the gradients do (2500 keys, gradients of 2^-10: 5e-3 off, of 2^-13: 5e-2).  So both meet their
+// leave that range long before the gradients do (4096 keys, gradients of 1e-3: 5e-3 off, of 1e-4: 5e-2).  So both meet their
 // product times a power of two, which the 32-bit sums are divided by at the end: p times 2^kLift, in the exponent; ds times a
 // factor of its row (dq) or key (dk) that puts a bound of it at 2^11 ... 2^12:
 //   |ds_ij| <= p_ij (|do_i . v_j| + |do_i . o_i|) <= 2 |do_i| max |v_j|,
@@ -528,7 +528,7 @@ __global__ __launch_bounds__(256) void attn_backward_join_kernel(const float* pa
 
 // ---- launches ----------------------------------------------------------------------------------------------------------
 // Parts of a key tile's rows: one workgroup fills a CU, so the parts are chosen that leave the fewest rows to walk in all rounds
-// of the 256 CUs (3 tiles of 128 or 64 keys on 3 heads of 256, fp32, in 8 / 6 parts: 336 / 252 workgroups, 501 / 340 us), the
+// of the 256 CUs (777 keys on 3 key heads of 256, fp32, in 8 / 6 parts: 336 / 252 workgroups, 501 / 324 us), the
 // more the better the balance: a causal tile at the start of a sequence has all the rows behind it (8192 tokens in 5 sequences,
 // 16/4 heads of 128, bf16: 1 / 2 / 3 parts 468 / 269 / 263 us, and 13 / 18 us to join the parts; 8000 tokens, 4 heads of 64, fp32:
 // 145 / 118 + 11 us).
